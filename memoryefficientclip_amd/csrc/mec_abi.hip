@@ -3,13 +3,11 @@
 // or synchronises the host.
 #include <atomic>
 #include <cmath>
-#include <cstdarg>
-#include <cstdio>
 #include <cstdlib>
 #include <cstring>
-#include <string>
 
 #include "mec.h"
+#include "mec_host.h"
 #include "mec_keep.h"
 #include "mec_kernels.h"
 #include "mec_rowops.h"
@@ -17,41 +15,6 @@
 using namespace mec;
 
 namespace {
-
-thread_local std::string g_err;
-
-int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
-int fail(int code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  g_err = buf;
-  return code;
-}
-
-// Compute units of the current device (cached per device; callers on any
-// thread may fill the cache, always with the same value).
-int compute_units(int* cus) {
-  static std::atomic<int> cache[64];
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess) return fail(MEC_ERR_HIP, "hipGetDevice failed");
-  const bool cached = dev >= 0 && dev < 64;
-  if (cached) {
-    const int v = cache[dev].load(std::memory_order_relaxed);
-    if (v > 0) {
-      *cus = v;
-      return MEC_OK;
-    }
-  }
-  int v = 0;
-  if (hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v < 1)
-    return fail(MEC_ERR_HIP, "hipDeviceGetAttribute(MultiprocessorCount) failed");
-  if (cached) cache[dev].store(v, std::memory_order_relaxed);
-  *cus = v;
-  return MEC_OK;
-}
 
 // Gradient scratch of mec_backward_noalloc: one array per GPU, held until the
 // process ends.  Host code never uses the name itself (on the host it is a
@@ -81,36 +44,6 @@ int noalloc_scratch(void** out) {
     return fail(MEC_ERR_HIP, "hipGetSymbolAddress(scratch): %s", hipGetErrorString(e));
   if (cached) cache[dev].store(p, std::memory_order_release);
   *out = p;
-  return MEC_OK;
-}
-
-int check_launch(const char* what) {
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return fail(MEC_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
-  return MEC_OK;
-}
-
-// Launches into a stream that is being captured into a HIP graph are
-// refused (MEC_ERR_UNSUPPORTED, before any launch): capturing a step of the
-// loss ended in a host segmentation fault during graph instantiation on the
-// MI355X, with no cause found in these launches.  A legacy default
-// stream implicitly joined to another stream's capture counts as capturing.
-// MEC_TEST_ASSUME_CAPTURING=1 makes the check report a capture without
-// asking HIP (tests of this refusal on machines without a GPU).
-int check_not_capturing(void* stream) {
-  const char* env = std::getenv("MEC_TEST_ASSUME_CAPTURING");
-  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-  const hipError_t e = (env && env[0] == '1') ? hipSuccess : hipStreamIsCapturing((hipStream_t)stream, &st);
-  if ((env && env[0] == '1') || e == hipErrorStreamCaptureImplicit ||
-      (e == hipSuccess && st != hipStreamCaptureStatusNone)) {
-    if (e != hipSuccess) (void)hipGetLastError();
-    return fail(MEC_ERR_UNSUPPORTED,
-                "the stream is being captured into a HIP graph; graph capture of these kernels is not supported");
-  }
-  if (e != hipSuccess) {
-    (void)hipGetLastError();
-    return fail(MEC_ERR_HIP, "hipStreamIsCapturing: %s", hipGetErrorString(e));
-  }
   return MEC_OK;
 }
 
