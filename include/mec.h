@@ -1,5 +1,6 @@
 /*
- * mec.h — C ABI of the MI355X (gfx950) memory-efficient CLIP / LiT loss.
+ * mec.h — C ABI of the MI355X (gfx950) memory-efficient CLIP / LiT loss, and of
+ * operators over a vocabulary for the text tower (the last part).
  *
  * This library replaces the four Triton kernels and the PyTorch glue of the
  * reference's autograd Functions (b0nce/MemoryEfficientCLIP):
@@ -404,6 +405,105 @@ int mec_backward(const void* x, int64_t ldx, const void* y, int64_t ldy, int64_t
 int mec_backward_noalloc(const void* x, int64_t ldx, const void* y, int64_t ldy, int64_t n, int64_t d, int dtype,
                          int mode, int normalize, float temperature, float grad_scale, const float* workspace,
                          const float* grad_output, float* acc_x, float* acc_y, void* dx, void* dy, void* stream);
+
+/* ---- The vocabulary side of a text tower ----
+ *
+ * Log probabilities of given tokens, distillation from a teacher's top logits,
+ * and the scaled token embedding, each with its gradient.  No counterpart in
+ * the reference.  The conventions above hold (error codes, streams, no
+ * allocation, no synchronisation, no graph capture), and:
+ *   - logits: `rows` rows of `vocab` elements with unit stride; row r starts at
+ *     (r / inner) * outer_stride + (r % inner) * inner_stride elements, so that
+ *     a 2-d matrix (inner = 1) and a slice of a 3-d tensor are both read in
+ *     place.  Any alignment and any strides >= 0 (rows that are one row in
+ *     memory, as after an expand, are only read).
+ *     1 <= vocab <= MEC_MAX_VOCAB, 1 <= rows <= 2^23 (MEC_ERR_UNSUPPORTED beyond).
+ *   - dtype: MEC_DTYPE_F32, MEC_DTYPE_BF16 or MEC_DTYPE_F16, of the logits and
+ *     their gradient; everything else is fp32, and sums are held in fp32.
+ *   - tokens: int64 or int32 (token_bytes 8 or 4), rows of them without gaps.
+ *   - gradients of logits are written as [rows, vocab] without gaps.
+ *   - all results are deterministic.
+ * A row of logits that is -inf throughout has log probability -inf for every
+ * token, entropy 0 and a gradient of 0.  NaN or +inf in a row makes its results
+ * NaN. */
+#define MEC_MAX_VOCAB (1LL << 19)
+#define MEC_MAX_TOP_K 128
+#define MEC_MAX_TEACHER_K 1024
+
+/* Bytes of mec_token_scores' workspace (16-byte aligned), on the current
+ * device; < 0 on bad arguments. */
+int64_t mec_token_scores_workspace_bytes(int64_t rows, int64_t vocab, int top_k, int dtype);
+
+/* p = softmax(logits / temperature) of each row; log_probs[r] = log p[tokens[r]],
+ * entropy[r] = -sum p log p, and the top_k (0: none; <= vocab, <= MEC_MAX_TOP_K)
+ * most probable tokens in order, top_tokens and top_log_probs [rows, top_k]:
+ * ties go to the lower token, NaN logits come first.  state: 2 * rows floats for
+ * mec_token_scores_backward.  A row whose token is ignore_index is not read: its
+ * log probability and entropy are 0, its top tokens -1 with 0.  A token outside
+ * [0, vocab) has log probability NaN. */
+int mec_token_scores(const void* logits, int64_t rows, int64_t inner, int64_t outer_stride, int64_t inner_stride,
+                     int64_t vocab, int dtype, const void* tokens, int token_bytes, int64_t ignore_index,
+                     float temperature, int top_k, float* log_probs, float* entropy, int64_t* top_tokens,
+                     float* top_log_probs, float* state, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Gradient of the logits for the gradients of log_probs and entropy (either may
+ * be NULL: zero), from what mec_token_scores left in state and entropy. */
+int mec_token_scores_backward(const void* logits, int64_t rows, int64_t inner, int64_t outer_stride,
+                              int64_t inner_stride, int64_t vocab, int dtype, const void* tokens, int token_bytes,
+                              int64_t ignore_index, float temperature, const float* state, const float* entropy,
+                              const float* grad_log_probs, const float* grad_entropy, void* grad_logits,
+                              void* stream);
+
+#define MEC_REDUCE_NONE 0 /* the loss of each row */
+#define MEC_REDUCE_SUM 1
+#define MEC_REDUCE_MEAN 2 /* over the rows that have a teacher; 0 if none has */
+
+/* Bytes of mec_distill_forward's workspace (16-byte aligned), on the current
+ * device; < 0 on bad arguments. */
+int64_t mec_distill_workspace_bytes(int64_t rows, int64_t vocab, int64_t k, int dtype, int with_grad);
+
+/* weight T^2 KL(q || p) of each row, T = temperature: p = softmax(logits / T) over
+ * the vocabulary, q = softmax(teacher_logits / T) over the row's k entries
+ * (teacher_tokens and teacher_logits [rows, k] without gaps, 1 <= k <=
+ * MEC_MAX_TEACHER_K; teacher_dtype as dtype).  Log probabilities serve as logits.
+ * An entry with a token < 0 is none; a row with no entry above -inf has no
+ * teacher: loss 0, gradient 0, not read.  A token >= vocab makes the row's loss
+ * and gradient NaN; entries of the same token add up.
+ * loss: rows floats for MEC_REDUCE_NONE, else one.  state: 2 * rows + 1 floats for
+ * mec_distill_backward.  grad_logits: NULL, or the gradient of the loss
+ * (MEC_REDUCE_SUM and _MEAN), made while a row of logits is at hand. */
+int mec_distill_forward(const void* logits, int64_t rows, int64_t inner, int64_t outer_stride, int64_t inner_stride,
+                        int64_t vocab, int dtype, const void* teacher_tokens, int token_bytes,
+                        const void* teacher_logits, int teacher_dtype, int64_t k, float temperature, float weight,
+                        int reduction, float* loss, float* state, void* grad_logits, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+
+/* Gradient of the logits for grad_output (device; rows floats for
+ * MEC_REDUCE_NONE, else one).  With made = 1 grad_logits holds what
+ * mec_distill_forward wrote there: then nothing is done where grad_output is 1,
+ * which the device finds out. */
+int mec_distill_backward(const void* logits, int64_t rows, int64_t inner, int64_t outer_stride, int64_t inner_stride,
+                         int64_t vocab, int dtype, const void* teacher_tokens, int token_bytes,
+                         const void* teacher_logits, int teacher_dtype, int64_t k, float temperature, float weight,
+                         int reduction, const float* state, const float* grad_output, int made, void* grad_logits,
+                         void* stream);
+
+/* out[t] = scale * weight[tokens[t]] ([n, d] without gaps, rounded to dtype once);
+ * weight [vocab, d] with row stride ldw >= d.  A token outside [0, vocab) gives a
+ * row of NaN.  1 <= n <= 2^23, 1 <= vocab <= 2^22, 1 <= d <= 2^16. */
+int mec_embedding(const void* tokens, int token_bytes, int64_t n, const void* weight, int64_t ldw, int64_t vocab,
+                  int64_t d, int dtype, float scale, void* out, void* stream);
+
+/* Bytes of mec_embedding_backward's workspace (16-byte aligned); < 0 on bad
+ * arguments. */
+int64_t mec_embedding_workspace_bytes(int64_t n, int64_t vocab, int64_t d, int dtype);
+
+/* grad_weight[v] = scale * the sum of grad_out's rows (row stride ldg >= d) whose
+ * token is v, in fp32, rounded to dtype once; 0 for a token that does not occur
+ * and for padding_idx (-1: none).  Tokens outside [0, vocab) are left out. */
+int mec_embedding_backward(const void* tokens, int token_bytes, int64_t n, const void* grad_out, int64_t ldg,
+                           int64_t vocab, int64_t d, int dtype, float scale, int64_t padding_idx, void* grad_weight,
+                           void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -66,7 +66,25 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                             _vp, _vp, _vp, _vp, _vp]),
     "mec_backward_noalloc": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _int, _int, _int, _f32, _f32, _vp, _vp,
                                     _vp, _vp, _vp, _vp, _vp]),
+    "mec_token_scores_workspace_bytes": (_i64, [_i64, _i64, _int, _int]),
+    "mec_token_scores": (_int, [_vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _int, _i64, _f32, _int, _vp, _vp, _vp,
+                                _vp, _vp, _vp, _i64, _vp]),
+    "mec_token_scores_backward": (_int, [_vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _int, _i64, _f32, _vp, _vp,
+                                         _vp, _vp, _vp, _vp]),
+    "mec_distill_workspace_bytes": (_i64, [_i64, _i64, _i64, _int, _int]),
+    "mec_distill_forward": (_int, [_vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _int, _vp, _int, _i64, _f32, _f32,
+                                   _int, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "mec_distill_backward": (_int, [_vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _int, _vp, _int, _i64, _f32, _f32,
+                                    _int, _vp, _vp, _int, _vp, _vp]),
+    "mec_embedding": (_int, [_vp, _int, _i64, _vp, _i64, _i64, _i64, _int, _f32, _vp, _vp]),
+    "mec_embedding_workspace_bytes": (_i64, [_i64, _i64, _i64, _int]),
+    "mec_embedding_backward": (_int, [_vp, _int, _i64, _vp, _i64, _i64, _i64, _int, _f32, _i64, _vp, _vp, _i64,
+                                      _vp]),
 }
+MAX_VOCAB = 1 << 19  # MEC_MAX_VOCAB
+MAX_TOP_K = 128  # MEC_MAX_TOP_K
+MAX_TEACHER_K = 1024  # MEC_MAX_TEACHER_K
+REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = 0, 1, 2
 NOALLOC_SCRATCH_BYTES = 256 << 20  # MEC_NOALLOC_SCRATCH_BYTES
 
 

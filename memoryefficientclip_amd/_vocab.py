@@ -1,0 +1,101 @@
+"""Host side shared by the operators over a vocabulary: argument checks, the
+layout of logits, scratch and the calls into the HIP library
+(``include/mec.h``)."""
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+from . import _function as _f
+from . import _lib
+
+
+def refuse_graph_capture() -> None:
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("memoryefficientclip_amd: the operators over a vocabulary do not support CUDA/HIP graph "
+                           "capture; call them outside the captured region")
+
+
+def check_gpu(name: str, t: torch.Tensor, device: torch.device | None = None) -> None:
+    """`t` is a tensor on the GPU (AssertionError else, as the losses raise it), on `device` if given."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise AssertionError(f"{name} must be a GPU tensor ({name}.is_cuda)")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the other inputs on {device}")
+
+
+def check_float(name: str, t: torch.Tensor) -> int:
+    """The C-ABI dtype code of a floating tensor."""
+    if t.dtype not in _f._DTYPES:
+        raise TypeError(f"unsupported dtype {t.dtype} of {name}; supported: float32, bfloat16, float16")
+    return _f._DTYPES[t.dtype]
+
+
+def check_tokens(name: str, t: torch.Tensor) -> int:
+    """Bytes of a token."""
+    if t.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"unsupported dtype {t.dtype} of {name}; supported: int64, int32")
+    return 8 if t.dtype == torch.int64 else 4
+
+
+def check_temperature(temperature: float) -> float:
+    temperature = float(temperature)
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"temperature must be in [1e-6, 1e6], got {temperature}")
+    return temperature
+
+
+def rows_of(logits: torch.Tensor) -> tuple[torch.Tensor, int, tuple[int, int, int, int]]:
+    """(tensor to hold, data pointer, (rows, inner, outer stride, inner stride)) of
+    logits [..., V]: read in place where the rows lie on a grid of two strides (any
+    2-d tensor with unit column stride, slices of a 3-d one), else copied."""
+    if logits.stride(-1) != 1 and logits.shape[-1] > 1:
+        logits = logits.contiguous()
+    dims = [(n, s) for n, s in zip(logits.shape[:-1], logits.stride()[:-1]) if n != 1]
+    # neighbouring dimensions that are one
+    merged: list[tuple[int, int]] = []
+    for n, s in dims:
+        if merged and merged[-1][1] == n * s:
+            merged[-1] = (merged[-1][0] * n, s)
+        else:
+            merged.append((n, s))
+    if len(merged) > 2:
+        return rows_of(logits.contiguous())
+    if not merged:
+        return logits, logits.data_ptr(), (1, 1, 0, 0)
+    if len(merged) == 1:
+        return logits, logits.data_ptr(), (merged[0][0], 1, merged[0][1], 0)
+    (n0, s0), (n1, s1) = merged
+    return logits, logits.data_ptr(), (n0 * n1, n1, s0, s1)
+
+
+@contextlib.contextmanager
+def on_device(index: int):
+    """The C-ABI calls launch on the current device."""
+    cur = torch.cuda.current_device()
+    if cur != index:
+        torch.cuda.set_device(index)
+    try:
+        yield _f._stream(index)
+    finally:
+        if cur != index:
+            torch.cuda.set_device(cur)
+
+
+@contextlib.contextmanager
+def scratch(nbytes: int, index: int):
+    """`nbytes` of the caching allocator's memory in the order of the current
+    stream of the current device `index`; < 0 is a size query's error code."""
+    if nbytes < 0:
+        raise _lib.error("size query", nbytes)
+    if nbytes == 0:
+        yield None
+        return
+    p = _f._alloc(nbytes, index)
+    try:
+        yield p
+    finally:
+        torch.cuda.caching_allocator_delete(p)

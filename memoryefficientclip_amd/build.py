@@ -9,6 +9,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -27,7 +28,6 @@ HIPCC_FLAGS = [
     "-O3",
     "-std=c++17",
     "-fPIC",
-    "-shared",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wno-unused-result",
 ]
@@ -45,14 +45,10 @@ def hipcc() -> str:
 
 
 def sources() -> list[Path]:
-    return [CSRC / "mec_abi.hip"]
+    return [CSRC / "mec_abi.hip", CSRC / "mec_vocab.hip"]
 
 
-def build(verbose: bool = False) -> Path:
-    """Compile the library (always recompiles) and return its path."""
-    LIB_DIR.mkdir(parents=True, exist_ok=True)
-    tmp = LIB.with_suffix(".so.tmp")
-    cmd = [hipcc(), *HIPCC_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", *map(str, sources()), "-o", str(tmp)]
+def _run(cmd: list[str], verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
@@ -63,6 +59,17 @@ def build(verbose: bool = False) -> Path:
         raise RuntimeError(f"hipcc failed ({res.returncode}):\n{err}")
     if verbose and err.strip():
         print(err, file=sys.stderr)
+
+
+def build(verbose: bool = False) -> Path:
+    """Compile the library (always recompiles, its sources side by side) and return its path."""
+    LIB_DIR.mkdir(parents=True, exist_ok=True)
+    tmp = LIB.with_suffix(".so.tmp")
+    objects = [LIB_DIR / f"{src.stem}.o" for src in sources()]
+    with ThreadPoolExecutor() as pool:
+        list(pool.map(lambda so: _run([hipcc(), *HIPCC_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", "-c", str(so[0]), "-o",
+                                       str(so[1])], verbose), zip(sources(), objects)))
+    _run([hipcc(), f"--offload-arch={ARCH}", "-fPIC", "-shared", *map(str, objects), "-o", str(tmp)], verbose)
     os.replace(tmp, LIB)
     return LIB
 

@@ -1,0 +1,297 @@
+// C-ABI entry points of the operators over a vocabulary (include/mec.h):
+// argument validation in plain host code, then stream-ordered kernel launches.
+// Nothing here allocates device memory or synchronises the host.
+#include <cmath>
+
+#include "mec_embed.h"
+#include "mec_host.h"
+#include "mec_vocab.h"
+
+using namespace mec;
+
+namespace {
+
+// (256 threads a row stay below 2^32 work-items)
+constexpr int64_t kMaxRows = int64_t(1) << 23;
+constexpr int64_t kMaxTokens = int64_t(1) << 23, kMaxEmbedVocab = int64_t(1) << 22, kMaxEmbedDim = int64_t(1) << 16;
+constexpr int64_t kMaxStride = int64_t(1) << 40;
+
+// float, bf16 bits or fp16 for dtype
+template <class F>
+void with_dtype(int dtype, F f) {
+  if (dtype == MEC_DTYPE_F32)
+    f((float*)nullptr);
+  else if (dtype == MEC_DTYPE_BF16)
+    f((uint16_t*)nullptr);
+  else
+    f((_Float16*)nullptr);
+}
+
+int check_dtype(int dtype) {
+  if (dtype != MEC_DTYPE_F32 && dtype != MEC_DTYPE_BF16 && dtype != MEC_DTYPE_F16)
+    return fail(MEC_ERR_INVALID, "dtype %d is not MEC_DTYPE_F32, _BF16 or _F16", dtype);
+  return MEC_OK;
+}
+
+int check_tokens(const void* tokens, int token_bytes) {
+  if (tokens == nullptr) return fail(MEC_ERR_INVALID, "tokens must be non-null");
+  if (token_bytes != 4 && token_bytes != 8) return fail(MEC_ERR_INVALID, "token_bytes=%d must be 4 or 8", token_bytes);
+  return MEC_OK;
+}
+
+int check_sizes(int64_t rows, int64_t vocab, int dtype) {
+  if (rows < 1) return fail(MEC_ERR_INVALID, "rows=%lld must be >= 1", (long long)rows);
+  if (rows > kMaxRows) return fail(MEC_ERR_UNSUPPORTED, "rows=%lld exceeds the maximum 2^23", (long long)rows);
+  if (vocab < 1) return fail(MEC_ERR_INVALID, "vocab=%lld must be >= 1", (long long)vocab);
+  if (vocab > MEC_MAX_VOCAB) return fail(MEC_ERR_UNSUPPORTED, "vocab=%lld exceeds the maximum 2^19", (long long)vocab);
+  return check_dtype(dtype);
+}
+
+// A matrix of logits as the callers give it.
+struct Logits {
+  const void* p;
+  int64_t rows, inner, outer_stride, inner_stride, vocab;
+  int dtype;
+  RowMap map() const { return RowMap{inner, outer_stride, inner_stride}; }
+};
+
+int check_logits(const Logits& x) {
+  if (int rc = check_sizes(x.rows, x.vocab, x.dtype)) return rc;
+  if (x.p == nullptr) return fail(MEC_ERR_INVALID, "logits must be non-null");
+  if (x.inner < 1) return fail(MEC_ERR_INVALID, "inner=%lld must be >= 1", (long long)x.inner);
+  if (x.outer_stride < 0 || x.inner_stride < 0 || x.outer_stride > kMaxStride || x.inner_stride > kMaxStride)
+    return fail(MEC_ERR_INVALID, "row strides %lld, %lld out of range [0, 2^40]", (long long)x.outer_stride,
+                (long long)x.inner_stride);
+  return MEC_OK;
+}
+
+int check_temperature(float t) {
+  // (1 / T and log2(e) / T are used: both have to be finite and not 0)
+  if (!(t >= 1e-6f && t <= 1e6f)) return fail(MEC_ERR_INVALID, "temperature must be in [1e-6, 1e6]");
+  return MEC_OK;
+}
+
+int check_top_k(int64_t vocab, int top_k) {
+  if (top_k < 0 || top_k > vocab)
+    return fail(MEC_ERR_INVALID, "top_k=%d out of range [0, vocab=%lld]", top_k, (long long)vocab);
+  if (top_k > MEC_MAX_TOP_K)
+    return fail(MEC_ERR_UNSUPPORTED, "top_k=%d exceeds the maximum %d", top_k, MEC_MAX_TOP_K);
+  return MEC_OK;
+}
+
+int check_workspace(const void* workspace, int64_t bytes, int64_t need) {
+  if (need > 0 && workspace == nullptr) return fail(MEC_ERR_INVALID, "workspace must be non-null");
+  if (bytes < need)
+    return fail(MEC_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)bytes, (long long)need);
+  if (((uintptr_t)workspace & 15) != 0) return fail(MEC_ERR_INVALID, "workspace must be 16-byte aligned");
+  return MEC_OK;
+}
+
+int check_teacher(const void* tokens, int token_bytes, const void* logits, int dtype, int64_t k) {
+  if (int rc = check_tokens(tokens, token_bytes)) return rc;
+  if (logits == nullptr) return fail(MEC_ERR_INVALID, "teacher_logits must be non-null");
+  if (k < 1) return fail(MEC_ERR_INVALID, "k=%lld must be >= 1", (long long)k);
+  if (k > MEC_MAX_TEACHER_K)
+    return fail(MEC_ERR_UNSUPPORTED, "k=%lld exceeds the maximum %d", (long long)k, MEC_MAX_TEACHER_K);
+  return check_dtype(dtype);
+}
+
+int check_loss(float temperature, float weight, int reduction) {
+  if (int rc = check_temperature(temperature)) return rc;
+  if (!std::isfinite(weight)) return fail(MEC_ERR_INVALID, "weight must be finite");
+  if (reduction != MEC_REDUCE_NONE && reduction != MEC_REDUCE_SUM && reduction != MEC_REDUCE_MEAN)
+    return fail(MEC_ERR_INVALID, "unknown reduction %d", reduction);
+  return MEC_OK;
+}
+
+int check_embedding(const void* tokens, int token_bytes, int64_t n, int64_t vocab, int64_t d, int dtype, float scale) {
+  if (int rc = check_tokens(tokens, token_bytes)) return rc;
+  if (n < 1 || vocab < 1 || d < 1)
+    return fail(MEC_ERR_INVALID, "n=%lld, vocab=%lld, d=%lld must be >= 1", (long long)n, (long long)vocab,
+                (long long)d);
+  if (n > kMaxTokens || vocab > kMaxEmbedVocab || d > kMaxEmbedDim)
+    return fail(MEC_ERR_UNSUPPORTED, "n=%lld, vocab=%lld, d=%lld exceed the maxima 2^23, 2^22, 2^16", (long long)n,
+                (long long)vocab, (long long)d);
+  if (!std::isfinite(scale)) return fail(MEC_ERR_INVALID, "scale must be finite");
+  return check_dtype(dtype);
+}
+
+int64_t round16(int64_t b) { return (b + 15) & ~int64_t(15); }
+
+}  // namespace
+
+extern "C" {
+
+int64_t mec_token_scores_workspace_bytes(int64_t rows, int64_t vocab, int top_k, int dtype) {
+  g_err.clear();
+  int rc = check_sizes(rows, vocab, dtype);
+  if (!rc) rc = check_top_k(vocab, top_k);
+  return rc ? rc : 0;
+}
+
+int mec_token_scores(const void* logits, int64_t rows, int64_t inner, int64_t outer_stride, int64_t inner_stride,
+                     int64_t vocab, int dtype, const void* tokens, int token_bytes, int64_t ignore_index,
+                     float temperature, int top_k, float* log_probs, float* entropy, int64_t* top_tokens,
+                     float* top_log_probs, float* state, void* workspace, int64_t workspace_bytes, void* stream) {
+  g_err.clear();
+  const Logits x{logits, rows, inner, outer_stride, inner_stride, vocab, dtype};
+  int rc = check_logits(x);
+  if (!rc) rc = check_tokens(tokens, token_bytes);
+  if (!rc) rc = check_temperature(temperature);
+  if (!rc) rc = check_top_k(vocab, top_k);
+  if (!rc && (!log_probs || !entropy || !state || (top_k > 0 && (!top_tokens || !top_log_probs))))
+    rc = fail(MEC_ERR_INVALID, "outputs and state must be non-null");
+  if (!rc)
+    rc = check_workspace(workspace, workspace_bytes, mec_token_scores_workspace_bytes(rows, vocab, top_k, dtype));
+  if (!rc) rc = check_not_capturing(stream);
+  if (rc) return rc;
+  with_dtype(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    k_token_scores<T><<<(unsigned)rows, kRowThreads, 0, (hipStream_t)stream>>>(
+        (const T*)logits, x.map(), (int)vocab, Tokens{tokens, token_bytes == 8}, ignore_index, 1.f / temperature, top_k,
+        log_probs, entropy, top_tokens, top_log_probs, state, rows);
+  });
+  return check_launch("mec_token_scores");
+}
+
+int mec_token_scores_backward(const void* logits, int64_t rows, int64_t inner, int64_t outer_stride,
+                              int64_t inner_stride, int64_t vocab, int dtype, const void* tokens, int token_bytes,
+                              int64_t ignore_index, float temperature, const float* state, const float* entropy,
+                              const float* grad_log_probs, const float* grad_entropy, void* grad_logits,
+                              void* stream) {
+  g_err.clear();
+  const Logits x{logits, rows, inner, outer_stride, inner_stride, vocab, dtype};
+  int rc = check_logits(x);
+  if (!rc) rc = check_tokens(tokens, token_bytes);
+  if (!rc) rc = check_temperature(temperature);
+  if (!rc && (!state || !entropy || !grad_logits))
+    rc = fail(MEC_ERR_INVALID, "state, entropy and grad_logits must be non-null");
+  if (!rc) rc = check_not_capturing(stream);
+  if (rc) return rc;
+  with_dtype(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    k_token_scores_grad<T><<<(unsigned)rows, kRowThreads, 0, (hipStream_t)stream>>>(
+        (const T*)logits, x.map(), (int)vocab, Tokens{tokens, token_bytes == 8}, ignore_index, 1.f / temperature, state,
+        entropy, grad_log_probs, grad_entropy, (T*)grad_logits, rows);
+  });
+  return check_launch("mec_token_scores_backward");
+}
+
+int64_t mec_distill_workspace_bytes(int64_t rows, int64_t vocab, int64_t k, int dtype, int with_grad) {
+  g_err.clear();
+  int rc = check_sizes(rows, vocab, dtype);
+  if (!rc && (k < 1 || k > MEC_MAX_TEACHER_K))
+    rc = fail(MEC_ERR_INVALID, "k=%lld out of range [1, %d]", (long long)k, MEC_MAX_TEACHER_K);
+  (void)with_grad;
+  return rc ? rc : round16(rows * 4);
+}
+
+int mec_distill_forward(const void* logits, int64_t rows, int64_t inner, int64_t outer_stride, int64_t inner_stride,
+                        int64_t vocab, int dtype, const void* teacher_tokens, int token_bytes,
+                        const void* teacher_logits, int teacher_dtype, int64_t k, float temperature, float weight,
+                        int reduction, float* loss, float* state, void* grad_logits, void* workspace,
+                        int64_t workspace_bytes, void* stream) {
+  g_err.clear();
+  const Logits x{logits, rows, inner, outer_stride, inner_stride, vocab, dtype};
+  int rc = check_logits(x);
+  if (!rc) rc = check_teacher(teacher_tokens, token_bytes, teacher_logits, teacher_dtype, k);
+  if (!rc) rc = check_loss(temperature, weight, reduction);
+  if (!rc && (!loss || !state)) rc = fail(MEC_ERR_INVALID, "loss and state must be non-null");
+  if (!rc && grad_logits && reduction == MEC_REDUCE_NONE)
+    rc = fail(MEC_ERR_INVALID, "grad_logits needs MEC_REDUCE_SUM or MEC_REDUCE_MEAN");
+  if (!rc)
+    rc = check_workspace(workspace, workspace_bytes,
+                         mec_distill_workspace_bytes(rows, vocab, k, dtype, grad_logits != nullptr));
+  if (!rc) rc = check_not_capturing(stream);
+  if (rc) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  const Teacher teacher{{teacher_tokens, token_bytes == 8}, teacher_logits, teacher_dtype, (int)k};
+  int* count = reduction == MEC_REDUCE_MEAN ? (int*)(state + 2 * rows) : nullptr;
+  if (count) {
+    k_zero_word<<<1, 1, 0, st>>>(count);
+    k_teacher_count<<<(unsigned)rows, 64, 0, st>>>(teacher, count);
+  }
+  float* row_loss = reduction == MEC_REDUCE_NONE ? loss : (float*)workspace;
+  with_dtype(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    k_distill<T><<<(unsigned)rows, kRowThreads, 0, st>>>((const T*)logits, x.map(), (int)vocab, teacher,
+                                                         1.f / temperature, weight, count, row_loss, state,
+                                                         (T*)grad_logits, rows);
+  });
+  if (reduction != MEC_REDUCE_NONE) k_loss_sum<<<1, kRowThreads, 0, st>>>(row_loss, rows, count, loss);
+  return check_launch("mec_distill_forward");
+}
+
+int mec_distill_backward(const void* logits, int64_t rows, int64_t inner, int64_t outer_stride, int64_t inner_stride,
+                         int64_t vocab, int dtype, const void* teacher_tokens, int token_bytes,
+                         const void* teacher_logits, int teacher_dtype, int64_t k, float temperature, float weight,
+                         int reduction, const float* state, const float* grad_output, int made, void* grad_logits,
+                         void* stream) {
+  g_err.clear();
+  const Logits x{logits, rows, inner, outer_stride, inner_stride, vocab, dtype};
+  int rc = check_logits(x);
+  if (!rc) rc = check_teacher(teacher_tokens, token_bytes, teacher_logits, teacher_dtype, k);
+  if (!rc) rc = check_loss(temperature, weight, reduction);
+  if (!rc && (!state || !grad_output || !grad_logits))
+    rc = fail(MEC_ERR_INVALID, "state, grad_output and grad_logits must be non-null");
+  if (!rc && made && reduction == MEC_REDUCE_NONE)
+    rc = fail(MEC_ERR_INVALID, "made needs MEC_REDUCE_SUM or MEC_REDUCE_MEAN");
+  if (!rc) rc = check_not_capturing(stream);
+  if (rc) return rc;
+  const Teacher teacher{{teacher_tokens, token_bytes == 8}, teacher_logits, teacher_dtype, (int)k};
+  const int* count = reduction == MEC_REDUCE_MEAN ? (const int*)(state + 2 * rows) : nullptr;
+  with_dtype(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    k_distill_grad<T><<<(unsigned)rows, kRowThreads, 0, (hipStream_t)stream>>>(
+        (const T*)logits, x.map(), (int)vocab, teacher, 1.f / temperature, weight, count, state, grad_output,
+        reduction == MEC_REDUCE_NONE, made, (T*)grad_logits, rows);
+  });
+  return check_launch("mec_distill_backward");
+}
+
+int mec_embedding(const void* tokens, int token_bytes, int64_t n, const void* weight, int64_t ldw, int64_t vocab,
+                  int64_t d, int dtype, float scale, void* out, void* stream) {
+  g_err.clear();
+  int rc = check_embedding(tokens, token_bytes, n, vocab, d, dtype, scale);
+  if (!rc && (!weight || !out)) rc = fail(MEC_ERR_INVALID, "weight and out must be non-null");
+  if (!rc && (ldw < d || ldw > kMaxStride))
+    rc = fail(MEC_ERR_INVALID, "row stride ldw=%lld must be in [d=%lld, 2^40]", (long long)ldw, (long long)d);
+  if (!rc) rc = check_not_capturing(stream);
+  if (rc) return rc;
+  with_dtype(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    k_embed<T><<<(unsigned)n, 256, 0, (hipStream_t)stream>>>(Tokens{tokens, token_bytes == 8}, (const T*)weight, ldw,
+                                                            vocab, (int)d, scale, (T*)out);
+  });
+  return check_launch("mec_embedding");
+}
+
+int64_t mec_embedding_workspace_bytes(int64_t n, int64_t vocab, int64_t d, int dtype) {
+  g_err.clear();
+  int rc = check_embedding((const void*)1, 8, n, vocab, d, dtype, 1.f);
+  return rc ? rc : 0;
+}
+
+int mec_embedding_backward(const void* tokens, int token_bytes, int64_t n, const void* grad_out, int64_t ldg,
+                           int64_t vocab, int64_t d, int dtype, float scale, int64_t padding_idx, void* grad_weight,
+                           void* workspace, int64_t workspace_bytes, void* stream) {
+  g_err.clear();
+  int rc = check_embedding(tokens, token_bytes, n, vocab, d, dtype, scale);
+  if (!rc && (!grad_out || !grad_weight)) rc = fail(MEC_ERR_INVALID, "grad_out and grad_weight must be non-null");
+  if (!rc && (ldg < d || ldg > kMaxStride))
+    rc = fail(MEC_ERR_INVALID, "row stride ldg=%lld must be in [d=%lld, 2^40]", (long long)ldg, (long long)d);
+  if (!rc && (padding_idx < -1 || padding_idx >= vocab))
+    rc = fail(MEC_ERR_INVALID, "padding_idx=%lld out of range [-1, vocab=%lld)", (long long)padding_idx,
+              (long long)vocab);
+  if (!rc) rc = check_workspace(workspace, workspace_bytes, mec_embedding_workspace_bytes(n, vocab, d, dtype));
+  if (!rc) rc = check_not_capturing(stream);
+  if (rc) return rc;
+  with_dtype(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    k_embed_grad<T><<<dim3((unsigned)vocab, (unsigned)((d + 255) / 256)), 256, 0, (hipStream_t)stream>>>(
+        Tokens{tokens, token_bytes == 8}, n, (const T*)grad_out, ldg, (int)d, scale, padding_idx, (T*)grad_weight);
+  });
+  return check_launch("mec_embedding_backward");
+}
+
+}  // extern "C"

@@ -1,0 +1,135 @@
+"""Distillation from a teacher's top logits: the student's distribution over the
+whole vocabulary against the teacher's over the k tokens it kept.
+
+    from memoryefficientclip_amd import TopKDistillationLoss, token_log_probs
+    t = token_log_probs(teacher_logits, tokens, top_k=32)            # once, or stored with the data
+    loss = TopKDistillationLoss(temperature=2.0)(student_logits, t.top_tokens, t.top_log_probs)
+
+Loss of a position:  T^2 KL(q || p),  q = softmax(teacher / T) over the k entries,
+p = softmax(student / T) over the vocabulary.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from . import _vocab as _v
+
+_REDUCTIONS = {"none": _lib.REDUCE_NONE, "sum": _lib.REDUCE_SUM, "mean": _lib.REDUCE_MEAN}
+
+
+class _DistillFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, teacher_tokens, teacher_logits, temperature, weight, reduction):
+        code, teacher_code = _v.check_float("student_logits", logits), _v.check_float("teacher_logits", teacher_logits)
+        token_bytes = _v.check_tokens("teacher_tokens", teacher_tokens)
+        held, px, rows = _v.rows_of(logits)
+        teacher_tokens, teacher_logits = teacher_tokens.contiguous(), teacher_logits.contiguous()
+        vocab, k, dev = logits.shape[-1], teacher_tokens.shape[-1], logits.device
+        di = dev.index
+        loss = torch.empty(logits.shape[:-1] if reduction == _lib.REDUCE_NONE else (), dtype=torch.float32, device=dev)
+        state = torch.empty(2 * rows[0] + 1, dtype=torch.float32, device=dev)
+        need = ctx.needs_input_grad[0]
+        # The gradient for grad_output 1 is made while the row is at hand: the
+        # logits are read once for loss and gradient.  fp16 programs scale their
+        # losses, so there grad_output is not 1 and the backward makes it.
+        dx = None
+        if need and reduction != _lib.REDUCE_NONE and logits.dtype != torch.float16:
+            dx = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        lib = _lib.load()
+        with _v.on_device(di) as stream:
+            nbytes = lib.mec_distill_workspace_bytes(rows[0], vocab, k, code, int(dx is not None))
+            with _v.scratch(nbytes, di) as ws:
+                rc = lib.mec_distill_forward(px, *rows, vocab, code, teacher_tokens.data_ptr(), token_bytes,
+                                             teacher_logits.data_ptr(), teacher_code, k, temperature, weight,
+                                             reduction, loss.data_ptr(), state.data_ptr(),
+                                             None if dx is None else dx.data_ptr(), ws, nbytes, stream)
+        if rc:
+            raise _lib.error("mec_distill_forward", rc)
+        if need:
+            ctx.save_for_backward(held, teacher_tokens, teacher_logits, state)
+            ctx.made = dx
+            ctx.mec = (rows, vocab, code, token_bytes, teacher_code, k, temperature, weight, reduction, logits.shape)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_output):
+        if not ctx.needs_input_grad[0]:
+            return (None,) * 6
+        _v.refuse_graph_capture()
+        held, teacher_tokens, teacher_logits, state = ctx.saved_tensors
+        rows, vocab, code, token_bytes, teacher_code, k, temperature, weight, reduction, shape = ctx.mec
+        go = grad_output.to(torch.float32).contiguous()
+        # (handed out once: its new owner may change it)
+        dx, ctx.made = ctx.made, None
+        made = dx is not None
+        if not made:
+            dx = torch.empty(shape, dtype=held.dtype, device=held.device)
+        with _v.on_device(held.device.index) as stream:
+            _lib.call("mec_distill_backward", held.data_ptr(), *rows, vocab, code, teacher_tokens.data_ptr(),
+                      token_bytes, teacher_logits.data_ptr(), teacher_code, k, temperature, weight, reduction,
+                      state.data_ptr(), go.data_ptr(), int(made), dx.data_ptr(), stream)
+        return dx, None, None, None, None, None
+
+
+class TopKDistillationLoss(nn.Module):
+    """``forward(student_logits [..., V], teacher_tokens [..., k], teacher_logits [..., k])``.
+
+    ``teacher_logits`` are the teacher's logits or log probabilities of
+    ``teacher_tokens`` (both mean the same to the softmax over them); an entry
+    with a token < 0 is none, and a position with no entry has loss 0, gradient
+    0 and no part in the mean.  ``reduction``: "mean" over the positions that
+    have a teacher, "sum" or "none"; fp32.  ``weight`` multiplies the loss.
+    Gradients flow to the student's logits only.
+
+    With "mean" and "sum" the forward leaves the gradient for ``grad_output`` 1
+    beside the loss (fp32 and bf16 logits), so that a training step reads the logits
+    once; with any other ``grad_output`` the backward makes it anew.  To
+    weight the loss against another, use ``weight``; to have the loss alone,
+    ``torch.no_grad()``.
+    """
+
+    def __init__(self, temperature=1.0, reduction="mean", weight=1.0):
+        super().__init__()
+        if reduction not in _REDUCTIONS:
+            raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
+        self.temperature = _v.check_temperature(temperature)
+        self.reduction = reduction
+        self.weight = float(weight)
+        if not math.isfinite(self.weight):
+            raise ValueError(f"weight must be finite, got {weight}")
+
+    def forward(self, student_logits, teacher_tokens, teacher_logits):
+        _v.check_gpu("student_logits", student_logits)
+        _v.check_gpu("teacher_tokens", teacher_tokens, student_logits.device)
+        _v.check_gpu("teacher_logits", teacher_logits, student_logits.device)
+        _v.refuse_graph_capture()
+        _v.check_float("student_logits", student_logits)
+        _v.check_float("teacher_logits", teacher_logits)
+        _v.check_tokens("teacher_tokens", teacher_tokens)
+        if teacher_tokens.shape != teacher_logits.shape:
+            raise ValueError(f"teacher_tokens {tuple(teacher_tokens.shape)} and teacher_logits "
+                             f"{tuple(teacher_logits.shape)} differ in shape")
+        if student_logits.dim() < 1 or teacher_tokens.dim() < 1 or student_logits.shape[:-1] != teacher_tokens.shape[:-1]:
+            raise ValueError(f"student_logits {tuple(student_logits.shape)} and teacher_tokens "
+                             f"{tuple(teacher_tokens.shape)} need the same positions")
+        vocab, k = student_logits.shape[-1], teacher_tokens.shape[-1]
+        if not 1 <= vocab <= _lib.MAX_VOCAB:
+            raise ValueError(f"the vocabulary must have 1 to {_lib.MAX_VOCAB} tokens, got {vocab}")
+        if not 1 <= k <= _lib.MAX_TEACHER_K:
+            raise ValueError(f"a position needs 1 to {_lib.MAX_TEACHER_K} teacher entries, got {k}")
+        reduction = _REDUCTIONS[self.reduction]
+        if student_logits.numel() == 0:
+            # no position: the graph's link to the logits
+            return student_logits.sum(-1, dtype=torch.float32) if reduction == _lib.REDUCE_NONE else \
+                student_logits.sum(dtype=torch.float32)
+        return _DistillFn.apply(student_logits, teacher_tokens, teacher_logits.detach(), self.temperature, self.weight,
+                                reduction)
+
+
+__all__ = ["TopKDistillationLoss"]
