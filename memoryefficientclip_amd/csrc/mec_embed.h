@@ -1,56 +1,511 @@
 // Scaled token embedding: y_t = scale W[tok_t], and its gradient
 // dW_v = scale sum_{t: tok_t = v} dy_t.
+//
+// The gradient sorts the tokens (stable, so that a token's positions stay in
+// order), sums long runs of one token in pieces, and then writes every row of
+// dW once: no atomics, sums in fp32 in an order that depends on the tokens alone.
 #pragma once
 #include "mec_vocab.h"
 
 namespace mec {
 
-// The product in 32 bits, then rounded: not contracted into one instruction that
-// rounds the exact product to 16 bits.
+// 16 bytes in memory at the alignment of a 2- or 4-byte element.
+template <int ALIGN>
+struct Bytes16;
+template <>
+struct Bytes16<2> {
+  typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2)));
+};
+template <>
+struct Bytes16<4> {
+  typedef uint32_t type __attribute__((ext_vector_type(4), aligned(4)));
+};
+
+// 16 bytes of elements at any alignment, as floats.
 template <class T>
-__device__ __forceinline__ void put_scaled(T* p, float scale, float v) {
-#pragma clang fp contract(off)
+struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+  using raw = typename Bytes16<sizeof(T)>::type;
+  static __device__ __forceinline__ void unpack(const raw& r, float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, float>::value) {
+        v[i] = __uint_as_float(r[i]);
+      } else if constexpr (std::is_same<T, uint16_t>::value) {
+        v[2 * i] = __uint_as_float(r[i] << 16);
+        v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+      } else {
+        const f16x2 h = __builtin_bit_cast(f16x2, (uint32_t)r[i]);
+        v[2 * i] = (float)h[0];
+        v[2 * i + 1] = (float)h[1];
+      }
+    }
+  }
+  static __device__ __forceinline__ raw pack(const float (&v)[N]) {
+    raw r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, float>::value)
+        r[i] = __float_as_uint(v[i]);
+      else if constexpr (std::is_same<T, uint16_t>::value)
+        r[i] = pack2_bf16(v[2 * i], v[2 * i + 1]);
+      else
+        r[i] = pack2_f16(v[2 * i], v[2 * i + 1]);
+    }
+    return r;
+  }
+};
+
+// v[i] = p[i] for i < n (n may be <= 0), 0 beyond.
+template <class T>
+__device__ __forceinline__ void load_row(const T* p, int n, float (&v)[Vec<T>::N]) {
+  constexpr int N = Vec<T>::N;
+  if (n >= N) {
+    Vec<T>::unpack(*(const typename Vec<T>::raw*)p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = i < n ? value(p[i]) : 0.f;
+  }
+}
+template <class T>
+__device__ __forceinline__ void store_row(T* p, int n, const float (&v)[Vec<T>::N]) {
+  constexpr int N = Vec<T>::N;
+  if (n >= N) {
+    *(typename Vec<T>::raw*)p = Vec<T>::pack(v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < n) put(p + i, v[i]);
+  }
+}
+
+// scale * v in 32 bits, to be rounded after: not contracted with the rounding
+// into one instruction that rounds the exact product to 16 bits.
+__device__ __forceinline__ float scaled(float scale, float v) {
   float s = scale * v;
   asm("" : "+v"(s));
-  put(p, s);
+  return s;
 }
 
-// One workgroup per token.  A token outside [0, vocab) gives a row of NaN.
-template <class T>
-__global__ __launch_bounds__(256) void k_embed(Tokens tokens, const T* weight, int64_t ldw, int64_t vocab, int d,
-                                               float scale, T* out) {
-  const int64_t t = blockIdx.x, tok = tokens[t];
-  const bool ok = tok >= 0 && tok < vocab;
-  for (int j = threadIdx.x; j < d; j += 256)
-    put_scaled(out + t * d + j, scale, ok ? value(weight[tok * ldw + j]) : NAN);
-}
+constexpr int kEmbedThreads = 256;
+constexpr int kEmbedTokens = 4;  // rows in flight per lane group
 
-// One workgroup per vocabulary row and 256 features: it looks through all
-// tokens and adds the rows of dy of its own, in order.
+// A group of 2^lg lanes takes a token's row, kEmbedTokens rows at a time.  A
+// token outside [0, vocab) gives a row of NaN.
 template <class T>
-__global__ __launch_bounds__(256) void k_embed_grad(Tokens tokens, int64_t rows, const T* dy, int64_t lddy, int d,
-                                                    float scale, int64_t padding, T* dw) {
-  __shared__ int hits[256];
-  __shared__ int wave_hits[4];
-  const int64_t v = blockIdx.x;
-  const int j = blockIdx.y * 256 + threadIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  float s = 0.f;
-  if (v != padding)
-    for (int64_t t0 = 0; t0 < rows; t0 += 256) {
-      const int64_t t = t0 + threadIdx.x;
-      const bool hit = t < rows && tokens[t] == v;
-      const uint64_t mask = __ballot(hit);
-      if (lane == 0) wave_hits[w] = __popcll(mask);
-      if (!__syncthreads_or(hit)) continue;
-      int at = __popcll(mask & ((1ull << lane) - 1)), n = 0;
-      for (int i = 0; i < 4; ++i) at += i < w ? wave_hits[i] : 0, n += wave_hits[i];
-      if (hit) hits[at] = threadIdx.x;
-      __syncthreads();
-      if (j < d)
-        for (int i = 0; i < n; ++i) s += value(dy[(t0 + hits[i]) * lddy + j]);
-      __syncthreads();
+__global__ __launch_bounds__(kEmbedThreads) void k_embed(Tokens tokens, int64_t n, const T* weight, int64_t ldw,
+                                                         int64_t vocab, int d, int lg, float scale, T* out) {
+  constexpr int N = Vec<T>::N;
+  const int lane = threadIdx.x & ((1 << lg) - 1);
+  const int groups = kEmbedThreads >> lg;
+  const int64_t t0 = (int64_t)blockIdx.x * groups * kEmbedTokens + (threadIdx.x >> lg);
+  int64_t tok[kEmbedTokens];
+#pragma unroll
+  for (int i = 0; i < kEmbedTokens; ++i) {
+    const int64_t t = t0 + i * groups;
+    tok[i] = t < n ? tokens[t] : -1;
+    if (tok[i] >= vocab) tok[i] = -1;
+  }
+  for (int col = lane * N; col < d; col += N << lg) {
+    float v[kEmbedTokens][N];
+#pragma unroll
+    for (int i = 0; i < kEmbedTokens; ++i) {
+      if (tok[i] >= 0) {
+        load_row(weight + tok[i] * ldw + col, d - col, v[i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[i][e] = NAN;
+      }
     }
-  if (j < d) put_scaled(dw + v * d + j, scale, s);
+#pragma unroll
+    for (int i = 0; i < kEmbedTokens; ++i) {
+      const int64_t t = t0 + i * groups;
+      if (t >= n) break;
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[i][e] = scaled(scale, v[i][e]);
+      store_row(out + t * d + col, d - col, v[i]);
+    }
+  }
+}
+
+// ---- stable radix sort of (token, position) by token ----
+//
+// Digits of up to 9 bits.  The array is cut into tiles, a tile into a chunk for
+// each wave, which takes 64 pairs at a time: lanes with the same digit find each
+// other with ballots, and the first of them moves the wave's own counter of that
+// digit.  A pass is two launches (tile counts, scatter); up to kSortOne pairs are
+// sorted by one workgroup in one launch.
+
+constexpr int kSortThreads = 512, kSortWaves = kSortThreads / 64;
+constexpr int kSortBins = 512;
+constexpr int kSortTiles = 128;  // at most: every workgroup reads all tile counts
+constexpr int kSortOne = 4096;
+
+struct SortShape {
+  int64_t n;
+  int tile;  // pairs per tile, a multiple of kSortThreads
+  int tiles;
+  int vocab;  // tokens outside [0, vocab) and the padding get this key and come last
+  int64_t padding;
+};
+
+struct SortSource {
+  Tokens tokens;      // the first pass
+  const uint2* pairs; // (key, position), the later ones; null in the first
+};
+
+__device__ __forceinline__ uint2 sort_item(const SortSource& src, const SortShape& s, int64_t i) {
+  if (src.pairs) return src.pairs[i];
+  const int64_t tok = src.tokens[i];
+  const bool ok = tok >= 0 && tok < s.vocab && tok != s.padding;
+  return make_uint2(ok ? (uint32_t)tok : (uint32_t)s.vocab, (uint32_t)i);
+}
+
+// Lanes of the wave with the same digit (of the active ones).
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool active) {
+  uint64_t mask = __ballot(active);
+  for (int b = 0; b < bits; ++b) {
+    const uint64_t one = __ballot((digit >> b) & 1);
+    mask &= (digit >> b) & 1 ? one : ~one;
+  }
+  return mask;
+}
+
+// Adds the chunk's digits to the wave's counters; f(pair, digit, place), place =
+// the counter's value for this pair.
+template <class F>
+__device__ __forceinline__ void sort_chunk(const SortSource& src, const SortShape& s, int64_t from, int64_t to,
+                                           int shift, int bits, int* counters, F f) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t i0 = from; i0 < to; i0 += 64) {
+    const int64_t i = i0 + lane;
+    const bool active = i < to;
+    const uint2 p = active ? sort_item(src, s, i) : make_uint2(0, 0);
+    const uint32_t digit = (p.x >> shift) & ((1u << bits) - 1);
+    const uint64_t mask = same_digit(digit, bits, active);
+    const int first = active ? __ffsll((unsigned long long)mask) - 1 : lane;
+    int old = 0;
+    if (active && lane == first) old = atomicAdd(&counters[digit], __popcll(mask));
+    old = __shfl(old, first, 64);
+    if (active) f(p, digit, old + __popcll(mask & ((1ull << lane) - 1)));
+  }
+}
+
+__device__ __forceinline__ void sort_tile_chunk(const SortShape& s, int64_t tile, int64_t& from, int64_t& to) {
+  const int64_t begin = tile * s.tile, end = begin + s.tile < s.n ? begin + s.tile : s.n;
+  from = begin + (int64_t)(threadIdx.x >> 6) * (s.tile / kSortWaves);
+  to = from + s.tile / kSortWaves;
+  if (from > end) from = end;
+  if (to > end) to = end;
+}
+
+struct SortLds {
+  int counters[kSortWaves][kSortBins];
+  int scan[kSortWaves];
+};
+
+__device__ __forceinline__ void sort_zero(SortLds& l) {
+  for (int i = threadIdx.x; i < kSortWaves * kSortBins; i += kSortThreads) (&l.counters[0][0])[i] = 0;
+  __syncthreads();
+}
+
+// Exclusive sum over the workgroup's 512 threads.
+__device__ __forceinline__ int sort_scan(int v, SortLds& l) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int s = v;
+  for (int i = 1; i < 64; i <<= 1) {
+    const int o = __shfl_up(s, i, 64);
+    if (lane >= i) s += o;
+  }
+  __syncthreads();
+  if (lane == 63) l.scan[w] = s;
+  __syncthreads();
+  int base = 0;
+  for (int i = 0; i < w; ++i) base += l.scan[i];
+  return base + s - v;
+}
+
+// counts[tile][digit]
+__global__ __launch_bounds__(kSortThreads) void k_sort_count(SortSource src, SortShape s, int shift, int bits,
+                                                             int* counts) {
+  __shared__ SortLds l;
+  sort_zero(l);
+  int64_t from, to;
+  sort_tile_chunk(s, blockIdx.x, from, to);
+  sort_chunk(src, s, from, to, shift, bits, l.counters[threadIdx.x >> 6], [](uint2, uint32_t, int) {});
+  __syncthreads();
+  int sum = 0;
+  for (int w = 0; w < kSortWaves; ++w) sum += l.counters[w][threadIdx.x];
+  counts[blockIdx.x * kSortBins + threadIdx.x] = sum;
+}
+
+// Turns the waves' counts into the places where their digits begin, given where
+// the tile's digits begin (one digit per thread).
+__device__ __forceinline__ void sort_places(SortLds& l, int begin) {
+  for (int w = 0; w < kSortWaves; ++w) {
+    const int c = l.counters[w][threadIdx.x];
+    l.counters[w][threadIdx.x] = begin;
+    begin += c;
+  }
+  __syncthreads();
+}
+
+struct SortOut {
+  uint2* pairs;   // all passes but the last
+  int* keys;      // the last
+  int* positions;
+  __device__ __forceinline__ void write(int64_t i, uint2 p) const {
+    if (pairs) {
+      pairs[i] = p;
+    } else {
+      keys[i] = (int)p.x;
+      positions[i] = (int)p.y;
+    }
+  }
+};
+
+__global__ __launch_bounds__(kSortThreads) void k_sort_scatter(SortSource src, SortShape s, int shift, int bits,
+                                                               const int* counts, SortOut out) {
+  __shared__ SortLds l;
+  sort_zero(l);
+  int64_t from, to;
+  sort_tile_chunk(s, blockIdx.x, from, to);
+  int* mine = l.counters[threadIdx.x >> 6];
+  sort_chunk(src, s, from, to, shift, bits, mine, [](uint2, uint32_t, int) {});
+  int before = 0, total = 0;
+#pragma unroll 16
+  for (int t = 0; t < s.tiles; ++t) {
+    const int c = counts[t * kSortBins + threadIdx.x];
+    total += c;
+    before += t < (int)blockIdx.x ? c : 0;
+  }
+  const int begin = sort_scan(total, l) + before;
+  sort_places(l, begin);
+  sort_chunk(src, s, from, to, shift, bits, mine, [&](uint2 p, uint32_t, int place) { out.write(place, p); });
+}
+
+// All passes by one workgroup (n <= kSortOne, one tile).
+__global__ __launch_bounds__(kSortThreads) void k_sort_one(Tokens tokens, SortShape s, int passes, int bits,
+                                                           uint2* even, uint2* odd, SortOut last) {
+  __shared__ SortLds l;
+  int64_t from, to;
+  sort_tile_chunk(s, 0, from, to);
+  int* mine = l.counters[threadIdx.x >> 6];
+  for (int pass = 0; pass < passes; ++pass) {
+    const SortSource src{tokens, pass == 0 ? nullptr : pass & 1 ? even : odd};
+    const SortOut out = pass == passes - 1 ? last : SortOut{pass & 1 ? odd : even, nullptr, nullptr};
+    sort_zero(l);
+    sort_chunk(src, s, from, to, pass * bits, bits, mine, [](uint2, uint32_t, int) {});
+    __syncthreads();
+    int total = 0;
+    for (int w = 0; w < kSortWaves; ++w) total += l.counters[w][threadIdx.x];
+    const int begin = sort_scan(total, l);
+    sort_places(l, begin);
+    sort_chunk(src, s, from, to, pass * bits, bits, mine, [&](uint2 p, uint32_t, int place) { out.write(place, p); });
+    __syncthreads();
+  }
+}
+
+// ---- sums of runs ----
+//
+// Pieces: 64 sorted positions, and blocks of 16 pieces, each at a multiple of its
+// size.  A piece (block) of one token alone is summed on its own, so that a
+// token that fills half the batch is summed by as many waves as any others.
+
+constexpr int kPiece = 64, kBlockPieces = 16, kBlock = kPiece * kBlockPieces;
+
+// acc += the rows of dy at positions [from, to) of the sorted order, in order;
+// columns col + lane * N of each of NC stretches of 64 N columns.
+template <class T, int NC>
+struct RowSum {
+  static constexpr int N = Vec<T>::N;
+  float acc[NC][N];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[c][e] = 0.f;
+  }
+  // rows of `src`, row(i) for i in [0, count)
+  template <class S, int U, class F>
+  __device__ __forceinline__ void add(const S* src, int count, int col, int d, F row) {
+    constexpr int M = Vec<S>::N, P = N / M;  // vectors of S per stretch and lane
+    int i = 0;
+    for (; i + U <= count; i += U) {
+      float v[U][NC][P][M];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const S* p = src + row(i + u);
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int q = 0; q < P; ++q) {
+            const int at = col + c * 64 * N + q * M;
+            load_row(p + at, d - at, v[u][c][q]);
+          }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int e = 0; e < N; ++e) acc[c][e] += v[u][c][e / M][e % M];
+    }
+    for (; i < count; ++i) {
+      const S* p = src + row(i);
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+          const int at = col + c * 64 * N + q * M;
+          float v[M];
+          load_row(p + at, d - at, v);
+#pragma unroll
+          for (int e = 0; e < M; ++e) acc[c][q * M + e] += v[e];
+        }
+    }
+  }
+};
+
+struct Runs {
+  const int* keys;       // sorted
+  const int* positions;
+  int64_t n;
+  int vocab;
+};
+
+// One workgroup of 16 waves per block of 1024 positions, each wave a piece:
+// piece_sums[piece] for a piece of one token, block_sums[block] if the whole
+// block is of one (then no piece_sums).
+template <class T>
+__global__ __launch_bounds__(kBlockPieces * 64) void k_embed_pieces(Runs runs, const T* dy, int64_t lddy, int d,
+                                                                    float* piece_sums, float* block_sums) {
+  constexpr int N = Vec<T>::N;
+  __shared__ float lds[kBlockPieces][64 * N];
+  const int64_t b0 = (int64_t)blockIdx.x * kBlock;
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t p0 = b0 + w * kPiece;
+  const bool all = b0 + kBlock <= runs.n && runs.keys[b0] == runs.keys[b0 + kBlock - 1] && runs.keys[b0] < runs.vocab;
+  const bool one = p0 + kPiece <= runs.n && runs.keys[p0] == runs.keys[p0 + kPiece - 1] && runs.keys[p0] < runs.vocab;
+  if (!__syncthreads_or(one)) return;
+  const int col = blockIdx.y * 64 * N + lane * N;
+  RowSum<T, 1> sum;
+  sum.zero();
+  if (one) {
+    const int pos = runs.positions[p0 + lane];
+    sum.template add<T, 8>(dy, kPiece, col, d, [&](int i) { return (int64_t)__builtin_amdgcn_readlane(pos, i) * lddy; });
+  }
+  if (!all) {
+    if (one) {
+#pragma unroll
+      for (int q = 0; q < N / 4; ++q) {
+        const float v[4] = {sum.acc[0][q * 4], sum.acc[0][q * 4 + 1], sum.acc[0][q * 4 + 2], sum.acc[0][q * 4 + 3]};
+        store_row(piece_sums + (p0 / kPiece) * d + col + q * 4, d - col - q * 4, v);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e) lds[w][e * 64 + lane] = sum.acc[0][e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 64 * N; i += kBlockPieces * 64) {
+    const int c = blockIdx.y * 64 * N + (i & 63) * N + (i >> 6);
+    float s = 0.f;
+    for (int p = 0; p < kBlockPieces; ++p) s += lds[p][i];
+    if (c < d) block_sums[(int64_t)blockIdx.x * d + c] = s;
+  }
+}
+
+// First index whose key is >= v.
+__device__ __forceinline__ int64_t lower_bound(const Runs& r, int v) {
+  int64_t lo = 0, hi = r.n;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (r.keys[mid] < v)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+constexpr int kDwRows = 16;  // vocabulary rows per workgroup
+
+// Every row of dW: a wave per row for runs of up to 64 positions, the
+// workgroup's 4 waves together for longer ones, with the pieces' sums.
+template <class T, int NC>
+__global__ __launch_bounds__(256) void k_embed_rows(Runs runs, const T* dy, int64_t lddy, int d, float scale,
+                                                    const float* piece_sums, const float* block_sums, T* dw) {
+  constexpr int N = Vec<T>::N;
+  constexpr int U = NC >= 4 ? 2 : 8 / NC;
+  __shared__ int64_t starts[kDwRows + 1];
+  __shared__ float lds[3][NC * N * 64];
+  const int v0 = blockIdx.x * kDwRows;
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int col = blockIdx.y * NC * 64 * N + lane * N;
+  if (threadIdx.x <= kDwRows) starts[threadIdx.x] = lower_bound(runs, v0 + threadIdx.x < runs.vocab ? v0 + threadIdx.x : runs.vocab);
+  __syncthreads();
+  auto write = [&](int v, RowSum<T, NC>& sum) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) sum.acc[c][e] = scaled(scale, sum.acc[c][e]);
+      const int at = col + c * 64 * N;
+      store_row(dw + (int64_t)v * d + at, d - at, sum.acc[c]);
+    }
+  };
+  RowSum<T, NC> sum;
+  for (int r = w; r < kDwRows && v0 + r < runs.vocab; r += 4) {
+    const int64_t lo = starts[r];
+    const int count = (int)(starts[r + 1] - lo < 65 ? starts[r + 1] - lo : 65);
+    if (count > 64) continue;
+    sum.zero();
+    const int pos = lane < count ? runs.positions[lo + lane] : 0;
+    sum.template add<T, U>(dy, count, col, d, [&](int i) { return (int64_t)__builtin_amdgcn_readlane(pos, i) * lddy; });
+    write(v0 + r, sum);
+  }
+  for (int r = 0; r < kDwRows && v0 + r < runs.vocab; ++r) {
+    const int64_t lo = starts[r], hi = starts[r + 1];
+    if (hi - lo <= 64) continue;
+    // [lo, a) positions, [a, a2) pieces, [a2, b2) blocks, [b2, b) pieces, [b, hi) positions
+    const int64_t a = (lo + kPiece - 1) / kPiece * kPiece, b = hi / kPiece * kPiece;
+    int64_t a2 = (a + kBlock - 1) / kBlock * kBlock, b2 = b / kBlock * kBlock;
+    if (a2 >= b2) a2 = b2 = b;
+    sum.zero();
+    auto positions = [&](int64_t from, int64_t to) {  // at most 63, a quarter for each wave
+      const int count = (int)(to - from), q = (count + 3) / 4;
+      const int at = w * q < count ? w * q : count, mine = count - at < q ? count - at : q;
+      const int pos = lane < mine ? runs.positions[from + at + lane] : 0;
+      sum.template add<T, U>(dy, mine, col, d, [&](int i) { return (int64_t)__builtin_amdgcn_readlane(pos, i) * lddy; });
+    };
+    auto sums = [&](const float* s, int64_t from, int64_t to) {
+      const int64_t count = to - from, q = (count + 3) / 4;
+      const int64_t at = w * q < count ? w * q : count;
+      const int mine = (int)(count - at < q ? count - at : q);
+      sum.template add<float, U>(s, mine, col, d, [&](int i) { return (from + at + i) * (int64_t)d; });
+    };
+    positions(lo, a);
+    sums(piece_sums, a / kPiece, a2 / kPiece);
+    sums(block_sums, a2 / kBlock, b2 / kBlock);
+    sums(piece_sums, b2 / kPiece, b / kPiece);
+    positions(b, hi);
+    __syncthreads();
+    if (w > 0) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < N; ++e) lds[w - 1][(c * N + e) * 64 + lane] = sum.acc[c][e];
+    }
+    __syncthreads();
+    if (w == 0) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          for (int p = 0; p < 3; ++p) sum.acc[c][e] += lds[p][(c * N + e) * 64 + lane];
+      write(v0 + r, sum);
+    }
+  }
 }
 
 }  // namespace mec

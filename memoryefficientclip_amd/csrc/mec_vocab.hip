@@ -117,6 +117,57 @@ int check_embedding(const void* tokens, int token_bytes, int64_t n, int64_t voca
 }
 
 int64_t round16(int64_t b) { return (b + 15) & ~int64_t(15); }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Workspace of mec_embedding_backward, in bytes from its start.
+struct EmbedWorkspace {
+  int64_t even, odd, keys, positions, counts, pieces, blocks, total;
+};
+EmbedWorkspace embed_workspace(int64_t n, int64_t d) {
+  EmbedWorkspace w;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t p = at;
+    at += round16(bytes);
+    return p;
+  };
+  w.even = take(n * 8);
+  w.odd = take(n * 8);
+  w.keys = take(n * 4);
+  w.positions = take(n * 4);
+  w.counts = take((int64_t)kSortTiles * kSortBins * 4);
+  w.pieces = take(n / kPiece * d * 4);
+  w.blocks = take(n / kBlock * d * 4);
+  w.total = at;
+  return w;
+}
+
+// Sorted tokens and their positions into the workspace.
+Runs sort_tokens(const void* tokens, int token_bytes, int64_t n, int64_t vocab, int64_t padding,
+                 const EmbedWorkspace& w, char* ws, hipStream_t st) {
+  int key_bits = 1;
+  while ((vocab >> key_bits) != 0) ++key_bits;
+  const int passes = (key_bits + 8) / 9, bits = (key_bits + passes - 1) / passes;
+  SortShape s{n, 0, 1, (int)vocab, padding};
+  const Tokens tok{tokens, token_bytes == 8};
+  uint2 *even = (uint2*)(ws + w.even), *odd = (uint2*)(ws + w.odd);
+  const SortOut last{nullptr, (int*)(ws + w.keys), (int*)(ws + w.positions)};
+  if (n <= kSortOne) {
+    s.tile = (int)(ceil_div(n, kSortThreads) * kSortThreads);
+    k_sort_one<<<1, kSortThreads, 0, st>>>(tok, s, passes, bits, even, odd, last);
+  } else {
+    s.tile = (int)(ceil_div(ceil_div(n, kSortTiles), kSortThreads) * kSortThreads);
+    s.tiles = (int)ceil_div(n, s.tile);
+    int* counts = (int*)(ws + w.counts);
+    for (int pass = 0; pass < passes; ++pass) {
+      const SortSource src{tok, pass == 0 ? nullptr : pass & 1 ? even : odd};
+      const SortOut out = pass == passes - 1 ? last : SortOut{pass & 1 ? odd : even, nullptr, nullptr};
+      k_sort_count<<<s.tiles, kSortThreads, 0, st>>>(src, s, pass * bits, bits, counts);
+      k_sort_scatter<<<s.tiles, kSortThreads, 0, st>>>(src, s, pass * bits, bits, counts, out);
+    }
+  }
+  return Runs{last.keys, last.positions, n, (int)vocab};
+}
 
 }  // namespace
 
@@ -260,8 +311,11 @@ int mec_embedding(const void* tokens, int token_bytes, int64_t n, const void* we
   if (rc) return rc;
   with_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    k_embed<T><<<(unsigned)n, 256, 0, (hipStream_t)stream>>>(Tokens{tokens, token_bytes == 8}, (const T*)weight, ldw,
-                                                            vocab, (int)d, scale, (T*)out);
+    int lg = 0;  // lanes for a row: up to a wave, one vector each
+    while (lg < 6 && (int64_t)Vec<T>::N << lg < d) ++lg;
+    const int64_t per_group = (kEmbedThreads >> lg) * kEmbedTokens;
+    k_embed<T><<<(unsigned)ceil_div(n, per_group), kEmbedThreads, 0, (hipStream_t)stream>>>(
+        Tokens{tokens, token_bytes == 8}, n, (const T*)weight, ldw, vocab, (int)d, lg, scale, (T*)out);
   });
   return check_launch("mec_embedding");
 }
@@ -269,7 +323,7 @@ int mec_embedding(const void* tokens, int token_bytes, int64_t n, const void* we
 int64_t mec_embedding_workspace_bytes(int64_t n, int64_t vocab, int64_t d, int dtype) {
   g_err.clear();
   int rc = check_embedding((const void*)1, 8, n, vocab, d, dtype, 1.f);
-  return rc ? rc : 0;
+  return rc ? rc : embed_workspace(n, d).total;
 }
 
 int mec_embedding_backward(const void* tokens, int token_bytes, int64_t n, const void* grad_out, int64_t ldg,
@@ -283,13 +337,32 @@ int mec_embedding_backward(const void* tokens, int token_bytes, int64_t n, const
   if (!rc && (padding_idx < -1 || padding_idx >= vocab))
     rc = fail(MEC_ERR_INVALID, "padding_idx=%lld out of range [-1, vocab=%lld)", (long long)padding_idx,
               (long long)vocab);
-  if (!rc) rc = check_workspace(workspace, workspace_bytes, mec_embedding_workspace_bytes(n, vocab, d, dtype));
+  const EmbedWorkspace w = rc ? EmbedWorkspace{} : embed_workspace(n, d);
+  if (!rc) rc = check_workspace(workspace, workspace_bytes, w.total);
   if (!rc) rc = check_not_capturing(stream);
   if (rc) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  char* ws = (char*)workspace;
+  float *pieces = (float*)(ws + w.pieces), *blocks = (float*)(ws + w.blocks);
+  const Runs runs = sort_tokens(tokens, token_bytes, n, vocab, padding_idx, w, ws, st);
   with_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    k_embed_grad<T><<<dim3((unsigned)vocab, (unsigned)((d + 255) / 256)), 256, 0, (hipStream_t)stream>>>(
-        Tokens{tokens, token_bytes == 8}, n, (const T*)grad_out, ldg, (int)d, scale, padding_idx, (T*)grad_weight);
+    constexpr int N = Vec<T>::N;
+    if (n >= kPiece)
+      k_embed_pieces<T><<<dim3((unsigned)ceil_div(n, kBlock), (unsigned)ceil_div(d, 64 * N)), kBlockPieces * 64, 0, st>>>(
+          runs, (const T*)grad_out, ldg, (int)d, pieces, blocks);
+    const unsigned groups = (unsigned)ceil_div(vocab, kDwRows);
+    auto rows = [&](auto nc) {
+      constexpr int NC = decltype(nc)::value;
+      k_embed_rows<T, NC><<<dim3(groups, (unsigned)ceil_div(d, NC * 64 * N)), 256, 0, st>>>(
+          runs, (const T*)grad_out, ldg, (int)d, scale, pieces, blocks, (T*)grad_weight);
+    };
+    if (d <= 64 * N)
+      rows(std::integral_constant<int, 1>{});
+    else if (d <= 128 * N)
+      rows(std::integral_constant<int, 2>{});
+    else
+      rows(std::integral_constant<int, 4>{});
   });
   return check_launch("mec_embedding_backward");
 }
