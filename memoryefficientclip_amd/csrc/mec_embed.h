@@ -56,16 +56,25 @@ struct Vec {
   }
 };
 
-// v[i] = p[i] for i < n (n may be <= 0), 0 beyond.
+// p[i] for i < n (n may be <= 0), zero bits beyond.
+template <class T>
+__device__ __forceinline__ typename Vec<T>::raw load_raw(const T* p, int n) {
+  constexpr int N = Vec<T>::N;
+  if (n >= N) return *(const typename Vec<T>::raw*)p;
+  typename Vec<T>::raw r = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < n) {
+      if constexpr (sizeof(T) == 4)
+        r[i] = __float_as_uint(p[i]);
+      else
+        r[i / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, p[i]) << (16 * (i & 1));
+    }
+  return r;
+}
 template <class T>
 __device__ __forceinline__ void load_row(const T* p, int n, float (&v)[Vec<T>::N]) {
-  constexpr int N = Vec<T>::N;
-  if (n >= N) {
-    Vec<T>::unpack(*(const typename Vec<T>::raw*)p, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = i < n ? value(p[i]) : 0.f;
-  }
+  Vec<T>::unpack(load_raw(p, n), v);
 }
 template <class T>
 __device__ __forceinline__ void store_row(T* p, int n, const float (&v)[Vec<T>::N]) {
@@ -308,11 +317,11 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_one(Tokens tokens, SortSh
 
 // ---- sums of runs ----
 //
-// Pieces: 64 sorted positions, and blocks of 16 pieces, each at a multiple of its
+// Pieces: 32 sorted positions, and blocks of 8 pieces, each at a multiple of its
 // size.  A piece (block) of one token alone is summed on its own, so that a
 // token that fills half the batch is summed by as many waves as any others.
 
-constexpr int kPiece = 64, kBlockPieces = 16, kBlock = kPiece * kBlockPieces;
+constexpr int kPiece = 32, kBlockPieces = 8, kBlock = kPiece * kBlockPieces;
 
 // acc += the rows of dy at positions [from, to) of the sorted order, in order;
 // columns col + lane * N of each of NC stretches of 64 N columns.
@@ -332,7 +341,7 @@ struct RowSum {
     constexpr int M = Vec<S>::N, P = N / M;  // vectors of S per stretch and lane
     int i = 0;
     for (; i + U <= count; i += U) {
-      float v[U][NC][P][M];
+      typename Vec<S>::raw v[U][NC][P];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const S* p = src + row(i + u);
@@ -341,7 +350,7 @@ struct RowSum {
 #pragma unroll
           for (int q = 0; q < P; ++q) {
             const int at = col + c * 64 * N + q * M;
-            load_row(p + at, d - at, v[u][c][q]);
+            v[u][c][q] = load_raw(p + at, d - at);
           }
       }
 #pragma unroll
@@ -349,7 +358,12 @@ struct RowSum {
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int e = 0; e < N; ++e) acc[c][e] += v[u][c][e / M][e % M];
+          for (int q = 0; q < P; ++q) {
+            float f[M];
+            Vec<S>::unpack(v[u][c][q], f);
+#pragma unroll
+            for (int e = 0; e < M; ++e) acc[c][q * M + e] += f[e];
+          }
     }
     for (; i < count; ++i) {
       const S* p = src + row(i);
@@ -372,11 +386,13 @@ struct Runs {
   const int* positions;
   int64_t n;
   int vocab;
+  int2* bounds;          // of each token's run: first and last + 1; 0, 0 for none
 };
 
-// One workgroup of 16 waves per block of 1024 positions, each wave a piece:
+// One workgroup of 8 waves per block of 256 positions, each wave a piece:
 // piece_sums[piece] for a piece of one token, block_sums[block] if the whole
-// block is of one (then no piece_sums).
+// block is of one (then no piece_sums).  The first column's workgroups also note
+// where the runs begin and end.
 template <class T>
 __global__ __launch_bounds__(kBlockPieces * 64) void k_embed_pieces(Runs runs, const T* dy, int64_t lddy, int d,
                                                                     float* piece_sums, float* block_sums) {
@@ -384,17 +400,26 @@ __global__ __launch_bounds__(kBlockPieces * 64) void k_embed_pieces(Runs runs, c
   __shared__ float lds[kBlockPieces][64 * N];
   const int64_t b0 = (int64_t)blockIdx.x * kBlock;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t p0 = b0 + w * kPiece;
-  const bool all = b0 + kBlock <= runs.n && runs.keys[b0] == runs.keys[b0 + kBlock - 1] && runs.keys[b0] < runs.vocab;
-  const bool one = p0 + kPiece <= runs.n && runs.keys[p0] == runs.keys[p0 + kPiece - 1] && runs.keys[p0] < runs.vocab;
+  const int64_t p0 = b0 + w * kPiece, at = p0 + lane;
+  // the wave's keys, and the one before and after
+  const bool in = lane < kPiece && at < runs.n;
+  const int key = in ? runs.keys[at] : runs.vocab;
+  const int pos = in ? runs.positions[at] : 0;
+  const int last = b0 + kBlock <= runs.n ? runs.keys[b0 + kBlock - 1] : runs.vocab;
+  const int first = runs.keys[b0];
+  if (blockIdx.y == 0 && in && key < runs.vocab) {
+    if (at == 0 || runs.keys[at - 1] != key) runs.bounds[key].x = (int)at;
+    if (at + 1 == runs.n || runs.keys[at + 1] != key) runs.bounds[key].y = (int)at + 1;
+  }
+  const bool all = first == last && first < runs.vocab;
+  const int key0 = __builtin_amdgcn_readlane(key, 0);
+  const bool one = key0 < runs.vocab && key0 == __builtin_amdgcn_readlane(key, kPiece - 1);
   if (!__syncthreads_or(one)) return;
   const int col = blockIdx.y * 64 * N + lane * N;
   RowSum<T, 1> sum;
   sum.zero();
-  if (one) {
-    const int pos = runs.positions[p0 + lane];
-    sum.template add<T, 8>(dy, kPiece, col, d, [&](int i) { return (int64_t)__builtin_amdgcn_readlane(pos, i) * lddy; });
-  }
+  if (one)
+    sum.template add<T, 16>(dy, kPiece, col, d, [&](int i) { return (int64_t)__builtin_amdgcn_readlane(pos, i) * lddy; });
   if (!all) {
     if (one) {
 #pragma unroll
@@ -416,36 +441,30 @@ __global__ __launch_bounds__(kBlockPieces * 64) void k_embed_pieces(Runs runs, c
   }
 }
 
-// First index whose key is >= v.
-__device__ __forceinline__ int64_t lower_bound(const Runs& r, int v) {
-  int64_t lo = 0, hi = r.n;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (r.keys[mid] < v)
-      lo = mid + 1;
-    else
-      hi = mid;
-  }
-  return lo;
+__global__ __launch_bounds__(256) void k_embed_clear(int2* bounds, int vocab) {
+  const int v = blockIdx.x * 256 + threadIdx.x;
+  if (v < vocab) bounds[v] = make_int2(0, 0);
 }
 
-constexpr int kDwRows = 16;  // vocabulary rows per workgroup
+constexpr int kWaveRows = 4, kDwRows = 4 * kWaveRows;  // vocabulary rows per wave, per workgroup
+constexpr int kShortRun = 2 * kPiece;
 
-// Every row of dW: a wave per row for runs of up to 64 positions, the
-// workgroup's 4 waves together for longer ones, with the pieces' sums.
+// Every row of dW, four to a wave: the positions of their runs of up to 64 are
+// one list, whose rows of dy are loaded one after another across the ends of the
+// runs.  Longer runs are summed by the workgroup's 4 waves together, with the
+// pieces' sums.
 template <class T, int NC>
 __global__ __launch_bounds__(256) void k_embed_rows(Runs runs, const T* dy, int64_t lddy, int d, float scale,
                                                     const float* piece_sums, const float* block_sums, T* dw) {
   constexpr int N = Vec<T>::N;
   constexpr int U = NC >= 4 ? 2 : 8 / NC;
-  __shared__ int64_t starts[kDwRows + 1];
   __shared__ float lds[3][NC * N * 64];
   const int v0 = blockIdx.x * kDwRows;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int col = blockIdx.y * NC * 64 * N + lane * N;
-  if (threadIdx.x <= kDwRows) starts[threadIdx.x] = lower_bound(runs, v0 + threadIdx.x < runs.vocab ? v0 + threadIdx.x : runs.vocab);
-  __syncthreads();
-  auto write = [&](int v, RowSum<T, NC>& sum) {
+  const int2 bound = lane < kDwRows && v0 + lane < runs.vocab ? runs.bounds[v0 + lane] : make_int2(0, 0);
+  RowSum<T, NC> sum;
+  auto write = [&](int v) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
 #pragma unroll
@@ -453,35 +472,74 @@ __global__ __launch_bounds__(256) void k_embed_rows(Runs runs, const T* dy, int6
       const int at = col + c * 64 * N;
       store_row(dw + (int64_t)v * d + at, d - at, sum.acc[c]);
     }
-  };
-  RowSum<T, NC> sum;
-  for (int r = w; r < kDwRows && v0 + r < runs.vocab; r += 4) {
-    const int64_t lo = starts[r];
-    const int count = (int)(starts[r + 1] - lo < 65 ? starts[r + 1] - lo : 65);
-    if (count > 64) continue;
     sum.zero();
-    const int pos = lane < count ? runs.positions[lo + lane] : 0;
-    sum.template add<T, U>(dy, count, col, d, [&](int i) { return (int64_t)__builtin_amdgcn_readlane(pos, i) * lddy; });
-    write(v0 + r, sum);
+  };
+  // the wave's short runs as one list
+  int begin[kWaveRows], end[kWaveRows + 1];  // of the run; of its part of the list
+  end[0] = 0;
+  sum.zero();
+#pragma unroll
+  for (int r = 0; r < kWaveRows; ++r) {
+    const int q = w * kWaveRows + r;
+    begin[r] = __builtin_amdgcn_readlane(bound.x, q);
+    const int count = __builtin_amdgcn_readlane(bound.y, q) - begin[r];
+    end[r + 1] = end[r] + (count <= kShortRun ? count : 0);
+    if (count == 0 && v0 + q < runs.vocab) write(v0 + q);
   }
-  for (int r = 0; r < kDwRows && v0 + r < runs.vocab; ++r) {
-    const int64_t lo = starts[r], hi = starts[r + 1];
-    if (hi - lo <= 64) continue;
+  const int total = end[kWaveRows];
+  int r = 0;
+  for (int i0 = 0; i0 < total; i0 += 64) {
+    const int i = i0 + lane;
+    int at = begin[0];
+#pragma unroll
+    for (int k = 1; k < kWaveRows; ++k) at = i >= end[k] ? begin[k] - end[k] : at;
+    const int pos = i < total ? runs.positions[at + i] : 0;
+    const int n = total - i0 < 64 ? total - i0 : 64;
+    for (int j = 0; j < n; j += U) {
+      typename Vec<T>::raw v[U][NC];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const T* p = dy + (int64_t)__builtin_amdgcn_readlane(pos, j + u < n ? j + u : n - 1) * lddy;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) v[u][c] = load_raw(p + col + c * 64 * N, d - col - c * 64 * N);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (j + u >= n) break;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          float f[N];
+          Vec<T>::unpack(v[u][c], f);
+#pragma unroll
+          for (int e = 0; e < N; ++e) sum.acc[c][e] += f[e];
+        }
+        // (the list's runs are not empty but for those that were written above or are long)
+        const int done = i0 + j + u + 1;
+#pragma unroll
+        for (int k = 0; k < kWaveRows; ++k)
+          if (done == end[k + 1] && end[k] < done) write(v0 + w * kWaveRows + k);
+      }
+    }
+  }
+  const uint64_t longer = __ballot(bound.y - bound.x > kShortRun);
+  for (uint64_t left = longer; left; left &= left - 1) {
+    const int q = __ffsll((unsigned long long)left) - 1;
+    const int64_t lo = __builtin_amdgcn_readlane(bound.x, q), hi = __builtin_amdgcn_readlane(bound.y, q);
     // [lo, a) positions, [a, a2) pieces, [a2, b2) blocks, [b2, b) pieces, [b, hi) positions
     const int64_t a = (lo + kPiece - 1) / kPiece * kPiece, b = hi / kPiece * kPiece;
     int64_t a2 = (a + kBlock - 1) / kBlock * kBlock, b2 = b / kBlock * kBlock;
     if (a2 >= b2) a2 = b2 = b;
     sum.zero();
-    auto positions = [&](int64_t from, int64_t to) {  // at most 63, a quarter for each wave
-      const int count = (int)(to - from), q = (count + 3) / 4;
-      const int at = w * q < count ? w * q : count, mine = count - at < q ? count - at : q;
+    auto positions = [&](int64_t from, int64_t to) {  // fewer than a piece, a quarter for each wave
+      const int count = (int)(to - from), each = (count + 3) / 4;
+      const int at = w * each < count ? w * each : count, mine = count - at < each ? count - at : each;
       const int pos = lane < mine ? runs.positions[from + at + lane] : 0;
       sum.template add<T, U>(dy, mine, col, d, [&](int i) { return (int64_t)__builtin_amdgcn_readlane(pos, i) * lddy; });
     };
     auto sums = [&](const float* s, int64_t from, int64_t to) {
-      const int64_t count = to - from, q = (count + 3) / 4;
-      const int64_t at = w * q < count ? w * q : count;
-      const int mine = (int)(count - at < q ? count - at : q);
+      const int64_t count = to - from, each = (count + 3) / 4;
+      const int64_t at = w * each < count ? w * each : count;
+      const int mine = (int)(count - at < each ? count - at : each);
       sum.template add<float, U>(s, mine, col, d, [&](int i) { return (from + at + i) * (int64_t)d; });
     };
     positions(lo, a);
@@ -503,7 +561,7 @@ __global__ __launch_bounds__(256) void k_embed_rows(Runs runs, const T* dy, int6
 #pragma unroll
         for (int e = 0; e < N; ++e)
           for (int p = 0; p < 3; ++p) sum.acc[c][e] += lds[p][(c * N + e) * 64 + lane];
-      write(v0 + r, sum);
+      write(v0 + q);
     }
   }
 }

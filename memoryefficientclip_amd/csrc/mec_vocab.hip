@@ -121,9 +121,9 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Workspace of mec_embedding_backward, in bytes from its start.
 struct EmbedWorkspace {
-  int64_t even, odd, keys, positions, counts, pieces, blocks, total;
+  int64_t even, odd, keys, positions, bounds, counts, pieces, blocks, total;
 };
-EmbedWorkspace embed_workspace(int64_t n, int64_t d) {
+EmbedWorkspace embed_workspace(int64_t n, int64_t vocab, int64_t d) {
   EmbedWorkspace w;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -135,6 +135,7 @@ EmbedWorkspace embed_workspace(int64_t n, int64_t d) {
   w.odd = take(n * 8);
   w.keys = take(n * 4);
   w.positions = take(n * 4);
+  w.bounds = take(vocab * 8);
   w.counts = take((int64_t)kSortTiles * kSortBins * 4);
   w.pieces = take(n / kPiece * d * 4);
   w.blocks = take(n / kBlock * d * 4);
@@ -166,7 +167,9 @@ Runs sort_tokens(const void* tokens, int token_bytes, int64_t n, int64_t vocab, 
       k_sort_scatter<<<s.tiles, kSortThreads, 0, st>>>(src, s, pass * bits, bits, counts, out);
     }
   }
-  return Runs{last.keys, last.positions, n, (int)vocab};
+  int2* bounds = (int2*)(ws + w.bounds);
+  k_embed_clear<<<(unsigned)ceil_div(vocab, 256), 256, 0, st>>>(bounds, (int)vocab);
+  return Runs{last.keys, last.positions, n, (int)vocab, bounds};
 }
 
 }  // namespace
@@ -323,7 +326,7 @@ int mec_embedding(const void* tokens, int token_bytes, int64_t n, const void* we
 int64_t mec_embedding_workspace_bytes(int64_t n, int64_t vocab, int64_t d, int dtype) {
   g_err.clear();
   int rc = check_embedding((const void*)1, 8, n, vocab, d, dtype, 1.f);
-  return rc ? rc : embed_workspace(n, d).total;
+  return rc ? rc : embed_workspace(n, vocab, d).total;
 }
 
 int mec_embedding_backward(const void* tokens, int token_bytes, int64_t n, const void* grad_out, int64_t ldg,
@@ -337,7 +340,7 @@ int mec_embedding_backward(const void* tokens, int token_bytes, int64_t n, const
   if (!rc && (padding_idx < -1 || padding_idx >= vocab))
     rc = fail(MEC_ERR_INVALID, "padding_idx=%lld out of range [-1, vocab=%lld)", (long long)padding_idx,
               (long long)vocab);
-  const EmbedWorkspace w = rc ? EmbedWorkspace{} : embed_workspace(n, d);
+  const EmbedWorkspace w = rc ? EmbedWorkspace{} : embed_workspace(n, vocab, d);
   if (!rc) rc = check_workspace(workspace, workspace_bytes, w.total);
   if (!rc) rc = check_not_capturing(stream);
   if (rc) return rc;
@@ -348,9 +351,8 @@ int mec_embedding_backward(const void* tokens, int token_bytes, int64_t n, const
   with_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int N = Vec<T>::N;
-    if (n >= kPiece)
-      k_embed_pieces<T><<<dim3((unsigned)ceil_div(n, kBlock), (unsigned)ceil_div(d, 64 * N)), kBlockPieces * 64, 0, st>>>(
-          runs, (const T*)grad_out, ldg, (int)d, pieces, blocks);
+    k_embed_pieces<T><<<dim3((unsigned)ceil_div(n, kBlock), (unsigned)ceil_div(d, 64 * N)), kBlockPieces * 64, 0, st>>>(
+        runs, (const T*)grad_out, ldg, (int)d, pieces, blocks);
     const unsigned groups = (unsigned)ceil_div(vocab, kDwRows);
     auto rows = [&](auto nc) {
       constexpr int NC = decltype(nc)::value;
