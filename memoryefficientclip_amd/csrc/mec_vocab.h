@@ -8,7 +8,7 @@
 // A row of nothing but -inf has S = 0: p = 0, log p = -inf, entropy 0.  A NaN or
 // +inf makes S NaN, and with it all that is formed from the row.
 #pragma once
-#include "mec_common.h"
+#include "mec_vec.h"
 
 namespace mec {
 
@@ -19,16 +19,11 @@ constexpr float kLn2 = 0.69314718055994531f;
 struct RowMap {
   int64_t inner, outer_stride, inner_stride;
   __device__ __forceinline__ int64_t operator()(int64_t r) const {
-    return inner == 1 ? r * outer_stride : (r / inner) * outer_stride + (r % inner) * inner_stride;
+    if (inner == 1) return r * outer_stride;
+    const uint32_t q = (uint32_t)r / (uint32_t)inner;  // (r < 2^23)
+    return q * outer_stride + ((uint32_t)r - q * (uint32_t)inner) * inner_stride;
   }
 };
-
-__device__ __forceinline__ float value(float v) { return v; }
-__device__ __forceinline__ float value(uint16_t v) { return bf16_to_f32(v); }
-__device__ __forceinline__ float value(_Float16 v) { return (float)v; }
-__device__ __forceinline__ void put(float* p, float v) { *p = v; }
-__device__ __forceinline__ void put(uint16_t* p, float v) { *p = f32_to_bf16(v); }
-__device__ __forceinline__ void put(_Float16* p, float v) { *p = (_Float16)v; }
 
 // Token i of an int64 or int32 array.
 struct Tokens {
@@ -97,45 +92,429 @@ __device__ __forceinline__ RowSums row_sums(const T* x, int n, float c, float* l
   return {ref, s, u};
 }
 
-// One workgroup per row.
+// t = (x - m) c as one fma with m c rounded beforehand.  The rounding of m c, below
+// 2^-2, moves every t of the row alike and drops out of p and log p, which are formed
+// from t.  Where m c is larger, up to fp32's end, the difference is taken first.
+struct Reference {
+  float m, c, mc;
+  bool far;
+  __device__ __forceinline__ Reference(float row_max, float scale) {
+    m = row_max == -INFINITY ? 0.f : row_max;
+    c = scale;
+    mc = m * c;
+    far = !(fabsf(mc) < 4194304.f);
+  }
+  __device__ __forceinline__ float t(float x) const { return far ? 2.f * c * (0.5f * x - 0.5f * m) : fmaf(x, c, -mc); }
+  // what to add to t of this one to have it relative to `to`
+  __device__ __forceinline__ float shift(const Reference& to) const {
+    if (far) return to.t(m);
+    return to.far ? fmaf(-to.m, c, mc) : mc - to.mc;
+  }
+};
+
+// ---- token log probabilities ----
+//
+// A row is cut into segments that a workgroup holds in registers: up to 8
+// vectors of 16 bytes a thread.  A segment is read once; maximum, sums and the
+// top k come from the registers.  Rows of more than one segment are joined by
+// k_scores_join.
+
+constexpr int kSegChunks = 8;
+constexpr int kMaxSegments = 64;  // a lane each in the join
+
+// A vector's words with -inf in the first `skip` elements.
 template <class T>
-__global__ __launch_bounds__(kRowThreads) void k_token_scores(const T* logits, RowMap map, int n, Tokens tokens,
-                                                              int64_t ignore, float inv_t, int k, float* log_probs,
-                                                              float* entropy, int64_t* top_tokens,
-                                                              float* top_log_probs, float* stats, int64_t rows) {
-  __shared__ float lds[kRowThreads / 64];
-  __shared__ uint64_t lds64[kRowThreads / 64];
+__device__ __forceinline__ typename Vec<T>::raw skip_elements(typename Vec<T>::raw r, int skip) {
+  constexpr uint32_t kInf = std::is_same<T, float>::value      ? 0xff800000u
+                            : std::is_same<T, uint16_t>::value ? 0xff80ff80u
+                                                               : 0xfc00fc00u;
+  constexpr int kPer = 4 / sizeof(T);  // elements in a word
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int in_word = skip - i * kPer;
+    const uint32_t mask = in_word <= 0 ? 0u : in_word >= kPer ? ~0u : 0xffffu;
+    r[i] = (r[i] & ~mask) | (kInf & mask);
+  }
+  return r;
+}
+
+template <class T>
+struct Segment {
+  static constexpr int N = Vec<T>::N, kChunk = kRowThreads * N;
+  typename Vec<T>::raw v[kSegChunks];
+  int n, first;  // elements; the thread's first one
+  // n elements at p.  A vector that would pass the end is the last one that
+  // does not, with -inf for the elements that belong to the thread before.
+  __device__ __forceinline__ void load(const T* p, int count) {
+    n = count;
+    first = threadIdx.x * N;
+    if (n < N) {
+      v[0] = first == 0 ? load_small(p) : skip_elements<T>(v[0], N);
+      return;
+    }
+#pragma unroll
+    for (int c = 0; c < kSegChunks; ++c) {
+      // (set in any case: a register set in one trip alone is kept through the next)
+      if (c * kChunk < n)
+        v[c] = *(const typename Vec<T>::raw*)(p + begin(c));
+      else
+        v[c] = skip_elements<T>(v[c], N);
+    }
+#pragma unroll
+    for (int c = 0; c < kSegChunks; ++c)
+      if (c * kChunk < n && (c + 1) * kChunk > n) v[c] = skip_elements<T>(v[c], c * kChunk + first - begin(c));
+  }
+  __device__ __forceinline__ typename Vec<T>::raw load_small(const T* p) {
+    typename Vec<T>::raw r = {0, 0, 0, 0};
+    r = skip_elements<T>(r, N);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < n) {
+        constexpr int kPer = 4 / sizeof(T);
+        if constexpr (kPer == 1) {
+          r[i] = __float_as_uint(p[i]);
+        } else {
+          const uint32_t at = 16 * (i & 1), q = __builtin_bit_cast(uint16_t, p[i]);
+          r[i / 2] = (r[i / 2] & ~(0xffffu << at)) | (q << at);
+        }
+      }
+    return r;
+  }
+  // where chunk c's vector begins
+  __device__ __forceinline__ int begin(int c) const {
+    const int at = c * kChunk + first;
+    return n < N ? 0 : at < n - N ? at : n - N;
+  }
+  // Unpacked anew by every pass: what one pass unpacks is not kept for the next
+  // (twice the registers, and spills).
+  __device__ __forceinline__ void values(int c, float (&x)[N]) const {
+    typename Vec<T>::raw r = v[c];
+    asm volatile("" : "+v"(r));
+    Vec<T>::unpack(r, x);
+  }
+  // f(element, its index) over the thread's elements that pred holds for: few
+  template <class P, class F>
+  __device__ __forceinline__ void each_of(P pred, F f) const {
+#pragma unroll
+    for (int c = 0; c < kSegChunks; ++c) {
+      if (c * kChunk >= n) break;
+      float x[N];
+      values(c, x);
+      uint32_t hits = 0;
+#pragma unroll
+      for (int e = 0; e < N; ++e) hits |= pred(x[e]) ? 1u << e : 0u;
+      if (hits == 0) continue;
+      const int i0 = begin(c);
+#pragma unroll 1
+      for (; hits; hits &= hits - 1) {
+        const int e = __ffs(hits) - 1;
+        float y = x[0];
+#pragma unroll
+        for (int q = 1; q < N; ++q) y = e == q ? x[q] : y;
+        if (i0 + e >= c * kChunk + first && i0 + e < n) f(y, i0 + e);
+      }
+    }
+  }
+  // f(element) over the thread's elements (and -inf in place of others')
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+    for (int c = 0; c < kSegChunks; ++c) {
+      if (c * kChunk >= n) break;
+      float x[N];
+      values(c, x);
+#pragma unroll
+      for (int e = 0; e < N; ++e) f(x[e]);
+    }
+  }
+};
+
+// Of the keys that the lanes hold through key(i), i < per_lane: the largest
+// number (its lowest `low` bits 0) that at least k keys reach, or a smaller one
+// that no more than `enough` reach.
+template <class K, class F>
+__device__ __forceinline__ K kth_largest(int per_lane, int low, int k, int enough, F key) {
+  K cut = 0;
+  for (int bit = sizeof(K) * 8 - 1; bit >= low; --bit) {
+    const K trial = cut | ((K)1 << bit);
+    int reach = 0;
+    for (int i = 0; i < per_lane; ++i) reach += __popcll(__ballot(key(i) >= trial));
+    if (reach >= k) {
+      cut = trial;
+      if (reach <= enough) break;
+    }
+  }
+  return cut;
+}
+
+constexpr int kCandidates = 1024;
+
+struct TopLds {
+  float thread_max[kRowThreads];
+  uint64_t found[kCandidates];
+  int count, scan[kRowThreads / 64];
+  float cut;
+};
+
+// After thread_max is there (and count is 0): by the first wave, a value that at
+// least k elements of the segment reach: so many threads' maxima do.
+__device__ __forceinline__ void top_cut(TopLds& l, int k) {
+  constexpr int kPer = kRowThreads / 64;
+  const int lane = threadIdx.x;
+  uint32_t key[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) key[i] = order_bits(l.thread_max[i * 64 + lane]);
+  uint32_t cut = 0;
+  for (int bit = 31; bit >= 16; --bit) {
+    const uint32_t trial = cut | (1u << bit);
+    int reach = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) reach += __popcll(__ballot(key[i] >= trial));
+    if (reach >= k) {
+      cut = trial;
+      if (reach <= k + k / 4) break;
+    }
+  }
+  // (0: too few threads have elements; as NaN it keeps nothing out)
+  if (lane == 0) l.cut = key_value((uint64_t)cut << 32);
+}
+
+// The k largest of n elements at x, where more of them reach `cut` than there is
+// room for (equal values, or a few threads with most of the large ones): the
+// k-th largest value exactly, the elements above it, and the first of those equal
+// to it.  Reads them again, from the cache; rare.
+template <class T>
+__device__ __attribute__((noinline)) void top_exactly(TopLds& l, const T* x, int n, int base, int k) {
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  auto count_from = [&](uint32_t from) {
+    int c = 0;
+    for (int i = tid; i < n; i += kRowThreads) c += order_bits(value(x[i])) >= from;
+    for (int s = 32; s >= 1; s >>= 1) c += __shfl_xor(c, s, 64);
+    __syncthreads();
+    if (lane == 0) l.scan[w] = c;
+    __syncthreads();
+    return l.scan[0] + l.scan[1] + l.scan[2] + l.scan[3];
+  };
+  const float cut = l.cut;
+  uint32_t kth = cut != cut ? 0u : order_bits(cut);  // reached by k at least
+  if (kth == 0 || count_from(kth + 1) >= k) {
+    kth = 0;
+    for (int bit = 31; bit >= 0; --bit)
+      if (count_from(kth | (1u << bit)) >= k) kth |= 1u << bit;
+  }
+  __syncthreads();
+  if (tid == 0) l.count = 0;
+  __syncthreads();
+  for (int i = tid; i < n; i += kRowThreads)
+    if (order_bits(value(x[i])) > kth) l.found[atomicAdd(&l.count, 1)] = order_key(value(x[i]), base + i);
+  __syncthreads();
+  int have = l.count;
+  for (int i0 = 0; i0 < n && have < k; i0 += kRowThreads) {
+    const int i = i0 + tid;
+    const bool mine = i < n && order_bits(value(x[i])) == kth;
+    const uint64_t mask = __ballot(mine);
+    __syncthreads();
+    if (lane == 0) l.scan[w] = __popcll(mask);
+    __syncthreads();
+    int at = have + __popcll(mask & ((1ull << lane) - 1));
+    for (int q = 0; q < w; ++q) at += l.scan[q];
+    if (mine && at < k) l.found[at] = order_key(value(x[i]), base + i);
+    have += l.scan[0] + l.scan[1] + l.scan[2] + l.scan[3];
+  }
+  __syncthreads();
+  if (tid == 0) l.count = k;
+  __syncthreads();
+}
+
+// The k largest of the segment (and perhaps others), keys with indexes from
+// `base`, at found[0 .. count) in no order; k <= the segment's elements.
+template <class T>
+__device__ __forceinline__ void top_collect(TopLds& l, const Segment<T>& v, const T* x, int base, int k) {
+  const float cut = l.cut;
+  v.each_of([&](float f) { return !(f < cut); },
+            [&](float f, int i) {
+              const int at = atomicAdd(&l.count, 1);
+              if (at < kCandidates) l.found[at] = order_key(f, base + i);
+            });
+  __syncthreads();
+  if (l.count > kCandidates) top_exactly(l, x, v.n, base, k);
+}
+
+struct ScoresOut {
+  float* log_probs;
+  float* entropy;
+  int64_t* top_tokens;
+  float* top_log_probs;
+  float* stats;  // m, S
+};
+
+// One row's result from its sums.
+struct RowResult {
+  Reference ref;
+  float s, ls, inv_t;
+  __device__ __forceinline__ RowResult(const Reference& r, float sum, float it)
+      : ref(r), s(sum), ls(logf(sum)), inv_t(it) {}
+  __device__ __forceinline__ float log_prob(float x) const {
+    if (s == 0.f) return -INFINITY;
+    const float t = ref.t(x);  // (log2's units pass fp32's range before the result does)
+    return (t > -1e30f ? kLn2 * t : scaled_difference(x, ref.m, inv_t)) - ls;
+  }
+  __device__ __forceinline__ float entropy(float u) const { return s == 0.f ? 0.f : ls - kLn2 * (u / s); }
+};
+
+__device__ __forceinline__ void write_ignored(const ScoresOut& out, int64_t r, int64_t rows, int k, int tid,
+                                              int threads) {
+  if (tid == 0) out.log_probs[r] = 0.f, out.entropy[r] = 0.f, out.stats[r] = 0.f, out.stats[rows + r] = 0.f;
+  for (int j = tid; j < k; j += threads) out.top_tokens[r * k + j] = -1, out.top_log_probs[r * k + j] = 0.f;
+}
+
+// blockIdx.x: the row; blockIdx.y: its segment, of `len` elements.
+// With one segment the row's results, else part[row][seg] = (m, S, U) and the
+// segment's top k keys.
+template <class T, bool TOP>
+__global__ __launch_bounds__(kRowThreads) void k_scores(const T* logits, RowMap map, int n, Tokens tokens,
+                                                        int64_t ignore, float inv_t, int k, ScoresOut out,
+                                                        int64_t rows, int len, float4* parts, uint64_t* part_top) {
+  constexpr int kWaves = kRowThreads / 64;
+  __shared__ float wave_max[kWaves], wave_s[kWaves], wave_u[kWaves];
+  __shared__ std::conditional_t<TOP, TopLds, char> top;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const float c = inv_t * (1.f / kLn2);
+  const int segments = gridDim.y, seg = blockIdx.y, base = seg * len;
+  const int64_t r = blockIdx.x, item = r * segments + seg;
+  {
+    const int64_t tok = tokens[r];
+    if (tok == ignore) {
+      if (segments == 1) write_ignored(out, r, rows, k, tid, kRowThreads);
+      return;
+    }
+    const T* x = logits + map(r) + base;
+    Segment<T> v;
+    v.load(x, n - base < len ? n - base : len);
+    float m = -INFINITY;
+    v.each([&](float f) { m = fmaxf(m, f); });
+    if constexpr (TOP) {
+      top.thread_max[tid] = m;
+      if (tid == 0) top.count = 0;
+    }
+    for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
+    if (lane == 0) wave_max[w] = m;
+    __syncthreads();
+    m = wave_max[0];
+    for (int i = 1; i < kWaves; ++i) m = fmaxf(m, wave_max[i]);
+    const int kk = TOP ? (k < v.n ? k : v.n) : 0;
+    if constexpr (TOP) {
+      if (w == 0) top_cut(top, kk);
+    }
+    const Reference ref(m, c);
+    float s = 0.f, u = 0.f;
+    auto sums = [&](auto far) {
+      v.each([&](float f) {
+        const float t = decltype(far)::value ? ref.t(f) : fmaf(f, c, -ref.mc);
+        const float e = fast_exp2(t);
+        s += e;
+        // (2^t is 0 below -200, where t may be -inf)
+        u = fmaf(e, fmaxf(t, -200.f), u);
+      });
+    };
+    if (ref.far)
+      sums(std::true_type{});
+    else
+      sums(std::false_type{});
+    s = wave_sum(s);
+    u = wave_sum(u);
+    if (lane == 0) wave_s[w] = s, wave_u[w] = u;
+    __syncthreads();
+    s = u = 0.f;
+    for (int i = 0; i < kWaves; ++i) s += wave_s[i], u += wave_u[i];
+    if constexpr (TOP) top_collect(top, v, x, base, kk);
+    const RowResult row(ref, s, inv_t);
+    if (tid == 0) {
+      if (segments == 1) {
+        out.log_probs[r] = tok >= 0 && tok < n ? row.log_prob(value(x[tok])) : NAN;
+        out.entropy[r] = row.entropy(u);
+        out.stats[r] = ref.m;
+        out.stats[rows + r] = s;
+      } else {
+        parts[item] = make_float4(m, s, u, 0.f);
+      }
+    }
+    if constexpr (TOP) {
+      const int count = top.count;
+      for (int i = tid; i < count; i += kRowThreads) {
+        const uint64_t key = top.found[i];
+        int rank = 0;
+        for (int j = 0; j < count; ++j) rank += top.found[j] > key;
+        if (rank >= kk) continue;
+        if (segments == 1) {
+          out.top_tokens[r * k + rank] = key_index(key);
+          out.top_log_probs[r * k + rank] = row.log_prob(key_value(key));
+        } else {
+          part_top[item * k + rank] = key;
+        }
+      }
+      if (segments > 1)
+        for (int i = kk + tid; i < k; i += kRowThreads) part_top[item * k + i] = 0;
+    }
+  }
+}
+
+constexpr int kJoinThreads = 64;
+
+// One wave per row: its segments' sums, a lane each, and the k largest of their
+// top keys (all different, so that exactly k reach the k-th).
+template <class T>
+__global__ __launch_bounds__(kJoinThreads) void k_scores_join(const T* logits, RowMap map, int n, Tokens tokens,
+                                                              int64_t ignore, float inv_t, int k, ScoresOut out,
+                                                              int64_t rows, int segments, const float4* parts,
+                                                              const uint64_t* part_top) {
+  extern __shared__ uint64_t keys[];  // segments * k, then k
   const int64_t r = blockIdx.x;
+  const int lane = threadIdx.x;
   const int64_t tok = tokens[r];
-  const int tid = threadIdx.x;
   if (tok == ignore) {
-    if (tid == 0) log_probs[r] = 0.f, entropy[r] = 0.f, stats[r] = 0.f, stats[rows + r] = 0.f;
-    for (int j = tid; j < k; j += kRowThreads) top_tokens[r * k + j] = -1, top_log_probs[r * k + j] = 0.f;
+    write_ignored(out, r, rows, k, lane, kJoinThreads);
     return;
   }
-  const T* x = logits + map(r);
-  const RowSums a = row_sums<T, true>(x, n, inv_t / kLn2, lds);
-  const float ls = logf(a.s);
-  auto log_prob = [&](float v) { return a.s == 0.f ? -INFINITY : scaled_difference(v, a.m, inv_t) - ls; };
-  if (tid == 0) {
-    log_probs[r] = tok >= 0 && tok < n ? log_prob(value(x[tok])) : NAN;
-    entropy[r] = a.s == 0.f ? 0.f : ls - kLn2 * (a.u / a.s);
-    stats[r] = a.m;
-    stats[rows + r] = a.s;
+  const float at = tok >= 0 && tok < n ? value(logits[map(r) + tok]) : 0.f;
+  const int count = segments * k;
+  for (int i = lane; i < count; i += 64) keys[i] = part_top[r * count + i];
+  const float c = inv_t * (1.f / kLn2);
+  const float4 p = lane < segments ? parts[r * segments + lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+  float m = p.x;
+  for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
+  const Reference ref(m, c);
+  // (S = 0: nothing of the segment can occur, and its shift may be -inf)
+  const float shift = Reference(p.x, c).shift(ref), scale = fast_exp2(shift);
+  const float s = wave_sum(p.y == 0.f ? 0.f : p.y * scale);
+  const float u = wave_sum(p.y == 0.f ? 0.f : scale * fmaf(p.y, fmaxf(shift, -200.f), p.z));
+  const RowResult row(ref, s, inv_t);
+  if (lane == 0) {
+    out.log_probs[r] = tok >= 0 && tok < n ? row.log_prob(at) : NAN;
+    out.entropy[r] = row.entropy(u);
+    out.stats[r] = ref.m;
+    out.stats[rows + r] = s;
   }
-  uint64_t last = 0;
-  for (int j = 0; j < k; ++j) {
-    uint64_t best = 0;
-    for (int v = tid; v < n; v += kRowThreads) {
-      const uint64_t q = order_key(value(x[v]), v);
-      if ((j == 0 || q < last) && q > best) best = q;
-    }
-    best = block_reduce(best, lds64, [](uint64_t p, uint64_t q) { return p > q ? p : q; });
-    last = best;
-    if (tid == 0) {
-      top_tokens[r * k + j] = key_index(best);
-      top_log_probs[r * k + j] = log_prob(value(x[key_index(best)]));
-    }
+  if (k == 0) return;
+  __syncthreads();
+  const uint64_t cut = kth_largest<uint64_t>((count + 63) / 64, 0, k, k, [&](int i) {
+    return i * 64 + lane < count ? keys[i * 64 + lane] : 0;
+  });
+  uint64_t* best = keys + count;
+  int have = 0;
+  for (int i0 = 0; i0 < count; i0 += 64) {
+    const uint64_t key = i0 + lane < count ? keys[i0 + lane] : 0;
+    const uint64_t mask = __ballot(key >= cut);
+    if (key >= cut) best[have + __popcll(mask & ((1ull << lane) - 1))] = key;
+    have += __popcll(mask);
+  }
+  __syncthreads();
+  for (int i = lane; i < k; i += 64) {
+    const uint64_t key = best[i];
+    int rank = 0;
+    for (int j = 0; j < k; ++j) rank += best[j] > key;
+    out.top_tokens[r * k + rank] = key_index(key);
+    out.top_log_probs[r * k + rank] = row.log_prob(key_value(key));
   }
 }
 
@@ -152,13 +531,14 @@ __global__ __launch_bounds__(kRowThreads) void k_token_scores_grad(const T* logi
   const float m = stats[r], s = stats[rows + r], h = entropy[r];
   const bool none = tok == ignore || s == 0.f, bad = tok < 0 || tok >= n;
   const float gl = g_log_probs ? g_log_probs[r] : 0.f, gh = g_entropy ? g_entropy[r] : 0.f;
+  const Reference ref(m, inv_t * (1.f / kLn2));
   const float ls = logf(s), inv_s = 1.f / s;
   for (int v = threadIdx.x; v < n; v += kRowThreads) {
     float d = 0.f;
     if (!none) {
-      const float z = fmaxf((value(x[v]) - m) * inv_t, -200.f);
-      const float p = fast_exp2(z * (1.f / kLn2)) * inv_s;
-      d = inv_t * ((v == tok ? gl : 0.f) - p * (gl + gh * (z - ls + h)));
+      const float t = ref.t(value(x[v]));
+      const float p = fast_exp2(t) * inv_s;
+      d = inv_t * ((v == tok ? gl : 0.f) - p * (gl + gh * (kLn2 * fmaxf(t, -200.f) - ls + h)));
       if (value(x[v]) != value(x[v]) || bad) d = NAN;
     }
     put(y + v, d);

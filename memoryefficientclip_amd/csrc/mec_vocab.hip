@@ -119,6 +119,27 @@ int check_embedding(const void* tokens, int token_bytes, int64_t n, int64_t voca
 int64_t round16(int64_t b) { return (b + 15) & ~int64_t(15); }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// How token scores cut a row.
+struct Cut {
+  int segments, len;
+};
+Cut cut_rows(int64_t rows, int64_t vocab, int dtype) {
+  const int64_t chunk = kRowThreads * (dtype == MEC_DTYPE_F32 ? 4 : 8);  // a vector per thread
+  int64_t s = ceil_div(vocab, chunk * kSegChunks);
+  // few rows: more, shorter segments, so that there are workgroups for every CU
+  const int64_t want = ceil_div(1024, rows);
+  if (s < want) s = want;
+  if (s > ceil_div(vocab, chunk)) s = ceil_div(vocab, chunk);
+  if (s > kMaxSegments) s = kMaxSegments;
+  const int64_t len = ceil_div(ceil_div(vocab, s), chunk) * chunk;
+  return Cut{(int)ceil_div(vocab, len), (int)len};
+}
+int64_t scores_parts_bytes(int64_t rows, const Cut& c) { return c.segments > 1 ? rows * c.segments * 16 : 0; }
+int64_t scores_workspace(int64_t rows, int64_t vocab, int top_k, int dtype) {
+  const Cut c = cut_rows(rows, vocab, dtype);
+  return c.segments > 1 ? scores_parts_bytes(rows, c) + round16(rows * c.segments * top_k * 8) : 0;
+}
+
 // Workspace of mec_embedding_backward, in bytes from its start.
 struct EmbedWorkspace {
   int64_t even, odd, keys, positions, bounds, counts, pieces, blocks, total;
@@ -180,7 +201,7 @@ int64_t mec_token_scores_workspace_bytes(int64_t rows, int64_t vocab, int top_k,
   g_err.clear();
   int rc = check_sizes(rows, vocab, dtype);
   if (!rc) rc = check_top_k(vocab, top_k);
-  return rc ? rc : 0;
+  return rc ? rc : scores_workspace(rows, vocab, top_k, dtype);
 }
 
 int mec_token_scores(const void* logits, int64_t rows, int64_t inner, int64_t outer_stride, int64_t inner_stride,
@@ -195,15 +216,29 @@ int mec_token_scores(const void* logits, int64_t rows, int64_t inner, int64_t ou
   if (!rc) rc = check_top_k(vocab, top_k);
   if (!rc && (!log_probs || !entropy || !state || (top_k > 0 && (!top_tokens || !top_log_probs))))
     rc = fail(MEC_ERR_INVALID, "outputs and state must be non-null");
-  if (!rc)
-    rc = check_workspace(workspace, workspace_bytes, mec_token_scores_workspace_bytes(rows, vocab, top_k, dtype));
+  if (!rc) rc = check_workspace(workspace, workspace_bytes, scores_workspace(rows, vocab, top_k, dtype));
   if (!rc) rc = check_not_capturing(stream);
   if (rc) return rc;
+  hipStream_t st = (hipStream_t)stream;
   with_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    k_token_scores<T><<<(unsigned)rows, kRowThreads, 0, (hipStream_t)stream>>>(
-        (const T*)logits, x.map(), (int)vocab, Tokens{tokens, token_bytes == 8}, ignore_index, 1.f / temperature, top_k,
-        log_probs, entropy, top_tokens, top_log_probs, state, rows);
+    const T* p = (const T*)logits;
+    const Tokens tok{tokens, token_bytes == 8};
+    const Cut cut = cut_rows(rows, vocab, dtype);
+    float4* parts = (float4*)workspace;
+    uint64_t* part_top = (uint64_t*)((char*)workspace + scores_parts_bytes(rows, cut));
+    const ScoresOut out{log_probs, entropy, top_tokens, top_log_probs, state};
+    const dim3 grid((unsigned)rows, cut.segments);
+    const float inv_t = 1.f / temperature;
+    if (top_k > 0)
+      k_scores<T, true><<<grid, kRowThreads, 0, st>>>(p, x.map(), (int)vocab, tok, ignore_index, inv_t, top_k, out, rows,
+                                                      cut.len, parts, part_top);
+    else
+      k_scores<T, false><<<grid, kRowThreads, 0, st>>>(p, x.map(), (int)vocab, tok, ignore_index, inv_t, 0, out, rows,
+                                                       cut.len, parts, part_top);
+    if (cut.segments > 1)
+      k_scores_join<T><<<(unsigned)rows, kJoinThreads, (size_t)(cut.segments + 1) * top_k * 8, st>>>(
+          p, x.map(), (int)vocab, tok, ignore_index, inv_t, top_k, out, rows, cut.segments, parts, part_top);
   });
   return check_launch("mec_token_scores");
 }
