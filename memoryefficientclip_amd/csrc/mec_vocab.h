@@ -144,7 +144,8 @@ struct Segment {
   typename Vec<T>::raw v[kSegChunks];
   int n, first;  // elements; the thread's first one
   // n elements at p.  A vector that would pass the end is the last one that
-  // does not, with -inf for the elements that belong to the thread before.
+  // does not; with ONCE the elements in it that belong to another thread are -inf.
+  template <bool ONCE>
   __device__ __forceinline__ void load(const T* p, int count) {
     n = count;
     first = threadIdx.x * N;
@@ -160,6 +161,7 @@ struct Segment {
       else
         v[c] = skip_elements<T>(v[c], N);
     }
+    if constexpr (!ONCE) return;
 #pragma unroll
     for (int c = 0; c < kSegChunks; ++c)
       if (c * kChunk < n && (c + 1) * kChunk > n) v[c] = skip_elements<T>(v[c], c * kChunk + first - begin(c));
@@ -179,6 +181,16 @@ struct Segment {
         }
       }
     return r;
+  }
+  // chunk c's vector to a segment of the same shape
+  __device__ __forceinline__ void store(T* p, int c, const float (&x)[N]) const {
+    if (n >= N) {
+      *(typename Vec<T>::raw*)(p + begin(c)) = Vec<T>::pack(x);
+    } else if (first == 0) {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (e < n) put(p + e, x[e]);
+    }
   }
   // where chunk c's vector begins
   __device__ __forceinline__ int begin(int c) const {
@@ -382,93 +394,92 @@ __global__ __launch_bounds__(kRowThreads) void k_scores(const T* logits, RowMap 
   const float c = inv_t * (1.f / kLn2);
   const int segments = gridDim.y, seg = blockIdx.y, base = seg * len;
   const int64_t r = blockIdx.x, item = r * segments + seg;
-  {
-    const int64_t tok = tokens[r];
-    if (tok == ignore) {
-      if (segments == 1) write_ignored(out, r, rows, k, tid, kRowThreads);
-      return;
+  const int64_t tok = tokens[r];
+  if (tok == ignore) {
+    if (segments == 1) write_ignored(out, r, rows, k, tid, kRowThreads);
+    return;
+  }
+  const T* x = logits + map(r) + base;
+  Segment<T> v;
+  v.template load<true>(x, n - base < len ? n - base : len);
+  float m = -INFINITY;
+  v.each([&](float f) { m = fmaxf(m, f); });
+  if constexpr (TOP) {
+    top.thread_max[tid] = m;
+    if (tid == 0) top.count = 0;
+  }
+  for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
+  if (lane == 0) wave_max[w] = m;
+  __syncthreads();
+  m = wave_max[0];
+  for (int i = 1; i < kWaves; ++i) m = fmaxf(m, wave_max[i]);
+  const int kk = TOP ? (k < v.n ? k : v.n) : 0;
+  if constexpr (TOP) {
+    if (w == 0) top_cut(top, kk);
+  }
+  const Reference ref(m, c);
+  float s = 0.f, u = 0.f;
+  auto sums = [&](auto far) {
+    v.each([&](float f) {
+      const float t = decltype(far)::value ? ref.t(f) : fmaf(f, c, -ref.mc);
+      const float e = fast_exp2(t);
+      s += e;
+      // (2^t is 0 below -200, where t may be -inf)
+      u = fmaf(e, fmaxf(t, -200.f), u);
+    });
+  };
+  if (ref.far)
+    sums(std::true_type{});
+  else
+    sums(std::false_type{});
+  s = wave_sum(s);
+  u = wave_sum(u);
+  if (lane == 0) wave_s[w] = s, wave_u[w] = u;
+  __syncthreads();
+  s = u = 0.f;
+  for (int i = 0; i < kWaves; ++i) s += wave_s[i], u += wave_u[i];
+  if constexpr (TOP) top_collect(top, v, x, base, kk);
+  const RowResult row(ref, s, inv_t);
+  if (tid == 0) {
+    if (segments == 1) {
+      out.log_probs[r] = tok >= 0 && tok < n ? row.log_prob(value(x[tok])) : NAN;
+      out.entropy[r] = row.entropy(u);
+      out.stats[r] = ref.m;
+      out.stats[rows + r] = s;
+    } else {
+      parts[item] = make_float4(m, s, u, 0.f);
     }
-    const T* x = logits + map(r) + base;
-    Segment<T> v;
-    v.load(x, n - base < len ? n - base : len);
-    float m = -INFINITY;
-    v.each([&](float f) { m = fmaxf(m, f); });
-    if constexpr (TOP) {
-      top.thread_max[tid] = m;
-      if (tid == 0) top.count = 0;
-    }
-    for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
-    if (lane == 0) wave_max[w] = m;
-    __syncthreads();
-    m = wave_max[0];
-    for (int i = 1; i < kWaves; ++i) m = fmaxf(m, wave_max[i]);
-    const int kk = TOP ? (k < v.n ? k : v.n) : 0;
-    if constexpr (TOP) {
-      if (w == 0) top_cut(top, kk);
-    }
-    const Reference ref(m, c);
-    float s = 0.f, u = 0.f;
-    auto sums = [&](auto far) {
-      v.each([&](float f) {
-        const float t = decltype(far)::value ? ref.t(f) : fmaf(f, c, -ref.mc);
-        const float e = fast_exp2(t);
-        s += e;
-        // (2^t is 0 below -200, where t may be -inf)
-        u = fmaf(e, fmaxf(t, -200.f), u);
-      });
-    };
-    if (ref.far)
-      sums(std::true_type{});
-    else
-      sums(std::false_type{});
-    s = wave_sum(s);
-    u = wave_sum(u);
-    if (lane == 0) wave_s[w] = s, wave_u[w] = u;
-    __syncthreads();
-    s = u = 0.f;
-    for (int i = 0; i < kWaves; ++i) s += wave_s[i], u += wave_u[i];
-    if constexpr (TOP) top_collect(top, v, x, base, kk);
-    const RowResult row(ref, s, inv_t);
-    if (tid == 0) {
+  }
+  if constexpr (TOP) {
+    const int count = top.count;
+    for (int i = tid; i < count; i += kRowThreads) {
+      const uint64_t key = top.found[i];
+      int rank = 0;
+      for (int j = 0; j < count; ++j) rank += top.found[j] > key;
+      if (rank >= kk) continue;
       if (segments == 1) {
-        out.log_probs[r] = tok >= 0 && tok < n ? row.log_prob(value(x[tok])) : NAN;
-        out.entropy[r] = row.entropy(u);
-        out.stats[r] = ref.m;
-        out.stats[rows + r] = s;
+        out.top_tokens[r * k + rank] = key_index(key);
+        out.top_log_probs[r * k + rank] = row.log_prob(key_value(key));
       } else {
-        parts[item] = make_float4(m, s, u, 0.f);
+        part_top[item * k + rank] = key;
       }
     }
-    if constexpr (TOP) {
-      const int count = top.count;
-      for (int i = tid; i < count; i += kRowThreads) {
-        const uint64_t key = top.found[i];
-        int rank = 0;
-        for (int j = 0; j < count; ++j) rank += top.found[j] > key;
-        if (rank >= kk) continue;
-        if (segments == 1) {
-          out.top_tokens[r * k + rank] = key_index(key);
-          out.top_log_probs[r * k + rank] = row.log_prob(key_value(key));
-        } else {
-          part_top[item * k + rank] = key;
-        }
-      }
-      if (segments > 1)
-        for (int i = kk + tid; i < k; i += kRowThreads) part_top[item * k + i] = 0;
-    }
+    if (segments > 1)
+      for (int i = kk + tid; i < k; i += kRowThreads) part_top[item * k + i] = 0;
   }
 }
 
 constexpr int kJoinThreads = 64;
+constexpr int kJoinRank = 256;  // above it, a search for the k-th key is shorter than ranking all
 
 // One wave per row: its segments' sums, a lane each, and the k largest of their
-// top keys (all different, so that exactly k reach the k-th).
+// top keys (all different: exactly k reach the k-th).
 template <class T>
 __global__ __launch_bounds__(kJoinThreads) void k_scores_join(const T* logits, RowMap map, int n, Tokens tokens,
                                                               int64_t ignore, float inv_t, int k, ScoresOut out,
                                                               int64_t rows, int segments, const float4* parts,
                                                               const uint64_t* part_top) {
-  extern __shared__ uint64_t keys[];  // segments * k, then k
+  extern __shared__ uint64_t keys[];  // segments * k
   const int64_t r = blockIdx.x;
   const int lane = threadIdx.x;
   const int64_t tok = tokens[r];
@@ -497,51 +508,93 @@ __global__ __launch_bounds__(kJoinThreads) void k_scores_join(const T* logits, R
   }
   if (k == 0) return;
   __syncthreads();
-  const uint64_t cut = kth_largest<uint64_t>((count + 63) / 64, 0, k, k, [&](int i) {
-    return i * 64 + lane < count ? keys[i * 64 + lane] : 0;
-  });
-  uint64_t* best = keys + count;
-  int have = 0;
-  for (int i0 = 0; i0 < count; i0 += 64) {
-    const uint64_t key = i0 + lane < count ? keys[i0 + lane] : 0;
-    const uint64_t mask = __ballot(key >= cut);
-    if (key >= cut) best[have + __popcll(mask & ((1ull << lane) - 1))] = key;
-    have += __popcll(mask);
+  // The lists are in order: if q lists have their p-th key at or above a cut, p q
+  // keys are.  The cut is the q-th of the p-th keys, p q >= k.
+  const int p_th = (k + segments - 1) / segments, q_th = (k + p_th - 1) / p_th;
+  const uint64_t head = lane < segments ? keys[lane * k + p_th - 1] : 0;
+  int above = 0;
+  for (int i = 0; i < segments; ++i) {
+    const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(head >> 32), i) << 32 |
+                           (uint32_t)__builtin_amdgcn_readlane((int)head, i);
+    above += other > head || (other == head && i < lane);
   }
-  __syncthreads();
-  for (int i = lane; i < k; i += 64) {
-    const uint64_t key = best[i];
+  uint64_t cut = __shfl(head, __ffsll((unsigned long long)__ballot(above == q_th - 1)) - 1, 64);
+  // (0: lists shorter than k; keys are not 0)
+  if (cut == 0) cut = 1;
+  // of the first n keys those from `cut` on, moved to the front
+  auto keep = [&](int n_keys) {
+    int kept = 0;
+    for (int i0 = 0; i0 < n_keys; i0 += 64) {
+      const uint64_t key = i0 + lane < n_keys ? keys[i0 + lane] : 0;
+      const uint64_t mask = __ballot(key >= cut);
+      __syncthreads();
+      if (key >= cut) keys[kept + __popcll(mask & ((1ull << lane) - 1))] = key;
+      kept += __popcll(mask);
+    }
+    __syncthreads();
+    return kept;
+  };
+  int have = keep(count);
+  if (have > kJoinRank) {
+    cut = kth_largest<uint64_t>((have + 63) / 64, 0, k, k,
+                                [&](int i) { return i * 64 + lane < have ? keys[i * 64 + lane] : 0; });
+    have = keep(have);
+  }
+  for (int i = lane; i < have; i += 64) {
+    const uint64_t key = keys[i];
     int rank = 0;
-    for (int j = 0; j < k; ++j) rank += best[j] > key;
+    for (int j = 0; j < have; ++j) rank += keys[j] > key;
+    if (rank >= k) continue;
     out.top_tokens[r * k + rank] = key_index(key);
     out.top_log_probs[r * k + rank] = row.log_prob(key_value(key));
   }
 }
 
-// dx_v = (1/T) (g_l (1[v = tok] - p_v) - g_h p_v (log p_v + entropy))
+// dx_v = (1/T) (g_l (1[v = tok] - p_v) - g_h p_v (log p_v + entropy)).
+// blockIdx.x: the row; blockIdx.y: its segment.  A vector that would pass the end
+// is the last one that does not: two threads then store the same values.
 template <class T>
-__global__ __launch_bounds__(kRowThreads) void k_token_scores_grad(const T* logits, RowMap map, int n, Tokens tokens,
-                                                                   int64_t ignore, float inv_t, const float* stats,
-                                                                   const float* entropy, const float* g_log_probs,
-                                                                   const float* g_entropy, T* dx, int64_t rows) {
+__global__ __launch_bounds__(kRowThreads) void k_scores_grad(const T* logits, RowMap map, int n, Tokens tokens,
+                                                             int64_t ignore, float inv_t, const float* stats,
+                                                             const float* entropy, const float* g_log_probs,
+                                                             const float* g_entropy, T* dx, int64_t rows, int len) {
+  constexpr int N = Vec<T>::N;
   const int64_t r = blockIdx.x;
+  const int base = blockIdx.y * len, count = n - base < len ? n - base : len;
   const int64_t tok = tokens[r];
-  const T* x = logits + map(r);
-  T* y = dx + r * n;
-  const float m = stats[r], s = stats[rows + r], h = entropy[r];
+  T* y = dx + r * n + base;
+  const float s = stats[rows + r];
   const bool none = tok == ignore || s == 0.f, bad = tok < 0 || tok >= n;
-  const float gl = g_log_probs ? g_log_probs[r] : 0.f, gh = g_entropy ? g_entropy[r] : 0.f;
-  const Reference ref(m, inv_t * (1.f / kLn2));
-  const float ls = logf(s), inv_s = 1.f / s;
-  for (int v = threadIdx.x; v < n; v += kRowThreads) {
-    float d = 0.f;
-    if (!none) {
-      const float t = ref.t(value(x[v]));
-      const float p = fast_exp2(t) * inv_s;
-      d = inv_t * ((v == tok ? gl : 0.f) - p * (gl + gh * (kLn2 * fmaxf(t, -200.f) - ls + h)));
-      if (value(x[v]) != value(x[v]) || bad) d = NAN;
+  Segment<T> v;
+  if (!none) v.template load<false>(logits + map(r) + base, count);
+  const Reference ref(stats[r], inv_t * (1.f / kLn2));
+  const float ls = logf(s), gl = bad ? NAN : g_log_probs ? g_log_probs[r] : 0.f, gh = g_entropy ? g_entropy[r] : 0.f;
+  // e (a + b t) = -(1/T) p (g_l + g_h (log p + entropy))
+  const float f = none ? 0.f : -inv_t / s, a = f * (gl + gh * (entropy[r] - ls)), b = f * gh * kLn2;
+  const int at = (int)(bad ? 0 : tok) - base;
+  v.n = count;
+  v.first = threadIdx.x * N;
+#pragma unroll
+  for (int c = 0; c < kSegChunks; ++c) {
+    if (c * Segment<T>::kChunk >= count) break;
+    float x[N];
+    if (none) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[e] = 0.f;
+    } else {
+      v.values(c, x);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float t = ref.t(x[e]);
+        x[e] = fast_exp2(t) * fmaf(b, fmaxf(t, -200.f), a);
+      }
+      const int own = at - v.begin(c);
+      if (own >= 0 && own < N) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] += e == own ? gl * inv_t : 0.f;
+      }
     }
-    put(y + v, d);
+    v.store(y, c, x);
   }
 }
 

@@ -123,11 +123,12 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 struct Cut {
   int segments, len;
 };
+constexpr int64_t kManyRows = 1024;  // a workgroup each fills the device
 Cut cut_rows(int64_t rows, int64_t vocab, int dtype) {
   const int64_t chunk = kRowThreads * (dtype == MEC_DTYPE_F32 ? 4 : 8);  // a vector per thread
   int64_t s = ceil_div(vocab, chunk * kSegChunks);
   // few rows: more, shorter segments, so that there are workgroups for every CU
-  const int64_t want = ceil_div(1024, rows);
+  const int64_t want = ceil_div(kManyRows, rows);
   if (s < want) s = want;
   if (s > ceil_div(vocab, chunk)) s = ceil_div(vocab, chunk);
   if (s > kMaxSegments) s = kMaxSegments;
@@ -237,7 +238,7 @@ int mec_token_scores(const void* logits, int64_t rows, int64_t inner, int64_t ou
       k_scores<T, false><<<grid, kRowThreads, 0, st>>>(p, x.map(), (int)vocab, tok, ignore_index, inv_t, 0, out, rows,
                                                        cut.len, parts, part_top);
     if (cut.segments > 1)
-      k_scores_join<T><<<(unsigned)rows, kJoinThreads, (size_t)(cut.segments + 1) * top_k * 8, st>>>(
+      k_scores_join<T><<<(unsigned)rows, kJoinThreads, (size_t)cut.segments * top_k * 8, st>>>(
           p, x.map(), (int)vocab, tok, ignore_index, inv_t, top_k, out, rows, cut.segments, parts, part_top);
   });
   return check_launch("mec_token_scores");
@@ -259,9 +260,10 @@ int mec_token_scores_backward(const void* logits, int64_t rows, int64_t inner, i
   if (rc) return rc;
   with_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    k_token_scores_grad<T><<<(unsigned)rows, kRowThreads, 0, (hipStream_t)stream>>>(
+    const Cut cut = cut_rows(kManyRows, vocab, dtype);
+    k_scores_grad<T><<<dim3((unsigned)rows, cut.segments), kRowThreads, 0, (hipStream_t)stream>>>(
         (const T*)logits, x.map(), (int)vocab, Tokens{tokens, token_bytes == 8}, ignore_index, 1.f / temperature, state,
-        entropy, grad_log_probs, grad_entropy, (T*)grad_logits, rows);
+        entropy, grad_log_probs, grad_entropy, (T*)grad_logits, rows, cut.len);
   });
   return check_launch("mec_token_scores_backward");
 }
