@@ -57,41 +57,6 @@ __device__ __forceinline__ float scaled_difference(float x, float m, float inv_t
 
 constexpr int kRowThreads = 256;
 
-template <class V, class Op>
-__device__ __forceinline__ V block_reduce(V v, V* lds, Op op) {
-  for (int m = 32; m >= 1; m >>= 1) v = op(v, (V)__shfl_xor(v, m, 64));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = lds[0];
-  for (int w = 1; w < kRowThreads / 64; ++w) v = op(v, lds[w]);
-  return v;
-}
-
-struct RowSums {
-  float m, s, u;
-};
-
-// m, S and U of a row, in every thread.
-template <class T, bool U>
-__device__ __forceinline__ RowSums row_sums(const T* x, int n, float c, float* lds) {
-  float m = -INFINITY;
-  for (int v = threadIdx.x; v < n; v += kRowThreads) m = fmaxf(m, value(x[v]));
-  m = block_reduce(m, lds, [](float a, float b) { return fmaxf(a, b); });
-  const float ref = m == -INFINITY ? 0.f : m;
-  float s = 0.f, u = 0.f;
-  for (int v = threadIdx.x; v < n; v += kRowThreads) {
-    const float t = (value(x[v]) - ref) * c;
-    const float e = fast_exp2(t);
-    s += e;
-    // (2^t is 0 below -200, where t may be -inf)
-    if (U) u += e * fmaxf(t, -200.f);
-  }
-  s = block_reduce(s, lds, [](float a, float b) { return a + b; });
-  if (U) u = block_reduce(u, lds, [](float a, float b) { return a + b; });
-  return {ref, s, u};
-}
-
 // t = (x - m) c as one fma with m c rounded beforehand.  The rounding of m c, below
 // 2^-2, moves every t of the row alike and drops out of p and log p, which are formed
 // from t.  Where m c is larger, up to fp32's end, the difference is taken first.
@@ -138,9 +103,9 @@ __device__ __forceinline__ typename Vec<T>::raw skip_elements(typename Vec<T>::r
   return r;
 }
 
-template <class T>
+template <class T, int THREADS = kRowThreads>
 struct Segment {
-  static constexpr int N = Vec<T>::N, kChunk = kRowThreads * N;
+  static constexpr int N = Vec<T>::N, kChunk = THREADS * N;
   typename Vec<T>::raw v[kSegChunks];
   int n, first;  // elements; the thread's first one
   // n elements at p.  A vector that would pass the end is the last one that
@@ -190,6 +155,18 @@ struct Segment {
 #pragma unroll
       for (int e = 0; e < N; ++e)
         if (e < n) put(p + e, x[e]);
+    }
+  }
+  // the same after load<true>: elements of another thread are left to it
+  __device__ __forceinline__ void store_own(T* p, int c, const float (&x)[N]) const {
+    const int at = c * kChunk + first;
+    if (at + N <= n) {
+      *(typename Vec<T>::raw*)(p + at) = Vec<T>::pack(x);
+    } else if (at < n) {
+      const int i0 = begin(c);
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (i0 + e >= at && i0 + e < n) put(p + i0 + e, x[e]);
     }
   }
   // where chunk c's vector begins
@@ -607,8 +584,6 @@ __global__ __launch_bounds__(kRowThreads) void k_scores_grad(const T* logits, Ro
 // A row whose teacher has nothing above -inf has loss 0 and gradient 0; a token
 // past the vocabulary makes both NaN.
 
-constexpr int kMaxTeacher = 1024;  // entries per row
-
 struct Teacher {
   Tokens tokens;
   const void* logits;
@@ -619,133 +594,300 @@ struct Teacher {
            : dtype == 1 ? value(((const uint16_t*)logits)[i])
                         : value(((const _Float16*)logits)[i]);
   }
+  __device__ __forceinline__ bool entry(int64_t i) const { return tokens[i] >= 0 && logit(i) != -INFINITY; }
 };
 
-// One row's teacher in shared memory.
-struct TeacherRow {
-  float q[kMaxTeacher], log_q[kMaxTeacher];
-  int tok[kMaxTeacher];
-  int some, bad;
-};
+constexpr int kTeacherRows = 64, kTeacherThreads = 256;
 
-// By the first wave of the workgroup; the caller synchronizes.
-__device__ __forceinline__ void load_teacher(const Teacher& t, int64_t r, int n, float inv_t, TeacherRow& row) {
-  const int lane = threadIdx.x;
-  if (lane >= 64) return;
-  const float c = inv_t / kLn2;
-  float m = -INFINITY;
-  bool bad = false;
-  for (int j = lane; j < t.k; j += 64) {
-    const int64_t tok = t.tokens[r * t.k + j];
-    const float z = tok < 0 ? -INFINITY : t.logit(r * t.k + j);
-    bad |= tok >= n;
-    row.tok[j] = tok < 0 || tok >= n ? -1 : (int)tok;
-    row.log_q[j] = z;
-    m = fmaxf(m, z);
-  }
-  for (int i = 32; i >= 1; i >>= 1) m = fmaxf(m, __shfl_xor(m, i, 64));
-  if (m == -INFINITY) m = 0.f;
-  float s = 0.f;
-  for (int j = lane; j < t.k; j += 64) s += fast_exp2((row.log_q[j] - m) * c);
-  s = wave_sum(s);
-  const float ls = logf(s);
-  for (int j = lane; j < t.k; j += 64) {
-    const float z = row.log_q[j] - m;
-    row.q[j] = s == 0.f ? 0.f : fast_exp2(z * c) / s;
-    row.log_q[j] = z * inv_t - ls;
-  }
-  bad = __any(bad);
-  if (lane == 0) row.some = !(s == 0.f), row.bad = bad;
-}
-
-// Rows that have a teacher: one wave per row.
-__global__ __launch_bounds__(64) void k_teacher_count(Teacher t, int* count) {
-  const int64_t r = blockIdx.x;
-  bool some = false;
-  for (int j = threadIdx.x; j < t.k; j += 64)
-    some |= t.tokens[r * t.k + j] >= 0 && t.logit(r * t.k + j) != -INFINITY;
-  if (__any(some) && threadIdx.x == 0) atomicAdd(count, 1);
-}
-
-// dx of a row: g (p_v - q at the teacher's tokens).
-template <class T>
-__device__ __forceinline__ void distill_row_grad(const T* x, T* y, int n, float inv_t, float m, float s, float g,
-                                                 const TeacherRow& row, int k) {
-  const float c = inv_t / kLn2;
-  const bool zero = !row.some || s == 0.f;
-  const float gs = row.bad ? NAN : g / s;
-  for (int v = threadIdx.x; v < n; v += kRowThreads)
-    put(y + v, zero ? 0.f : fast_exp2((value(x[v]) - m) * c) * gs);
-  if (zero || row.bad) return;
+// some[r]: row r has a teacher; *count: how many rows do (0 before; not counted if null).
+__global__ __launch_bounds__(kTeacherThreads) void k_teacher_rows(Teacher t, int64_t rows, int* some, int* count) {
+  __shared__ int has[kTeacherRows];
+  const int tid = threadIdx.x;
+  const int64_t r0 = (int64_t)blockIdx.x * kTeacherRows;
+  const int n = rows - r0 < kTeacherRows ? (int)(rows - r0) : kTeacherRows;
+  if (tid < kTeacherRows) has[tid] = 0;
   __syncthreads();
-  // the teacher's tokens once more, each by one thread with all its entries
-  for (int j = threadIdx.x; j < k; j += kRowThreads) {
-    const int v = row.tok[j];
-    if (v < 0) continue;
-    float q = 0.f;
-    for (int i = 0; i < k; ++i) q += row.tok[i] == v ? row.q[i] : 0.f;
-    put(y + v, g * (fast_exp2((value(x[v]) - m) * c) / s - q));
-  }
-}
-
-// loss, and with dx its gradient for grad_output 1.  count: rows that have a
-// teacher (mean), null for 1.
-template <class T>
-__global__ __launch_bounds__(kRowThreads) void k_distill(const T* logits, RowMap map, int n, Teacher teacher,
-                                                         float inv_t, float scale, const int* count, float* row_loss,
-                                                         float* stats, T* dx, int64_t rows) {
-  __shared__ float lds[kRowThreads / 64];
-  __shared__ TeacherRow row;
-  const int64_t r = blockIdx.x;
-  load_teacher(teacher, r, n, inv_t, row);
+#pragma unroll 4
+  for (int i = tid; i < n * t.k; i += kTeacherThreads)
+    if (t.entry(r0 * t.k + i)) has[i / t.k] = 1;
   __syncthreads();
-  const T* x = logits + map(r);
-  RowSums a{0.f, 1.f, 0.f};
-  if (row.some) a = row_sums<T, false>(x, n, inv_t / kLn2, lds);
-  const float ls = logf(a.s);
-  float loss = 0.f;
-  for (int j = threadIdx.x; j < teacher.k; j += kRowThreads)
-    if (!(row.q[j] == 0.f) && row.tok[j] >= 0)
-      loss += row.q[j] * (row.log_q[j] - (a.s == 0.f ? -INFINITY : scaled_difference(value(x[row.tok[j]]), a.m, inv_t) - ls));
-  loss = block_reduce(loss, lds, [](float p, float q) { return p + q; });
-  if (threadIdx.x == 0) {
-    row_loss[r] = row.bad ? NAN : loss * (scale / (inv_t * inv_t));
-    stats[r] = a.m;
-    stats[rows + r] = a.s;
+  if (tid < 64) {
+    const bool mine = tid < n && has[tid];
+    if (tid < n) some[r0 + tid] = mine;
+    const int c = __popcll(__ballot(mine));
+    if (tid == 0 && count) atomicAdd(count, c);
   }
-  if (!dx) return;
-  const float rows_in = count ? fmaxf((float)*count, 1.f) : 1.f;
-  distill_row_grad(x, dx + r * n, n, inv_t, a.m, a.s, scale / (inv_t * rows_in), row, teacher.k);
-}
-
-// dx for a given grad_output (one number, or one for each row).  With
-// made = 1 the forward has left the gradient for grad_output 1 in dx.
-template <class T>
-__global__ __launch_bounds__(kRowThreads) void k_distill_grad(const T* logits, RowMap map, int n, Teacher teacher,
-                                                              float inv_t, float scale, const int* count,
-                                                              const float* stats, const float* grad_output,
-                                                              int per_row, int made, T* dx, int64_t rows) {
-  __shared__ TeacherRow row;
-  const int64_t r = blockIdx.x;
-  const float go = grad_output[per_row ? r : 0];
-  if (made && go == 1.f) return;
-  load_teacher(teacher, r, n, inv_t, row);
-  __syncthreads();
-  const float rows_in = count ? fmaxf((float)*count, 1.f) : 1.f;
-  distill_row_grad(logits + map(r), dx + r * n, n, inv_t, stats[r], stats[rows + r], go * scale / (inv_t * rows_in),
-                   row, teacher.k);
-}
-
-// loss = sum of the row losses (/ count), one workgroup, in a fixed order.
-__global__ __launch_bounds__(kRowThreads) void k_loss_sum(const float* row_loss, int64_t rows, const int* count,
-                                                          float* loss) {
-  __shared__ double lds[kRowThreads / 64];
-  double s = 0.;
-  for (int64_t r = threadIdx.x; r < rows; r += kRowThreads) s += row_loss[r];
-  s = block_reduce(s, lds, [](double a, double b) { return a + b; });
-  if (threadIdx.x == 0) *loss = (float)(count ? s / (*count > 0 ? *count : 1) : s);
 }
 
 __global__ void k_zero_word(int* p) { *p = 0; }
+
+// One row's teacher in shared memory: q, log q and the tokens (-1: none).
+struct TeacherRow {
+  float *q, *log_q;
+  int* tok;
+  int k;
+  __device__ __forceinline__ TeacherRow(float* lds, int entries)
+      : q(lds), log_q(lds + entries), tok((int*)lds + 2 * entries), k(entries) {}
+  // By one wave; true if a token lies past the vocabulary.
+  __device__ __forceinline__ bool load(const Teacher& t, int64_t r, int n, float inv_t) {
+    const int lane = threadIdx.x & 63;
+    const float c = inv_t * (1.f / kLn2);
+    float m = -INFINITY;
+    bool bad = false;
+    for (int j = lane; j < k; j += 64) {
+      const int64_t v = t.tokens[r * k + j];
+      const float z = v < 0 ? -INFINITY : t.logit(r * k + j);
+      bad |= v >= n;
+      tok[j] = v < 0 || v >= n ? -1 : (int)v;
+      log_q[j] = z;
+      m = fmaxf(m, z);
+    }
+    for (int i = 32; i >= 1; i >>= 1) m = fmaxf(m, __shfl_xor(m, i, 64));
+    const Reference ref(m, c);
+    float s = 0.f;
+    for (int j = lane; j < k; j += 64) s += fast_exp2(ref.t(log_q[j]));
+    s = wave_sum(s);
+    const float ls = logf(s);
+    for (int j = lane; j < k; j += 64) {
+      const float z = ref.t(log_q[j]);
+      q[j] = s == 0.f ? 0.f : fast_exp2(z) / s;
+      log_q[j] = kLn2 * z - ls;
+    }
+    return __any(bad);
+  }
+  // sum_j q_j (log q_j - log p_j) by the wave that loaded it; x: the row's logits
+  template <class T>
+  __device__ __forceinline__ float divergence(const T* x, const Reference& ref, float s, float inv_t) const {
+    const RowResult row(ref, s, inv_t);
+    float loss = 0.f;
+    for (int j = threadIdx.x & 63; j < k; j += 64)
+      if (!(q[j] == 0.f) && tok[j] >= 0) loss += q[j] * (log_q[j] - row.log_prob(value(x[tok[j]])));
+    return wave_sum(loss);
+  }
+  // After y = g p over [base, base + count) of a row: y at the teacher's tokens
+  // there, each by one thread from all its entries.
+  template <class T>
+  __device__ __forceinline__ void subtract(const T* x, T* y, int base, int count, const Reference& ref, float gs,
+                                           float g) const {
+    for (int j = threadIdx.x; j < k; j += blockDim.x) {
+      const int v = tok[j];
+      if (v < base || v >= base + count) continue;
+      float sum = 0.f;
+      for (int i = 0; i < k; ++i) sum += tok[i] == v ? q[i] : 0.f;
+      put(y + v, fast_exp2(ref.t(value(x[v]))) * gs - g * sum);
+    }
+  }
+};
+
+// What the backward has to know of a row: m and S; S < 0: the row has no
+// teacher, S = 0: nothing can occur (both: no gradient), NaN: no result.
+struct DistillState {
+  float* m;
+  float* s;
+};
+
+// A row of at most 8 vectors a thread, held by one workgroup from its only read
+// to the gradient's write.  dx: the gradient for grad_output 1.
+template <class T, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap map, int n, Teacher teacher,
+                                                         float inv_t, float scale, const int* some, const int* count,
+                                                         float* row_loss, DistillState state, T* dx) {
+  constexpr int N = Vec<T>::N, kWaves = THREADS / 64;
+  extern __shared__ float teacher_lds[];
+  __shared__ float wave_max[kWaves], wave_s[kWaves];
+  __shared__ int bad_row;
+  const int64_t r = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const T* x = logits + map(r);
+  T* y = dx + r * n;
+  Segment<T, THREADS> v;
+  if (!some[r]) {
+    if (tid == 0) row_loss[r] = 0.f, state.m[r] = 0.f, state.s[r] = -1.f;
+    v.n = n;
+    v.first = tid * N;
+    const float zero[N] = {};
+#pragma unroll
+    for (int c = 0; c < kSegChunks; ++c)
+      if (c * Segment<T, THREADS>::kChunk < n) v.store(y, c, zero);
+    return;
+  }
+  v.template load<true>(x, n);
+  TeacherRow row(teacher_lds, teacher.k);
+  if (w == 0) {
+    const bool bad = row.load(teacher, r, n, inv_t);
+    if (lane == 0) bad_row = bad;
+  }
+  float m = -INFINITY;
+  v.each([&](float f) { m = fmaxf(m, f); });
+  for (int i = 32; i >= 1; i >>= 1) m = fmaxf(m, __shfl_xor(m, i, 64));
+  if (lane == 0) wave_max[w] = m;
+  __syncthreads();
+  m = wave_max[0];
+#pragma unroll
+  for (int i = 1; i < kWaves; ++i) m = fmaxf(m, wave_max[i]);
+  const Reference ref(m, inv_t * (1.f / kLn2));
+  float s = 0.f;
+  v.each([&](float f) { s += fast_exp2(ref.t(f)); });
+  s = wave_sum(s);
+  if (lane == 0) wave_s[w] = s;
+  __syncthreads();
+  s = 0.f;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) s += wave_s[i];
+  const bool bad = bad_row;
+  const float rows_in = count ? fmaxf((float)*count, 1.f) : 1.f;
+  const float g = scale / (inv_t * rows_in), gs = bad ? NAN : s == 0.f ? 0.f : g / s;
+#pragma unroll
+  for (int c = 0; c < kSegChunks; ++c) {
+    if (c * Segment<T, THREADS>::kChunk >= n) break;
+    float f[N];
+    v.values(c, f);
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = fast_exp2(ref.t(f[e])) * gs;
+    v.store_own(y, c, f);
+  }
+  if (w == 0) {
+    const float loss = row.divergence(x, ref, s, inv_t);
+    if (lane == 0) {
+      row_loss[r] = bad ? NAN : loss * (scale / (inv_t * inv_t));
+      state.m[r] = ref.m;
+      state.s[r] = bad ? NAN : s;
+    }
+  }
+  if (bad || s == 0.f) return;
+  __syncthreads();
+  row.subtract(x, y, 0, n, ref, gs, g);
+}
+
+// m and S of a segment (blockIdx.x: the row, blockIdx.y: its segment).
+template <class T>
+__global__ __launch_bounds__(kRowThreads) void k_distill_sums(const T* logits, RowMap map, int n, float inv_t,
+                                                              const int* some, int len, float2* parts) {
+  constexpr int kWaves = kRowThreads / 64;
+  __shared__ float wave_max[kWaves], wave_s[kWaves];
+  const int64_t r = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, base = blockIdx.y * len;
+  if (!some[r]) return;
+  Segment<T> v;
+  v.template load<true>(logits + map(r) + base, n - base < len ? n - base : len);
+  float m = -INFINITY;
+  v.each([&](float f) { m = fmaxf(m, f); });
+  for (int i = 32; i >= 1; i >>= 1) m = fmaxf(m, __shfl_xor(m, i, 64));
+  if (lane == 0) wave_max[w] = m;
+  __syncthreads();
+  m = wave_max[0];
+#pragma unroll
+  for (int i = 1; i < kWaves; ++i) m = fmaxf(m, wave_max[i]);
+  const Reference ref(m, inv_t * (1.f / kLn2));
+  float s = 0.f;
+  v.each([&](float f) { s += fast_exp2(ref.t(f)); });
+  s = wave_sum(s);
+  if (lane == 0) wave_s[w] = s;
+  __syncthreads();
+  if (tid == 0) {
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) s += wave_s[i];
+    parts[r * gridDim.y + blockIdx.y] = make_float2(m, s);
+  }
+}
+
+// A row's m, S and loss from its segments' sums, a lane each: one wave per row.
+template <class T>
+__global__ __launch_bounds__(64) void k_distill_join(const T* logits, RowMap map, int n, Teacher teacher, float inv_t,
+                                                     float scale, const int* some, const float2* parts, int segments,
+                                                     float* row_loss, DistillState state) {
+  extern __shared__ float teacher_lds[];
+  const int64_t r = blockIdx.x;
+  const int lane = threadIdx.x;
+  if (!some[r]) {
+    if (lane == 0) row_loss[r] = 0.f, state.m[r] = 0.f, state.s[r] = -1.f;
+    return;
+  }
+  TeacherRow row(teacher_lds, teacher.k);
+  const float2 p = lane < segments ? parts[r * segments + lane] : make_float2(-INFINITY, 0.f);
+  const bool bad = row.load(teacher, r, n, inv_t);
+  float m = p.x;
+  for (int i = 32; i >= 1; i >>= 1) m = fmaxf(m, __shfl_xor(m, i, 64));
+  const float c = inv_t * (1.f / kLn2);
+  const Reference ref(m, c);
+  const float s = wave_sum(p.y == 0.f ? 0.f : p.y * fast_exp2(Reference(p.x, c).shift(ref)));
+  __syncthreads();
+  const float loss = row.divergence(logits + map(r), ref, s, inv_t);
+  if (lane == 0) {
+    row_loss[r] = bad ? NAN : loss * (scale / (inv_t * inv_t));
+    state.m[r] = ref.m;
+    state.s[r] = bad ? NAN : s;
+  }
+}
+
+// dx from the rows' m and S.  grad_output: one number, one for each row, or
+// null for 1.  With `made` dx holds the gradient for grad_output 1, and only
+// another one makes it anew (few workgroups then, each for many segments).
+template <class T>
+__global__ __launch_bounds__(kRowThreads) void k_distill_grad(const T* logits, RowMap map, int n, Teacher teacher,
+                                                              float inv_t, float scale, const int* count,
+                                                              DistillState state, const float* grad_output,
+                                                              int per_row, int made, T* dx, int64_t rows, int len,
+                                                              int segments) {
+  constexpr int N = Vec<T>::N;
+  extern __shared__ float teacher_lds[];
+  if (made && *grad_output == 1.f) return;
+  const int tid = threadIdx.x;
+  const float rows_in = count ? fmaxf((float)*count, 1.f) : 1.f;
+  const uint32_t items = (uint32_t)rows * segments;  // (< 2^29)
+  for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const uint32_t r = item / segments;
+    const int base = (int)(item - r * segments) * len, size = n - base < len ? n - base : len;
+    const T* x = logits + map(r);
+    T* y = dx + (int64_t)r * n;
+    const float s = state.s[r];
+    const bool none = s <= 0.f;
+    Segment<T> v;
+    v.n = size;
+    v.first = tid * N;
+    if (none) {
+      const float zero[N] = {};
+#pragma unroll
+      for (int c = 0; c < kSegChunks; ++c)
+        if (c * Segment<T>::kChunk < size) v.store(y + base, c, zero);
+      continue;
+    }
+    v.template load<false>(x + base, size);
+    TeacherRow row(teacher_lds, teacher.k);
+    if (tid < 64) row.load(teacher, r, n, inv_t);
+    const Reference ref(state.m[r], inv_t * (1.f / kLn2));
+    const float g = (grad_output ? grad_output[per_row ? r : 0] : 1.f) * scale / (inv_t * rows_in), gs = g / s;
+#pragma unroll
+    for (int c = 0; c < kSegChunks; ++c) {
+      if (c * Segment<T>::kChunk >= size) break;
+      float f[N];
+      v.values(c, f);
+#pragma unroll
+      for (int e = 0; e < N; ++e) f[e] = fast_exp2(ref.t(f[e])) * gs;
+      v.store(y + base, c, f);
+    }
+    __syncthreads();
+    if (s == s) row.subtract(x, y, base, size, ref, gs, g);
+    __syncthreads();
+  }
+}
+
+// loss = sum of the row losses (/ count), one workgroup, in a fixed order.
+constexpr int kSumThreads = 1024;
+__global__ __launch_bounds__(kSumThreads) void k_loss_sum(const float* row_loss, int64_t rows, const int* count,
+                                                          float* loss) {
+  __shared__ double lds[kSumThreads / 64];
+  double s = 0.;
+#pragma unroll 8
+  for (int64_t r = threadIdx.x; r < rows; r += kSumThreads) s += row_loss[r];
+  s = wave_sum_f64(s);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kSumThreads / 64; ++w) s += lds[w];
+    *loss = (float)(count ? s / (*count > 0 ? *count : 1) : s);
+  }
+}
 
 }  // namespace mec

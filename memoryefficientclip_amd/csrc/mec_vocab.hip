@@ -141,6 +141,41 @@ int64_t scores_workspace(int64_t rows, int64_t vocab, int top_k, int dtype) {
   return c.segments > 1 ? scores_parts_bytes(rows, c) + round16(rows * c.segments * top_k * 8) : 0;
 }
 
+// Threads of the workgroup that holds a row of logits in registers, 0 if none does.
+int row_threads(int64_t vocab, int dtype) {
+  const int64_t per_thread = (dtype == MEC_DTYPE_F32 ? 4 : 8) * kSegChunks;
+  for (int threads = 256; threads <= 1024; threads *= 2)
+    if (vocab <= per_thread * threads) return threads;
+  return 0;
+}
+
+// Workspace of mec_distill_forward, in bytes from its start.
+struct DistillWorkspace {
+  int64_t some, row_loss, parts, total;
+};
+DistillWorkspace distill_workspace(int64_t rows, int64_t vocab, int dtype, bool with_grad) {
+  DistillWorkspace w;
+  w.some = 0;
+  w.row_loss = round16(rows * 4);
+  w.parts = 2 * round16(rows * 4);
+  const bool whole = with_grad && row_threads(vocab, dtype) != 0;
+  w.total = w.parts + (whole ? 0 : round16(rows * cut_rows(rows, vocab, dtype).segments * 8));
+  return w;
+}
+
+template <class T>
+void distill_grad(const Logits& x, const Teacher& teacher, float inv_t, float weight, const int* count,
+                  const DistillState& state, const float* grad_output, int per_row, int made, void* dx,
+                  hipStream_t st) {
+  const Cut cut = cut_rows(kManyRows, x.vocab, x.dtype);
+  const int64_t items = x.rows * cut.segments;
+  // (made: to find grad_output 1 few workgroups are enough)
+  const int64_t most = made ? 2048 : int64_t(1) << 22;
+  k_distill_grad<T><<<(unsigned)(items < most ? items : most), kRowThreads, (size_t)teacher.k * 12, st>>>(
+      (const T*)x.p, x.map(), (int)x.vocab, teacher, inv_t, weight, count, state, grad_output, per_row, made, (T*)dx,
+      x.rows, cut.len, cut.segments);
+}
+
 // Workspace of mec_embedding_backward, in bytes from its start.
 struct EmbedWorkspace {
   int64_t even, odd, keys, positions, bounds, counts, pieces, blocks, total;
@@ -273,8 +308,7 @@ int64_t mec_distill_workspace_bytes(int64_t rows, int64_t vocab, int64_t k, int 
   int rc = check_sizes(rows, vocab, dtype);
   if (!rc && (k < 1 || k > MEC_MAX_TEACHER_K))
     rc = fail(MEC_ERR_INVALID, "k=%lld out of range [1, %d]", (long long)k, MEC_MAX_TEACHER_K);
-  (void)with_grad;
-  return rc ? rc : round16(rows * 4);
+  return rc ? rc : distill_workspace(rows, vocab, dtype, with_grad != 0).total;
 }
 
 int mec_distill_forward(const void* logits, int64_t rows, int64_t inner, int64_t outer_stride, int64_t inner_stride,
@@ -290,26 +324,44 @@ int mec_distill_forward(const void* logits, int64_t rows, int64_t inner, int64_t
   if (!rc && (!loss || !state)) rc = fail(MEC_ERR_INVALID, "loss and state must be non-null");
   if (!rc && grad_logits && reduction == MEC_REDUCE_NONE)
     rc = fail(MEC_ERR_INVALID, "grad_logits needs MEC_REDUCE_SUM or MEC_REDUCE_MEAN");
-  if (!rc)
-    rc = check_workspace(workspace, workspace_bytes,
-                         mec_distill_workspace_bytes(rows, vocab, k, dtype, grad_logits != nullptr));
+  const DistillWorkspace w = rc ? DistillWorkspace{} : distill_workspace(rows, vocab, dtype, grad_logits != nullptr);
+  if (!rc) rc = check_workspace(workspace, workspace_bytes, w.total);
   if (!rc) rc = check_not_capturing(stream);
   if (rc) return rc;
   hipStream_t st = (hipStream_t)stream;
   const Teacher teacher{{teacher_tokens, token_bytes == 8}, teacher_logits, teacher_dtype, (int)k};
   int* count = reduction == MEC_REDUCE_MEAN ? (int*)(state + 2 * rows) : nullptr;
-  if (count) {
-    k_zero_word<<<1, 1, 0, st>>>(count);
-    k_teacher_count<<<(unsigned)rows, 64, 0, st>>>(teacher, count);
-  }
-  float* row_loss = reduction == MEC_REDUCE_NONE ? loss : (float*)workspace;
+  char* ws = (char*)workspace;
+  int* some = (int*)(ws + w.some);
+  float2* parts = (float2*)(ws + w.parts);
+  if (count) k_zero_word<<<1, 1, 0, st>>>(count);
+  k_teacher_rows<<<(unsigned)ceil_div(rows, kTeacherRows), kTeacherThreads, 0, st>>>(teacher, rows, some, count);
+  float* row_loss = reduction == MEC_REDUCE_NONE ? loss : (float*)(ws + w.row_loss);
+  const DistillState ds{state, state + rows};
+  const float inv_t = 1.f / temperature;
+  const size_t lds = (size_t)k * 12;
   with_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    k_distill<T><<<(unsigned)rows, kRowThreads, 0, st>>>((const T*)logits, x.map(), (int)vocab, teacher,
-                                                         1.f / temperature, weight, count, row_loss, state,
-                                                         (T*)grad_logits, rows);
+    const T* p = (const T*)logits;
+    const int n = (int)vocab;
+    const int threads = grad_logits ? row_threads(vocab, dtype) : 0;
+    auto whole = [&](auto th) {
+      constexpr int THREADS = decltype(th)::value;
+      k_distill_row<T, THREADS><<<(unsigned)rows, THREADS, lds, st>>>(p, x.map(), n, teacher, inv_t, weight, some, count,
+                                                                      row_loss, ds, (T*)grad_logits);
+    };
+    if (threads == 256) return whole(std::integral_constant<int, 256>{});
+    if (threads == 512) return whole(std::integral_constant<int, 512>{});
+    if (threads == 1024) return whole(std::integral_constant<int, 1024>{});
+    const Cut cut = cut_rows(rows, vocab, dtype);
+    k_distill_sums<T><<<dim3((unsigned)rows, cut.segments), kRowThreads, 0, st>>>(p, x.map(), n, inv_t, some, cut.len,
+                                                                                   parts);
+    k_distill_join<T><<<(unsigned)rows, 64, lds, st>>>(p, x.map(), n, teacher, inv_t, weight, some, parts, cut.segments,
+                                                       row_loss, ds);
+    if (grad_logits)
+      distill_grad<T>(x, teacher, inv_t, weight, count, ds, nullptr, 0, 0, grad_logits, st);
   });
-  if (reduction != MEC_REDUCE_NONE) k_loss_sum<<<1, kRowThreads, 0, st>>>(row_loss, rows, count, loss);
+  if (reduction != MEC_REDUCE_NONE) k_loss_sum<<<1, kSumThreads, 0, st>>>(row_loss, rows, count, loss);
   return check_launch("mec_distill_forward");
 }
 
@@ -333,9 +385,9 @@ int mec_distill_backward(const void* logits, int64_t rows, int64_t inner, int64_
   const int* count = reduction == MEC_REDUCE_MEAN ? (const int*)(state + 2 * rows) : nullptr;
   with_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    k_distill_grad<T><<<(unsigned)rows, kRowThreads, 0, (hipStream_t)stream>>>(
-        (const T*)logits, x.map(), (int)vocab, teacher, 1.f / temperature, weight, count, state, grad_output,
-        reduction == MEC_REDUCE_NONE, made, (T*)grad_logits, rows);
+    distill_grad<T>(x, teacher, 1.f / temperature, weight, count,
+                    DistillState{const_cast<float*>(state), const_cast<float*>(state) + rows}, grad_output,
+                    reduction == MEC_REDUCE_NONE, made != 0, grad_logits, (hipStream_t)stream);
   });
   return check_launch("mec_distill_backward");
 }
