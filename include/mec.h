@@ -438,7 +438,7 @@ int64_t mec_token_scores_workspace_bytes(int64_t rows, int64_t vocab, int top_k,
  * entropy[r] = -sum p log p, and the top_k (0: none; <= vocab, <= MEC_MAX_TOP_K)
  * most probable tokens in order, top_tokens and top_log_probs [rows, top_k]:
  * ties go to the lower token, NaN logits come first.  state: 2 * rows floats for
- * mec_token_scores_backward.  A row whose token is ignore_index is not read: its
+ * mec_token_scores_backward, NULL without one.  A row whose token is ignore_index is not read: its
  * log probability and entropy are 0, its top tokens -1 with 0.  A token outside
  * [0, vocab) has log probability NaN. */
 int mec_token_scores(const void* logits, int64_t rows, int64_t inner, int64_t outer_stride, int64_t inner_stride,

@@ -3,8 +3,6 @@ layout of logits, scratch and the calls into the HIP library
 (``include/mec.h``)."""
 from __future__ import annotations
 
-import contextlib
-
 import torch
 
 from . import _function as _f
@@ -27,18 +25,19 @@ def check_gpu(name: str, t: torch.Tensor, device: torch.device | None = None) ->
         raise ValueError(f"{name} is on {t.device}, the other inputs on {device}")
 
 
-def check_float(name: str, t: torch.Tensor) -> int:
-    """The C-ABI dtype code of a floating tensor."""
+def check_float(name: str, t: torch.Tensor) -> None:
     if t.dtype not in _f._DTYPES:
         raise TypeError(f"unsupported dtype {t.dtype} of {name}; supported: float32, bfloat16, float16")
+
+
+def code_of(t: torch.Tensor) -> int:
+    """The C-ABI dtype code of a tensor that passed check_float."""
     return _f._DTYPES[t.dtype]
 
 
-def check_tokens(name: str, t: torch.Tensor) -> int:
-    """Bytes of a token."""
+def check_tokens(name: str, t: torch.Tensor) -> None:
     if t.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"unsupported dtype {t.dtype} of {name}; supported: int64, int32")
-    return 8 if t.dtype == torch.int64 else 4
 
 
 def check_temperature(temperature: float) -> float:
@@ -72,30 +71,23 @@ def rows_of(logits: torch.Tensor) -> tuple[torch.Tensor, int, tuple[int, int, in
     return logits, logits.data_ptr(), (n0 * n1, n1, s0, s1)
 
 
-@contextlib.contextmanager
-def on_device(index: int):
-    """The C-ABI calls launch on the current device."""
+def launch(index: int, nbytes: int, call) -> int:
+    """``call(workspace, stream)``, a C-ABI call, on device `index` with `nbytes` of
+    the caching allocator's memory in the order of the current stream (< 0: a
+    size query's error code).  Returns its status."""
+    if nbytes < 0:
+        raise _lib.error("size query", nbytes)
+    # (the C-ABI calls launch on the current device)
     cur = torch.cuda.current_device()
     if cur != index:
         torch.cuda.set_device(index)
+    ws = None
     try:
-        yield _f._stream(index)
+        if nbytes:
+            ws = _f._alloc(nbytes, index)
+        return call(ws, _f._stream(index))
     finally:
+        if ws is not None:
+            torch.cuda.caching_allocator_delete(ws)
         if cur != index:
             torch.cuda.set_device(cur)
-
-
-@contextlib.contextmanager
-def scratch(nbytes: int, index: int):
-    """`nbytes` of the caching allocator's memory in the order of the current
-    stream of the current device `index`; < 0 is a size query's error code."""
-    if nbytes < 0:
-        raise _lib.error("size query", nbytes)
-    if nbytes == 0:
-        yield None
-        return
-    p = _f._alloc(nbytes, index)
-    try:
-        yield p
-    finally:
-        torch.cuda.caching_allocator_delete(p)

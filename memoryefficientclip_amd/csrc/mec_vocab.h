@@ -181,12 +181,29 @@ struct Segment {
     asm volatile("" : "+v"(r));
     Vec<T>::unpack(r, x);
   }
-  // f(element, its index) over the thread's elements that pred holds for: few
-  template <class P, class F>
-  __device__ __forceinline__ void each_of(P pred, F f) const {
+  // The largest element of each of the thread's vectors (not NaN), and of all.
+  __device__ __forceinline__ float maxima(float (&most)[kSegChunks]) const {
+    float m = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < kSegChunks; ++c) {
+      most[c] = -INFINITY;
+      if (c * kChunk >= n) continue;
+      float x[N];
+      values(c, x);
+#pragma unroll
+      for (int e = 0; e < N; ++e) most[c] = fmaxf(most[c], x[e]);
+      m = fmaxf(m, most[c]);
+    }
+    return m;
+  }
+  // f(element, its index) over the thread's elements that pred holds for, few,
+  // all in vectors that look(vector) holds for
+  template <class L, class P, class F>
+  __device__ __forceinline__ void each_of(L look, P pred, F f) const {
 #pragma unroll
     for (int c = 0; c < kSegChunks; ++c) {
       if (c * kChunk >= n) break;
+      if (!look(c)) continue;
       float x[N];
       values(c, x);
       uint32_t hits = 0;
@@ -210,6 +227,7 @@ struct Segment {
 #pragma unroll
     for (int c = 0; c < kSegChunks; ++c) {
       if (c * kChunk >= n) break;
+      if (c * kChunk + first >= n) continue;
       float x[N];
       values(c, x);
 #pragma unroll
@@ -316,11 +334,13 @@ __device__ __attribute__((noinline)) void top_exactly(TopLds& l, const T* x, int
 }
 
 // The k largest of the segment (and perhaps others), keys with indexes from
-// `base`, at found[0 .. count) in no order; k <= the segment's elements.
+// `base`, at found[0 .. count) in no order; k <= the segment's elements.  Only
+// vectors whose maximum reaches the cut are looked into, all where there is a NaN.
 template <class T>
-__device__ __forceinline__ void top_collect(TopLds& l, const Segment<T>& v, const T* x, int base, int k) {
+__device__ __forceinline__ void top_collect(TopLds& l, const Segment<T>& v, const float (&most)[kSegChunks], bool nan,
+                                            const T* x, int base, int k) {
   const float cut = l.cut;
-  v.each_of([&](float f) { return !(f < cut); },
+  v.each_of([&](int c) { return nan || !(most[c] < cut); }, [&](float f) { return !(f < cut); },
             [&](float f, int i) {
               const int at = atomicAdd(&l.count, 1);
               if (at < kCandidates) l.found[at] = order_key(f, base + i);
@@ -334,7 +354,7 @@ struct ScoresOut {
   float* entropy;
   int64_t* top_tokens;
   float* top_log_probs;
-  float* stats;  // m, S
+  float* stats;  // m, S; or null
 };
 
 // One row's result from its sums.
@@ -353,7 +373,10 @@ struct RowResult {
 
 __device__ __forceinline__ void write_ignored(const ScoresOut& out, int64_t r, int64_t rows, int k, int tid,
                                               int threads) {
-  if (tid == 0) out.log_probs[r] = 0.f, out.entropy[r] = 0.f, out.stats[r] = 0.f, out.stats[rows + r] = 0.f;
+  if (tid == 0) {
+    out.log_probs[r] = 0.f, out.entropy[r] = 0.f;
+    if (out.stats) out.stats[r] = 0.f, out.stats[rows + r] = 0.f;
+  }
   for (int j = tid; j < k; j += threads) out.top_tokens[r * k + j] = -1, out.top_log_probs[r * k + j] = 0.f;
 }
 
@@ -379,8 +402,8 @@ __global__ __launch_bounds__(kRowThreads) void k_scores(const T* logits, RowMap 
   const T* x = logits + map(r) + base;
   Segment<T> v;
   v.template load<true>(x, n - base < len ? n - base : len);
-  float m = -INFINITY;
-  v.each([&](float f) { m = fmaxf(m, f); });
+  float most[kSegChunks];
+  float m = v.maxima(most);
   if constexpr (TOP) {
     top.thread_max[tid] = m;
     if (tid == 0) top.count = 0;
@@ -396,33 +419,33 @@ __global__ __launch_bounds__(kRowThreads) void k_scores(const T* logits, RowMap 
   }
   const Reference ref(m, c);
   float s = 0.f, u = 0.f;
-  auto sums = [&](auto far) {
+  auto sums = [&](auto plain) {
+    s = u = 0.f;
     v.each([&](float f) {
-      const float t = decltype(far)::value ? ref.t(f) : fmaf(f, c, -ref.mc);
+      const float t = decltype(plain)::value ? fmaf(f, c, -ref.mc) : ref.t(f);
       const float e = fast_exp2(t);
       s += e;
       // (2^t is 0 below -200, where t may be -inf)
-      u = fmaf(e, fmaxf(t, -200.f), u);
+      u = fmaf(e, decltype(plain)::value ? t : fmaxf(t, -200.f), u);
     });
+    s = wave_sum(s);
+    u = wave_sum(u);
   };
-  if (ref.far)
-    sums(std::true_type{});
-  else
-    sums(std::false_type{});
-  s = wave_sum(s);
-  u = wave_sum(u);
+  // Where no t is -inf the plain form is enough, one operation in eleven less; a
+  // wave that meets one has a U of NaN and takes the other.
+  if (!ref.far) sums(std::true_type{});
+  if (ref.far || u != u) sums(std::false_type{});
   if (lane == 0) wave_s[w] = s, wave_u[w] = u;
   __syncthreads();
   s = u = 0.f;
   for (int i = 0; i < kWaves; ++i) s += wave_s[i], u += wave_u[i];
-  if constexpr (TOP) top_collect(top, v, x, base, kk);
+  if constexpr (TOP) top_collect(top, v, most, s != s, x, base, kk);
   const RowResult row(ref, s, inv_t);
   if (tid == 0) {
     if (segments == 1) {
       out.log_probs[r] = tok >= 0 && tok < n ? row.log_prob(value(x[tok])) : NAN;
       out.entropy[r] = row.entropy(u);
-      out.stats[r] = ref.m;
-      out.stats[rows + r] = s;
+      if (out.stats) out.stats[r] = ref.m, out.stats[rows + r] = s;
     } else {
       parts[item] = make_float4(m, s, u, 0.f);
     }
@@ -446,81 +469,98 @@ __global__ __launch_bounds__(kRowThreads) void k_scores(const T* logits, RowMap 
   }
 }
 
-constexpr int kJoinThreads = 64;
+constexpr int kJoinThreads = 256;
 constexpr int kJoinRank = 256;  // above it, a search for the k-th key is shorter than ranking all
 
-// One wave per row: its segments' sums, a lane each, and the k largest of their
-// top keys (all different: exactly k reach the k-th).
+// One workgroup per row: its segments' sums, a lane of the first wave each, and
+// the k largest of their top keys (all different: exactly k reach the k-th).
 template <class T>
 __global__ __launch_bounds__(kJoinThreads) void k_scores_join(const T* logits, RowMap map, int n, Tokens tokens,
                                                               int64_t ignore, float inv_t, int k, ScoresOut out,
                                                               int64_t rows, int segments, const float4* parts,
                                                               const uint64_t* part_top) {
   extern __shared__ uint64_t keys[];  // segments * k
+  __shared__ uint64_t cut_at;
+  __shared__ int kept;
+  __shared__ float2 sums;
   const int64_t r = blockIdx.x;
-  const int lane = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63;
   const int64_t tok = tokens[r];
   if (tok == ignore) {
-    write_ignored(out, r, rows, k, lane, kJoinThreads);
+    write_ignored(out, r, rows, k, tid, kJoinThreads);
     return;
   }
-  const float at = tok >= 0 && tok < n ? value(logits[map(r) + tok]) : 0.f;
   const int count = segments * k;
-  for (int i = lane; i < count; i += 64) keys[i] = part_top[r * count + i];
+  part_top += r * count;
   const float c = inv_t * (1.f / kLn2);
-  const float4 p = lane < segments ? parts[r * segments + lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
-  float m = p.x;
-  for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
-  const Reference ref(m, c);
-  // (S = 0: nothing of the segment can occur, and its shift may be -inf)
-  const float shift = Reference(p.x, c).shift(ref), scale = fast_exp2(shift);
-  const float s = wave_sum(p.y == 0.f ? 0.f : p.y * scale);
-  const float u = wave_sum(p.y == 0.f ? 0.f : scale * fmaf(p.y, fmaxf(shift, -200.f), p.z));
-  const RowResult row(ref, s, inv_t);
-  if (lane == 0) {
-    out.log_probs[r] = tok >= 0 && tok < n ? row.log_prob(at) : NAN;
-    out.entropy[r] = row.entropy(u);
-    out.stats[r] = ref.m;
-    out.stats[rows + r] = s;
+  if (tid < 64) {
+    const float at = tok >= 0 && tok < n ? value(logits[map(r) + tok]) : 0.f;
+    const float4 p = lane < segments ? parts[r * segments + lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    // The lists are in order: if q lists have their p-th key at or above a cut,
+    // p q keys are.  The cut is the q-th of the p-th keys, p q >= k.
+    const int p_th = k ? (k + segments - 1) / segments : 1, q_th = k ? (k + p_th - 1) / p_th : 1;
+    const uint64_t head = k && lane < segments ? part_top[lane * k + p_th - 1] : 0;
+    float m = p.x;
+    for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
+    const Reference ref(m, c);
+    // (S = 0: nothing of the segment can occur, and its shift may be -inf)
+    const float shift = Reference(p.x, c).shift(ref), scale = fast_exp2(shift);
+    const float s = wave_sum(p.y == 0.f ? 0.f : p.y * scale);
+    const float u = wave_sum(p.y == 0.f ? 0.f : scale * fmaf(p.y, fmaxf(shift, -200.f), p.z));
+    const RowResult row(ref, s, inv_t);
+    if (lane == 0) {
+      out.log_probs[r] = tok >= 0 && tok < n ? row.log_prob(at) : NAN;
+      out.entropy[r] = row.entropy(u);
+      if (out.stats) {
+        out.stats[r] = ref.m;
+        out.stats[rows + r] = s;
+      }
+      sums = make_float2(ref.m, s);
+      kept = 0;
+    }
+    if (k) {
+      int above = 0;
+      for (int i = 0; i < segments; ++i) {
+        const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(head >> 32), i) << 32 |
+                               (uint32_t)__builtin_amdgcn_readlane((int)head, i);
+        above += other > head || (other == head && i < lane);
+      }
+      // (lists shorter than k end in 0; keys are not 0)
+      if (lane < segments && above == q_th - 1) cut_at = head ? head : 1;
+    }
   }
   if (k == 0) return;
   __syncthreads();
-  // The lists are in order: if q lists have their p-th key at or above a cut, p q
-  // keys are.  The cut is the q-th of the p-th keys, p q >= k.
-  const int p_th = (k + segments - 1) / segments, q_th = (k + p_th - 1) / p_th;
-  const uint64_t head = lane < segments ? keys[lane * k + p_th - 1] : 0;
-  int above = 0;
-  for (int i = 0; i < segments; ++i) {
-    const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(head >> 32), i) << 32 |
-                           (uint32_t)__builtin_amdgcn_readlane((int)head, i);
-    above += other > head || (other == head && i < lane);
+  uint64_t cut = cut_at;
+  uint64_t* found = keys;
+#pragma unroll 4
+  for (int i = tid; i < count; i += kJoinThreads) {
+    const uint64_t key = part_top[i];
+    if (key >= cut) found[atomicAdd(&kept, 1)] = key;
   }
-  uint64_t cut = __shfl(head, __ffsll((unsigned long long)__ballot(above == q_th - 1)) - 1, 64);
-  // (0: lists shorter than k; keys are not 0)
-  if (cut == 0) cut = 1;
-  // of the first n keys those from `cut` on, moved to the front
-  auto keep = [&](int n_keys) {
-    int kept = 0;
-    for (int i0 = 0; i0 < n_keys; i0 += 64) {
-      const uint64_t key = i0 + lane < n_keys ? keys[i0 + lane] : 0;
-      const uint64_t mask = __ballot(key >= cut);
-      __syncthreads();
-      if (key >= cut) keys[kept + __popcll(mask & ((1ull << lane) - 1))] = key;
-      kept += __popcll(mask);
-    }
-    __syncthreads();
-    return kept;
-  };
-  int have = keep(count);
+  __syncthreads();
+  int have = kept;
   if (have > kJoinRank) {
-    cut = kth_largest<uint64_t>((have + 63) / 64, 0, k, k,
-                                [&](int i) { return i * 64 + lane < have ? keys[i * 64 + lane] : 0; });
-    have = keep(have);
+    // the k-th key itself, and the keys from it on to the front, by the first wave
+    if (tid < 64) {
+      cut = kth_largest<uint64_t>((have + 63) / 64, 0, k, k,
+                                  [&](int i) { return i * 64 + lane < have ? found[i * 64 + lane] : 0; });
+      int at = 0;
+      for (int i0 = 0; i0 < have; i0 += 64) {
+        const uint64_t key = i0 + lane < have ? found[i0 + lane] : 0;
+        const uint64_t mask = __ballot(key >= cut);
+        if (key >= cut) found[at + __popcll(mask & ((1ull << lane) - 1))] = key;
+        at += __popcll(mask);
+      }
+    }
+    have = k;
+    __syncthreads();
   }
-  for (int i = lane; i < have; i += 64) {
-    const uint64_t key = keys[i];
+  const RowResult row(Reference(sums.x, c), sums.y, inv_t);
+  for (int i = tid; i < have; i += kJoinThreads) {
+    const uint64_t key = found[i];
     int rank = 0;
-    for (int j = 0; j < have; ++j) rank += keys[j] > key;
+    for (int j = 0; j < have; ++j) rank += found[j] > key;
     if (rank >= k) continue;
     out.top_tokens[r * k + rank] = key_index(key);
     out.top_log_probs[r * k + rank] = row.log_prob(key_value(key));

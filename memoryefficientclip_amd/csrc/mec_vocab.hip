@@ -250,8 +250,8 @@ int mec_token_scores(const void* logits, int64_t rows, int64_t inner, int64_t ou
   if (!rc) rc = check_tokens(tokens, token_bytes);
   if (!rc) rc = check_temperature(temperature);
   if (!rc) rc = check_top_k(vocab, top_k);
-  if (!rc && (!log_probs || !entropy || !state || (top_k > 0 && (!top_tokens || !top_log_probs))))
-    rc = fail(MEC_ERR_INVALID, "outputs and state must be non-null");
+  if (!rc && (!log_probs || !entropy || (top_k > 0 && (!top_tokens || !top_log_probs))))
+    rc = fail(MEC_ERR_INVALID, "outputs must be non-null");
   if (!rc) rc = check_workspace(workspace, workspace_bytes, scores_workspace(rows, vocab, top_k, dtype));
   if (!rc) rc = check_not_capturing(stream);
   if (rc) return rc;

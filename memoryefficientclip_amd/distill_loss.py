@@ -22,45 +22,44 @@ from . import _vocab as _v
 _REDUCTIONS = {"none": _lib.REDUCE_NONE, "sum": _lib.REDUCE_SUM, "mean": _lib.REDUCE_MEAN}
 
 
+def _loss(logits, teacher_tokens, teacher_logits, temperature, weight, reduction, need):
+    """The loss, and with `need` what the backward needs."""
+    code, teacher_code, token_bytes = _v.code_of(logits), _v.code_of(teacher_logits), teacher_tokens.element_size()
+    held, px, rows = _v.rows_of(logits)
+    teacher_tokens, teacher_logits = teacher_tokens.contiguous(), teacher_logits.contiguous()
+    vocab, k, dev = logits.shape[-1], teacher_tokens.shape[-1], logits.device
+    loss = torch.empty(logits.shape[:-1] if reduction == _lib.REDUCE_NONE else (), dtype=torch.float32, device=dev)
+    state = torch.empty(2 * rows[0] + 1, dtype=torch.float32, device=dev)
+    # The gradient for grad_output 1 is made while the row is at hand: the
+    # logits are read once for loss and gradient.  fp16 programs scale their
+    # losses, so there grad_output is not 1 and the backward makes it.
+    dx = None
+    if need and reduction != _lib.REDUCE_NONE and logits.dtype != torch.float16:
+        dx = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    lib = _lib.load()
+    nbytes = lib.mec_distill_workspace_bytes(rows[0], vocab, k, code, int(dx is not None))
+    rc = _v.launch(dev.index, nbytes, lambda ws, stream: lib.mec_distill_forward(
+        px, *rows, vocab, code, teacher_tokens.data_ptr(), token_bytes, teacher_logits.data_ptr(), teacher_code, k,
+        temperature, weight, reduction, loss.data_ptr(), state.data_ptr(), None if dx is None else dx.data_ptr(), ws,
+        nbytes, stream))
+    if rc:
+        raise _lib.error("mec_distill_forward", rc)
+    kept = (held, teacher_tokens, teacher_logits, state,
+            (rows, vocab, code, token_bytes, teacher_code, k, temperature, weight, reduction, logits.shape), dx)
+    return loss, kept
+
+
 class _DistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher_tokens, teacher_logits, temperature, weight, reduction):
-        code, teacher_code = _v.check_float("student_logits", logits), _v.check_float("teacher_logits", teacher_logits)
-        token_bytes = _v.check_tokens("teacher_tokens", teacher_tokens)
-        held, px, rows = _v.rows_of(logits)
-        teacher_tokens, teacher_logits = teacher_tokens.contiguous(), teacher_logits.contiguous()
-        vocab, k, dev = logits.shape[-1], teacher_tokens.shape[-1], logits.device
-        di = dev.index
-        loss = torch.empty(logits.shape[:-1] if reduction == _lib.REDUCE_NONE else (), dtype=torch.float32, device=dev)
-        state = torch.empty(2 * rows[0] + 1, dtype=torch.float32, device=dev)
-        need = ctx.needs_input_grad[0]
-        # The gradient for grad_output 1 is made while the row is at hand: the
-        # logits are read once for loss and gradient.  fp16 programs scale their
-        # losses, so there grad_output is not 1 and the backward makes it.
-        dx = None
-        if need and reduction != _lib.REDUCE_NONE and logits.dtype != torch.float16:
-            dx = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-        lib = _lib.load()
-        with _v.on_device(di) as stream:
-            nbytes = lib.mec_distill_workspace_bytes(rows[0], vocab, k, code, int(dx is not None))
-            with _v.scratch(nbytes, di) as ws:
-                rc = lib.mec_distill_forward(px, *rows, vocab, code, teacher_tokens.data_ptr(), token_bytes,
-                                             teacher_logits.data_ptr(), teacher_code, k, temperature, weight,
-                                             reduction, loss.data_ptr(), state.data_ptr(),
-                                             None if dx is None else dx.data_ptr(), ws, nbytes, stream)
-        if rc:
-            raise _lib.error("mec_distill_forward", rc)
-        if need:
-            ctx.save_for_backward(held, teacher_tokens, teacher_logits, state)
-            ctx.made = dx
-            ctx.mec = (rows, vocab, code, token_bytes, teacher_code, k, temperature, weight, reduction, logits.shape)
+        loss, kept = _loss(logits, teacher_tokens, teacher_logits, temperature, weight, reduction, True)
+        ctx.save_for_backward(*kept[:4])
+        ctx.mec, ctx.made = kept[4:]
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_output):
-        if not ctx.needs_input_grad[0]:
-            return (None,) * 6
         _v.refuse_graph_capture()
         held, teacher_tokens, teacher_logits, state = ctx.saved_tensors
         rows, vocab, code, token_bytes, teacher_code, k, temperature, weight, reduction, shape = ctx.mec
@@ -70,10 +69,13 @@ class _DistillFn(torch.autograd.Function):
         made = dx is not None
         if not made:
             dx = torch.empty(shape, dtype=held.dtype, device=held.device)
-        with _v.on_device(held.device.index) as stream:
-            _lib.call("mec_distill_backward", held.data_ptr(), *rows, vocab, code, teacher_tokens.data_ptr(),
-                      token_bytes, teacher_logits.data_ptr(), teacher_code, k, temperature, weight, reduction,
-                      state.data_ptr(), go.data_ptr(), int(made), dx.data_ptr(), stream)
+        lib = _lib.load()
+        rc = _v.launch(held.device.index, 0, lambda ws, stream: lib.mec_distill_backward(
+            held.data_ptr(), *rows, vocab, code, teacher_tokens.data_ptr(), token_bytes, teacher_logits.data_ptr(),
+            teacher_code, k, temperature, weight, reduction, state.data_ptr(), go.data_ptr(), int(made), dx.data_ptr(),
+            stream))
+        if rc:
+            raise _lib.error("mec_distill_backward", rc)
         return dx, None, None, None, None, None
 
 
@@ -128,8 +130,10 @@ class TopKDistillationLoss(nn.Module):
             # no position: the graph's link to the logits
             return student_logits.sum(-1, dtype=torch.float32) if reduction == _lib.REDUCE_NONE else \
                 student_logits.sum(dtype=torch.float32)
-        return _DistillFn.apply(student_logits, teacher_tokens, teacher_logits.detach(), self.temperature, self.weight,
-                                reduction)
+        args = (student_logits, teacher_tokens, teacher_logits.detach(), self.temperature, self.weight, reduction)
+        if student_logits.requires_grad and torch.is_grad_enabled():
+            return _DistillFn.apply(*args)
+        return _loss(*args, False)[0]
 
 
 __all__ = ["TopKDistillationLoss"]

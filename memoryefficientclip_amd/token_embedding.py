@@ -19,40 +19,40 @@ from . import _vocab as _v
 _MAX_TOKENS, _MAX_VOCAB, _MAX_DIM = 1 << 23, 1 << 22, 1 << 16
 
 
+def _lookup(tokens, weight, scale):
+    w, ldw = _f._rows(weight)
+    vocab, d = w.shape
+    out = torch.empty((*tokens.shape, d), dtype=w.dtype, device=w.device)
+    lib = _lib.load()
+    rc = _v.launch(w.device.index, 0, lambda ws, stream: lib.mec_embedding(
+        tokens.data_ptr(), tokens.element_size(), tokens.numel(), w.data_ptr(), ldw, vocab, d, _v.code_of(w), scale,
+        out.data_ptr(), stream))
+    if rc:
+        raise _lib.error("mec_embedding", rc)
+    return out
+
+
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, weight, scale, padding_idx):
-        code, token_bytes = _v.check_float("weight", weight), _v.check_tokens("tokens", tokens)
-        tokens = tokens.contiguous()
-        w, ldw = _f._rows(weight)
-        vocab, d = w.shape
-        out = torch.empty((*tokens.shape, d), dtype=w.dtype, device=w.device)
-        with _v.on_device(w.device.index) as stream:
-            _lib.call("mec_embedding", tokens.data_ptr(), token_bytes, tokens.numel(), w.data_ptr(), ldw, vocab, d, code,
-                      scale, out.data_ptr(), stream)
-        if ctx.needs_input_grad[1]:
-            ctx.save_for_backward(tokens)
-            ctx.mec = (vocab, d, code, token_bytes, scale, padding_idx)
-        return out
+        ctx.save_for_backward(tokens)
+        ctx.mec = (weight.shape, scale, padding_idx)
+        return _lookup(tokens, weight, scale)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_output):
-        if not ctx.needs_input_grad[1]:
-            return None, None, None, None
         _v.refuse_graph_capture()
         tokens, = ctx.saved_tensors
-        vocab, d, code, token_bytes, scale, padding_idx = ctx.mec
+        (vocab, d), scale, padding_idx = ctx.mec
         dy, ldg = _f._rows(grad_output.reshape(-1, d))
-        dev = dy.device
-        dw = torch.empty((vocab, d), dtype=dy.dtype, device=dev)
+        dw = torch.empty((vocab, d), dtype=dy.dtype, device=dy.device)
+        n, code = tokens.numel(), _v.code_of(dy)
         lib = _lib.load()
-        with _v.on_device(dev.index) as stream:
-            n = tokens.numel()
-            nbytes = lib.mec_embedding_workspace_bytes(n, vocab, d, code)
-            with _v.scratch(nbytes, dev.index) as ws:
-                rc = lib.mec_embedding_backward(tokens.data_ptr(), token_bytes, n, dy.data_ptr(), ldg, vocab, d, code,
-                                                scale, padding_idx, dw.data_ptr(), ws, nbytes, stream)
+        nbytes = lib.mec_embedding_workspace_bytes(n, vocab, d, code)
+        rc = _v.launch(dy.device.index, nbytes, lambda ws, stream: lib.mec_embedding_backward(
+            tokens.data_ptr(), tokens.element_size(), n, dy.data_ptr(), ldg, vocab, d, code, scale, padding_idx,
+            dw.data_ptr(), ws, nbytes, stream))
         if rc:
             raise _lib.error("mec_embedding_backward", rc)
         return None, dw, None, None
@@ -90,7 +90,10 @@ def scaled_embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 
         padding_idx += vocab
     if tokens.numel() == 0:
         return weight[:0].sum() * scale + torch.empty((*tokens.shape, d), dtype=weight.dtype, device=weight.device)
-    return _EmbeddingFn.apply(tokens, weight, scale, int(padding_idx))
+    tokens = tokens.contiguous()
+    if weight.requires_grad and torch.is_grad_enabled():
+        return _EmbeddingFn.apply(tokens, weight, scale, int(padding_idx))
+    return _lookup(tokens, weight, scale)
 
 
 class ScaledTokenEmbedding(nn.Module):

@@ -28,35 +28,42 @@ class TokenScores(NamedTuple):
     top_log_probs: torch.Tensor | None
 
 
+def _scores(logits, tokens, top_k, temperature, ignore_index, keep):
+    """Results, and with `keep` what the backward needs of them."""
+    code, token_bytes = _v.code_of(logits), tokens.element_size()
+    held, px, rows = _v.rows_of(logits)
+    tokens = tokens.contiguous()
+    vocab, dev, shape = logits.shape[-1], logits.device, tokens.shape
+    log_probs = torch.empty(shape, dtype=torch.float32, device=dev)
+    entropy = torch.empty(shape, dtype=torch.float32, device=dev)
+    top_tokens = top_log_probs = state = None
+    if top_k:
+        top_tokens = torch.empty((*shape, top_k), dtype=torch.int64, device=dev)
+        top_log_probs = torch.empty((*shape, top_k), dtype=torch.float32, device=dev)
+    if keep:
+        state = torch.empty(2 * rows[0], dtype=torch.float32, device=dev)
+    lib = _lib.load()
+    nbytes = lib.mec_token_scores_workspace_bytes(rows[0], vocab, top_k, code)
+    rc = _v.launch(dev.index, nbytes, lambda ws, stream: lib.mec_token_scores(
+        px, *rows, vocab, code, tokens.data_ptr(), token_bytes, ignore_index, temperature, top_k,
+        log_probs.data_ptr(), entropy.data_ptr(), top_tokens.data_ptr() if top_k else None,
+        top_log_probs.data_ptr() if top_k else None, state.data_ptr() if keep else None, ws, nbytes, stream))
+    if rc:
+        raise _lib.error("mec_token_scores", rc)
+    kept = (held, tokens, entropy, state, (rows, vocab, code, token_bytes, ignore_index, temperature, logits.shape))
+    return (log_probs, entropy, top_tokens, top_log_probs), kept
+
+
 class _TokenScoresFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top_k, temperature, ignore_index):
-        code, token_bytes = _v.check_float("logits", logits), _v.check_tokens("tokens", tokens)
-        held, px, rows = _v.rows_of(logits)
-        tokens = tokens.contiguous()
-        vocab, dev = logits.shape[-1], logits.device
-        di = dev.index
-        log_probs = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
-        entropy = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
-        top_tokens = torch.empty((*tokens.shape, top_k), dtype=torch.int64, device=dev)
-        top_log_probs = torch.empty((*tokens.shape, top_k), dtype=torch.float32, device=dev)
-        state = torch.empty(2 * rows[0], dtype=torch.float32, device=dev)
-        lib = _lib.load()
-        with _v.on_device(di) as stream:
-            nbytes = lib.mec_token_scores_workspace_bytes(rows[0], vocab, top_k, code)
-            with _v.scratch(nbytes, di) as ws:
-                rc = lib.mec_token_scores(px, *rows, vocab, code, tokens.data_ptr(), token_bytes, ignore_index,
-                                          temperature, top_k, log_probs.data_ptr(), entropy.data_ptr(),
-                                          top_tokens.data_ptr(), top_log_probs.data_ptr(), state.data_ptr(), ws,
-                                          nbytes, stream)
-        if rc:
-            raise _lib.error("mec_token_scores", rc)
-        ctx.mark_non_differentiable(top_tokens, top_log_probs)
+        out, kept = _scores(logits, tokens, top_k, temperature, ignore_index, True)
+        if top_k:
+            ctx.mark_non_differentiable(out[2], out[3])
         ctx.set_materialize_grads(False)
-        if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(held, tokens, entropy, state)
-            ctx.mec = (rows, vocab, code, token_bytes, ignore_index, temperature, logits.shape)
-        return log_probs, entropy, top_tokens, top_log_probs
+        ctx.save_for_backward(*kept[:4])
+        ctx.mec = kept[4]
+        return out
 
     @staticmethod
     @once_differentiable
@@ -69,11 +76,13 @@ class _TokenScoresFn(torch.autograd.Function):
         gl = None if g_log_probs is None else g_log_probs.to(torch.float32).contiguous()
         gh = None if g_entropy is None else g_entropy.to(torch.float32).contiguous()
         dx = torch.empty(shape, dtype=held.dtype, device=held.device)
-        with _v.on_device(held.device.index) as stream:
-            _lib.call("mec_token_scores_backward", held.data_ptr(), *rows, vocab, code, tokens.data_ptr(), token_bytes,
-                      ignore_index, temperature, state.data_ptr(), entropy.data_ptr(),
-                      None if gl is None else gl.data_ptr(), None if gh is None else gh.data_ptr(), dx.data_ptr(),
-                      stream)
+        lib = _lib.load()
+        rc = _v.launch(held.device.index, 0, lambda ws, stream: lib.mec_token_scores_backward(
+            held.data_ptr(), *rows, vocab, code, tokens.data_ptr(), token_bytes, ignore_index, temperature,
+            state.data_ptr(), entropy.data_ptr(), None if gl is None else gl.data_ptr(),
+            None if gh is None else gh.data_ptr(), dx.data_ptr(), stream))
+        if rc:
+            raise _lib.error("mec_token_scores_backward", rc)
         return dx, None, None, None, None
 
 
@@ -98,10 +107,10 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, 
     _v.check_gpu("logits", logits)
     _v.check_gpu("tokens", tokens, logits.device)
     _v.refuse_graph_capture()
-    _v.check_float("logits", logits)
-    _v.check_tokens("tokens", tokens)
     if logits.dim() < 1 or logits.shape[:-1] != tokens.shape:
         raise ValueError(f"logits {tuple(logits.shape)} need one row for each of the tokens {tuple(tokens.shape)}")
+    _v.check_float("logits", logits)
+    _v.check_tokens("tokens", tokens)
     vocab, top_k = logits.shape[-1], int(top_k)
     if not 1 <= vocab <= _lib.MAX_VOCAB:
         raise ValueError(f"the vocabulary must have 1 to {_lib.MAX_VOCAB} tokens, got {vocab}")
@@ -113,8 +122,9 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, 
         return TokenScores(zero, zero.clone(),
                            torch.empty((*tokens.shape, top_k), dtype=torch.int64, device=logits.device) if top_k else None,
                            zero.detach()[..., None].expand(*tokens.shape, top_k) if top_k else None)
-    lp, h, tt, tlp = _TokenScoresFn.apply(logits, tokens, top_k, temperature, int(ignore_index))
-    return TokenScores(lp, h, tt if top_k else None, tlp if top_k else None)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return TokenScores(*_TokenScoresFn.apply(logits, tokens, top_k, temperature, int(ignore_index)))
+    return TokenScores(*_scores(logits, tokens, top_k, temperature, int(ignore_index), False)[0])
 
 
 __all__ = ["TokenScores", "token_log_probs"]

@@ -176,7 +176,7 @@ LOGITS_BAD = [(0, None, -1), (1, 0, -1), (1, 1 << 24, -2), (2, 0, -1), (3, -1, -
 
 @pytest.mark.parametrize("name,good,more", [
     ("mec_token_scores", SCORES, [(10, 0.0, -1), (10, math.nan, -1), (11, -1, -1), (11, 101, -1), (12, None, -1),
-                                  (13, None, -1), (14, None, -1), (15, None, -1), (16, None, -1)]),
+                                  (13, None, -1), (14, None, -1), (15, None, -1)]),
     ("mec_token_scores_backward", SCORES_BACK, [(10, 0.0, -1), (11, None, -1), (12, None, -1), (15, None, -1)]),
     ("mec_distill_forward", DISTILL, [(9, None, -1), (10, 4, -1), (11, 0, -1), (11, 1025, -2), (12, -1.0, -1),
                                       (13, math.inf, -1), (14, 3, -1), (15, None, -1), (16, None, -1), (18, None, -1),
