@@ -57,6 +57,31 @@ __device__ __forceinline__ float scaled_difference(float x, float m, float inv_t
 
 constexpr int kRowThreads = 256;
 
+// The wave's sum (largest), the same in every lane and in the same order on
+// every run: six lane moves of the vector unit instead of trips to LDS.
+template <class Op>
+__device__ __forceinline__ float wave_all(float v, float none, Op op) {
+  auto step = [&](auto ctrl, auto rows) {
+    const int moved = __builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(v), decltype(ctrl)::value,
+                                                  decltype(rows)::value, 0xf, false);
+    v = op(v, __int_as_float(moved));
+  };
+  using std::integral_constant;
+  step(integral_constant<int, 0xb1>{}, integral_constant<int, 0xf>{});   // lane ^ 1
+  step(integral_constant<int, 0x4e>{}, integral_constant<int, 0xf>{});   // lane ^ 2
+  step(integral_constant<int, 0x141>{}, integral_constant<int, 0xf>{});  // mirrored in 8 lanes
+  step(integral_constant<int, 0x140>{}, integral_constant<int, 0xf>{});  // mirrored in 16
+  step(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // lane 15 of a row of 16 to the next
+  step(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});  // lane 31 to the upper half
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+__device__ __forceinline__ float wave_total(float v) {
+  return wave_all(v, 0.f, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ float wave_most(float v) {
+  return wave_all(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
+}
+
 // t = (x - m) c as one fma with m c rounded beforehand.  The rounding of m c, below
 // 2^-2, moves every t of the row alike and drops out of p and log p, which are formed
 // from t.  Where m c is larger, up to fp32's end, the difference is taken first.
@@ -85,6 +110,20 @@ struct Reference {
 // k_scores_join.
 
 constexpr int kSegChunks = 8;
+
+// Workgroups of a launch over all segments of all rows: neighbours are the
+// segments of one row, then the next row's.  A row of workgroups of the grid
+// holds `rows_x` rows (below 2^32 work-items).
+struct SegmentGrid {
+  int segments, len;
+  uint32_t rows_x;
+  __device__ __forceinline__ bool place(int64_t rows, int64_t& r, int& seg) const {
+    const uint32_t q = blockIdx.x / (uint32_t)segments;
+    seg = (int)(blockIdx.x - q * segments);
+    r = (int64_t)blockIdx.y * rows_x + q;
+    return r < rows;
+  }
+};
 constexpr int kMaxSegments = 64;  // a lane each in the join
 
 // A vector's words with -inf in the first `skip` elements.
@@ -176,13 +215,12 @@ struct Segment {
   }
   // Unpacked anew by every pass: what one pass unpacks is not kept for the next
   // (twice the registers, and spills).
-  __device__ __forceinline__ void values(int c, float (&x)[N]) const {
-    typename Vec<T>::raw r = v[c];
-    asm volatile("" : "+v"(r));
-    Vec<T>::unpack(r, x);
+  __device__ __forceinline__ void values(int c, float (&x)[N]) {
+    asm volatile("" : "+v"(v[c]));
+    Vec<T>::unpack(v[c], x);
   }
   // The largest element of each of the thread's vectors (not NaN), and of all.
-  __device__ __forceinline__ float maxima(float (&most)[kSegChunks]) const {
+  __device__ __forceinline__ float maxima(float (&most)[kSegChunks]) {
     float m = -INFINITY;
 #pragma unroll
     for (int c = 0; c < kSegChunks; ++c) {
@@ -199,7 +237,7 @@ struct Segment {
   // f(element, its index) over the thread's elements that pred holds for, few,
   // all in vectors that look(vector) holds for
   template <class L, class P, class F>
-  __device__ __forceinline__ void each_of(L look, P pred, F f) const {
+  __device__ __forceinline__ void each_of(L look, P pred, F f) {
 #pragma unroll
     for (int c = 0; c < kSegChunks; ++c) {
       if (c * kChunk >= n) break;
@@ -223,7 +261,7 @@ struct Segment {
   }
   // f(element) over the thread's elements (and -inf in place of others')
   template <class F>
-  __device__ __forceinline__ void each(F f) const {
+  __device__ __forceinline__ void each(F f) {
 #pragma unroll
     for (int c = 0; c < kSegChunks; ++c) {
       if (c * kChunk >= n) break;
@@ -337,7 +375,7 @@ __device__ __attribute__((noinline)) void top_exactly(TopLds& l, const T* x, int
 // `base`, at found[0 .. count) in no order; k <= the segment's elements.  Only
 // vectors whose maximum reaches the cut are looked into, all where there is a NaN.
 template <class T>
-__device__ __forceinline__ void top_collect(TopLds& l, const Segment<T>& v, const float (&most)[kSegChunks], bool nan,
+__device__ __forceinline__ void top_collect(TopLds& l, Segment<T>& v, const float (&most)[kSegChunks], bool nan,
                                             const T* x, int base, int k) {
   const float cut = l.cut;
   v.each_of([&](int c) { return nan || !(most[c] < cut); }, [&](float f) { return !(f < cut); },
@@ -380,20 +418,25 @@ __device__ __forceinline__ void write_ignored(const ScoresOut& out, int64_t r, i
   for (int j = tid; j < k; j += threads) out.top_tokens[r * k + j] = -1, out.top_log_probs[r * k + j] = 0.f;
 }
 
-// blockIdx.x: the row; blockIdx.y: its segment, of `len` elements.
+// One workgroup per segment of a row.
 // With one segment the row's results, else part[row][seg] = (m, S, U) and the
 // segment's top k keys.
 template <class T, bool TOP>
 __global__ __launch_bounds__(kRowThreads) void k_scores(const T* logits, RowMap map, int n, Tokens tokens,
                                                         int64_t ignore, float inv_t, int k, ScoresOut out,
-                                                        int64_t rows, int len, float4* parts, uint64_t* part_top) {
+                                                        int64_t rows, SegmentGrid grid, float4* parts,
+                                                        uint64_t* part_top) {
   constexpr int kWaves = kRowThreads / 64;
   __shared__ float wave_max[kWaves], wave_s[kWaves], wave_u[kWaves];
   __shared__ std::conditional_t<TOP, TopLds, char> top;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const float c = inv_t * (1.f / kLn2);
-  const int segments = gridDim.y, seg = blockIdx.y, base = seg * len;
-  const int64_t r = blockIdx.x, item = r * segments + seg;
+  const int segments = grid.segments, len = grid.len;
+  int64_t r;
+  int seg;
+  if (!grid.place(rows, r, seg)) return;
+  const int base = seg * len;
+  const int64_t item = r * segments + seg;
   const int64_t tok = tokens[r];
   if (tok == ignore) {
     if (segments == 1) write_ignored(out, r, rows, k, tid, kRowThreads);
@@ -408,7 +451,7 @@ __global__ __launch_bounds__(kRowThreads) void k_scores(const T* logits, RowMap 
     top.thread_max[tid] = m;
     if (tid == 0) top.count = 0;
   }
-  for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
+  m = wave_most(m);
   if (lane == 0) wave_max[w] = m;
   __syncthreads();
   m = wave_max[0];
@@ -428,8 +471,8 @@ __global__ __launch_bounds__(kRowThreads) void k_scores(const T* logits, RowMap 
       // (2^t is 0 below -200, where t may be -inf)
       u = fmaf(e, decltype(plain)::value ? t : fmaxf(t, -200.f), u);
     });
-    s = wave_sum(s);
-    u = wave_sum(u);
+    s = wave_total(s);
+    u = wave_total(u);
   };
   // Where no t is -inf the plain form is enough, one operation in eleven less; a
   // wave that meets one has a U of NaN and takes the other.
@@ -440,9 +483,9 @@ __global__ __launch_bounds__(kRowThreads) void k_scores(const T* logits, RowMap 
   s = u = 0.f;
   for (int i = 0; i < kWaves; ++i) s += wave_s[i], u += wave_u[i];
   if constexpr (TOP) top_collect(top, v, most, s != s, x, base, kk);
-  const RowResult row(ref, s, inv_t);
   if (tid == 0) {
     if (segments == 1) {
+      const RowResult row(ref, s, inv_t);
       out.log_probs[r] = tok >= 0 && tok < n ? row.log_prob(value(x[tok])) : NAN;
       out.entropy[r] = row.entropy(u);
       if (out.stats) out.stats[r] = ref.m, out.stats[rows + r] = s;
@@ -459,7 +502,7 @@ __global__ __launch_bounds__(kRowThreads) void k_scores(const T* logits, RowMap 
       if (rank >= kk) continue;
       if (segments == 1) {
         out.top_tokens[r * k + rank] = key_index(key);
-        out.top_log_probs[r * k + rank] = row.log_prob(key_value(key));
+        out.top_log_probs[r * k + rank] = RowResult(ref, s, inv_t).log_prob(key_value(key));
       } else {
         part_top[item * k + rank] = key;
       }
@@ -501,12 +544,12 @@ __global__ __launch_bounds__(kJoinThreads) void k_scores_join(const T* logits, R
     const int p_th = k ? (k + segments - 1) / segments : 1, q_th = k ? (k + p_th - 1) / p_th : 1;
     const uint64_t head = k && lane < segments ? part_top[lane * k + p_th - 1] : 0;
     float m = p.x;
-    for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
+    m = wave_most(m);
     const Reference ref(m, c);
     // (S = 0: nothing of the segment can occur, and its shift may be -inf)
     const float shift = Reference(p.x, c).shift(ref), scale = fast_exp2(shift);
-    const float s = wave_sum(p.y == 0.f ? 0.f : p.y * scale);
-    const float u = wave_sum(p.y == 0.f ? 0.f : scale * fmaf(p.y, fmaxf(shift, -200.f), p.z));
+    const float s = wave_total(p.y == 0.f ? 0.f : p.y * scale);
+    const float u = wave_total(p.y == 0.f ? 0.f : scale * fmaf(p.y, fmaxf(shift, -200.f), p.z));
     const RowResult row(ref, s, inv_t);
     if (lane == 0) {
       out.log_probs[r] = tok >= 0 && tok < n ? row.log_prob(at) : NAN;
@@ -568,16 +611,20 @@ __global__ __launch_bounds__(kJoinThreads) void k_scores_join(const T* logits, R
 }
 
 // dx_v = (1/T) (g_l (1[v = tok] - p_v) - g_h p_v (log p_v + entropy)).
-// blockIdx.x: the row; blockIdx.y: its segment.  A vector that would pass the end
+// One workgroup per segment of a row.  A vector that would pass the end
 // is the last one that does not: two threads then store the same values.
 template <class T>
 __global__ __launch_bounds__(kRowThreads) void k_scores_grad(const T* logits, RowMap map, int n, Tokens tokens,
                                                              int64_t ignore, float inv_t, const float* stats,
                                                              const float* entropy, const float* g_log_probs,
-                                                             const float* g_entropy, T* dx, int64_t rows, int len) {
+                                                             const float* g_entropy, T* dx, int64_t rows,
+                                                             SegmentGrid grid) {
   constexpr int N = Vec<T>::N;
-  const int64_t r = blockIdx.x;
-  const int base = blockIdx.y * len, count = n - base < len ? n - base : len;
+  const int len = grid.len;
+  int64_t r;
+  int seg;
+  if (!grid.place(rows, r, seg)) return;
+  const int base = seg * len, count = n - base < len ? n - base : len;
   const int64_t tok = tokens[r];
   T* y = dx + r * n + base;
   const float s = stats[rows + r];
@@ -682,11 +729,11 @@ struct TeacherRow {
       log_q[j] = z;
       m = fmaxf(m, z);
     }
-    for (int i = 32; i >= 1; i >>= 1) m = fmaxf(m, __shfl_xor(m, i, 64));
+    m = wave_most(m);
     const Reference ref(m, c);
     float s = 0.f;
     for (int j = lane; j < k; j += 64) s += fast_exp2(ref.t(log_q[j]));
-    s = wave_sum(s);
+    s = wave_total(s);
     const float ls = logf(s);
     for (int j = lane; j < k; j += 64) {
       const float z = ref.t(log_q[j]);
@@ -702,7 +749,7 @@ struct TeacherRow {
     float loss = 0.f;
     for (int j = threadIdx.x & 63; j < k; j += 64)
       if (!(q[j] == 0.f) && tok[j] >= 0) loss += q[j] * (log_q[j] - row.log_prob(value(x[tok[j]])));
-    return wave_sum(loss);
+    return wave_total(loss);
   }
   // After y = g p over [base, base + count) of a row: y at the teacher's tokens
   // there, each by one thread from all its entries.
@@ -759,7 +806,7 @@ __global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap
   }
   float m = -INFINITY;
   v.each([&](float f) { m = fmaxf(m, f); });
-  for (int i = 32; i >= 1; i >>= 1) m = fmaxf(m, __shfl_xor(m, i, 64));
+  m = wave_most(m);
   if (lane == 0) wave_max[w] = m;
   __syncthreads();
   m = wave_max[0];
@@ -768,7 +815,7 @@ __global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap
   const Reference ref(m, inv_t * (1.f / kLn2));
   float s = 0.f;
   v.each([&](float f) { s += fast_exp2(ref.t(f)); });
-  s = wave_sum(s);
+  s = wave_total(s);
   if (lane == 0) wave_s[w] = s;
   __syncthreads();
   s = 0.f;
@@ -799,20 +846,23 @@ __global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap
   row.subtract(x, y, 0, n, ref, gs, g);
 }
 
-// m and S of a segment (blockIdx.x: the row, blockIdx.y: its segment).
+// m and S of a segment.
 template <class T>
 __global__ __launch_bounds__(kRowThreads) void k_distill_sums(const T* logits, RowMap map, int n, float inv_t,
-                                                              const int* some, int len, float2* parts) {
+                                                              const int* some, int64_t rows, SegmentGrid grid,
+                                                              float2* parts) {
   constexpr int kWaves = kRowThreads / 64;
   __shared__ float wave_max[kWaves], wave_s[kWaves];
-  const int64_t r = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, base = blockIdx.y * len;
+  int64_t r;
+  int seg;
+  if (!grid.place(rows, r, seg)) return;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, len = grid.len, base = seg * len;
   if (!some[r]) return;
   Segment<T> v;
   v.template load<true>(logits + map(r) + base, n - base < len ? n - base : len);
   float m = -INFINITY;
   v.each([&](float f) { m = fmaxf(m, f); });
-  for (int i = 32; i >= 1; i >>= 1) m = fmaxf(m, __shfl_xor(m, i, 64));
+  m = wave_most(m);
   if (lane == 0) wave_max[w] = m;
   __syncthreads();
   m = wave_max[0];
@@ -821,14 +871,14 @@ __global__ __launch_bounds__(kRowThreads) void k_distill_sums(const T* logits, R
   const Reference ref(m, inv_t * (1.f / kLn2));
   float s = 0.f;
   v.each([&](float f) { s += fast_exp2(ref.t(f)); });
-  s = wave_sum(s);
+  s = wave_total(s);
   if (lane == 0) wave_s[w] = s;
   __syncthreads();
   if (tid == 0) {
     s = 0.f;
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) s += wave_s[i];
-    parts[r * gridDim.y + blockIdx.y] = make_float2(m, s);
+    parts[r * grid.segments + seg] = make_float2(m, s);
   }
 }
 
@@ -848,10 +898,10 @@ __global__ __launch_bounds__(64) void k_distill_join(const T* logits, RowMap map
   const float2 p = lane < segments ? parts[r * segments + lane] : make_float2(-INFINITY, 0.f);
   const bool bad = row.load(teacher, r, n, inv_t);
   float m = p.x;
-  for (int i = 32; i >= 1; i >>= 1) m = fmaxf(m, __shfl_xor(m, i, 64));
+  m = wave_most(m);
   const float c = inv_t * (1.f / kLn2);
   const Reference ref(m, c);
-  const float s = wave_sum(p.y == 0.f ? 0.f : p.y * fast_exp2(Reference(p.x, c).shift(ref)));
+  const float s = wave_total(p.y == 0.f ? 0.f : p.y * fast_exp2(Reference(p.x, c).shift(ref)));
   __syncthreads();
   const float loss = row.divergence(logits + map(r), ref, s, inv_t);
   if (lane == 0) {

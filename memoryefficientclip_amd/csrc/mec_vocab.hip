@@ -122,6 +122,14 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // How token scores cut a row.
 struct Cut {
   int segments, len;
+  uint32_t rows_x(int64_t rows) const {
+    const int64_t most = (int64_t(1) << 23) / segments;
+    return (uint32_t)(rows < most ? rows : most);
+  }
+  SegmentGrid grid(int64_t rows) const { return SegmentGrid{segments, len, rows_x(rows)}; }
+  dim3 dims(int64_t rows) const {
+    return dim3(rows_x(rows) * segments, (unsigned)((rows + rows_x(rows) - 1) / rows_x(rows)));
+  }
 };
 constexpr int64_t kManyRows = 1024;  // a workgroup each fills the device
 Cut cut_rows(int64_t rows, int64_t vocab, int dtype) {
@@ -264,14 +272,14 @@ int mec_token_scores(const void* logits, int64_t rows, int64_t inner, int64_t ou
     float4* parts = (float4*)workspace;
     uint64_t* part_top = (uint64_t*)((char*)workspace + scores_parts_bytes(rows, cut));
     const ScoresOut out{log_probs, entropy, top_tokens, top_log_probs, state};
-    const dim3 grid((unsigned)rows, cut.segments);
+    const dim3 grid = cut.dims(rows);
     const float inv_t = 1.f / temperature;
     if (top_k > 0)
       k_scores<T, true><<<grid, kRowThreads, 0, st>>>(p, x.map(), (int)vocab, tok, ignore_index, inv_t, top_k, out, rows,
-                                                      cut.len, parts, part_top);
+                                                      cut.grid(rows), parts, part_top);
     else
       k_scores<T, false><<<grid, kRowThreads, 0, st>>>(p, x.map(), (int)vocab, tok, ignore_index, inv_t, 0, out, rows,
-                                                       cut.len, parts, part_top);
+                                                       cut.grid(rows), parts, part_top);
     if (cut.segments > 1)
       k_scores_join<T><<<(unsigned)rows, kJoinThreads, (size_t)cut.segments * top_k * 8, st>>>(
           p, x.map(), (int)vocab, tok, ignore_index, inv_t, top_k, out, rows, cut.segments, parts, part_top);
@@ -296,9 +304,9 @@ int mec_token_scores_backward(const void* logits, int64_t rows, int64_t inner, i
   with_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     const Cut cut = cut_rows(kManyRows, vocab, dtype);
-    k_scores_grad<T><<<dim3((unsigned)rows, cut.segments), kRowThreads, 0, (hipStream_t)stream>>>(
+    k_scores_grad<T><<<cut.dims(rows), kRowThreads, 0, (hipStream_t)stream>>>(
         (const T*)logits, x.map(), (int)vocab, Tokens{tokens, token_bytes == 8}, ignore_index, 1.f / temperature, state,
-        entropy, grad_log_probs, grad_entropy, (T*)grad_logits, rows, cut.len);
+        entropy, grad_log_probs, grad_entropy, (T*)grad_logits, rows, cut.grid(rows));
   });
   return check_launch("mec_token_scores_backward");
 }
@@ -354,8 +362,7 @@ int mec_distill_forward(const void* logits, int64_t rows, int64_t inner, int64_t
     if (threads == 512) return whole(std::integral_constant<int, 512>{});
     if (threads == 1024) return whole(std::integral_constant<int, 1024>{});
     const Cut cut = cut_rows(rows, vocab, dtype);
-    k_distill_sums<T><<<dim3((unsigned)rows, cut.segments), kRowThreads, 0, st>>>(p, x.map(), n, inv_t, some, cut.len,
-                                                                                   parts);
+    k_distill_sums<T><<<cut.dims(rows), kRowThreads, 0, st>>>(p, x.map(), n, inv_t, some, rows, cut.grid(rows), parts);
     k_distill_join<T><<<(unsigned)rows, 64, lds, st>>>(p, x.map(), n, teacher, inv_t, weight, some, parts, cut.segments,
                                                        row_loss, ds);
     if (grad_logits)
