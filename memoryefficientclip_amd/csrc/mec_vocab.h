@@ -151,6 +151,9 @@ struct Segment {
   // does not; with ONCE the elements in it that belong to another thread are -inf.
   template <bool ONCE>
   __device__ __forceinline__ void load(const T* p, int count) {
+    // (opaque: in a loop over segments the compiler else makes a copy of the code for
+    // each number of vectors)
+    asm volatile("" : "+s"(count));
     n = count;
     first = threadIdx.x * N;
     if (n < N) {
@@ -681,32 +684,49 @@ struct Teacher {
            : dtype == 1 ? value(((const uint16_t*)logits)[i])
                         : value(((const _Float16*)logits)[i]);
   }
-  __device__ __forceinline__ bool entry(int64_t i) const { return tokens[i] >= 0 && logit(i) != -INFINITY; }
 };
 
-constexpr int kTeacherRows = 64, kTeacherThreads = 256;
-
-// some[r]: row r has a teacher; *count: how many rows do (0 before; not counted if null).
-__global__ __launch_bounds__(kTeacherThreads) void k_teacher_rows(Teacher t, int64_t rows, int* some, int* count) {
-  __shared__ int has[kTeacherRows];
-  const int tid = threadIdx.x;
-  const int64_t r0 = (int64_t)blockIdx.x * kTeacherRows;
-  const int n = rows - r0 < kTeacherRows ? (int)(rows - r0) : kTeacherRows;
-  if (tid < kTeacherRows) has[tid] = 0;
-  __syncthreads();
-#pragma unroll 4
-  for (int i = tid; i < n * t.k; i += kTeacherThreads)
-    if (t.entry(r0 * t.k + i)) has[i / t.k] = 1;
-  __syncthreads();
-  if (tid < 64) {
-    const bool mine = tid < n && has[tid];
-    if (tid < n) some[r0 + tid] = mine;
-    const int c = __popcll(__ballot(mine));
-    if (tid == 0 && count) atomicAdd(count, c);
+// Which rows have a teacher, and how many of each workgroup's.
+struct TeacherRows {
+  int* some;    // [rows]
+  int* counts;  // [groups]
+  int groups, rows_each;
+  // by one wave, in every lane
+  __device__ __forceinline__ int total() const {
+    int c = 0;
+    for (int i = threadIdx.x & 63; i < groups; i += 64) c += counts[i];
+    for (int i = 32; i >= 1; i >>= 1) c += __shfl_xor(c, i, 64);
+    return c;
   }
-}
+};
+constexpr int kTeacherThreads = 256, kTeacherRows = 16, kTeacherGroups = 1024;
 
-__global__ void k_zero_word(int* p) { *p = 0; }
+__global__ __launch_bounds__(kTeacherThreads) void k_teacher_rows(Teacher t, int64_t rows, TeacherRows out) {
+  __shared__ int has[kTeacherRows];
+  __shared__ int count;
+  const int tid = threadIdx.x;
+  if (tid == 0) count = 0;
+  const int64_t first = (int64_t)blockIdx.x * out.rows_each, end = first + out.rows_each < rows ? first + out.rows_each : rows;
+  for (int64_t r0 = first; r0 < end; r0 += kTeacherRows) {
+    const int n = end - r0 < kTeacherRows ? (int)(end - r0) : kTeacherRows;
+    if (tid < kTeacherRows) has[tid] = 0;
+    __syncthreads();
+    const int entries = n * t.k;
+#pragma unroll 4
+    for (int i = tid; i < entries; i += kTeacherThreads) {
+      const int64_t tok = t.tokens[r0 * t.k + i];
+      const float z = t.logit(r0 * t.k + i);
+      if (tok >= 0 && z != -INFINITY) has[(uint32_t)i / (uint32_t)t.k] = 1;
+    }
+    __syncthreads();
+    if (tid < n) {
+      out.some[r0 + tid] = has[tid];
+      if (has[tid]) atomicAdd(&count, 1);
+    }
+  }
+  __syncthreads();
+  if (tid == 0) out.counts[blockIdx.x] = count;
+}
 
 // One row's teacher in shared memory: q, log q and the tokens (-1: none).
 struct TeacherRow {
@@ -773,65 +793,98 @@ struct DistillState {
   float* s;
 };
 
-// A row of at most 8 vectors a thread, held by one workgroup from its only read
-// to the gradient's write.  dx: the gradient for grad_output 1.
-template <class T, int THREADS>
+// Loss and gradient (for grad_output 1) of a row by one workgroup.  With ONE the
+// row is one segment and stays in registers from its only read to the
+// gradient's write.  Longer rows are read a second time, from the last-level
+// cache that the device's rows at hand fit into; the last segment is still in
+// registers then, and comes first.
+template <class T, int THREADS, bool ONE>
 __global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap map, int n, Teacher teacher,
-                                                         float inv_t, float scale, const int* some, const int* count,
-                                                         float* row_loss, DistillState state, T* dx) {
+                                                         float inv_t, float scale, TeacherRows have, int mean,
+                                                         float* row_loss, DistillState state, T* dx, int segments,
+                                                         int len) {
   constexpr int N = Vec<T>::N, kWaves = THREADS / 64;
   extern __shared__ float teacher_lds[];
-  __shared__ float wave_max[kWaves], wave_s[kWaves];
-  __shared__ int bad_row;
+  __shared__ float2 wave_sums[kWaves];
+  __shared__ int bad_row, count;
   const int64_t r = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const T* x = logits + map(r);
   T* y = dx + r * n;
   Segment<T, THREADS> v;
-  if (!some[r]) {
+  auto each_segment = [&](auto f) {  // f(segment, its first element, its size)
+    if constexpr (ONE)
+      f(0, 0, n);
+    else
+      for (int i = 0; i < segments; ++i) f(i, i * len, n - i * len < len ? n - i * len : len);
+  };
+  if (!have.some[r]) {
     if (tid == 0) row_loss[r] = 0.f, state.m[r] = 0.f, state.s[r] = -1.f;
-    v.n = n;
-    v.first = tid * N;
-    const float zero[N] = {};
+    each_segment([&](int, int base, int size) {
+      v.n = size;
+      v.first = tid * N;
+      const float zero[N] = {};
 #pragma unroll
-    for (int c = 0; c < kSegChunks; ++c)
-      if (c * Segment<T, THREADS>::kChunk < n) v.store(y, c, zero);
+      for (int c = 0; c < kSegChunks; ++c)
+        if (c * Segment<T, THREADS>::kChunk < size) v.store(y + base, c, zero);
+    });
     return;
   }
-  v.template load<true>(x, n);
   TeacherRow row(teacher_lds, teacher.k);
-  if (w == 0) {
-    const bool bad = row.load(teacher, r, n, inv_t);
-    if (lane == 0) bad_row = bad;
-  }
-  float m = -INFINITY;
-  v.each([&](float f) { m = fmaxf(m, f); });
-  m = wave_most(m);
-  if (lane == 0) wave_max[w] = m;
-  __syncthreads();
-  m = wave_max[0];
-#pragma unroll
-  for (int i = 1; i < kWaves; ++i) m = fmaxf(m, wave_max[i]);
-  const Reference ref(m, inv_t * (1.f / kLn2));
-  float s = 0.f;
-  v.each([&](float f) { s += fast_exp2(ref.t(f)); });
+  const float c_log2 = inv_t * (1.f / kLn2);
+  // each wave's own largest and sum: no waiting for others until all is read
+  float m = -INFINITY, s = 0.f;
+  each_segment([&](int i, int base, int size) {
+    v.template load<true>(x + base, size);
+    if (i == 0 && w == 0) {
+      const bool bad = row.load(teacher, r, n, inv_t);
+      if (lane == 0) bad_row = bad;
+    }
+    if (i == 0 && w == 1) {
+      const int rows_in = mean ? have.total() : 1;
+      if (lane == 0) count = rows_in;
+    }
+    float most[kSegChunks];
+    const float m_old = m;
+    m = fmaxf(m, wave_most(v.maxima(most)));
+    const Reference ref(m, c_log2);
+    if (!ONE && i > 0 && s != 0.f) s *= fast_exp2(Reference(m_old, c_log2).shift(ref));
+    v.each([&](float f) { s += fast_exp2(ref.t(f)); });
+  });
   s = wave_total(s);
-  if (lane == 0) wave_s[w] = s;
+  if (lane == 0) wave_sums[w] = make_float2(m, s);
   __syncthreads();
+  m = wave_sums[0].x;
+#pragma unroll
+  for (int i = 1; i < kWaves; ++i) m = fmaxf(m, wave_sums[i].x);
+  const Reference ref(m, c_log2);
   s = 0.f;
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) s += wave_s[i];
+  for (int i = 0; i < kWaves; ++i) {
+    const float2 p = wave_sums[i];
+    s += p.y == 0.f ? 0.f : p.y * fast_exp2(Reference(p.x, c_log2).shift(ref));
+  }
   const bool bad = bad_row;
-  const float rows_in = count ? fmaxf((float)*count, 1.f) : 1.f;
-  const float g = scale / (inv_t * rows_in), gs = bad ? NAN : s == 0.f ? 0.f : g / s;
+  const float g = scale / (inv_t * fmaxf((float)count, 1.f)), gs = bad ? NAN : s == 0.f ? 0.f : g / s;
+  auto write = [&](int base) {
 #pragma unroll
-  for (int c = 0; c < kSegChunks; ++c) {
-    if (c * Segment<T, THREADS>::kChunk >= n) break;
-    float f[N];
-    v.values(c, f);
+    for (int c = 0; c < kSegChunks; ++c) {
+      if (c * Segment<T, THREADS>::kChunk >= v.n) break;
+      float f[N];
+      v.values(c, f);
 #pragma unroll
-    for (int e = 0; e < N; ++e) f[e] = fast_exp2(ref.t(f[e])) * gs;
-    v.store_own(y, c, f);
+      for (int e = 0; e < N; ++e) f[e] = fast_exp2(ref.t(f[e])) * gs;
+      v.store_own(y + base, c, f);
+    }
+  };
+  if constexpr (ONE) {
+    write(0);
+  } else {
+    write((segments - 1) * len);
+    for (int i = segments - 2; i >= 0; --i) {
+      v.template load<true>(x + i * len, len);
+      write(i * len);
+    }
   }
   if (w == 0) {
     const float loss = row.divergence(x, ref, s, inv_t);
@@ -911,8 +964,7 @@ __global__ __launch_bounds__(64) void k_distill_join(const T* logits, RowMap map
   }
 }
 
-// dx from the rows' m and S.  grad_output: one number, one for each row, or
-// null for 1.  With `made` dx holds the gradient for grad_output 1, and only
+// dx from the rows' m and S.  grad_output: one number, or one for each row.  With `made` dx holds the gradient for grad_output 1, and only
 // another one makes it anew (few workgroups then, each for many segments).
 template <class T>
 __global__ __launch_bounds__(kRowThreads) void k_distill_grad(const T* logits, RowMap map, int n, Teacher teacher,
@@ -927,8 +979,8 @@ __global__ __launch_bounds__(kRowThreads) void k_distill_grad(const T* logits, R
   const float rows_in = count ? fmaxf((float)*count, 1.f) : 1.f;
   const uint32_t items = (uint32_t)rows * segments;  // (< 2^29)
   for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const uint32_t r = item / segments;
-    const int base = (int)(item - r * segments) * len, size = n - base < len ? n - base : len;
+    const uint32_t q = item / segments, r = (uint32_t)rows - 1 - q;  // the last ones first: they are still cached
+    const int base = (int)(item - q * segments) * len, size = n - base < len ? n - base : len;
     const T* x = logits + map(r);
     T* y = dx + (int64_t)r * n;
     const float s = state.s[r];
@@ -947,7 +999,7 @@ __global__ __launch_bounds__(kRowThreads) void k_distill_grad(const T* logits, R
     TeacherRow row(teacher_lds, teacher.k);
     if (tid < 64) row.load(teacher, r, n, inv_t);
     const Reference ref(state.m[r], inv_t * (1.f / kLn2));
-    const float g = (grad_output ? grad_output[per_row ? r : 0] : 1.f) * scale / (inv_t * rows_in), gs = g / s;
+    const float g = grad_output[per_row ? r : 0] * scale / (inv_t * rows_in), gs = g / s;
 #pragma unroll
     for (int c = 0; c < kSegChunks; ++c) {
       if (c * Segment<T>::kChunk >= size) break;
@@ -963,10 +1015,11 @@ __global__ __launch_bounds__(kRowThreads) void k_distill_grad(const T* logits, R
   }
 }
 
-// loss = sum of the row losses (/ count), one workgroup, in a fixed order.
+// loss = sum of the row losses (/ the rows that have a teacher, noted in *count for
+// the backward), one workgroup, in a fixed order.
 constexpr int kSumThreads = 1024;
-__global__ __launch_bounds__(kSumThreads) void k_loss_sum(const float* row_loss, int64_t rows, const int* count,
-                                                          float* loss) {
+__global__ __launch_bounds__(kSumThreads) void k_loss_sum(const float* row_loss, int64_t rows, TeacherRows have,
+                                                          int mean, int* count, float* loss) {
   __shared__ double lds[kSumThreads / 64];
   double s = 0.;
 #pragma unroll 8
@@ -974,9 +1027,12 @@ __global__ __launch_bounds__(kSumThreads) void k_loss_sum(const float* row_loss,
   s = wave_sum_f64(s);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
   __syncthreads();
+  if (threadIdx.x >= 64) return;
+  const int rows_in = mean ? have.total() : 1;
   if (threadIdx.x == 0) {
     for (int w = 1; w < kSumThreads / 64; ++w) s += lds[w];
-    *loss = (float)(count ? s / (*count > 0 ? *count : 1) : s);
+    *loss = (float)(s / (rows_in > 0 ? rows_in : 1));
+    *count = rows_in;
   }
 }
 

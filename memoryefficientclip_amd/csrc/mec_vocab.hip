@@ -149,39 +149,38 @@ int64_t scores_workspace(int64_t rows, int64_t vocab, int top_k, int dtype) {
   return c.segments > 1 ? scores_parts_bytes(rows, c) + round16(rows * c.segments * top_k * 8) : 0;
 }
 
-// Threads of the workgroup that holds a row of logits in registers, 0 if none does.
-int row_threads(int64_t vocab, int dtype) {
-  const int64_t per_thread = (dtype == MEC_DTYPE_F32 ? 4 : 8) * kSegChunks;
+// The workgroup that makes a row's loss and gradient: the fewest threads that hold
+// it in registers, else 1024 and several segments.
+struct RowShape {
+  int threads, segments, len;
+};
+RowShape row_shape(int64_t vocab, int dtype) {
+  const int64_t chunk = dtype == MEC_DTYPE_F32 ? 4 : 8;
   for (int threads = 256; threads <= 1024; threads *= 2)
-    if (vocab <= per_thread * threads) return threads;
-  return 0;
+    if (vocab <= chunk * kSegChunks * threads) return RowShape{threads, 1, (int)vocab};
+  const int64_t s = ceil_div(vocab, chunk * kSegChunks * 1024);
+  const int64_t len = ceil_div(ceil_div(vocab, s), chunk * 1024) * chunk * 1024;
+  return RowShape{1024, (int)ceil_div(vocab, len), (int)len};
 }
 
 // Workspace of mec_distill_forward, in bytes from its start.
 struct DistillWorkspace {
-  int64_t some, row_loss, parts, total;
+  int64_t some, counts, row_loss, parts, total;
 };
 DistillWorkspace distill_workspace(int64_t rows, int64_t vocab, int dtype, bool with_grad) {
   DistillWorkspace w;
-  w.some = 0;
-  w.row_loss = round16(rows * 4);
-  w.parts = 2 * round16(rows * 4);
-  const bool whole = with_grad && row_threads(vocab, dtype) != 0;
-  w.total = w.parts + (whole ? 0 : round16(rows * cut_rows(rows, vocab, dtype).segments * 8));
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t p = at;
+    at += round16(bytes);
+    return p;
+  };
+  w.some = take(rows * 4);
+  w.counts = take(kTeacherGroups * 4);
+  w.row_loss = take(rows * 4);
+  w.parts = take(with_grad ? 0 : rows * cut_rows(rows, vocab, dtype).segments * 8);
+  w.total = at;
   return w;
-}
-
-template <class T>
-void distill_grad(const Logits& x, const Teacher& teacher, float inv_t, float weight, const int* count,
-                  const DistillState& state, const float* grad_output, int per_row, int made, void* dx,
-                  hipStream_t st) {
-  const Cut cut = cut_rows(kManyRows, x.vocab, x.dtype);
-  const int64_t items = x.rows * cut.segments;
-  // (made: to find grad_output 1 few workgroups are enough)
-  const int64_t most = made ? 2048 : int64_t(1) << 22;
-  k_distill_grad<T><<<(unsigned)(items < most ? items : most), kRowThreads, (size_t)teacher.k * 12, st>>>(
-      (const T*)x.p, x.map(), (int)x.vocab, teacher, inv_t, weight, count, state, grad_output, per_row, made, (T*)dx,
-      x.rows, cut.len, cut.segments);
 }
 
 // Workspace of mec_embedding_backward, in bytes from its start.
@@ -338,37 +337,45 @@ int mec_distill_forward(const void* logits, int64_t rows, int64_t inner, int64_t
   if (rc) return rc;
   hipStream_t st = (hipStream_t)stream;
   const Teacher teacher{{teacher_tokens, token_bytes == 8}, teacher_logits, teacher_dtype, (int)k};
-  int* count = reduction == MEC_REDUCE_MEAN ? (int*)(state + 2 * rows) : nullptr;
   char* ws = (char*)workspace;
-  int* some = (int*)(ws + w.some);
-  float2* parts = (float2*)(ws + w.parts);
-  if (count) k_zero_word<<<1, 1, 0, st>>>(count);
-  k_teacher_rows<<<(unsigned)ceil_div(rows, kTeacherRows), kTeacherThreads, 0, st>>>(teacher, rows, some, count);
+  const int64_t each = ceil_div(ceil_div(rows, kTeacherGroups), kTeacherRows) * kTeacherRows;
+  const TeacherRows have{(int*)(ws + w.some), (int*)(ws + w.counts), (int)ceil_div(rows, each), (int)each};
+  k_teacher_rows<<<have.groups, kTeacherThreads, 0, st>>>(teacher, rows, have);
   float* row_loss = reduction == MEC_REDUCE_NONE ? loss : (float*)(ws + w.row_loss);
   const DistillState ds{state, state + rows};
   const float inv_t = 1.f / temperature;
+  const int mean = reduction == MEC_REDUCE_MEAN;
   const size_t lds = (size_t)k * 12;
   with_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     const T* p = (const T*)logits;
     const int n = (int)vocab;
-    const int threads = grad_logits ? row_threads(vocab, dtype) : 0;
-    auto whole = [&](auto th) {
-      constexpr int THREADS = decltype(th)::value;
-      k_distill_row<T, THREADS><<<(unsigned)rows, THREADS, lds, st>>>(p, x.map(), n, teacher, inv_t, weight, some, count,
-                                                                      row_loss, ds, (T*)grad_logits);
-    };
-    if (threads == 256) return whole(std::integral_constant<int, 256>{});
-    if (threads == 512) return whole(std::integral_constant<int, 512>{});
-    if (threads == 1024) return whole(std::integral_constant<int, 1024>{});
+    if (grad_logits) {
+      const RowShape shape = row_shape(vocab, dtype);
+      auto run = [&](auto threads, auto one) {
+        constexpr int THREADS = decltype(threads)::value;
+        k_distill_row<T, THREADS, decltype(one)::value><<<(unsigned)rows, THREADS, lds, st>>>(
+            p, x.map(), n, teacher, inv_t, weight, have, mean, row_loss, ds, (T*)grad_logits, shape.segments, shape.len);
+      };
+      if (shape.segments > 1)
+        run(std::integral_constant<int, 1024>{}, std::false_type{});
+      else if (shape.threads == 256)
+        run(std::integral_constant<int, 256>{}, std::true_type{});
+      else if (shape.threads == 512)
+        run(std::integral_constant<int, 512>{}, std::true_type{});
+      else
+        run(std::integral_constant<int, 1024>{}, std::true_type{});
+      return;
+    }
     const Cut cut = cut_rows(rows, vocab, dtype);
-    k_distill_sums<T><<<cut.dims(rows), kRowThreads, 0, st>>>(p, x.map(), n, inv_t, some, rows, cut.grid(rows), parts);
-    k_distill_join<T><<<(unsigned)rows, 64, lds, st>>>(p, x.map(), n, teacher, inv_t, weight, some, parts, cut.segments,
-                                                       row_loss, ds);
-    if (grad_logits)
-      distill_grad<T>(x, teacher, inv_t, weight, count, ds, nullptr, 0, 0, grad_logits, st);
+    float2* parts = (float2*)(ws + w.parts);
+    k_distill_sums<T><<<cut.dims(rows), kRowThreads, 0, st>>>(p, x.map(), n, inv_t, have.some, rows, cut.grid(rows),
+                                                              parts);
+    k_distill_join<T><<<(unsigned)rows, 64, lds, st>>>(p, x.map(), n, teacher, inv_t, weight, have.some, parts,
+                                                       cut.segments, row_loss, ds);
   });
-  if (reduction != MEC_REDUCE_NONE) k_loss_sum<<<1, kSumThreads, 0, st>>>(row_loss, rows, count, loss);
+  if (reduction != MEC_REDUCE_NONE)
+    k_loss_sum<<<1, kSumThreads, 0, st>>>(row_loss, rows, have, mean, (int*)(state + 2 * rows), loss);
   return check_launch("mec_distill_forward");
 }
 
@@ -392,9 +399,14 @@ int mec_distill_backward(const void* logits, int64_t rows, int64_t inner, int64_
   const int* count = reduction == MEC_REDUCE_MEAN ? (const int*)(state + 2 * rows) : nullptr;
   with_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    distill_grad<T>(x, teacher, 1.f / temperature, weight, count,
-                    DistillState{const_cast<float*>(state), const_cast<float*>(state) + rows}, grad_output,
-                    reduction == MEC_REDUCE_NONE, made != 0, grad_logits, (hipStream_t)stream);
+    const Cut cut = cut_rows(kManyRows, vocab, dtype);
+    const int64_t items = rows * cut.segments;
+    // (made: few workgroups are enough to find that grad_output is 1)
+    const int64_t most = made ? 2048 : int64_t(1) << 22;
+    k_distill_grad<T><<<(unsigned)(items < most ? items : most), kRowThreads, (size_t)k * 12, (hipStream_t)stream>>>(
+        (const T*)logits, x.map(), (int)vocab, teacher, 1.f / temperature, weight, count,
+        DistillState{const_cast<float*>(state), const_cast<float*>(state) + rows}, grad_output,
+        reduction == MEC_REDUCE_NONE, made, (T*)grad_logits, rows, cut.len, cut.segments);
   });
   return check_launch("mec_distill_backward");
 }
