@@ -192,7 +192,7 @@ struct Segment {
   // chunk c's vector to a segment of the same shape
   __device__ __forceinline__ void store(T* p, int c, const float (&x)[N]) const {
     if (n >= N) {
-      *(typename Vec<T>::raw*)(p + begin(c)) = Vec<T>::pack(x);
+      __builtin_nontemporal_store(Vec<T>::pack(x), (typename Vec<T>::raw*)(p + begin(c)));
     } else if (first == 0) {
 #pragma unroll
       for (int e = 0; e < N; ++e)
@@ -203,7 +203,7 @@ struct Segment {
   __device__ __forceinline__ void store_own(T* p, int c, const float (&x)[N]) const {
     const int at = c * kChunk + first;
     if (at + N <= n) {
-      *(typename Vec<T>::raw*)(p + at) = Vec<T>::pack(x);
+      __builtin_nontemporal_store(Vec<T>::pack(x), (typename Vec<T>::raw*)(p + at));
     } else if (at < n) {
       const int i0 = begin(c);
 #pragma unroll
