@@ -627,6 +627,8 @@ __global__ __launch_bounds__(kRowThreads) void k_scores_grad(const T* logits, Ro
   int64_t r;
   int seg;
   if (!grid.place(rows, r, seg)) return;
+  // the last rows first: what the forward read last is still cached
+  r = rows - 1 - r;
   const int base = seg * len, count = n - base < len ? n - base : len;
   const int64_t tok = tokens[r];
   T* y = dx + r * n + base;
