@@ -22,7 +22,7 @@ constexpr int kEmbedTokens = 4;  // rows in flight per lane group
 
 // A group of 2^lg lanes takes a token's row, kEmbedTokens rows at a time.  A
 // token outside [0, vocab) gives a row of NaN.
-template <class T>
+template <class T, bool PAST>
 __global__ __launch_bounds__(kEmbedThreads) void k_embed(Tokens tokens, int64_t n, const T* weight, int64_t ldw,
                                                          int64_t vocab, int d, int lg, float scale, T* out) {
   constexpr int N = Vec<T>::N;
@@ -53,7 +53,7 @@ __global__ __launch_bounds__(kEmbedThreads) void k_embed(Tokens tokens, int64_t 
       if (t >= n) break;
 #pragma unroll
       for (int e = 0; e < N; ++e) v[i][e] = scaled(scale, v[i][e]);
-      store_row(out + t * d + col, d - col, v[i]);
+      store_row<PAST>(out + t * d + col, d - col, v[i]);
     }
   }
 }
@@ -374,7 +374,7 @@ constexpr int kShortRun = 2 * kPiece;
 // one list, whose rows of dy are loaded one after another across the ends of the
 // runs.  Longer runs are summed by the workgroup's 4 waves together, with the
 // pieces' sums.
-template <class T, int NC>
+template <class T, int NC, bool PAST>
 __global__ __launch_bounds__(256) void k_embed_rows(Runs runs, const T* dy, int64_t lddy, int d, float scale,
                                                     const float* piece_sums, const float* block_sums, T* dw) {
   constexpr int N = Vec<T>::N;
@@ -391,7 +391,7 @@ __global__ __launch_bounds__(256) void k_embed_rows(Runs runs, const T* dy, int6
 #pragma unroll
       for (int e = 0; e < N; ++e) sum.acc[c][e] = scaled(scale, sum.acc[c][e]);
       const int at = col + c * 64 * N;
-      store_row(dw + (int64_t)v * d + at, d - at, sum.acc[c]);
+      store_row<PAST>(dw + (int64_t)v * d + at, d - at, sum.acc[c]);
     }
     sum.zero();
   };

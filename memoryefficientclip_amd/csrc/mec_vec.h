@@ -79,11 +79,25 @@ template <class T>
 __device__ __forceinline__ void load_row(const T* p, int n, float (&v)[Vec<T>::N]) {
   Vec<T>::unpack(load_raw(p, n), v);
 }
-template <class T>
+// Outputs that pass half of the last-level cache (256 MB) are stored past it: there
+// they would only push out what is read next, and their lines hold up the kernel
+// that follows while they are written back.  Smaller ones stay for their reader.
+// (PAST is a template argument: the compiler joins the two stores of a branch into
+// one without the hint.)
+constexpr int64_t kKeepBytes = int64_t(128) << 20;
+
+template <bool PAST, class T>
+__device__ __forceinline__ void store_vec(T* p, const typename Vec<T>::raw& v) {
+  if constexpr (PAST)
+    __builtin_nontemporal_store(v, (typename Vec<T>::raw*)p);
+  else
+    *(typename Vec<T>::raw*)p = v;
+}
+template <bool PAST = false, class T>
 __device__ __forceinline__ void store_row(T* p, int n, const float (&v)[Vec<T>::N]) {
   constexpr int N = Vec<T>::N;
   if (n >= N) {
-    *(typename Vec<T>::raw*)p = Vec<T>::pack(v);
+    store_vec<PAST>(p, Vec<T>::pack(v));
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i)

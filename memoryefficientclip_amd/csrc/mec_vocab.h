@@ -190,9 +190,10 @@ struct Segment {
     return r;
   }
   // chunk c's vector to a segment of the same shape
+  template <bool PAST>
   __device__ __forceinline__ void store(T* p, int c, const float (&x)[N]) const {
     if (n >= N) {
-      __builtin_nontemporal_store(Vec<T>::pack(x), (typename Vec<T>::raw*)(p + begin(c)));
+      store_vec<PAST>(p + begin(c), Vec<T>::pack(x));
     } else if (first == 0) {
 #pragma unroll
       for (int e = 0; e < N; ++e)
@@ -200,10 +201,11 @@ struct Segment {
     }
   }
   // the same after load<true>: elements of another thread are left to it
+  template <bool PAST>
   __device__ __forceinline__ void store_own(T* p, int c, const float (&x)[N]) const {
     const int at = c * kChunk + first;
     if (at + N <= n) {
-      __builtin_nontemporal_store(Vec<T>::pack(x), (typename Vec<T>::raw*)(p + at));
+      store_vec<PAST>(p + at, Vec<T>::pack(x));
     } else if (at < n) {
       const int i0 = begin(c);
 #pragma unroll
@@ -616,7 +618,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_scores_join(const T* logits, R
 // dx_v = (1/T) (g_l (1[v = tok] - p_v) - g_h p_v (log p_v + entropy)).
 // One workgroup per segment of a row.  A vector that would pass the end
 // is the last one that does not: two threads then store the same values.
-template <class T>
+template <class T, bool PAST>
 __global__ __launch_bounds__(kRowThreads) void k_scores_grad(const T* logits, RowMap map, int n, Tokens tokens,
                                                              int64_t ignore, float inv_t, const float* stats,
                                                              const float* entropy, const float* g_log_probs,
@@ -663,7 +665,7 @@ __global__ __launch_bounds__(kRowThreads) void k_scores_grad(const T* logits, Ro
         for (int e = 0; e < N; ++e) x[e] += e == own ? gl * inv_t : 0.f;
       }
     }
-    v.store(y, c, x);
+    v.template store<PAST>(y, c, x);
   }
 }
 
@@ -800,7 +802,7 @@ struct DistillState {
 // gradient's write.  Longer rows are read a second time, from the last-level
 // cache that the device's rows at hand fit into; the last segment is still in
 // registers then, and comes first.
-template <class T, int THREADS, bool ONE>
+template <class T, int THREADS, bool ONE, bool PAST>
 __global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap map, int n, Teacher teacher,
                                                          float inv_t, float scale, TeacherRows have, int mean,
                                                          float* row_loss, DistillState state, T* dx, int segments,
@@ -828,7 +830,7 @@ __global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap
       const float zero[N] = {};
 #pragma unroll
       for (int c = 0; c < kSegChunks; ++c)
-        if (c * Segment<T, THREADS>::kChunk < size) v.store(y + base, c, zero);
+        if (c * Segment<T, THREADS>::kChunk < size) v.template store<PAST>(y + base, c, zero);
     });
     return;
   }
@@ -876,7 +878,7 @@ __global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap
       v.values(c, f);
 #pragma unroll
       for (int e = 0; e < N; ++e) f[e] = fast_exp2(ref.t(f[e])) * gs;
-      v.store_own(y + base, c, f);
+      v.template store_own<PAST>(y + base, c, f);
     }
   };
   if constexpr (ONE) {
@@ -968,7 +970,7 @@ __global__ __launch_bounds__(64) void k_distill_join(const T* logits, RowMap map
 
 // dx from the rows' m and S.  grad_output: one number, or one for each row.  With `made` dx holds the gradient for grad_output 1, and only
 // another one makes it anew (few workgroups then, each for many segments).
-template <class T>
+template <class T, bool PAST>
 __global__ __launch_bounds__(kRowThreads) void k_distill_grad(const T* logits, RowMap map, int n, Teacher teacher,
                                                               float inv_t, float scale, const int* count,
                                                               DistillState state, const float* grad_output,
@@ -994,7 +996,7 @@ __global__ __launch_bounds__(kRowThreads) void k_distill_grad(const T* logits, R
       const float zero[N] = {};
 #pragma unroll
       for (int c = 0; c < kSegChunks; ++c)
-        if (c * Segment<T>::kChunk < size) v.store(y + base, c, zero);
+        if (c * Segment<T>::kChunk < size) v.template store<PAST>(y + base, c, zero);
       continue;
     }
     v.template load<false>(x + base, size);
@@ -1009,7 +1011,7 @@ __global__ __launch_bounds__(kRowThreads) void k_distill_grad(const T* logits, R
       v.values(c, f);
 #pragma unroll
       for (int e = 0; e < N; ++e) f[e] = fast_exp2(ref.t(f[e])) * gs;
-      v.store(y + base, c, f);
+      v.template store<PAST>(y + base, c, f);
     }
     __syncthreads();
     if (s == s) row.subtract(x, y, base, size, ref, gs, g);

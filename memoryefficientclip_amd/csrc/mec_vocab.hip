@@ -27,6 +27,16 @@ void with_dtype(int dtype, F f) {
     f((_Float16*)nullptr);
 }
 
+// f(true_type or false_type): whether an output of this size is stored past the
+// last-level cache
+template <class F>
+void with_past(int64_t bytes, F f) {
+  if (bytes > kKeepBytes)
+    f(std::true_type{});
+  else
+    f(std::false_type{});
+}
+
 int check_dtype(int dtype) {
   if (dtype != MEC_DTYPE_F32 && dtype != MEC_DTYPE_BF16 && dtype != MEC_DTYPE_F16)
     return fail(MEC_ERR_INVALID, "dtype %d is not MEC_DTYPE_F32, _BF16 or _F16", dtype);
@@ -303,9 +313,11 @@ int mec_token_scores_backward(const void* logits, int64_t rows, int64_t inner, i
   with_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     const Cut cut = cut_rows(kManyRows, vocab, dtype);
-    k_scores_grad<T><<<cut.dims(rows), kRowThreads, 0, (hipStream_t)stream>>>(
-        (const T*)logits, x.map(), (int)vocab, Tokens{tokens, token_bytes == 8}, ignore_index, 1.f / temperature, state,
-        entropy, grad_log_probs, grad_entropy, (T*)grad_logits, rows, cut.grid(rows));
+    with_past(rows * vocab * sizeof(T), [&](auto past) {
+      k_scores_grad<T, decltype(past)::value><<<cut.dims(rows), kRowThreads, 0, (hipStream_t)stream>>>(
+          (const T*)logits, x.map(), (int)vocab, Tokens{tokens, token_bytes == 8}, ignore_index, 1.f / temperature,
+          state, entropy, grad_log_probs, grad_entropy, (T*)grad_logits, rows, cut.grid(rows));
+    });
   });
   return check_launch("mec_token_scores_backward");
 }
@@ -354,8 +366,11 @@ int mec_distill_forward(const void* logits, int64_t rows, int64_t inner, int64_t
       const RowShape shape = row_shape(vocab, dtype);
       auto run = [&](auto threads, auto one) {
         constexpr int THREADS = decltype(threads)::value;
-        k_distill_row<T, THREADS, decltype(one)::value><<<(unsigned)rows, THREADS, lds, st>>>(
-            p, x.map(), n, teacher, inv_t, weight, have, mean, row_loss, ds, (T*)grad_logits, shape.segments, shape.len);
+        with_past(rows * vocab * sizeof(T), [&](auto past) {
+          k_distill_row<T, THREADS, decltype(one)::value, decltype(past)::value><<<(unsigned)rows, THREADS, lds, st>>>(
+              p, x.map(), n, teacher, inv_t, weight, have, mean, row_loss, ds, (T*)grad_logits, shape.segments,
+              shape.len);
+        });
       };
       if (shape.segments > 1)
         run(std::integral_constant<int, 1024>{}, std::false_type{});
@@ -403,10 +418,13 @@ int mec_distill_backward(const void* logits, int64_t rows, int64_t inner, int64_
     const int64_t items = rows * cut.segments;
     // (made: few workgroups are enough to find that grad_output is 1)
     const int64_t most = made ? 2048 : int64_t(1) << 22;
-    k_distill_grad<T><<<(unsigned)(items < most ? items : most), kRowThreads, (size_t)k * 12, (hipStream_t)stream>>>(
-        (const T*)logits, x.map(), (int)vocab, teacher, 1.f / temperature, weight, count,
-        DistillState{const_cast<float*>(state), const_cast<float*>(state) + rows}, grad_output,
-        reduction == MEC_REDUCE_NONE, made, (T*)grad_logits, rows, cut.len, cut.segments);
+    with_past(rows * vocab * sizeof(T), [&](auto past) {
+      k_distill_grad<T, decltype(past)::value>
+          <<<(unsigned)(items < most ? items : most), kRowThreads, (size_t)k * 12, (hipStream_t)stream>>>(
+              (const T*)logits, x.map(), (int)vocab, teacher, 1.f / temperature, weight, count,
+              DistillState{const_cast<float*>(state), const_cast<float*>(state) + rows}, grad_output,
+              reduction == MEC_REDUCE_NONE, made, (T*)grad_logits, rows, cut.len, cut.segments);
+    });
   });
   return check_launch("mec_distill_backward");
 }
@@ -425,8 +443,11 @@ int mec_embedding(const void* tokens, int token_bytes, int64_t n, const void* we
     int lg = 0;  // lanes for a row: up to a wave, one vector each
     while (lg < 6 && (int64_t)Vec<T>::N << lg < d) ++lg;
     const int64_t per_group = (kEmbedThreads >> lg) * kEmbedTokens;
-    k_embed<T><<<(unsigned)ceil_div(n, per_group), kEmbedThreads, 0, (hipStream_t)stream>>>(
-        Tokens{tokens, token_bytes == 8}, n, (const T*)weight, ldw, vocab, (int)d, lg, scale, (T*)out);
+    with_past(n * d * sizeof(T), [&](auto past) {
+      k_embed<T, decltype(past)::value>
+          <<<(unsigned)ceil_div(n, per_group), kEmbedThreads, 0, (hipStream_t)stream>>>(
+              Tokens{tokens, token_bytes == 8}, n, (const T*)weight, ldw, vocab, (int)d, lg, scale, (T*)out);
+    });
   });
   return check_launch("mec_embedding");
 }
@@ -464,8 +485,10 @@ int mec_embedding_backward(const void* tokens, int token_bytes, int64_t n, const
     const unsigned groups = (unsigned)ceil_div(vocab, kDwRows);
     auto rows = [&](auto nc) {
       constexpr int NC = decltype(nc)::value;
-      k_embed_rows<T, NC><<<dim3(groups, (unsigned)ceil_div(d, NC * 64 * N)), 256, 0, st>>>(
-          runs, (const T*)grad_out, ldg, (int)d, scale, pieces, blocks, (T*)grad_weight);
+      with_past(vocab * d * sizeof(T), [&](auto past) {
+        k_embed_rows<T, NC, decltype(past)::value><<<dim3(groups, (unsigned)ceil_div(d, NC * 64 * N)), 256, 0, st>>>(
+            runs, (const T*)grad_out, ldg, (int)d, scale, pieces, blocks, (T*)grad_weight);
+      });
     };
     if (d <= 64 * N)
       rows(std::integral_constant<int, 1>{});
