@@ -60,20 +60,22 @@ __global__ __launch_bounds__(kEmbedThreads) void k_embed(Tokens tokens, int64_t 
 
 // ---- stable radix sort of (token, position) by token ----
 //
-// Digits of up to 9 bits.  The array is cut into tiles, a tile into a chunk for
-// each wave, which takes 64 pairs at a time: lanes with the same digit find each
-// other with ballots, and the first of them moves the wave's own counter of that
-// digit.  A pass is two launches (tile counts, scatter); up to kSortOne pairs are
-// sorted by one workgroup in one launch.
+// Digits of up to 9 bits.  The array is cut into tiles, a tile into a chunk of up
+// to 8 x 64 pairs for each wave, which holds them in registers: lanes with the same
+// digit find each other with ballots, and the first of them moves the wave's own
+// counter of that digit.  A pass is two launches (tile counts, scatter; a third
+// between them for more than 128 tiles); up to kSortOne pairs are sorted by one
+// workgroup in one launch.
 
 constexpr int kSortThreads = 512, kSortWaves = kSortThreads / 64;
 constexpr int kSortBins = 512;
-constexpr int kSortTiles = 128;  // at most: every workgroup reads all tile counts
-constexpr int kSortOne = 4096;
+constexpr int kSortItems = 8;    // pairs per lane, at most
+constexpr int kSortTiles = 128;  // up to here every workgroup reads all tiles' counts
+constexpr int kSortOne = kSortThreads * kSortItems;
 
 struct SortShape {
   int64_t n;
-  int tile;  // pairs per tile, a multiple of kSortThreads
+  int items;  // pairs per lane
   int tiles;
   int vocab;  // tokens outside [0, vocab) and the padding get this key and come last
   int64_t padding;
@@ -84,12 +86,24 @@ struct SortSource {
   const uint2* pairs; // (key, position), the later ones; null in the first
 };
 
-__device__ __forceinline__ uint2 sort_item(const SortSource& src, const SortShape& s, int64_t i) {
-  if (src.pairs) return src.pairs[i];
-  const int64_t tok = src.tokens[i];
-  const bool ok = tok >= 0 && tok < s.vocab && tok != s.padding;
-  return make_uint2(ok ? (uint32_t)tok : (uint32_t)s.vocab, (uint32_t)i);
-}
+struct SortOut {
+  uint2* pairs;   // all passes but the last
+  int* keys;      // the last
+  int* positions;
+  __device__ __forceinline__ void write(int64_t i, uint2 p) const {
+    if (pairs) {
+      pairs[i] = p;
+    } else {
+      keys[i] = (int)p.x;
+      positions[i] = (int)p.y;
+    }
+  }
+};
+
+struct SortLds {
+  int counters[kSortWaves][kSortBins];
+  int scan[kSortWaves];
+};
 
 // Lanes of the wave with the same digit (of the active ones).
 __device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool active) {
@@ -101,37 +115,51 @@ __device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool ac
   return mask;
 }
 
-// Adds the chunk's digits to the wave's counters; f(pair, digit, place), place =
-// the counter's value for this pair.
-template <class F>
-__device__ __forceinline__ void sort_chunk(const SortSource& src, const SortShape& s, int64_t from, int64_t to,
-                                           int shift, int bits, int* counters, F f) {
-  const int lane = threadIdx.x & 63;
-  for (int64_t i0 = from; i0 < to; i0 += 64) {
-    const int64_t i = i0 + lane;
-    const bool active = i < to;
-    const uint2 p = active ? sort_item(src, s, i) : make_uint2(0, 0);
-    const uint32_t digit = (p.x >> shift) & ((1u << bits) - 1);
-    const uint64_t mask = same_digit(digit, bits, active);
-    const int first = active ? __ffsll((unsigned long long)mask) - 1 : lane;
-    int old = 0;
-    if (active && lane == first) old = atomicAdd(&counters[digit], __popcll(mask));
-    old = __shfl(old, first, 64);
-    if (active) f(p, digit, old + __popcll(mask & ((1ull << lane) - 1)));
+// A wave's pairs of a tile, in order: lane, then the next 64.
+struct SortChunk {
+  uint2 pair[kSortItems];
+  int place[kSortItems];  // among the wave's pairs of the same digit
+  int count;              // pairs
+  __device__ __forceinline__ void load(const SortSource& src, const SortShape& s, int64_t tile) {
+    const int lane = threadIdx.x & 63, per_wave = s.items * 64;
+    const int64_t from = tile * (int64_t)(per_wave * kSortWaves) + (int64_t)(threadIdx.x >> 6) * per_wave;
+    const int64_t left = s.n - from;
+    count = left < 0 ? 0 : left < per_wave ? (int)left : per_wave;
+#pragma unroll
+    for (int b = 0; b < kSortItems; ++b) {
+      const int i = b * 64 + lane;
+      pair[b] = make_uint2(0, 0);
+      if (i >= count) continue;
+      if (src.pairs) {
+        pair[b] = src.pairs[from + i];
+      } else {
+        const int64_t tok = src.tokens[from + i];
+        const bool ok = tok >= 0 && tok < s.vocab && tok != s.padding;
+        pair[b] = make_uint2(ok ? (uint32_t)tok : (uint32_t)s.vocab, (uint32_t)(from + i));
+      }
+    }
   }
-}
-
-__device__ __forceinline__ void sort_tile_chunk(const SortShape& s, int64_t tile, int64_t& from, int64_t& to) {
-  const int64_t begin = tile * s.tile, end = begin + s.tile < s.n ? begin + s.tile : s.n;
-  from = begin + (int64_t)(threadIdx.x >> 6) * (s.tile / kSortWaves);
-  to = from + s.tile / kSortWaves;
-  if (from > end) from = end;
-  if (to > end) to = end;
-}
-
-struct SortLds {
-  int counters[kSortWaves][kSortBins];
-  int scan[kSortWaves];
+  // Adds the digits to the wave's counters, and notes the places.
+  __device__ __forceinline__ void rank(int shift, int bits, int* counters) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int b = 0; b < kSortItems; ++b) {
+      if (b * 64 >= count) break;
+      const bool active = b * 64 + lane < count;
+      const uint32_t digit = (pair[b].x >> shift) & ((1u << bits) - 1);
+      const uint64_t mask = same_digit(digit, bits, active);
+      const int first = active ? __ffsll((unsigned long long)mask) - 1 : lane;
+      int old = 0;
+      if (active && lane == first) old = atomicAdd(&counters[digit], __popcll(mask));
+      place[b] = __shfl(old, first, 64) + __popcll(mask & ((1ull << lane) - 1));
+    }
+  }
+  __device__ __forceinline__ void scatter(int shift, int bits, const int* begins, const SortOut& out) const {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int b = 0; b < kSortItems; ++b)
+      if (b * 64 + lane < count) out.write(begins[(pair[b].x >> shift) & ((1u << bits) - 1)] + place[b], pair[b]);
+  }
 };
 
 __device__ __forceinline__ void sort_zero(SortLds& l) {
@@ -155,23 +183,18 @@ __device__ __forceinline__ int sort_scan(int v, SortLds& l) {
   return base + s - v;
 }
 
-// counts[tile][digit]
-__global__ __launch_bounds__(kSortThreads) void k_sort_count(SortSource src, SortShape s, int shift, int bits,
-                                                             int* counts) {
-  __shared__ SortLds l;
-  sort_zero(l);
-  int64_t from, to;
-  sort_tile_chunk(s, blockIdx.x, from, to);
-  sort_chunk(src, s, from, to, shift, bits, l.counters[threadIdx.x >> 6], [](uint2, uint32_t, int) {});
-  __syncthreads();
+// The tile's count of the thread's digit.
+__device__ __forceinline__ int sort_digit_count(const SortLds& l) {
   int sum = 0;
+#pragma unroll
   for (int w = 0; w < kSortWaves; ++w) sum += l.counters[w][threadIdx.x];
-  counts[blockIdx.x * kSortBins + threadIdx.x] = sum;
+  return sum;
 }
 
 // Turns the waves' counts into the places where their digits begin, given where
 // the tile's digits begin (one digit per thread).
 __device__ __forceinline__ void sort_places(SortLds& l, int begin) {
+#pragma unroll
   for (int w = 0; w < kSortWaves; ++w) {
     const int c = l.counters[w][threadIdx.x];
     l.counters[w][threadIdx.x] = begin;
@@ -180,58 +203,94 @@ __device__ __forceinline__ void sort_places(SortLds& l, int begin) {
   __syncthreads();
 }
 
-struct SortOut {
-  uint2* pairs;   // all passes but the last
-  int* keys;      // the last
-  int* positions;
-  __device__ __forceinline__ void write(int64_t i, uint2 p) const {
-    if (pairs) {
-      pairs[i] = p;
-    } else {
-      keys[i] = (int)p.x;
-      positions[i] = (int)p.y;
-    }
+// Marks every token's run as empty, a part by each workgroup.
+__device__ __forceinline__ void clear_bounds(int2* bounds, int vocab, int block, int blocks) {
+  for (int v = block * kSortThreads + threadIdx.x; v < vocab; v += blocks * kSortThreads) bounds[v] = make_int2(0, 0);
+}
+
+// counts[tile][digit]; bounds (or null) is cleared on the way.
+__global__ __launch_bounds__(kSortThreads) void k_sort_count(SortSource src, SortShape s, int shift, int bits,
+                                                             int* counts, int2* bounds) {
+  __shared__ SortLds l;
+  SortChunk chunk;
+  chunk.load(src, s, blockIdx.x);
+  if (bounds) clear_bounds(bounds, s.vocab, blockIdx.x, gridDim.x);
+  sort_zero(l);
+  chunk.rank(shift, bits, l.counters[threadIdx.x >> 6]);
+  __syncthreads();
+  counts[blockIdx.x * kSortBins + threadIdx.x] = sort_digit_count(l);
+}
+
+// For more than kSortTiles tiles: counts[t] becomes the sum of the tiles before
+// t, counts[tiles] the sum of all.  A workgroup per 64 digits, a wave per eighth
+// of the tiles.
+__global__ __launch_bounds__(kSortThreads) void k_sort_prefix(int* counts, int tiles) {
+  __shared__ int sums[kSortWaves][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, digit = blockIdx.x * 64 + lane;
+  const int each = (tiles + kSortWaves - 1) / kSortWaves;
+  const int from = w * each < tiles ? w * each : tiles, to = from + each < tiles ? from + each : tiles;
+  int sum = 0;
+#pragma unroll 16
+  for (int t = from; t < to; ++t) sum += counts[t * kSortBins + digit];
+  sums[w][lane] = sum;
+  __syncthreads();
+  int before = 0;
+  for (int i = 0; i < w; ++i) before += sums[i][lane];
+#pragma unroll 16
+  for (int t = from; t < to; ++t) {
+    const int c = counts[t * kSortBins + digit];
+    counts[t * kSortBins + digit] = before;
+    before += c;
   }
-};
+  if (w == kSortWaves - 1) counts[tiles * kSortBins + digit] = before;
+}
 
 __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(SortSource src, SortShape s, int shift, int bits,
                                                                const int* counts, SortOut out) {
   __shared__ SortLds l;
-  sort_zero(l);
-  int64_t from, to;
-  sort_tile_chunk(s, blockIdx.x, from, to);
-  int* mine = l.counters[threadIdx.x >> 6];
-  sort_chunk(src, s, from, to, shift, bits, mine, [](uint2, uint32_t, int) {});
+  SortChunk chunk;
+  chunk.load(src, s, blockIdx.x);
   int before = 0, total = 0;
-#pragma unroll 16
-  for (int t = 0; t < s.tiles; ++t) {
-    const int c = counts[t * kSortBins + threadIdx.x];
-    total += c;
-    before += t < (int)blockIdx.x ? c : 0;
+  if (s.tiles > kSortTiles) {
+    before = counts[blockIdx.x * kSortBins + threadIdx.x];
+    total = counts[s.tiles * kSortBins + threadIdx.x];
+  } else {
+#pragma unroll 32
+    for (int t = 0; t < s.tiles; ++t) {
+      const int c = counts[t * kSortBins + threadIdx.x];
+      total += c;
+      before += t < (int)blockIdx.x ? c : 0;
+    }
   }
+  sort_zero(l);
+  int* mine = l.counters[threadIdx.x >> 6];
+  chunk.rank(shift, bits, mine);
   const int begin = sort_scan(total, l) + before;
   sort_places(l, begin);
-  sort_chunk(src, s, from, to, shift, bits, mine, [&](uint2 p, uint32_t, int place) { out.write(place, p); });
+  chunk.scatter(shift, bits, mine, out);
 }
 
-// All passes by one workgroup (n <= kSortOne, one tile).
+// All passes by the first workgroup (n <= kSortOne, one tile); the others clear
+// the bounds.
 __global__ __launch_bounds__(kSortThreads) void k_sort_one(Tokens tokens, SortShape s, int passes, int bits,
-                                                           uint2* even, uint2* odd, SortOut last) {
+                                                           uint2* even, uint2* odd, SortOut last, int2* bounds) {
   __shared__ SortLds l;
-  int64_t from, to;
-  sort_tile_chunk(s, 0, from, to);
+  if (blockIdx.x > 0) {
+    clear_bounds(bounds, s.vocab, blockIdx.x - 1, gridDim.x - 1);
+    return;
+  }
   int* mine = l.counters[threadIdx.x >> 6];
   for (int pass = 0; pass < passes; ++pass) {
     const SortSource src{tokens, pass == 0 ? nullptr : pass & 1 ? even : odd};
     const SortOut out = pass == passes - 1 ? last : SortOut{pass & 1 ? odd : even, nullptr, nullptr};
+    SortChunk chunk;
+    chunk.load(src, s, 0);
     sort_zero(l);
-    sort_chunk(src, s, from, to, pass * bits, bits, mine, [](uint2, uint32_t, int) {});
+    chunk.rank(pass * bits, bits, mine);
     __syncthreads();
-    int total = 0;
-    for (int w = 0; w < kSortWaves; ++w) total += l.counters[w][threadIdx.x];
-    const int begin = sort_scan(total, l);
+    const int begin = sort_scan(sort_digit_count(l), l);
     sort_places(l, begin);
-    sort_chunk(src, s, from, to, pass * bits, bits, mine, [&](uint2 p, uint32_t, int place) { out.write(place, p); });
+    chunk.scatter(pass * bits, bits, mine, out);
     __syncthreads();
   }
 }
@@ -360,11 +419,6 @@ __global__ __launch_bounds__(kBlockPieces * 64) void k_embed_pieces(Runs runs, c
     for (int p = 0; p < kBlockPieces; ++p) s += lds[p][i];
     if (c < d) block_sums[(int64_t)blockIdx.x * d + c] = s;
   }
-}
-
-__global__ __launch_bounds__(256) void k_embed_clear(int2* bounds, int vocab) {
-  const int v = blockIdx.x * 256 + threadIdx.x;
-  if (v < vocab) bounds[v] = make_int2(0, 0);
 }
 
 constexpr int kWaveRows = 4, kDwRows = 4 * kWaveRows;  // vocabulary rows per wave, per workgroup

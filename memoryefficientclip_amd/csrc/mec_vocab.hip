@@ -210,7 +210,7 @@ EmbedWorkspace embed_workspace(int64_t n, int64_t vocab, int64_t d) {
   w.keys = take(n * 4);
   w.positions = take(n * 4);
   w.bounds = take(vocab * 8);
-  w.counts = take((int64_t)kSortTiles * kSortBins * 4);
+  w.counts = take((ceil_div(n, (int64_t)kSortThreads * kSortItems) + kSortTiles + 1) * kSortBins * 4);
   w.pieces = take(n / kPiece * d * 4);
   w.blocks = take(n / kBlock * d * 4);
   w.total = at;
@@ -223,26 +223,27 @@ Runs sort_tokens(const void* tokens, int token_bytes, int64_t n, int64_t vocab, 
   int key_bits = 1;
   while ((vocab >> key_bits) != 0) ++key_bits;
   const int passes = (key_bits + 8) / 9, bits = (key_bits + passes - 1) / passes;
-  SortShape s{n, 0, 1, (int)vocab, padding};
+  // pairs per lane: as few as keep the tiles within kSortTiles
+  const int64_t per_lane = ceil_div(n, (int64_t)kSortThreads * (n <= kSortOne ? 1 : kSortTiles));
+  SortShape s{n, (int)(per_lane < kSortItems ? per_lane : kSortItems), 1, (int)vocab, padding};
   const Tokens tok{tokens, token_bytes == 8};
   uint2 *even = (uint2*)(ws + w.even), *odd = (uint2*)(ws + w.odd);
   const SortOut last{nullptr, (int*)(ws + w.keys), (int*)(ws + w.positions)};
+  int2* bounds = (int2*)(ws + w.bounds);
   if (n <= kSortOne) {
-    s.tile = (int)(ceil_div(n, kSortThreads) * kSortThreads);
-    k_sort_one<<<1, kSortThreads, 0, st>>>(tok, s, passes, bits, even, odd, last);
+    const unsigned clears = (unsigned)ceil_div(vocab, 4 * kSortThreads);
+    k_sort_one<<<1 + (clears < 256 ? clears : 256), kSortThreads, 0, st>>>(tok, s, passes, bits, even, odd, last, bounds);
   } else {
-    s.tile = (int)(ceil_div(ceil_div(n, kSortTiles), kSortThreads) * kSortThreads);
-    s.tiles = (int)ceil_div(n, s.tile);
+    s.tiles = (int)ceil_div(n, (int64_t)kSortThreads * s.items);
     int* counts = (int*)(ws + w.counts);
     for (int pass = 0; pass < passes; ++pass) {
       const SortSource src{tok, pass == 0 ? nullptr : pass & 1 ? even : odd};
       const SortOut out = pass == passes - 1 ? last : SortOut{pass & 1 ? odd : even, nullptr, nullptr};
-      k_sort_count<<<s.tiles, kSortThreads, 0, st>>>(src, s, pass * bits, bits, counts);
+      k_sort_count<<<s.tiles, kSortThreads, 0, st>>>(src, s, pass * bits, bits, counts, pass == 0 ? bounds : nullptr);
+      if (s.tiles > kSortTiles) k_sort_prefix<<<kSortBins / 64, kSortThreads, 0, st>>>(counts, s.tiles);
       k_sort_scatter<<<s.tiles, kSortThreads, 0, st>>>(src, s, pass * bits, bits, counts, out);
     }
   }
-  int2* bounds = (int2*)(ws + w.bounds);
-  k_embed_clear<<<(unsigned)ceil_div(vocab, 256), 256, 0, st>>>(bounds, (int)vocab);
   return Runs{last.keys, last.positions, n, (int)vocab, bounds};
 }
 
