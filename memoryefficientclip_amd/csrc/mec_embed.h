@@ -422,9 +422,9 @@ __global__ __launch_bounds__(kBlockPieces * 64) void k_embed_pieces(Runs runs, c
 }
 
 constexpr int kWaveRows = 4, kDwRows = 4 * kWaveRows;  // vocabulary rows per wave, per workgroup
-constexpr int kShortRun = 2 * kPiece;
+constexpr int kShortRun = 16;  // a wave's work alone; longer ones would be the launch's last
 
-// Every row of dW, four to a wave: the positions of their runs of up to 64 are
+// Every row of dW, four to a wave: the positions of their runs of up to 16 are
 // one list, whose rows of dy are loaded one after another across the ends of the
 // runs.  Longer runs are summed by the workgroup's 4 waves together, with the
 // pieces' sums.
@@ -432,7 +432,8 @@ template <class T, int NC, bool PAST>
 __global__ __launch_bounds__(256) void k_embed_rows(Runs runs, const T* dy, int64_t lddy, int d, float scale,
                                                     const float* piece_sums, const float* block_sums, T* dw) {
   constexpr int N = Vec<T>::N;
-  constexpr int U = NC >= 4 ? 2 : 8 / NC;
+  constexpr int U = 8 / NC;      // rows of dy in flight
+  constexpr int UF = U > 1 ? U / 2 : 1;  // rows of sums
   __shared__ float lds[3][NC * N * 64];
   const int v0 = blockIdx.x * kDwRows;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -501,7 +502,8 @@ __global__ __launch_bounds__(256) void k_embed_rows(Runs runs, const T* dy, int6
     const int q = __ffsll((unsigned long long)left) - 1;
     const int64_t lo = __builtin_amdgcn_readlane(bound.x, q), hi = __builtin_amdgcn_readlane(bound.y, q);
     // [lo, a) positions, [a, a2) pieces, [a2, b2) blocks, [b2, b) pieces, [b, hi) positions
-    const int64_t a = (lo + kPiece - 1) / kPiece * kPiece, b = hi / kPiece * kPiece;
+    int64_t a = (lo + kPiece - 1) / kPiece * kPiece, b = hi / kPiece * kPiece;
+    if (a > b) a = b = hi;
     int64_t a2 = (a + kBlock - 1) / kBlock * kBlock, b2 = b / kBlock * kBlock;
     if (a2 >= b2) a2 = b2 = b;
     sum.zero();
@@ -515,7 +517,7 @@ __global__ __launch_bounds__(256) void k_embed_rows(Runs runs, const T* dy, int6
       const int64_t count = to - from, each = (count + 3) / 4;
       const int64_t at = w * each < count ? w * each : count;
       const int mine = (int)(count - at < each ? count - at : each);
-      sum.template add<float, U>(s, mine, col, d, [&](int i) { return (from + at + i) * (int64_t)d; });
+      sum.template add<float, UF>(s, mine, col, d, [&](int i) { return (from + at + i) * (int64_t)d; });
     };
     positions(lo, a);
     sums(piece_sums, a / kPiece, a2 / kPiece);

@@ -491,12 +491,11 @@ int mec_embedding_backward(const void* tokens, int token_bytes, int64_t n, const
             runs, (const T*)grad_out, ldg, (int)d, scale, pieces, blocks, (T*)grad_weight);
       });
     };
-    if (d <= 64 * N)
-      rows(std::integral_constant<int, 1>{});
-    else if (d <= 128 * N)
-      rows(std::integral_constant<int, 2>{});
-    else
-      rows(std::integral_constant<int, 4>{});
+    // (1024 columns by a wave: more of them in 16 bits take too many registers)
+    if (d <= 64 * N) return rows(std::integral_constant<int, 1>{});
+    if constexpr (sizeof(T) == 4)
+      if (d > 128 * N) return rows(std::integral_constant<int, 4>{});
+    rows(std::integral_constant<int, 2>{});
   });
   return check_launch("mec_embedding_backward");
 }

@@ -56,6 +56,24 @@ def test_sizes(n, vocab, d, dtype):
     check(*make(n, vocab, d, dtype))
 
 
+@pytest.mark.parametrize("n,vocab,d", [(524288, 5000, 8), (600001, 70000, 12), (700000, 3, 4)])
+def test_many_tokens(n, vocab, d):
+    """More than 128 tiles of the sort."""
+    check(*make(n, vocab, d, torch.bfloat16, seed=10))
+
+
+@pytest.mark.parametrize("n", [17, 40, 70, 300, 2000])
+def test_runs_of_every_length(n):
+    """Token v occurs v times, in a random order: runs that end inside and at the
+    ends of pieces and blocks, at every offset."""
+    lengths = torch.arange(n % 7, 400)
+    tok = torch.repeat_interleave(lengths, lengths)
+    g = torch.Generator().manual_seed(n)
+    tok = tok[torch.randperm(tok.numel(), generator=g)][: n * 40]
+    _, w, dy = make(tok.numel(), 400, 20, torch.float32, seed=11)
+    check(tok, w, dy)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
 @pytest.mark.parametrize("n", [500, 5000, 60000])
 def test_tokens_that_occur_often(n, dtype):
