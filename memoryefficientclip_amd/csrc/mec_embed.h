@@ -71,7 +71,7 @@ constexpr int kSortThreads = 512, kSortWaves = kSortThreads / 64;
 constexpr int kSortBins = 512;
 constexpr int kSortItems = 8;    // pairs per lane, at most
 constexpr int kSortTiles = 128;  // up to here every workgroup reads all tiles' counts
-constexpr int kSortOne = kSortThreads * kSortItems;
+constexpr int kSortOneThreads = 1024, kSortOne = kSortOneThreads * kSortItems;
 
 struct SortShape {
   int64_t n;
@@ -100,9 +100,11 @@ struct SortOut {
   }
 };
 
+template <int THREADS>
 struct SortLds {
-  int counters[kSortWaves][kSortBins];
-  int scan[kSortWaves];
+  static constexpr int kWaves = THREADS / 64;
+  int counters[kWaves][kSortBins];
+  int scan[kWaves];
 };
 
 // Lanes of the wave with the same digit (of the active ones).
@@ -162,13 +164,15 @@ struct SortChunk {
   }
 };
 
-__device__ __forceinline__ void sort_zero(SortLds& l) {
-  for (int i = threadIdx.x; i < kSortWaves * kSortBins; i += kSortThreads) (&l.counters[0][0])[i] = 0;
+template <int THREADS>
+__device__ __forceinline__ void sort_zero(SortLds<THREADS>& l) {
+  for (int i = threadIdx.x; i < l.kWaves * kSortBins; i += THREADS) (&l.counters[0][0])[i] = 0;
   __syncthreads();
 }
 
-// Exclusive sum over the workgroup's 512 threads.
-__device__ __forceinline__ int sort_scan(int v, SortLds& l) {
+// Exclusive sum over the workgroup's threads.
+template <int THREADS>
+__device__ __forceinline__ int sort_scan(int v, SortLds<THREADS>& l) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int s = v;
   for (int i = 1; i < 64; i <<= 1) {
@@ -183,35 +187,41 @@ __device__ __forceinline__ int sort_scan(int v, SortLds& l) {
   return base + s - v;
 }
 
-// The tile's count of the thread's digit.
-__device__ __forceinline__ int sort_digit_count(const SortLds& l) {
+// The tile's count of the thread's digit (0: the thread has none).
+template <int THREADS>
+__device__ __forceinline__ int sort_digit_count(const SortLds<THREADS>& l) {
   int sum = 0;
+  if (threadIdx.x < kSortBins) {
 #pragma unroll
-  for (int w = 0; w < kSortWaves; ++w) sum += l.counters[w][threadIdx.x];
+    for (int w = 0; w < l.kWaves; ++w) sum += l.counters[w][threadIdx.x];
+  }
   return sum;
 }
 
 // Turns the waves' counts into the places where their digits begin, given where
 // the tile's digits begin (one digit per thread).
-__device__ __forceinline__ void sort_places(SortLds& l, int begin) {
+template <int THREADS>
+__device__ __forceinline__ void sort_places(SortLds<THREADS>& l, int begin) {
+  if (threadIdx.x < kSortBins) {
 #pragma unroll
-  for (int w = 0; w < kSortWaves; ++w) {
-    const int c = l.counters[w][threadIdx.x];
-    l.counters[w][threadIdx.x] = begin;
-    begin += c;
+    for (int w = 0; w < l.kWaves; ++w) {
+      const int c = l.counters[w][threadIdx.x];
+      l.counters[w][threadIdx.x] = begin;
+      begin += c;
+    }
   }
   __syncthreads();
 }
 
 // Marks every token's run as empty, a part by each workgroup.
 __device__ __forceinline__ void clear_bounds(int2* bounds, int vocab, int block, int blocks) {
-  for (int v = block * kSortThreads + threadIdx.x; v < vocab; v += blocks * kSortThreads) bounds[v] = make_int2(0, 0);
+  for (int v = block * blockDim.x + threadIdx.x; v < vocab; v += blocks * blockDim.x) bounds[v] = make_int2(0, 0);
 }
 
 // counts[tile][digit]; bounds (or null) is cleared on the way.
 __global__ __launch_bounds__(kSortThreads) void k_sort_count(SortSource src, SortShape s, int shift, int bits,
                                                              int* counts, int2* bounds) {
-  __shared__ SortLds l;
+  __shared__ SortLds<kSortThreads> l;
   SortChunk chunk;
   chunk.load(src, s, blockIdx.x);
   if (bounds) clear_bounds(bounds, s.vocab, blockIdx.x, gridDim.x);
@@ -247,7 +257,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_prefix(int* counts, int t
 
 __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(SortSource src, SortShape s, int shift, int bits,
                                                                const int* counts, SortOut out) {
-  __shared__ SortLds l;
+  __shared__ SortLds<kSortThreads> l;
   SortChunk chunk;
   chunk.load(src, s, blockIdx.x);
   int before = 0, total = 0;
@@ -272,9 +282,9 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(SortSource src, S
 
 // All passes by the first workgroup (n <= kSortOne, one tile); the others clear
 // the bounds.
-__global__ __launch_bounds__(kSortThreads) void k_sort_one(Tokens tokens, SortShape s, int passes, int bits,
+__global__ __launch_bounds__(kSortOneThreads) void k_sort_one(Tokens tokens, SortShape s, int passes, int bits,
                                                            uint2* even, uint2* odd, SortOut last, int2* bounds) {
-  __shared__ SortLds l;
+  __shared__ SortLds<kSortOneThreads> l;
   if (blockIdx.x > 0) {
     clear_bounds(bounds, s.vocab, blockIdx.x - 1, gridDim.x - 1);
     return;

@@ -224,15 +224,15 @@ Runs sort_tokens(const void* tokens, int token_bytes, int64_t n, int64_t vocab, 
   while ((vocab >> key_bits) != 0) ++key_bits;
   const int passes = (key_bits + 8) / 9, bits = (key_bits + passes - 1) / passes;
   // pairs per lane: as few as keep the tiles within kSortTiles
-  const int64_t per_lane = ceil_div(n, (int64_t)kSortThreads * (n <= kSortOne ? 1 : kSortTiles));
+  const int64_t per_lane = ceil_div(n, n <= kSortOne ? kSortOneThreads : (int64_t)kSortThreads * kSortTiles);
   SortShape s{n, (int)(per_lane < kSortItems ? per_lane : kSortItems), 1, (int)vocab, padding};
   const Tokens tok{tokens, token_bytes == 8};
   uint2 *even = (uint2*)(ws + w.even), *odd = (uint2*)(ws + w.odd);
   const SortOut last{nullptr, (int*)(ws + w.keys), (int*)(ws + w.positions)};
   int2* bounds = (int2*)(ws + w.bounds);
   if (n <= kSortOne) {
-    const unsigned clears = (unsigned)ceil_div(vocab, 4 * kSortThreads);
-    k_sort_one<<<1 + (clears < 256 ? clears : 256), kSortThreads, 0, st>>>(tok, s, passes, bits, even, odd, last, bounds);
+    const unsigned clears = (unsigned)ceil_div(vocab, 4 * kSortOneThreads);
+    k_sort_one<<<1 + (clears < 256 ? clears : 256), kSortOneThreads, 0, st>>>(tok, s, passes, bits, even, odd, last, bounds);
   } else {
     s.tiles = (int)ceil_div(n, (int64_t)kSortThreads * s.items);
     int* counts = (int*)(ws + w.counts);
