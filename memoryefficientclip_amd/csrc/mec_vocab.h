@@ -92,6 +92,7 @@ struct Reference {
     m = row_max == -INFINITY ? 0.f : row_max;
     c = scale;
     mc = m * c;
+    asm("" : "+v"(mc));  // one rounded number wherever it is used, not part of another fma
     far = !(fabsf(mc) < 4194304.f);
   }
   __device__ __forceinline__ float t(float x) const { return far ? 2.f * c * (0.5f * x - 0.5f * m) : fmaf(x, c, -mc); }

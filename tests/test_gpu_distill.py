@@ -129,6 +129,16 @@ def test_masked_students(dtype, vocab):
     ref.assert_close("dx", dx, grad, dtype, 2 * ref.score_tolerance(x, 1.0))
 
 
+@pytest.mark.parametrize("offset", [3e4, -3e6])
+@pytest.mark.parametrize("vocab", [300, 50001, 150000])
+def test_common_offset(vocab, offset):
+    x, tok, z = make(3, vocab, 12, torch.float32, seed=13)
+    x = (x + offset).float()
+    x[:, : vocab // 3] -= 40.0
+    for go in (1.0, 2.0):
+        check(x, tok, z + offset, 0.7, grad_output=go)
+
+
 def test_nan_spreads_over_its_row_alone():
     x, tok, z = make(5, 2500, 8, torch.float32, seed=5)
     x[0, 7] = math.nan

@@ -148,6 +148,22 @@ def test_large_values():
         check(x, tok, 4, temperature, atol=3e-6 * max(1.0, 3.0 / temperature))
 
 
+@pytest.mark.parametrize("offset", [3e4, -3e4, 3e6, -3e7])
+@pytest.mark.parametrize("vocab", [300, 50001, 131072])
+def test_common_offset(vocab, offset):
+    """Logits far from zero: their differences are exact in fp32, and so must the
+    results be, though scaled logits are rounded by far more than the tolerance."""
+    x, tok, g = make(3, vocab, torch.float32, seed=14)
+    x = (x + offset).float()
+    x[:, : vocab // 3] -= 40.0     # segments with other maxima
+    for temperature in (1.0, 0.7):
+        check(x, tok, 5, temperature)
+    gl, gh = torch.randn(3, generator=g), torch.randn(3, generator=g)
+    want = ref.token_scores_grad(x, tok, gl, gh, 0.7)
+    atol = ref.score_tolerance(x, 0.7) / 0.7 * (gl.abs().max() + gh.abs().max() * (1 + ref.spread(x, 0.7))).item()
+    ref.assert_close("dx", gradient(x, tok, gl, gh, 0.7), want, torch.float32, atol)
+
+
 def test_layouts():
     g = torch.Generator().manual_seed(5)
     base = torch.randn(4, 9, 1003, generator=g)
