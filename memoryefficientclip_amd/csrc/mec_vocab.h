@@ -241,27 +241,36 @@ struct Segment {
     return m;
   }
   // f(element, its index) over the thread's elements that pred holds for, few,
-  // all in vectors that look(vector) holds for
+  // all in vectors that look(vector) holds for.  Every lane goes to its own next
+  // vector and its own next element: a wave takes as many steps as its lane with
+  // the most, not one for each vector and element that any lane wants.
   template <class L, class P, class F>
   __device__ __forceinline__ void each_of(L look, P pred, F f) {
+    uint32_t vectors = 0;
 #pragma unroll
-    for (int c = 0; c < kSegChunks; ++c) {
-      if (c * kChunk >= n) break;
-      if (!look(c)) continue;
+    for (int c = 0; c < kSegChunks; ++c)
+      if (c * kChunk + first < n && look(c)) vectors |= 1u << c;
+#pragma unroll 1
+    for (; vectors; vectors &= vectors - 1) {
+      const int at = __ffs(vectors) - 1;
+      typename Vec<T>::raw r = v[0];
+#pragma unroll
+      for (int c = 1; c < kSegChunks; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = at == c ? v[c][i] : r[i];
       float x[N];
-      values(c, x);
+      Vec<T>::unpack(r, x);
       uint32_t hits = 0;
 #pragma unroll
       for (int e = 0; e < N; ++e) hits |= pred(x[e]) ? 1u << e : 0u;
-      if (hits == 0) continue;
-      const int i0 = begin(c);
+      const int i0 = begin(at);
 #pragma unroll 1
       for (; hits; hits &= hits - 1) {
         const int e = __ffs(hits) - 1;
         float y = x[0];
 #pragma unroll
         for (int q = 1; q < N; ++q) y = e == q ? x[q] : y;
-        if (i0 + e >= c * kChunk + first && i0 + e < n) f(y, i0 + e);
+        if (i0 + e >= at * kChunk + first && i0 + e < n) f(y, i0 + e);
       }
     }
   }
