@@ -551,6 +551,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_scores_join(const T* logits, R
   const int count = segments * k;
   part_top += r * count;
   const float c = inv_t * (1.f / kLn2);
+  const uint64_t early = tid < count ? part_top[tid] : 0;  // on its way while the cut is found
   if (tid < 64) {
     const float at = tok >= 0 && tok < n ? value(logits[map(r) + tok]) : 0.f;
     const float4 p = lane < segments ? parts[r * segments + lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
@@ -591,8 +592,9 @@ __global__ __launch_bounds__(kJoinThreads) void k_scores_join(const T* logits, R
   __syncthreads();
   uint64_t cut = cut_at;
   uint64_t* found = keys;
+  if (early >= cut) found[atomicAdd(&kept, 1)] = early;
 #pragma unroll 4
-  for (int i = tid; i < count; i += kJoinThreads) {
+  for (int i = tid + kJoinThreads; i < count; i += kJoinThreads) {
     const uint64_t key = part_top[i];
     if (key >= cut) found[atomicAdd(&kept, 1)] = key;
   }
