@@ -811,9 +811,9 @@ struct DistillState {
 
 // Loss and gradient (for grad_output 1) of a row by one workgroup.  With ONE the
 // row is one segment and stays in registers from its only read to the
-// gradient's write.  Longer rows are read a second time, from the last-level
-// cache that the device's rows at hand fit into; the last segment is still in
-// registers then, and comes first.
+// gradient's write.  Of a longer row the last segment stays in registers and
+// the one before it in LDS (128 KB: up to 131072 16-bit logits are read once);
+// what is left is read a second time.
 template <class T, int THREADS, bool ONE, bool PAST>
 __global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap map, int n, Teacher teacher,
                                                          float inv_t, float scale, TeacherRows have, int mean,
@@ -823,16 +823,19 @@ __global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap
   extern __shared__ float teacher_lds[];
   __shared__ float2 wave_sums[kWaves];
   __shared__ int bad_row, count;
+  __shared__ typename Vec<T>::raw held[ONE ? 1 : kSegChunks][ONE ? 1 : THREADS];
   const int64_t r = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const T* x = logits + map(r);
   T* y = dx + r * n;
   Segment<T, THREADS> v;
+  // (the first segment is the short one: the others fill the registers)
+  const int first_size = ONE ? n : n - (segments - 1) * len;
   auto each_segment = [&](auto f) {  // f(segment, its first element, its size)
     if constexpr (ONE)
       f(0, 0, n);
     else
-      for (int i = 0; i < segments; ++i) f(i, i * len, n - i * len < len ? n - i * len : len);
+      for (int i = 0; i < segments; ++i) f(i, i ? first_size + (i - 1) * len : 0, i ? len : first_size);
   };
   if (!have.some[r]) {
     if (tid == 0) row_loss[r] = 0.f, state.m[r] = 0.f, state.s[r] = -1.f;
@@ -866,6 +869,13 @@ __global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap
     const Reference ref(m, c_log2);
     if (!ONE && i > 0 && s != 0.f) s *= fast_exp2(Reference(m_old, c_log2).shift(ref));
     v.each([&](float f) { s += fast_exp2(ref.t(f)); });
+    if constexpr (!ONE) {
+      if (i == segments - 2) {
+#pragma unroll
+        for (int c = 0; c < kSegChunks; ++c)
+          if (c * Segment<T, THREADS>::kChunk < size) held[c][tid] = v.v[c];
+      }
+    }
   });
   s = wave_total(s);
   if (lane == 0) wave_sums[w] = make_float2(m, s);
@@ -896,10 +906,18 @@ __global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap
   if constexpr (ONE) {
     write(0);
   } else {
-    write((segments - 1) * len);
+    write(first_size + (segments - 2) * len);
     for (int i = segments - 2; i >= 0; --i) {
-      v.template load<true>(x + i * len, len);
-      write(i * len);
+      const int base = i ? first_size + (i - 1) * len : 0, size = i ? len : first_size;
+      if (i == segments - 2) {
+        v.n = size;
+#pragma unroll
+        for (int c = 0; c < kSegChunks; ++c)
+          if (c * Segment<T, THREADS>::kChunk < size) v.v[c] = held[c][tid];
+      } else {
+        v.template load<true>(x + base, size);
+      }
+      write(base);
     }
   }
   if (w == 0) {

@@ -168,8 +168,7 @@ RowShape row_shape(int64_t vocab, int dtype) {
   const int64_t chunk = dtype == MEC_DTYPE_F32 ? 4 : 8;
   for (int threads = 256; threads <= 1024; threads *= 2)
     if (vocab <= chunk * kSegChunks * threads) return RowShape{threads, 1, (int)vocab};
-  const int64_t s = ceil_div(vocab, chunk * kSegChunks * 1024);
-  const int64_t len = ceil_div(ceil_div(vocab, s), chunk * 1024) * chunk * 1024;
+  const int64_t len = chunk * kSegChunks * 1024;
   return RowShape{1024, (int)ceil_div(vocab, len), (int)len};
 }
 
