@@ -9,6 +9,15 @@
 
 namespace mec {
 
+// Where the vector of a row of d elements begins that a lane takes for column
+// `col`: one that would pass the end is the last one that does not (two lanes
+// then do the same for the columns they share).  n: its elements, 0 for none.
+template <int N>
+__device__ __forceinline__ int vec_begin(int col, int d, int& n) {
+  n = col >= d ? 0 : d < N ? d : N;
+  return d < N || col < d - N ? col : d - N;
+}
+
 // scale * v in 32 bits, to be rounded after: not contracted with the rounding
 // into one instruction that rounds the exact product to 16 bits.
 __device__ __forceinline__ float scaled(float scale, float v) {
@@ -36,12 +45,14 @@ __global__ __launch_bounds__(kEmbedThreads) void k_embed(Tokens tokens, int64_t 
     tok[i] = t < n ? tokens[t] : -1;
     if (tok[i] >= vocab) tok[i] = -1;
   }
-  for (int col = lane * N; col < d; col += N << lg) {
+  for (int col0 = lane * N; col0 < d; col0 += N << lg) {
+    int n_col;
+    const int col = vec_begin<N>(col0, d, n_col);
     float v[kEmbedTokens][N];
 #pragma unroll
     for (int i = 0; i < kEmbedTokens; ++i) {
       if (tok[i] >= 0) {
-        load_row(weight + tok[i] * ldw + col, d - col, v[i]);
+        load_row(weight + tok[i] * ldw + col, n_col, v[i]);
       } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) v[i][e] = NAN;
@@ -53,7 +64,7 @@ __global__ __launch_bounds__(kEmbedThreads) void k_embed(Tokens tokens, int64_t 
       if (t >= n) break;
 #pragma unroll
       for (int e = 0; e < N; ++e) v[i][e] = scaled(scale, v[i][e]);
-      store_row<PAST>(out + t * d + col, d - col, v[i]);
+      store_row<PAST>(out + t * d + col, n_col, v[i]);
     }
   }
 }
@@ -313,12 +324,18 @@ __global__ __launch_bounds__(kSortOneThreads) void k_sort_one(Tokens tokens, Sor
 
 constexpr int kPiece = 32, kBlockPieces = 8, kBlock = kPiece * kBlockPieces;
 
-// acc += the rows of dy at positions [from, to) of the sorted order, in order;
-// columns col + lane * N of each of NC stretches of 64 N columns.
+// Sums of rows, added in order: a lane's vector in each of NC stretches of 64 N
+// columns.
 template <class T, int NC>
 struct RowSum {
   static constexpr int N = Vec<T>::N;
   float acc[NC][N];
+  int at[NC], n[NC];  // the lane's vectors (vec_begin)
+  __device__ __forceinline__ RowSum(int col, int d) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) at[c] = vec_begin<N>(col + c * 64 * N, d, n[c]);
+    zero();
+  }
   __device__ __forceinline__ void zero() {
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -327,7 +344,7 @@ struct RowSum {
   }
   // rows of `src`, row(i) for i in [0, count)
   template <class S, int U, class F>
-  __device__ __forceinline__ void add(const S* src, int count, int col, int d, F row) {
+  __device__ __forceinline__ void add(const S* src, int count, F row) {
     constexpr int M = Vec<S>::N, P = N / M;  // vectors of S per stretch and lane
     int i = 0;
     for (; i + U <= count; i += U) {
@@ -338,10 +355,7 @@ struct RowSum {
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int q = 0; q < P; ++q) {
-            const int at = col + c * 64 * N + q * M;
-            v[u][c][q] = load_raw(p + at, d - at);
-          }
+          for (int q = 0; q < P; ++q) v[u][c][q] = load_raw(p + at[c] + q * M, n[c] - q * M);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -361,9 +375,8 @@ struct RowSum {
       for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int q = 0; q < P; ++q) {
-          const int at = col + c * 64 * N + q * M;
           float v[M];
-          load_row(p + at, d - at, v);
+          load_row(p + at[c] + q * M, n[c] - q * M, v);
 #pragma unroll
           for (int e = 0; e < M; ++e) acc[c][q * M + e] += v[e];
         }
@@ -406,16 +419,15 @@ __global__ __launch_bounds__(kBlockPieces * 64) void k_embed_pieces(Runs runs, c
   const bool one = key0 < runs.vocab && key0 == __builtin_amdgcn_readlane(key, kPiece - 1);
   if (!__syncthreads_or(one)) return;
   const int col = blockIdx.y * 64 * N + lane * N;
-  RowSum<T, 1> sum;
-  sum.zero();
+  RowSum<T, 1> sum(col, d);
   if (one)
-    sum.template add<T, 16>(dy, kPiece, col, d, [&](int i) { return (int64_t)__builtin_amdgcn_readlane(pos, i) * lddy; });
+    sum.template add<T, 16>(dy, kPiece, [&](int i) { return (int64_t)__builtin_amdgcn_readlane(pos, i) * lddy; });
   if (!all) {
     if (one) {
 #pragma unroll
       for (int q = 0; q < N / 4; ++q) {
         const float v[4] = {sum.acc[0][q * 4], sum.acc[0][q * 4 + 1], sum.acc[0][q * 4 + 2], sum.acc[0][q * 4 + 3]};
-        store_row(piece_sums + (p0 / kPiece) * d + col + q * 4, d - col - q * 4, v);
+        store_row(piece_sums + (p0 / kPiece) * d + sum.at[0] + q * 4, sum.n[0] - q * 4, v);
       }
     }
     return;
@@ -424,10 +436,11 @@ __global__ __launch_bounds__(kBlockPieces * 64) void k_embed_pieces(Runs runs, c
   for (int e = 0; e < N; ++e) lds[w][e * 64 + lane] = sum.acc[0][e];
   __syncthreads();
   for (int i = threadIdx.x; i < 64 * N; i += kBlockPieces * 64) {
-    const int c = blockIdx.y * 64 * N + (i & 63) * N + (i >> 6);
+    int n;
+    const int c = vec_begin<N>(blockIdx.y * 64 * N + (i & 63) * N, d, n);
     float s = 0.f;
     for (int p = 0; p < kBlockPieces; ++p) s += lds[p][i];
-    if (c < d) block_sums[(int64_t)blockIdx.x * d + c] = s;
+    if ((i >> 6) < n) block_sums[(int64_t)blockIdx.x * d + c + (i >> 6)] = s;
   }
 }
 
@@ -449,21 +462,19 @@ __global__ __launch_bounds__(256) void k_embed_rows(Runs runs, const T* dy, int6
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int col = blockIdx.y * NC * 64 * N + lane * N;
   const int2 bound = lane < kDwRows && v0 + lane < runs.vocab ? runs.bounds[v0 + lane] : make_int2(0, 0);
-  RowSum<T, NC> sum;
+  RowSum<T, NC> sum(col, d);
   auto write = [&](int v) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
 #pragma unroll
       for (int e = 0; e < N; ++e) sum.acc[c][e] = scaled(scale, sum.acc[c][e]);
-      const int at = col + c * 64 * N;
-      store_row<PAST>(dw + (int64_t)v * d + at, d - at, sum.acc[c]);
+      store_row<PAST>(dw + (int64_t)v * d + sum.at[c], sum.n[c], sum.acc[c]);
     }
     sum.zero();
   };
   // the wave's short runs as one list
   int begin[kWaveRows], end[kWaveRows + 1];  // of the run; of its part of the list
   end[0] = 0;
-  sum.zero();
 #pragma unroll
   for (int r = 0; r < kWaveRows; ++r) {
     const int q = w * kWaveRows + r;
@@ -487,7 +498,7 @@ __global__ __launch_bounds__(256) void k_embed_rows(Runs runs, const T* dy, int6
       for (int u = 0; u < U; ++u) {
         const T* p = dy + (int64_t)__builtin_amdgcn_readlane(pos, j + u < n ? j + u : n - 1) * lddy;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) v[u][c] = load_raw(p + col + c * 64 * N, d - col - c * 64 * N);
+        for (int c = 0; c < NC; ++c) v[u][c] = load_raw(p + sum.at[c], sum.n[c]);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -521,13 +532,13 @@ __global__ __launch_bounds__(256) void k_embed_rows(Runs runs, const T* dy, int6
       const int count = (int)(to - from), each = (count + 3) / 4;
       const int at = w * each < count ? w * each : count, mine = count - at < each ? count - at : each;
       const int pos = lane < mine ? runs.positions[from + at + lane] : 0;
-      sum.template add<T, U>(dy, mine, col, d, [&](int i) { return (int64_t)__builtin_amdgcn_readlane(pos, i) * lddy; });
+      sum.template add<T, U>(dy, mine, [&](int i) { return (int64_t)__builtin_amdgcn_readlane(pos, i) * lddy; });
     };
     auto sums = [&](const float* s, int64_t from, int64_t to) {
       const int64_t count = to - from, each = (count + 3) / 4;
       const int64_t at = w * each < count ? w * each : count;
       const int mine = (int)(count - at < each ? count - at : each);
-      sum.template add<float, UF>(s, mine, col, d, [&](int i) { return (from + at + i) * (int64_t)d; });
+      sum.template add<float, UF>(s, mine, [&](int i) { return (from + at + i) * (int64_t)d; });
     };
     positions(lo, a);
     sums(piece_sums, a / kPiece, a2 / kPiece);
