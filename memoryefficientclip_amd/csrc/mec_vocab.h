@@ -127,74 +127,101 @@ struct SegmentGrid {
 };
 constexpr int kMaxSegments = 64;  // a lane each in the join
 
-// A vector's words with -inf in the first `skip` elements.
+// A vector's words with -inf outside of its elements [lo, hi).
 template <class T>
-__device__ __forceinline__ typename Vec<T>::raw skip_elements(typename Vec<T>::raw r, int skip) {
+__device__ __forceinline__ typename Vec<T>::raw own_elements(typename Vec<T>::raw r, int lo, int hi) {
   constexpr uint32_t kInf = std::is_same<T, float>::value      ? 0xff800000u
                             : std::is_same<T, uint16_t>::value ? 0xff80ff80u
                                                                : 0xfc00fc00u;
   constexpr int kPer = 4 / sizeof(T);  // elements in a word
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int in_word = skip - i * kPer;
-    const uint32_t mask = in_word <= 0 ? 0u : in_word >= kPer ? ~0u : 0xffffu;
-    r[i] = (r[i] & ~mask) | (kInf & mask);
+    uint32_t mask = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      if (i * kPer + e >= lo && i * kPer + e < hi) mask |= (kPer == 1 ? ~0u : 0xffffu) << (16 * e);
+    r[i] = (r[i] & mask) | (kInf & ~mask);
   }
   return r;
 }
+
+// Elements between the last 4-byte boundary and p.  Vectors begin on these: off
+// them the loads take 1.35 times as long (8192 x 50001 bf16), while 16-byte
+// boundaries make no difference (50002, 50004 against 50008).
+template <class T>
+__device__ __forceinline__ int misaligned(const T* p) {
+  return (int)(((uintptr_t)p & 3) / sizeof(T));
+}
+
+// Elements [base, base + size) of a row of n that begins `shift` elements past a
+// boundary: segment `seg` (size <= 0: none).
+struct SegmentRange {
+  int base, size;
+  __device__ __forceinline__ SegmentRange(int seg, int len, int n, int shift) {
+    const int from = seg * len - shift, to = from + len < n ? from + len : n;
+    base = from > 0 ? from : 0;
+    size = to - base;
+  }
+};
 
 template <class T, int THREADS = kRowThreads>
 struct Segment {
   static constexpr int N = Vec<T>::N, kChunk = THREADS * N;
   typename Vec<T>::raw v[kSegChunks];
-  int n, first;  // elements; the thread's first one
-  // n elements at p.  A vector that would pass the end is the last one that
-  // does not; with ONCE the elements in it that belong to another thread are -inf.
-  template <bool ONCE>
-  __device__ __forceinline__ void load(const T* p, int count) {
+  // elements; where the thread's first vector would begin; elements from the
+  // boundary before the segment on
+  int n, first, span;
+  // The shape of a segment of `count` elements at p.  Vectors begin on boundaries
+  // (misaligned), but for one that would begin before the segment or end after it,
+  // which is moved into it.
+  __device__ __forceinline__ void shape(const T* p, int count) {
     // (opaque: in a loop over segments the compiler else makes a copy of the code for
     // each number of vectors)
+    count = __builtin_amdgcn_readfirstlane(count);
     asm volatile("" : "+s"(count));
     n = count;
-    first = threadIdx.x * N;
+    const int shift = n < N ? 0 : misaligned(p);
+    first = (int)threadIdx.x * N - shift;
+    span = n + shift;
+  }
+  // where chunk c's vector would begin, and where it does
+  __device__ __forceinline__ int place(int c) const { return c * kChunk + first; }
+  __device__ __forceinline__ int begin(int c) const {
+    const int at = place(c) > 0 ? place(c) : 0;
+    return n < N ? 0 : at < n - N ? at : n - N;
+  }
+  // n elements at p; with ONCE the elements that a moved vector shares with
+  // another thread's are -inf in it.
+  template <bool ONCE>
+  __device__ __forceinline__ void load(const T* p, int count) {
+    shape(p, count);
     if (n < N) {
-      v[0] = first == 0 ? load_small(p) : skip_elements<T>(v[0], N);
+      v[0] = load_raw(p, first == 0 ? n : 0);
+      v[0] = own_elements<T>(v[0], 0, first == 0 ? n : 0);
       return;
     }
 #pragma unroll
     for (int c = 0; c < kSegChunks; ++c) {
       // (set in any case: a register set in one trip alone is kept through the next)
-      if (c * kChunk < n)
+      if (c * kChunk < span)
         v[c] = *(const typename Vec<T>::raw*)(p + begin(c));
       else
-        v[c] = skip_elements<T>(v[c], N);
+        v[c] = own_elements<T>(v[c], 0, 0);
     }
     if constexpr (!ONCE) return;
+    if (first < 0) v[0] = own_elements<T>(v[0], 0, N + first);
 #pragma unroll
     for (int c = 0; c < kSegChunks; ++c)
-      if (c * kChunk < n && (c + 1) * kChunk > n) v[c] = skip_elements<T>(v[c], c * kChunk + first - begin(c));
-  }
-  __device__ __forceinline__ typename Vec<T>::raw load_small(const T* p) {
-    typename Vec<T>::raw r = {0, 0, 0, 0};
-    r = skip_elements<T>(r, N);
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i < n) {
-        constexpr int kPer = 4 / sizeof(T);
-        if constexpr (kPer == 1) {
-          r[i] = __float_as_uint(p[i]);
-        } else {
-          const uint32_t at = 16 * (i & 1), q = __builtin_bit_cast(uint16_t, p[i]);
-          r[i / 2] = (r[i / 2] & ~(0xffffu << at)) | (q << at);
-        }
+      if (c * kChunk < span && (c + 1) * kChunk > span) {
+        const int lo = place(c) - begin(c);
+        if (lo > 0) v[c] = own_elements<T>(v[c], lo, N);
       }
-    return r;
   }
   // chunk c's vector to a segment of the same shape
   template <bool PAST>
   __device__ __forceinline__ void store(T* p, int c, const float (&x)[N]) const {
     if (n >= N) {
-      store_vec<PAST>(p + begin(c), Vec<T>::pack(x));
+      if (place(c) < n) store_vec<PAST>(p + begin(c), Vec<T>::pack(x));
     } else if (first == 0) {
 #pragma unroll
       for (int e = 0; e < N; ++e)
@@ -204,20 +231,15 @@ struct Segment {
   // the same after load<true>: elements of another thread are left to it
   template <bool PAST>
   __device__ __forceinline__ void store_own(T* p, int c, const float (&x)[N]) const {
-    const int at = c * kChunk + first;
-    if (at + N <= n) {
+    const int at = place(c);
+    if (at >= 0 && at + N <= n) {
       store_vec<PAST>(p + at, Vec<T>::pack(x));
     } else if (at < n) {
       const int i0 = begin(c);
 #pragma unroll
       for (int e = 0; e < N; ++e)
-        if (i0 + e >= at && i0 + e < n) put(p + i0 + e, x[e]);
+        if (i0 + e >= at && i0 + e < at + N && i0 + e < n) put(p + i0 + e, x[e]);
     }
-  }
-  // where chunk c's vector begins
-  __device__ __forceinline__ int begin(int c) const {
-    const int at = c * kChunk + first;
-    return n < N ? 0 : at < n - N ? at : n - N;
   }
   // Unpacked anew by every pass: what one pass unpacks is not kept for the next
   // (twice the registers, and spills).
@@ -231,7 +253,7 @@ struct Segment {
 #pragma unroll
     for (int c = 0; c < kSegChunks; ++c) {
       most[c] = -INFINITY;
-      if (c * kChunk >= n) continue;
+      if (c * kChunk >= span) continue;
       float x[N];
       values(c, x);
 #pragma unroll
@@ -249,7 +271,7 @@ struct Segment {
     uint32_t vectors = 0;
 #pragma unroll
     for (int c = 0; c < kSegChunks; ++c)
-      if (c * kChunk + first < n && look(c)) vectors |= 1u << c;
+      if (place(c) < n && look(c)) vectors |= 1u << c;
 #pragma unroll 1
     for (; vectors; vectors &= vectors - 1) {
       const int at = __ffs(vectors) - 1;
@@ -270,7 +292,30 @@ struct Segment {
         float y = x[0];
 #pragma unroll
         for (int q = 1; q < N; ++q) y = e == q ? x[q] : y;
-        if (i0 + e >= at * kChunk + first && i0 + e < n) f(y, i0 + e);
+        if (i0 + e >= place(at) && i0 + e < place(at) + N && i0 + e < n) f(y, i0 + e);
+      }
+    }
+  }
+  // whether a vector of chunk c has -inf in place of another thread's elements
+  __device__ __forceinline__ bool edge(int c) const {
+    return (c == 0 && span != n) || ((c + 1) * kChunk > span && span % N != 0);
+  }
+  // f(element) over the thread's elements (and -inf in place of others'), in the
+  // chunks with an edge g(element)
+  template <class F, class G>
+  __device__ __forceinline__ void each(F f, G g) {
+#pragma unroll
+    for (int c = 0; c < kSegChunks; ++c) {
+      if (c * kChunk >= span) break;
+      if (place(c) >= n) continue;
+      float x[N];
+      values(c, x);
+      if (edge(c)) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) g(x[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) f(x[e]);
       }
     }
   }
@@ -279,8 +324,8 @@ struct Segment {
   __device__ __forceinline__ void each(F f) {
 #pragma unroll
     for (int c = 0; c < kSegChunks; ++c) {
-      if (c * kChunk >= n) break;
-      if (c * kChunk + first >= n) continue;
+      if (c * kChunk >= span) break;
+      if (place(c) >= n) continue;
       float x[N];
       values(c, x);
 #pragma unroll
@@ -450,16 +495,23 @@ __global__ __launch_bounds__(kRowThreads) void k_scores(const T* logits, RowMap 
   int64_t r;
   int seg;
   if (!grid.place(rows, r, seg)) return;
-  const int base = seg * len;
   const int64_t item = r * segments + seg;
   const int64_t tok = tokens[r];
   if (tok == ignore) {
     if (segments == 1) write_ignored(out, r, rows, k, tid, kRowThreads);
     return;
   }
-  const T* x = logits + map(r) + base;
+  const T* x = logits + map(r);
+  const SegmentRange range(seg, len, n, misaligned(x));
+  const int base = range.base;
+  if (range.size <= 0) {  // (the last one, of a row that needs one less)
+    if (tid == 0) parts[item] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    for (int i = tid; i < k; i += kRowThreads) part_top[item * k + i] = 0;
+    return;
+  }
+  x += base;
   Segment<T> v;
-  v.template load<true>(x, n - base < len ? n - base : len);
+  v.template load<true>(x, range.size);
   float most[kSegChunks];
   float m = v.maxima(most);
   if constexpr (TOP) {
@@ -477,22 +529,33 @@ __global__ __launch_bounds__(kRowThreads) void k_scores(const T* logits, RowMap 
   }
   const Reference ref(m, c);
   float s = 0.f, u = 0.f;
-  auto sums = [&](auto plain) {
-    s = u = 0.f;
-    v.each([&](float f) {
-      const float t = decltype(plain)::value ? fmaf(f, c, -ref.mc) : ref.t(f);
-      const float e = fast_exp2(t);
-      s += e;
-      // (2^t is 0 below -200, where t may be -inf)
-      u = fmaf(e, decltype(plain)::value ? t : fmaxf(t, -200.f), u);
-    });
+  auto careful = [&](float f) {
+    const float t = ref.t(f);
+    const float e = fast_exp2(t);
+    s += e;
+    // (2^t is 0 below -200, where t may be -inf)
+    u = fmaf(e, fmaxf(t, -200.f), u);
+  };
+  // Where no t is -inf the plain form does, with one operation in eleven less (138
+  // against 162 us for 8192 x 50008 bf16); a wave that meets one has a U of NaN and
+  // starts again.
+  if (!ref.far) {
+    v.each(
+        [&](float f) {
+          const float t = fmaf(f, c, -ref.mc), e = fast_exp2(t);
+          s += e;
+          u = fmaf(e, t, u);
+        },
+        careful);
     s = wave_total(s);
     u = wave_total(u);
-  };
-  // Where no t is -inf the plain form is enough, one operation in eleven less; a
-  // wave that meets one has a U of NaN and takes the other.
-  if (!ref.far) sums(std::true_type{});
-  if (ref.far || u != u) sums(std::false_type{});
+  }
+  if (ref.far || u != u) {
+    s = u = 0.f;
+    v.each(careful);
+    s = wave_total(s);
+    u = wave_total(u);
+  }
   if (lane == 0) wave_s[w] = s, wave_u[w] = u;
   __syncthreads();
   s = u = 0.f;
@@ -643,23 +706,27 @@ __global__ __launch_bounds__(kRowThreads) void k_scores_grad(const T* logits, Ro
   if (!grid.place(rows, r, seg)) return;
   // the last rows first: what the forward read last is still cached
   r = rows - 1 - r;
-  const int base = seg * len, count = n - base < len ? n - base : len;
   const int64_t tok = tokens[r];
+  const T* x0 = logits + map(r);
+  const SegmentRange range(seg, len, n, misaligned(x0));
+  const int base = range.base;
+  if (range.size <= 0) return;
   T* y = dx + r * n + base;
   const float s = stats[rows + r];
   const bool none = tok == ignore || s == 0.f, bad = tok < 0 || tok >= n;
   Segment<T> v;
-  if (!none) v.template load<false>(logits + map(r) + base, count);
+  if (none)
+    v.shape(x0 + base, range.size);
+  else
+    v.template load<false>(x0 + base, range.size);
   const Reference ref(stats[r], inv_t * (1.f / kLn2));
   const float ls = logf(s), gl = bad ? NAN : g_log_probs ? g_log_probs[r] : 0.f, gh = g_entropy ? g_entropy[r] : 0.f;
   // e (a + b t) = -(1/T) p (g_l + g_h (log p + entropy))
   const float f = none ? 0.f : -inv_t / s, a = f * (gl + gh * (entropy[r] - ls)), b = f * gh * kLn2;
   const int at = (int)(bad ? 0 : tok) - base;
-  v.n = count;
-  v.first = threadIdx.x * N;
 #pragma unroll
   for (int c = 0; c < kSegChunks; ++c) {
-    if (c * Segment<T>::kChunk >= count) break;
+    if (c * Segment<T>::kChunk >= v.span) break;
     float x[N];
     if (none) {
 #pragma unroll
@@ -829,23 +896,25 @@ __global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap
   const T* x = logits + map(r);
   T* y = dx + r * n;
   Segment<T, THREADS> v;
-  // (the first segment is the short one: the others fill the registers)
-  const int first_size = ONE ? n : n - (segments - 1) * len;
+  // (the first segment is the short one, up to a boundary: the others fill the registers)
+  const int shift = misaligned(x);
+  const int first_size = ONE ? n : (n - (segments - 1) * len + shift + N - 1) / N * N - shift;
+  auto seg_base = [&](int i) { return i ? first_size + (i - 1) * len : 0; };
+  auto seg_size = [&](int i) { return (i < segments - 1 ? seg_base(i + 1) : n) - seg_base(i); };
   auto each_segment = [&](auto f) {  // f(segment, its first element, its size)
     if constexpr (ONE)
       f(0, 0, n);
     else
-      for (int i = 0; i < segments; ++i) f(i, i ? first_size + (i - 1) * len : 0, i ? len : first_size);
+      for (int i = 0; i < segments; ++i) f(i, seg_base(i), seg_size(i));
   };
   if (!have.some[r]) {
     if (tid == 0) row_loss[r] = 0.f, state.m[r] = 0.f, state.s[r] = -1.f;
     each_segment([&](int, int base, int size) {
-      v.n = size;
-      v.first = tid * N;
+      v.shape(x + base, size);
       const float zero[N] = {};
 #pragma unroll
       for (int c = 0; c < kSegChunks; ++c)
-        if (c * Segment<T, THREADS>::kChunk < size) v.template store<PAST>(y + base, c, zero);
+        if (c * Segment<T, THREADS>::kChunk < v.span) v.template store<PAST>(y + base, c, zero);
     });
     return;
   }
@@ -873,7 +942,7 @@ __global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap
       if (i == segments - 2) {
 #pragma unroll
         for (int c = 0; c < kSegChunks; ++c)
-          if (c * Segment<T, THREADS>::kChunk < size) held[c][tid] = v.v[c];
+          if (c * Segment<T, THREADS>::kChunk < v.span) held[c][tid] = v.v[c];
       }
     }
   });
@@ -895,7 +964,7 @@ __global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap
   auto write = [&](int base) {
 #pragma unroll
     for (int c = 0; c < kSegChunks; ++c) {
-      if (c * Segment<T, THREADS>::kChunk >= v.n) break;
+      if (c * Segment<T, THREADS>::kChunk >= v.span) break;
       float f[N];
       v.values(c, f);
 #pragma unroll
@@ -906,14 +975,14 @@ __global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap
   if constexpr (ONE) {
     write(0);
   } else {
-    write(first_size + (segments - 2) * len);
+    write(seg_base(segments - 1));
     for (int i = segments - 2; i >= 0; --i) {
-      const int base = i ? first_size + (i - 1) * len : 0, size = i ? len : first_size;
+      const int base = seg_base(i), size = seg_size(i);
       if (i == segments - 2) {
-        v.n = size;
+        v.shape(x + base, size);
 #pragma unroll
         for (int c = 0; c < kSegChunks; ++c)
-          if (c * Segment<T, THREADS>::kChunk < size) v.v[c] = held[c][tid];
+          if (c * Segment<T, THREADS>::kChunk < v.span) v.v[c] = held[c][tid];
       } else {
         v.template load<true>(x + base, size);
       }
@@ -943,10 +1012,16 @@ __global__ __launch_bounds__(kRowThreads) void k_distill_sums(const T* logits, R
   int64_t r;
   int seg;
   if (!grid.place(rows, r, seg)) return;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, len = grid.len, base = seg * len;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   if (!some[r]) return;
+  const T* x = logits + map(r);
+  const SegmentRange range(seg, grid.len, n, misaligned(x));
+  if (range.size <= 0) {  // (the last one, of a row that needs one less)
+    if (tid == 0) parts[r * grid.segments + seg] = make_float2(-INFINITY, 0.f);
+    return;
+  }
   Segment<T> v;
-  v.template load<true>(logits + map(r) + base, n - base < len ? n - base : len);
+  v.template load<true>(x + range.base, range.size);
   float m = -INFINITY;
   v.each([&](float f) { m = fmaxf(m, f); });
   m = wave_most(m);
@@ -1014,19 +1089,20 @@ __global__ __launch_bounds__(kRowThreads) void k_distill_grad(const T* logits, R
   const uint32_t items = (uint32_t)rows * segments;  // (< 2^29)
   for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
     const uint32_t q = item / segments, r = (uint32_t)rows - 1 - q;  // the last ones first: they are still cached
-    const int base = (int)(item - q * segments) * len, size = n - base < len ? n - base : len;
     const T* x = logits + map(r);
+    const SegmentRange range((int)(item - q * segments), len, n, misaligned(x));
+    const int base = range.base, size = range.size;
+    if (size <= 0) continue;
     T* y = dx + (int64_t)r * n;
     const float s = state.s[r];
     const bool none = s <= 0.f;
     Segment<T> v;
-    v.n = size;
-    v.first = tid * N;
     if (none) {
+      v.shape(x + base, size);
       const float zero[N] = {};
 #pragma unroll
       for (int c = 0; c < kSegChunks; ++c)
-        if (c * Segment<T>::kChunk < size) v.template store<PAST>(y + base, c, zero);
+        if (c * Segment<T>::kChunk < v.span) v.template store<PAST>(y + base, c, zero);
       continue;
     }
     v.template load<false>(x + base, size);
@@ -1036,7 +1112,7 @@ __global__ __launch_bounds__(kRowThreads) void k_distill_grad(const T* logits, R
     const float g = grad_output[per_row ? r : 0] * scale / (inv_t * rows_in), gs = g / s;
 #pragma unroll
     for (int c = 0; c < kSegChunks; ++c) {
-      if (c * Segment<T>::kChunk >= size) break;
+      if (c * Segment<T>::kChunk >= v.span) break;
       float f[N];
       v.values(c, f);
 #pragma unroll

@@ -63,6 +63,11 @@ struct Logits {
   int64_t rows, inner, outer_stride, inner_stride, vocab;
   int dtype;
   RowMap map() const { return RowMap{inner, outer_stride, inner_stride}; }
+  // every row begins on a 4-byte boundary
+  bool aligned() const {
+    return dtype == MEC_DTYPE_F32 ||
+           (((uintptr_t)p & 3) == 0 && outer_stride % 2 == 0 && (inner == 1 || inner_stride % 2 == 0));
+  }
 };
 
 int check_logits(const Logits& x) {
@@ -142,8 +147,9 @@ struct Cut {
   }
 };
 constexpr int64_t kManyRows = 1024;  // a workgroup each fills the device
-Cut cut_rows(int64_t rows, int64_t vocab, int dtype) {
-  const int64_t chunk = kRowThreads * (dtype == MEC_DTYPE_F32 ? 4 : 8);  // a vector per thread
+Cut cut_rows(int64_t rows, int64_t vocab, int dtype, bool aligned) {
+  const int64_t vec = dtype == MEC_DTYPE_F32 ? 4 : 8, chunk = kRowThreads * vec;  // a vector per thread
+  if (!aligned) ++vocab;  // counted from the boundary before the row
   int64_t s = ceil_div(vocab, chunk * kSegChunks);
   // few rows: more, shorter segments, so that there are workgroups for every CU
   const int64_t want = ceil_div(kManyRows, rows);
@@ -153,10 +159,15 @@ Cut cut_rows(int64_t rows, int64_t vocab, int dtype) {
   const int64_t len = ceil_div(ceil_div(vocab, s), chunk) * chunk;
   return Cut{(int)ceil_div(vocab, len), (int)len};
 }
+// most segments of a row, wherever its rows begin
+int64_t most_segments(int64_t rows, int64_t vocab, int dtype) {
+  const int a = cut_rows(rows, vocab, dtype, true).segments, b = cut_rows(rows, vocab, dtype, false).segments;
+  return a > b ? a : b;
+}
 int64_t scores_parts_bytes(int64_t rows, const Cut& c) { return c.segments > 1 ? rows * c.segments * 16 : 0; }
 int64_t scores_workspace(int64_t rows, int64_t vocab, int top_k, int dtype) {
-  const Cut c = cut_rows(rows, vocab, dtype);
-  return c.segments > 1 ? scores_parts_bytes(rows, c) + round16(rows * c.segments * top_k * 8) : 0;
+  const int64_t s = most_segments(rows, vocab, dtype);
+  return s > 1 ? rows * s * 16 + round16(rows * s * top_k * 8) : 0;
 }
 
 // The workgroup that makes a row's loss and gradient: the fewest threads that hold
@@ -164,11 +175,12 @@ int64_t scores_workspace(int64_t rows, int64_t vocab, int top_k, int dtype) {
 struct RowShape {
   int threads, segments, len;
 };
-RowShape row_shape(int64_t vocab, int dtype) {
-  const int64_t chunk = dtype == MEC_DTYPE_F32 ? 4 : 8;
+RowShape row_shape(int64_t vocab, int dtype, bool aligned) {
+  const int64_t vec = dtype == MEC_DTYPE_F32 ? 4 : 8;
   for (int threads = 256; threads <= 1024; threads *= 2)
-    if (vocab <= chunk * kSegChunks * threads) return RowShape{threads, 1, (int)vocab};
-  const int64_t len = chunk * kSegChunks * 1024;
+    if (vocab + (aligned ? 0 : 1) <= vec * kSegChunks * threads) return RowShape{threads, 1, (int)vocab};
+  // (the first segment may begin off a boundary, and end up to a vector later for it)
+  const int64_t len = vec * kSegChunks * 1024 - (aligned ? 0 : vec);
   return RowShape{1024, (int)ceil_div(vocab, len), (int)len};
 }
 
@@ -187,7 +199,7 @@ DistillWorkspace distill_workspace(int64_t rows, int64_t vocab, int dtype, bool 
   w.some = take(rows * 4);
   w.counts = take(kTeacherGroups * 4);
   w.row_loss = take(rows * 4);
-  w.parts = take(with_grad ? 0 : rows * cut_rows(rows, vocab, dtype).segments * 8);
+  w.parts = take(with_grad ? 0 : rows * most_segments(rows, vocab, dtype) * 8);
   w.total = at;
   return w;
 }
@@ -277,7 +289,7 @@ int mec_token_scores(const void* logits, int64_t rows, int64_t inner, int64_t ou
     using T = std::remove_pointer_t<decltype(t)>;
     const T* p = (const T*)logits;
     const Tokens tok{tokens, token_bytes == 8};
-    const Cut cut = cut_rows(rows, vocab, dtype);
+    const Cut cut = cut_rows(rows, vocab, dtype, x.aligned());
     float4* parts = (float4*)workspace;
     uint64_t* part_top = (uint64_t*)((char*)workspace + scores_parts_bytes(rows, cut));
     const ScoresOut out{log_probs, entropy, top_tokens, top_log_probs, state};
@@ -312,7 +324,7 @@ int mec_token_scores_backward(const void* logits, int64_t rows, int64_t inner, i
   if (rc) return rc;
   with_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const Cut cut = cut_rows(kManyRows, vocab, dtype);
+    const Cut cut = cut_rows(kManyRows, vocab, dtype, x.aligned());
     with_past(rows * vocab * sizeof(T), [&](auto past) {
       k_scores_grad<T, decltype(past)::value><<<cut.dims(rows), kRowThreads, 0, (hipStream_t)stream>>>(
           (const T*)logits, x.map(), (int)vocab, Tokens{tokens, token_bytes == 8}, ignore_index, 1.f / temperature,
@@ -363,7 +375,7 @@ int mec_distill_forward(const void* logits, int64_t rows, int64_t inner, int64_t
     const T* p = (const T*)logits;
     const int n = (int)vocab;
     if (grad_logits) {
-      const RowShape shape = row_shape(vocab, dtype);
+      const RowShape shape = row_shape(vocab, dtype, x.aligned());
       auto run = [&](auto threads, auto one) {
         constexpr int THREADS = decltype(threads)::value;
         with_past(rows * vocab * sizeof(T), [&](auto past) {
@@ -382,7 +394,7 @@ int mec_distill_forward(const void* logits, int64_t rows, int64_t inner, int64_t
         run(std::integral_constant<int, 1024>{}, std::true_type{});
       return;
     }
-    const Cut cut = cut_rows(rows, vocab, dtype);
+    const Cut cut = cut_rows(rows, vocab, dtype, x.aligned());
     float2* parts = (float2*)(ws + w.parts);
     k_distill_sums<T><<<cut.dims(rows), kRowThreads, 0, st>>>(p, x.map(), n, inv_t, have.some, rows, cut.grid(rows),
                                                               parts);
@@ -414,7 +426,7 @@ int mec_distill_backward(const void* logits, int64_t rows, int64_t inner, int64_
   const int* count = reduction == MEC_REDUCE_MEAN ? (const int*)(state + 2 * rows) : nullptr;
   with_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const Cut cut = cut_rows(kManyRows, vocab, dtype);
+    const Cut cut = cut_rows(kManyRows, vocab, dtype, x.aligned());
     const int64_t items = rows * cut.segments;
     // (made: few workgroups are enough to find that grad_output is 1)
     const int64_t most = made ? 2048 : int64_t(1) << 22;

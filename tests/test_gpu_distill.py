@@ -224,6 +224,21 @@ def test_layouts_and_teacher_types(tz):
         check(base[..., off:off + 990], tok % 990, z, leaf=leaf)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("vocab", [8191, 8192, 16384, 16385, 32768, 65535, 65536, 65537, 131071, 131072, 131073])
+def test_full_segments_at_odd_addresses(dtype, vocab):
+    g = torch.Generator().manual_seed(16)
+    base = torch.randn(3 * (vocab + 1) + 8, generator=g).to(dtype)
+    dev = base.to(DEV)
+    tok = torch.randint(0, vocab, (3, 7), generator=g)
+    tok[0, :2] = torch.tensor([0, vocab - 1])
+    z = torch.randn(3, 7, generator=g)
+    for off, ld in ((0, vocab), (1, vocab), (1, vocab + 1), (3, vocab + 1)):
+        for go in (1.0, 2.0):
+            check(base.as_strided((3, vocab), (ld, 1), off), tok, z, grad_output=go,
+                  leaf=dev.as_strided((3, vocab), (ld, 1), off))
+
+
 def test_many_rows_and_repeats_bit_for_bit():
     x, tok, z = make(2000, 777, 9, torch.bfloat16, seed=11)
     tok[::3] = -1

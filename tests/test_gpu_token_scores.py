@@ -203,6 +203,24 @@ def test_every_alignment(dtype):
             check(x, torch.tensor([0, vocab - 1, 17]), 9, gpu_logits=dev.as_strided((3, vocab), (ld, 1), off))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("vocab", [2047, 2048, 2049, 16383, 16384, 16385, 32767, 32768, 65535, 65536, 65537, 131072])
+def test_full_segments_at_odd_addresses(dtype, vocab):
+    """Rows that fill their segments and begin off the boundaries of the vectors."""
+    g = torch.Generator().manual_seed(15)
+    base = torch.randn(3 * (vocab + 1) + 8, generator=g).to(dtype)
+    dev = base.to(DEV)
+    tok = torch.tensor([0, vocab - 1, vocab // 2])
+    gl, gh = torch.ones(3), torch.ones(3)
+    for off, ld in ((0, vocab), (1, vocab), (1, vocab + 1), (3, vocab + 1)):
+        x = base.as_strided((3, vocab), (ld, 1), off)
+        leaf = dev.as_strided((3, vocab), (ld, 1), off)
+        check(x, tok, 6, gpu_logits=leaf)
+        want = ref.token_scores_grad(x, tok, gl, gh)
+        ref.assert_close("dx", gradient(x, tok, gl, gh, leaf=leaf), want, dtype,
+                         ref.score_tolerance(x, 1.0) * (2 + ref.spread(x, 1.0)))
+
+
 def test_tokens_outside_the_vocabulary():
     x, tok, _ = make(5, 70, torch.float32)
     tok[1], tok[2], tok[3] = 70, -1, -100
