@@ -30,7 +30,9 @@ constexpr int kEmbedThreads = 256;
 constexpr int kEmbedTokens = 4;  // rows in flight per lane group
 
 // A group of 2^lg lanes takes a token's row, kEmbedTokens rows at a time.  A
-// token outside [0, vocab) gives a row of NaN.
+// token outside [0, vocab) gives a row of NaN.  Bound by memory: 524288 rows of 1024
+// bf16 in 300 us (1.07 GB written; as much gathered, about a quarter of it from
+// memory), 78848 rows of 768 in 37 us.
 template <class T, bool PAST>
 __global__ __launch_bounds__(kEmbedThreads) void k_embed(Tokens tokens, int64_t n, const T* weight, int64_t ldw,
                                                          int64_t vocab, int d, int lg, float scale, T* out) {
@@ -76,7 +78,8 @@ __global__ __launch_bounds__(kEmbedThreads) void k_embed(Tokens tokens, int64_t 
 // digit find each other with ballots, and the first of them moves the wave's own
 // counter of that digit.  A pass is two launches (tile counts, scatter; a third
 // between them for more than 128 tiles); up to kSortOne pairs are sorted by one
-// workgroup in one launch.
+// workgroup in one launch.  Two passes over 78848 pairs take 28 us, over 524288 48 us,
+// over 5003 (one launch) 17 us: waiting, not moving, 16 bytes a pair and pass.
 
 constexpr int kSortThreads = 512, kSortWaves = kSortThreads / 64;
 constexpr int kSortBins = 512;
@@ -395,7 +398,9 @@ struct Runs {
 // One workgroup of 8 waves per block of 256 positions, each wave a piece:
 // piece_sums[piece] for a piece of one token, block_sums[block] if the whole
 // block is of one (then no piece_sums).  The first column's workgroups also note
-// where the runs begin and end.
+// where the runs begin and end.  Small pieces, so that a few frequent tokens are
+// spread over all CUs: 524288 tokens, 1024 bf16 features 115 us, 78848 tokens, 768
+// features 16 us (pieces of 64 in blocks of 1024: 190 and 46).
 template <class T>
 __global__ __launch_bounds__(kBlockPieces * 64) void k_embed_pieces(Runs runs, const T* dy, int64_t lddy, int d,
                                                                     float* piece_sums, float* block_sums) {
@@ -447,6 +452,8 @@ __global__ __launch_bounds__(kBlockPieces * 64) void k_embed_pieces(Runs runs, c
 constexpr int kWaveRows = 4, kDwRows = 4 * kWaveRows;  // vocabulary rows per wave, per workgroup
 constexpr int kShortRun = 16;  // a wave's work alone; longer ones would be the launch's last
 
+// Bound by memory and, for few tokens, by the latency of positions, then rows of dy:
+// dW of 131072 x 1024 bf16 in 144 us, of 49408 x 768 in 32 us, of 32001 x 641 fp32 in 18.
 // Every row of dW, four to a wave: the positions of their runs of up to 16 are
 // one list, whose rows of dy are loaded one after another across the ends of the
 // runs.  Longer runs are summed by the workgroup's 4 waves together, with the

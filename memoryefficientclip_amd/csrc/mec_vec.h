@@ -79,6 +79,7 @@ template <class T>
 __device__ __forceinline__ void load_row(const T* p, int n, float (&v)[Vec<T>::N]) {
   Vec<T>::unpack(load_raw(p, n), v);
 }
+
 // Outputs that pass half of the last-level cache (256 MB) are stored past it: there
 // they would only push out what is read next, and their lines hold up the kernel
 // that follows while they are written back.  Smaller ones stay for their reader.

@@ -334,19 +334,18 @@ struct Segment {
   }
 };
 
-// Of the keys that the lanes hold through key(i), i < per_lane: the largest
-// number (its lowest `low` bits 0) that at least k keys reach, or a smaller one
-// that no more than `enough` reach.
-template <class K, class F>
-__device__ __forceinline__ K kth_largest(int per_lane, int low, int k, int enough, F key) {
-  K cut = 0;
-  for (int bit = sizeof(K) * 8 - 1; bit >= low; --bit) {
-    const K trial = cut | ((K)1 << bit);
+// Of the keys that the wave's lanes hold through key(i), i < per_lane, all
+// different: a number that exactly k of them reach.
+template <class F>
+__device__ __forceinline__ uint64_t kth_largest(int per_lane, int k, F key) {
+  uint64_t cut = 0;
+  for (int bit = 63; bit >= 0; --bit) {
+    const uint64_t trial = cut | (1ull << bit);
     int reach = 0;
     for (int i = 0; i < per_lane; ++i) reach += __popcll(__ballot(key(i) >= trial));
     if (reach >= k) {
       cut = trial;
-      if (reach <= enough) break;
+      if (reach == k) break;
     }
   }
   return cut;
@@ -478,9 +477,15 @@ __device__ __forceinline__ void write_ignored(const ScoresOut& out, int64_t r, i
   for (int j = tid; j < k; j += threads) out.top_tokens[r * k + j] = -1, out.top_log_probs[r * k + j] = 0.f;
 }
 
-// One workgroup per segment of a row.
-// With one segment the row's results, else part[row][seg] = (m, S, U) and the
-// segment's top k keys.
+// One workgroup per segment of a row.  With one segment the row's results, else
+// parts[row][seg] = (m, S, U) and the segment's top k keys.
+//
+// Bound by the read and by the vector unit about alike: a value costs an unpack
+// twice (maximum, sums), half a maximum, three fma-like operations and an
+// exponential, which takes four times their cycles.  256 threads and 8 vectors each:
+// 51 to 67 registers, so that seven or eight workgroups share a CU and one's sums
+// hide the others' loads.  8192 x 49408 bf16 in 138 us (5.9 TB/s); with the 32 top
+// tokens, 4096 x 131072 bf16, a tenth of them ignored, 190 us (5.1 TB/s).
 template <class T, bool TOP>
 __global__ __launch_bounds__(kRowThreads) void k_scores(const T* logits, RowMap map, int n, Tokens tokens,
                                                         int64_t ignore, float inv_t, int k, ScoresOut out,
@@ -595,6 +600,8 @@ constexpr int kJoinRank = 256;  // above it, a search for the k-th key is shorte
 
 // One workgroup per row: its segments' sums, a lane of the first wave each, and
 // the k largest of their top keys (all different: exactly k reach the k-th).
+// Bound by the latency of four dependent reads: 4096 rows of 8 lists of 32 keys
+// 11 us, one row of 64 lists of 20 keys 7 us (all keys ranked: 99 us).
 template <class T>
 __global__ __launch_bounds__(kJoinThreads) void k_scores_join(const T* logits, RowMap map, int n, Tokens tokens,
                                                               int64_t ignore, float inv_t, int k, ScoresOut out,
@@ -666,8 +673,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_scores_join(const T* logits, R
   if (have > kJoinRank) {
     // the k-th key itself, and the keys from it on to the front, by the first wave
     if (tid < 64) {
-      cut = kth_largest<uint64_t>((have + 63) / 64, 0, k, k,
-                                  [&](int i) { return i * 64 + lane < have ? found[i * 64 + lane] : 0; });
+      cut = kth_largest((have + 63) / 64, k, [&](int i) { return i * 64 + lane < have ? found[i * 64 + lane] : 0; });
       int at = 0;
       for (int i0 = 0; i0 < have; i0 += 64) {
         const uint64_t key = i0 + lane < have ? found[i0 + lane] : 0;
@@ -690,9 +696,12 @@ __global__ __launch_bounds__(kJoinThreads) void k_scores_join(const T* logits, R
   }
 }
 
-// dx_v = (1/T) (g_l (1[v = tok] - p_v) - g_h p_v (log p_v + entropy)).
-// One workgroup per segment of a row.  A vector that would pass the end
-// is the last one that does not: two threads then store the same values.
+// dx_v = (1/T) (g_l (1[v = tok] - p_v) - g_h p_v (log p_v + entropy)), which is
+// 2^t (a + b t) but for the token's own term.  One workgroup per segment of a row; a
+// vector that is moved into the segment (Segment::begin) stores values that another
+// thread stores as well, the same ones.  Bound by memory: 8192 x 49408 bf16, a quarter
+// of the rows ignored, 245 us for 0.61 GB read and 0.81 GB written (5.8 TB/s, some of
+// the reads from the cache).
 template <class T, bool PAST>
 __global__ __launch_bounds__(kRowThreads) void k_scores_grad(const T* logits, RowMap map, int n, Tokens tokens,
                                                              int64_t ignore, float inv_t, const float* stats,
@@ -789,7 +798,8 @@ __global__ __launch_bounds__(kTeacherThreads) void k_teacher_rows(Teacher t, int
   __shared__ int count;
   const int tid = threadIdx.x;
   if (tid == 0) count = 0;
-  const int64_t first = (int64_t)blockIdx.x * out.rows_each, end = first + out.rows_each < rows ? first + out.rows_each : rows;
+  const int64_t first = (int64_t)blockIdx.x * out.rows_each;
+  const int64_t end = first + out.rows_each < rows ? first + out.rows_each : rows;
   for (int64_t r0 = first; r0 < end; r0 += kTeacherRows) {
     const int n = end - r0 < kTeacherRows ? (int)(end - r0) : kTeacherRows;
     if (tid < kTeacherRows) has[tid] = 0;
@@ -877,10 +887,13 @@ struct DistillState {
 };
 
 // Loss and gradient (for grad_output 1) of a row by one workgroup.  With ONE the
-// row is one segment and stays in registers from its only read to the
-// gradient's write.  Of a longer row the last segment stays in registers and
-// the one before it in LDS (128 KB: up to 131072 16-bit logits are read once);
-// what is left is read a second time.
+// row is one segment and stays in registers from its only read to the gradient's
+// write.  Of a longer row the last segment stays in registers and the one before
+// it in LDS (128 KB: up to 131072 16-bit logits are read once); what is left is
+// read a second time.  Bound by memory: two workgroups of 1024 threads share a CU
+// with ONE, so that one reads while the other writes (8192 x 49408 bf16, a quarter
+// without a teacher: 288 us, 4.9 TB/s); a longer row has the CU to itself (4096 x
+// 200000 bf16: 750 us, 4.4 TB/s of what has to move, a third of the reads twice).
 template <class T, int THREADS, bool ONE, bool PAST>
 __global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap map, int n, Teacher teacher,
                                                          float inv_t, float scale, TeacherRows have, int mean,
@@ -1002,7 +1015,8 @@ __global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap
   row.subtract(x, y, 0, n, ref, gs, g);
 }
 
-// m and S of a segment.
+// m and S of a segment: the loss without its gradient (1003 x 32001 fp16 14 us,
+// 4096 x 200000 bf16 320 us, 5.1 TB/s).
 template <class T>
 __global__ __launch_bounds__(kRowThreads) void k_distill_sums(const T* logits, RowMap map, int n, float inv_t,
                                                               const int* some, int64_t rows, SegmentGrid grid,
@@ -1073,8 +1087,10 @@ __global__ __launch_bounds__(64) void k_distill_join(const T* logits, RowMap map
   }
 }
 
-// dx from the rows' m and S.  grad_output: one number, or one for each row.  With `made` dx holds the gradient for grad_output 1, and only
-// another one makes it anew (few workgroups then, each for many segments).
+// dx from the rows' m and S.  grad_output: one number, or one for each row.  With
+// `made` dx holds the gradient for grad_output 1, and only another one makes it anew
+// (few workgroups then, each for many segments).
+// Bound by memory: 1003 x 32001 fp16 21 us.
 template <class T, bool PAST>
 __global__ __launch_bounds__(kRowThreads) void k_distill_grad(const T* logits, RowMap map, int n, Teacher teacher,
                                                               float inv_t, float scale, const int* count,

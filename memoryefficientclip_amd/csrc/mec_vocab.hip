@@ -62,7 +62,8 @@ struct Logits {
   const void* p;
   int64_t rows, inner, outer_stride, inner_stride, vocab;
   int dtype;
-  RowMap map() const { return RowMap{inner, outer_stride, inner_stride}; }
+  // (an inner beyond the rows means the same as all of them, and fits the kernels' 32 bits)
+  RowMap map() const { return RowMap{inner < rows ? inner : rows, outer_stride, inner_stride}; }
   // every row begins on a 4-byte boundary
   bool aligned() const {
     return dtype == MEC_DTYPE_F32 ||
@@ -242,8 +243,9 @@ Runs sort_tokens(const void* tokens, int token_bytes, int64_t n, int64_t vocab, 
   const SortOut last{nullptr, (int*)(ws + w.keys), (int*)(ws + w.positions)};
   int2* bounds = (int2*)(ws + w.bounds);
   if (n <= kSortOne) {
-    const unsigned clears = (unsigned)ceil_div(vocab, 4 * kSortOneThreads);
-    k_sort_one<<<1 + (clears < 256 ? clears : 256), kSortOneThreads, 0, st>>>(tok, s, passes, bits, even, odd, last, bounds);
+    const int64_t clears = ceil_div(vocab, 4 * kSortOneThreads);
+    const unsigned groups = 1 + (unsigned)(clears < 256 ? clears : 256);
+    k_sort_one<<<groups, kSortOneThreads, 0, st>>>(tok, s, passes, bits, even, odd, last, bounds);
   } else {
     s.tiles = (int)ceil_div(n, (int64_t)kSortThreads * s.items);
     int* counts = (int*)(ws + w.counts);
@@ -296,8 +298,8 @@ int mec_token_scores(const void* logits, int64_t rows, int64_t inner, int64_t ou
     const dim3 grid = cut.dims(rows);
     const float inv_t = 1.f / temperature;
     if (top_k > 0)
-      k_scores<T, true><<<grid, kRowThreads, 0, st>>>(p, x.map(), (int)vocab, tok, ignore_index, inv_t, top_k, out, rows,
-                                                      cut.grid(rows), parts, part_top);
+      k_scores<T, true><<<grid, kRowThreads, 0, st>>>(p, x.map(), (int)vocab, tok, ignore_index, inv_t, top_k, out,
+                                                      rows, cut.grid(rows), parts, part_top);
     else
       k_scores<T, false><<<grid, kRowThreads, 0, st>>>(p, x.map(), (int)vocab, tok, ignore_index, inv_t, 0, out, rows,
                                                        cut.grid(rows), parts, part_top);

@@ -117,7 +117,7 @@ class TopKDistillationLoss(nn.Module):
         if teacher_tokens.shape != teacher_logits.shape:
             raise ValueError(f"teacher_tokens {tuple(teacher_tokens.shape)} and teacher_logits "
                              f"{tuple(teacher_logits.shape)} differ in shape")
-        if student_logits.dim() < 1 or teacher_tokens.dim() < 1 or student_logits.shape[:-1] != teacher_tokens.shape[:-1]:
+        if min(student_logits.dim(), teacher_tokens.dim()) < 1 or student_logits.shape[:-1] != teacher_tokens.shape[:-1]:
             raise ValueError(f"student_logits {tuple(student_logits.shape)} and teacher_tokens "
                              f"{tuple(teacher_tokens.shape)} need the same positions")
         vocab, k = student_logits.shape[-1], teacher_tokens.shape[-1]

@@ -119,9 +119,8 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, 
     temperature = _v.check_temperature(temperature)
     if tokens.numel() == 0:
         zero = logits.sum(-1, dtype=torch.float32)  # (no element: the graph's link to the logits)
-        return TokenScores(zero, zero.clone(),
-                           torch.empty((*tokens.shape, top_k), dtype=torch.int64, device=logits.device) if top_k else None,
-                           zero.detach()[..., None].expand(*tokens.shape, top_k) if top_k else None)
+        none = torch.empty((*tokens.shape, top_k), dtype=torch.int64, device=logits.device)
+        return TokenScores(zero, zero.clone(), none if top_k else None, none.float() if top_k else None)
     if logits.requires_grad and torch.is_grad_enabled():
         return TokenScores(*_TokenScoresFn.apply(logits, tokens, top_k, temperature, int(ignore_index)))
     return TokenScores(*_scores(logits, tokens, top_k, temperature, int(ignore_index), False)[0])

@@ -324,6 +324,22 @@ def test_gradient_layouts():
         ref.assert_close("dx", leaf.grad, full, torch.bfloat16, 1e-5)
 
 
+def test_c_abi_row_map():
+    """Rows on two strides through the C ABI; an `inner` beyond the rows is one stride."""
+    from memoryefficientclip_amd import _lib
+    x, tok, _ = make(6, 700, torch.float32, seed=17)
+    flat, tg = x.to(DEV), tok.to(DEV)
+    lp, _, _, _ = ref.token_scores(x, tok, 0)
+    st = torch.cuda.current_stream().cuda_stream
+    ws = torch.empty(_lib.load().mec_token_scores_workspace_bytes(6, 700, 0, _lib.DTYPE_F32), dtype=torch.uint8,
+                     device=DEV)
+    for inner, outer, step in ((1, 700, 0), (2, 1400, 700), (6, 0, 700), (1 << 32, 12345, 700), (7, 1, 700)):
+        out, h = torch.empty(6, device=DEV), torch.empty(6, device=DEV)
+        _lib.call("mec_token_scores", flat.data_ptr(), 6, inner, outer, step, 700, _lib.DTYPE_F32, tg.data_ptr(), 8, -100,
+                  1.0, 0, out.data_ptr(), h.data_ptr(), None, None, None, ws.data_ptr(), ws.numel(), st)
+        ref.assert_close("log_probs", out, lp, torch.float32, ref.score_tolerance(x, 1.0))
+
+
 def test_results_repeat_bit_for_bit():
     x, tok, _ = make(70, 50001, torch.bfloat16, seed=12)
     x, tok = x.to(DEV), tok.to(DEV)
