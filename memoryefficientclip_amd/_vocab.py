@@ -5,6 +5,8 @@ from __future__ import annotations
 
 import torch
 
+from torch.autograd.function import once_differentiable
+
 from . import _function as _f
 from . import _lib
 
@@ -69,6 +71,21 @@ def rows_of(logits: torch.Tensor) -> tuple[torch.Tensor, int, tuple[int, int, in
         return logits, logits.data_ptr(), (merged[0][0], 1, merged[0][1], 0)
     (n0, s0), (n1, s1) = merged
     return logits, logits.data_ptr(), (n0 * n1, n1, s0, s1)
+
+
+def backward_of(grad):
+    """``Function.backward`` from `grad(ctx, *grad_outputs)`, which is differentiable once.
+
+    The wrapper that says so costs as much as the rest of a small backward (autograd
+    runs it on a thread of its own, where Python code is several times slower than
+    on the caller's), so it is taken only where a second derivative could be asked
+    for: under ``create_graph``."""
+    guarded = once_differentiable(grad)
+
+    def backward(ctx, *grad_outputs):
+        return guarded(ctx, *grad_outputs) if torch.is_grad_enabled() else grad(ctx, *grad_outputs)
+
+    return staticmethod(backward)
 
 
 def launch(index: int, nbytes: int, call) -> int:

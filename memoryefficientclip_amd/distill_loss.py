@@ -14,7 +14,6 @@ import math
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from . import _vocab as _v
@@ -49,6 +48,25 @@ def _loss(logits, teacher_tokens, teacher_logits, temperature, weight, reduction
     return loss, kept
 
 
+def _logits_grad(ctx, grad_output):
+    held, teacher_tokens, teacher_logits, state = ctx.saved_tensors
+    rows, vocab, code, token_bytes, teacher_code, k, temperature, weight, reduction, shape = ctx.mec
+    go = grad_output.contiguous()
+    # (handed out once: its new owner may change it)
+    dx, ctx.made = ctx.made, None
+    made = dx is not None
+    if not made:
+        dx = held.new_empty(shape)
+    lib = _lib.load()
+    rc = _v.launch(held.device.index, 0, lambda ws, stream: lib.mec_distill_backward(
+        held.data_ptr(), *rows, vocab, code, teacher_tokens.data_ptr(), token_bytes, teacher_logits.data_ptr(),
+        teacher_code, k, temperature, weight, reduction, state.data_ptr(), go.data_ptr(), int(made), dx.data_ptr(),
+        stream))
+    if rc:
+        raise _lib.error("mec_distill_backward", rc)
+    return dx, None, None, None, None, None
+
+
 class _DistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher_tokens, teacher_logits, temperature, weight, reduction):
@@ -57,26 +75,7 @@ class _DistillFn(torch.autograd.Function):
         ctx.mec, ctx.made = kept[4:]
         return loss
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_output):
-        _v.refuse_graph_capture()
-        held, teacher_tokens, teacher_logits, state = ctx.saved_tensors
-        rows, vocab, code, token_bytes, teacher_code, k, temperature, weight, reduction, shape = ctx.mec
-        go = grad_output.to(torch.float32).contiguous()
-        # (handed out once: its new owner may change it)
-        dx, ctx.made = ctx.made, None
-        made = dx is not None
-        if not made:
-            dx = torch.empty(shape, dtype=held.dtype, device=held.device)
-        lib = _lib.load()
-        rc = _v.launch(held.device.index, 0, lambda ws, stream: lib.mec_distill_backward(
-            held.data_ptr(), *rows, vocab, code, teacher_tokens.data_ptr(), token_bytes, teacher_logits.data_ptr(),
-            teacher_code, k, temperature, weight, reduction, state.data_ptr(), go.data_ptr(), int(made), dx.data_ptr(),
-            stream))
-        if rc:
-            raise _lib.error("mec_distill_backward", rc)
-        return dx, None, None, None, None, None
+    backward = _v.backward_of(_logits_grad)
 
 
 class TopKDistillationLoss(nn.Module):

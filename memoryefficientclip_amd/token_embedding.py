@@ -10,7 +10,6 @@ import math
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import _function as _f
 from . import _lib
@@ -32,30 +31,31 @@ def _lookup(tokens, weight, scale):
     return out
 
 
+def _weight_grad(ctx, grad_output):
+    tokens, = ctx.saved_tensors
+    vocab, d, n, code, index, scale, padding_idx, nbytes = ctx.mec
+    dy, ldg = (grad_output, d) if grad_output.is_contiguous() else _f._rows(grad_output.reshape(-1, d))
+    dw = dy.new_empty((vocab, d))
+    lib = _lib.load()
+    rc = _v.launch(index, nbytes, lambda ws, stream: lib.mec_embedding_backward(
+        tokens.data_ptr(), tokens.element_size(), n, dy.data_ptr(), ldg, vocab, d, code, scale, padding_idx,
+        dw.data_ptr(), ws, nbytes, stream))
+    if rc:
+        raise _lib.error("mec_embedding_backward", rc)
+    return None, dw, None, None
+
+
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, weight, scale, padding_idx):
+        out = _lookup(tokens, weight, scale)
         ctx.save_for_backward(tokens)
-        ctx.mec = (weight.shape, scale, padding_idx)
-        return _lookup(tokens, weight, scale)
+        (vocab, d), n, code = weight.shape, tokens.numel(), _v.code_of(weight)
+        ctx.mec = (vocab, d, n, code, weight.device.index, scale, padding_idx,
+                   _lib.load().mec_embedding_workspace_bytes(n, vocab, d, code))
+        return out
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_output):
-        _v.refuse_graph_capture()
-        tokens, = ctx.saved_tensors
-        (vocab, d), scale, padding_idx = ctx.mec
-        dy, ldg = _f._rows(grad_output.reshape(-1, d))
-        dw = torch.empty((vocab, d), dtype=dy.dtype, device=dy.device)
-        n, code = tokens.numel(), _v.code_of(dy)
-        lib = _lib.load()
-        nbytes = lib.mec_embedding_workspace_bytes(n, vocab, d, code)
-        rc = _v.launch(dy.device.index, nbytes, lambda ws, stream: lib.mec_embedding_backward(
-            tokens.data_ptr(), tokens.element_size(), n, dy.data_ptr(), ldg, vocab, d, code, scale, padding_idx,
-            dw.data_ptr(), ws, nbytes, stream))
-        if rc:
-            raise _lib.error("mec_embedding_backward", rc)
-        return None, dw, None, None
+    backward = _v.backward_of(_weight_grad)
 
 
 def scaled_embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,

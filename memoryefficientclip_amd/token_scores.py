@@ -14,7 +14,6 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from . import _vocab as _v
@@ -54,6 +53,24 @@ def _scores(logits, tokens, top_k, temperature, ignore_index, keep):
     return (log_probs, entropy, top_tokens, top_log_probs), kept
 
 
+def _logits_grad(ctx, g_log_probs, g_entropy, _g_tokens, _g_top):
+    if g_log_probs is None and g_entropy is None:
+        return None, None, None, None, None
+    held, tokens, entropy, state = ctx.saved_tensors
+    rows, vocab, code, token_bytes, ignore_index, temperature, shape = ctx.mec
+    gl = None if g_log_probs is None else g_log_probs.contiguous()
+    gh = None if g_entropy is None else g_entropy.contiguous()
+    dx = held.new_empty(shape)
+    lib = _lib.load()
+    rc = _v.launch(held.device.index, 0, lambda ws, stream: lib.mec_token_scores_backward(
+        held.data_ptr(), *rows, vocab, code, tokens.data_ptr(), token_bytes, ignore_index, temperature,
+        state.data_ptr(), entropy.data_ptr(), None if gl is None else gl.data_ptr(),
+        None if gh is None else gh.data_ptr(), dx.data_ptr(), stream))
+    if rc:
+        raise _lib.error("mec_token_scores_backward", rc)
+    return dx, None, None, None, None
+
+
 class _TokenScoresFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top_k, temperature, ignore_index):
@@ -65,25 +82,7 @@ class _TokenScoresFn(torch.autograd.Function):
         ctx.mec = kept[4]
         return out
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_log_probs, g_entropy, _g_tokens, _g_top):
-        if not ctx.needs_input_grad[0] or (g_log_probs is None and g_entropy is None):
-            return None, None, None, None, None
-        _v.refuse_graph_capture()
-        held, tokens, entropy, state = ctx.saved_tensors
-        rows, vocab, code, token_bytes, ignore_index, temperature, shape = ctx.mec
-        gl = None if g_log_probs is None else g_log_probs.to(torch.float32).contiguous()
-        gh = None if g_entropy is None else g_entropy.to(torch.float32).contiguous()
-        dx = torch.empty(shape, dtype=held.dtype, device=held.device)
-        lib = _lib.load()
-        rc = _v.launch(held.device.index, 0, lambda ws, stream: lib.mec_token_scores_backward(
-            held.data_ptr(), *rows, vocab, code, tokens.data_ptr(), token_bytes, ignore_index, temperature,
-            state.data_ptr(), entropy.data_ptr(), None if gl is None else gl.data_ptr(),
-            None if gh is None else gh.data_ptr(), dx.data_ptr(), stream))
-        if rc:
-            raise _lib.error("mec_token_scores_backward", rc)
-        return dx, None, None, None, None
+    backward = _v.backward_of(_logits_grad)
 
 
 def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, temperature: float = 1.0,

@@ -60,7 +60,8 @@ def check(x, tok, z, temperature=1.0, weight=1.0, reduction="mean", grad_output=
 
 SIZES = [(1, 1, 1), (1, 2, 2), (3, 7, 3), (5, 63, 8), (4, 64, 64), (2, 65, 5), (7, 1000, 10), (2, 2048, 1),
          (3, 4097, 32), (2, 8192, 7), (2, 16385, 20), (3, 32001, 10), (2, 50001, 64), (2, 65536, 16), (1, 65544, 16),
-         (1, 131072, 128), (300, 517, 10), (2, 200003, 64), (3, 700, 700), (2, 5000, 1024), (1, 524288, 9)]
+         (1, 131072, 128), (300, 517, 10), (2, 200003, 64), (3, 700, 700), (2, 5000, 1024), (1, 524288, 9),
+         (2, 70000, 1024), (1, 140001, 700), (2, 300001, 33)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
@@ -237,6 +238,24 @@ def test_full_segments_at_odd_addresses(dtype, vocab):
         for go in (1.0, 2.0):
             check(base.as_strided((3, vocab), (ld, 1), off), tok, z, grad_output=go,
                   leaf=dev.as_strided((3, vocab), (ld, 1), off))
+
+
+def test_gradient_past_32_bits():
+    """A gradient of more than 2^32 elements (8.6 GB): all rows of the logits are one in memory."""
+    rows, vocab = 66001, 65600
+    x, tok, z = make(1, vocab, 5, torch.bfloat16, seed=18)
+    leaf = x.to(DEV).expand(rows, vocab).detach().requires_grad_(True)
+    tok_all, z_all = tok.to(DEV).repeat(rows, 1), z.to(DEV).repeat(rows, 1)
+    tok_all[-1], z_all[-2] = -1, 0.0
+    loss = mec.TopKDistillationLoss(reduction="sum")(leaf, tok_all, z_all)
+    dx, = torch.autograd.grad(loss, leaf)
+    one, _, grad = ref.distill(x, tok, z)
+    other, _, grad0 = ref.distill(x, tok, z * 0)
+    ref.assert_close("loss", loss, (one * (rows - 2) + other)[0], torch.float32, 2 * rows * ref.score_tolerance(x, 1.0))
+    for r in (0, 65471, 65472, rows - 3):   # 2^32 / vocab lies between
+        ref.assert_close("dx", dx[r], grad[0], torch.bfloat16, 2 * ref.score_tolerance(x, 1.0))
+    ref.assert_close("dx", dx[-2], grad0[0], torch.bfloat16, 2 * ref.score_tolerance(x, 1.0))
+    assert (dx[-1] == 0).all()
 
 
 def test_many_rows_and_repeats_bit_for_bit():

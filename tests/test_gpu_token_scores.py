@@ -245,6 +245,21 @@ def test_past_32_bits():
     ref.assert_close("dx", leaf.grad, want, torch.bfloat16, 1e-6)
 
 
+def test_gradient_past_32_bits():
+    """A gradient of more than 2^32 elements (8.6 GB): all rows of the logits are one in memory."""
+    rows, vocab = 66001, 65600
+    x, tok, _ = make(1, vocab, torch.bfloat16, seed=18)
+    leaf = x.to(DEV).expand(rows, vocab).detach().requires_grad_(True)
+    tok_all = tok.to(DEV).repeat(rows)
+    tok_all[-1] = -100
+    r = mec.token_log_probs(leaf, tok_all)
+    dx, = torch.autograd.grad(r.log_probs, leaf, torch.ones(rows, device=DEV))
+    want = ref.token_scores_grad(x, tok, torch.ones(1), torch.zeros(1))[0]
+    for row in (0, 65471, 65472, rows - 2):   # 2^32 / vocab lies between
+        ref.assert_close("dx", dx[row], want, torch.bfloat16, 2 * ref.score_tolerance(x, 1.0))
+    assert (dx[-1] == 0).all()
+
+
 def gradient(x, tok, gl, gh, temperature=1.0, leaf=None):
     leaf = x.to(DEV) if leaf is None else leaf
     leaf = leaf.detach().requires_grad_(True)
