@@ -294,8 +294,8 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(SortSource src, S
   chunk.scatter(shift, bits, mine, out);
 }
 
-// All passes by the first workgroup (n <= kSortOne, one tile); the others clear
-// the bounds.
+// All passes by the first workgroup (n <= kSortOne, one tile); the others, if
+// any, clear the bounds.
 __global__ __launch_bounds__(kSortOneThreads) void k_sort_one(Tokens tokens, SortShape s, int passes, int bits,
                                                            uint2* even, uint2* odd, SortOut last, int2* bounds) {
   __shared__ SortLds<kSortOneThreads> l;
@@ -392,7 +392,19 @@ struct Runs {
   const int* positions;
   int64_t n;
   int vocab;
-  int2* bounds;          // of each token's run: first and last + 1; 0, 0 for none
+  int2* bounds;          // of each token's run: first and last + 1; 0, 0 for none (null: to be searched for)
+  // First index whose key is >= v.
+  __device__ __forceinline__ int lower_bound(int v) const {
+    int lo = 0, hi = (int)n;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (keys[mid] < v)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    return lo;
+  }
 };
 
 // One workgroup of 8 waves per block of 256 positions, each wave a piece:
@@ -450,6 +462,10 @@ __global__ __launch_bounds__(kBlockPieces * 64) void k_embed_pieces(Runs runs, c
 }
 
 constexpr int kWaveRows = 4, kDwRows = 4 * kWaveRows;  // vocabulary rows per wave, per workgroup
+// Up to here there are no pieces, and the bounds of the runs are searched for: two
+// launches instead of three (a launch on autograd's thread takes longer than the
+// search; one token alone is 512 rows by four waves).
+constexpr int kDirect = 512;
 constexpr int kShortRun = 16;  // a wave's work alone; longer ones would be the launch's last
 
 // Bound by memory and, for few tokens, by the latency of positions, then rows of dy:
@@ -468,7 +484,14 @@ __global__ __launch_bounds__(256) void k_embed_rows(Runs runs, const T* dy, int6
   const int v0 = blockIdx.x * kDwRows;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int col = blockIdx.y * NC * 64 * N + lane * N;
-  const int2 bound = lane < kDwRows && v0 + lane < runs.vocab ? runs.bounds[v0 + lane] : make_int2(0, 0);
+  int2 bound = make_int2(0, 0);
+  if (runs.bounds) {
+    if (lane < kDwRows && v0 + lane < runs.vocab) bound = runs.bounds[v0 + lane];
+  } else {
+    const int v = v0 + (lane < kDwRows ? lane : kDwRows);
+    const int first = runs.lower_bound(v < runs.vocab ? v : runs.vocab), next = __shfl_down(first, 1, 64);
+    if (lane < kDwRows) bound = make_int2(first, next);
+  }
   RowSum<T, NC> sum(col, d);
   auto write = [&](int v) {
 #pragma unroll
@@ -531,15 +554,18 @@ __global__ __launch_bounds__(256) void k_embed_rows(Runs runs, const T* dy, int6
     const int64_t lo = __builtin_amdgcn_readlane(bound.x, q), hi = __builtin_amdgcn_readlane(bound.y, q);
     // [lo, a) positions, [a, a2) pieces, [a2, b2) blocks, [b2, b) pieces, [b, hi) positions
     int64_t a = (lo + kPiece - 1) / kPiece * kPiece, b = hi / kPiece * kPiece;
-    if (a > b) a = b = hi;
+    if (a > b || !runs.bounds) a = b = hi;
     int64_t a2 = (a + kBlock - 1) / kBlock * kBlock, b2 = b / kBlock * kBlock;
     if (a2 >= b2) a2 = b2 = b;
     sum.zero();
-    auto positions = [&](int64_t from, int64_t to) {  // fewer than a piece, a quarter for each wave
+    auto positions = [&](int64_t from, int64_t to) {  // a quarter for each wave
       const int count = (int)(to - from), each = (count + 3) / 4;
-      const int at = w * each < count ? w * each : count, mine = count - at < each ? count - at : each;
-      const int pos = lane < mine ? runs.positions[from + at + lane] : 0;
-      sum.template add<T, U>(dy, mine, [&](int i) { return (int64_t)__builtin_amdgcn_readlane(pos, i) * lddy; });
+      const int end = (w + 1) * each < count ? (w + 1) * each : count;
+      for (int at = w * each; at < end; at += 64) {
+        const int mine = end - at < 64 ? end - at : 64;
+        const int pos = lane < mine ? runs.positions[from + at + lane] : 0;
+        sum.template add<T, U>(dy, mine, [&](int i) { return (int64_t)__builtin_amdgcn_readlane(pos, i) * lddy; });
+      }
     };
     auto sums = [&](const float* s, int64_t from, int64_t to) {
       const int64_t count = to - from, each = (count + 3) / 4;

@@ -243,7 +243,8 @@ Runs sort_tokens(const void* tokens, int token_bytes, int64_t n, int64_t vocab, 
   const SortOut last{nullptr, (int*)(ws + w.keys), (int*)(ws + w.positions)};
   int2* bounds = (int2*)(ws + w.bounds);
   if (n <= kSortOne) {
-    const int64_t clears = ceil_div(vocab, 4 * kSortOneThreads);
+    if (n <= kDirect) bounds = nullptr;
+    const int64_t clears = bounds ? ceil_div(vocab, 4 * kSortOneThreads) : 0;
     const unsigned groups = 1 + (unsigned)(clears < 256 ? clears : 256);
     k_sort_one<<<groups, kSortOneThreads, 0, st>>>(tok, s, passes, bits, even, odd, last, bounds);
   } else {
@@ -494,8 +495,10 @@ int mec_embedding_backward(const void* tokens, int token_bytes, int64_t n, const
   with_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int N = Vec<T>::N;
-    k_embed_pieces<T><<<dim3((unsigned)ceil_div(n, kBlock), (unsigned)ceil_div(d, 64 * N)), kBlockPieces * 64, 0, st>>>(
-        runs, (const T*)grad_out, ldg, (int)d, pieces, blocks);
+    if (runs.bounds) {
+      const dim3 grid((unsigned)ceil_div(n, kBlock), (unsigned)ceil_div(d, 64 * N));
+      k_embed_pieces<T><<<grid, kBlockPieces * 64, 0, st>>>(runs, (const T*)grad_out, ldg, (int)d, pieces, blocks);
+    }
     const unsigned groups = (unsigned)ceil_div(vocab, kDwRows);
     auto rows = [&](auto nc) {
       constexpr int NC = decltype(nc)::value;

@@ -47,7 +47,8 @@ def check(tok, w, dy, scale=1.7, padding_idx=None, gpu_tokens=None, gpu_dy=None)
 
 SIZES = [(1, 1, 1), (1, 1000, 64), (2, 3, 7), (63, 10, 65), (64, 64, 128), (65, 5000, 8), (257, 300, 513),
          (1000, 100, 96), (1025, 2, 40), (4096, 9000, 48), (4097, 513, 33), (8193, 70000, 24), (20000, 1, 16),
-         (30000, 30000, 64), (3000, 300000, 8), (70000, 4000, 40), (300, 600, 2050), (5000, 20, 1536), (20000, 400000, 4), (9000, 1, 3)]
+         (30000, 30000, 64), (3000, 300000, 8), (70000, 4000, 40), (300, 600, 2050), (5000, 20, 1536),
+         (20000, 400000, 4), (9000, 1, 3), (511, 3, 40), (512, 1, 600), (513, 2, 1030), (512, 90, 136)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
