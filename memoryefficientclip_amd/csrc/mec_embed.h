@@ -294,8 +294,8 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(SortSource src, S
   chunk.scatter(shift, bits, mine, out);
 }
 
-// All passes by the first workgroup (n <= kSortOne, one tile); the others, if
-// any, clear the bounds.
+// All passes by the first workgroup (n <= kSortOne, one tile); the others clear
+// the bounds.
 __global__ __launch_bounds__(kSortOneThreads) void k_sort_one(Tokens tokens, SortShape s, int passes, int bits,
                                                            uint2* even, uint2* odd, SortOut last, int2* bounds) {
   __shared__ SortLds<kSortOneThreads> l;
@@ -392,19 +392,7 @@ struct Runs {
   const int* positions;
   int64_t n;
   int vocab;
-  int2* bounds;          // of each token's run: first and last + 1; 0, 0 for none (null: to be searched for)
-  // First index whose key is >= v.
-  __device__ __forceinline__ int lower_bound(int v) const {
-    int lo = 0, hi = (int)n;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (keys[mid] < v)
-        lo = mid + 1;
-      else
-        hi = mid;
-    }
-    return lo;
-  }
+  int2* bounds;          // of each token's run: first and last + 1; 0, 0 for none
 };
 
 // One workgroup of 8 waves per block of 256 positions, each wave a piece:
@@ -462,10 +450,64 @@ __global__ __launch_bounds__(kBlockPieces * 64) void k_embed_pieces(Runs runs, c
 }
 
 constexpr int kWaveRows = 4, kDwRows = 4 * kWaveRows;  // vocabulary rows per wave, per workgroup
-// Up to here there are no pieces, and the bounds of the runs are searched for: two
-// launches instead of three (a launch on autograd's thread takes longer than the
-// search; one token alone is 512 rows by four waves).
-constexpr int kDirect = 512;
+// Up to here nothing is sorted: every workgroup picks the positions of its own rows
+// out of all tokens.  One launch instead of three, and on autograd's thread a launch takes
+// longer than that (one token alone is 512 rows by four waves).
+constexpr int kFew = 512;
+
+// The positions of a workgroup's kDwRows rows among kFew tokens at most, in order.
+struct FewTokens {
+  Tokens tokens;
+  int64_t padding;
+};
+struct FewLds {
+  int positions[kFew];
+  int counts[4][kDwRows];
+};
+// Fills l.positions, and gives lane r < kDwRows of every wave the bounds of row r's.
+__device__ __forceinline__ int2 few_positions(const FewTokens& few, int n, int v0, int vocab, FewLds& l) {
+  constexpr int kPer = kFew / 256;  // tokens per lane
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  if (threadIdx.x < 4 * kDwRows) (&l.counts[0][0])[threadIdx.x] = 0;
+  __syncthreads();
+  int row[kPer], place[kPer];
+  uint64_t mask[kPer];
+#pragma unroll
+  for (int b = 0; b < kPer; ++b) {
+    const int i = w * (kFew / 4) + b * 64 + lane;
+    const int64_t tok = i < n ? few.tokens[i] : -1, r = tok - v0;
+    const bool mine = tok >= 0 && tok < vocab && tok != few.padding && r >= 0 && r < kDwRows;
+    row[b] = mine ? (int)r : -1;
+    mask[b] = same_digit(mine ? (uint32_t)r : 0u, 4, mine);
+    const int first = mine ? __ffsll((unsigned long long)mask[b]) - 1 : lane;
+    int old = 0;
+    if (mine && lane == first) old = atomicAdd(&l.counts[w][row[b]], __popcll(mask[b]));
+    place[b] = __shfl(old, first, 64) + __popcll(mask[b] & ((1ull << lane) - 1));
+  }
+  __syncthreads();
+  int total = 0, before = 0;
+  if (lane < kDwRows) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      total += l.counts[q][lane];
+      before += q < w ? l.counts[q][lane] : 0;
+    }
+  }
+  int end = total;
+  for (int i = 1; i < kDwRows; i <<= 1) {
+    const int o = __shfl_up(end, i, 64);
+    if (lane >= i) end += o;
+  }
+  const int begin = end - total;
+#pragma unroll
+  for (int b = 0; b < kPer; ++b) {
+    const int at = __shfl(begin + before, row[b] < 0 ? 0 : row[b], 64) + place[b];
+    if (row[b] >= 0) l.positions[at] = w * (kFew / 4) + b * 64 + lane;
+  }
+  __syncthreads();
+  return lane < kDwRows ? make_int2(begin, end) : make_int2(0, 0);
+}
+
 constexpr int kShortRun = 16;  // a wave's work alone; longer ones would be the launch's last
 
 // Bound by memory and, for few tokens, by the latency of positions, then rows of dy:
@@ -475,23 +517,23 @@ constexpr int kShortRun = 16;  // a wave's work alone; longer ones would be the 
 // runs.  Longer runs are summed by the workgroup's 4 waves together, with the
 // pieces' sums.
 template <class T, int NC, bool PAST>
-__global__ __launch_bounds__(256) void k_embed_rows(Runs runs, const T* dy, int64_t lddy, int d, float scale,
-                                                    const float* piece_sums, const float* block_sums, T* dw) {
+__global__ __launch_bounds__(256) void k_embed_rows(Runs runs, FewTokens few, const T* dy, int64_t lddy, int d,
+                                                    float scale, const float* piece_sums, const float* block_sums,
+                                                    T* dw) {
   constexpr int N = Vec<T>::N;
   constexpr int U = 8 / NC;      // rows of dy in flight
   constexpr int UF = U > 1 ? U / 2 : 1;  // rows of sums
   __shared__ float lds[3][NC * N * 64];
+  __shared__ FewLds few_lds;
   const int v0 = blockIdx.x * kDwRows;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int col = blockIdx.y * NC * 64 * N + lane * N;
   int2 bound = make_int2(0, 0);
-  if (runs.bounds) {
-    if (lane < kDwRows && v0 + lane < runs.vocab) bound = runs.bounds[v0 + lane];
-  } else {
-    const int v = v0 + (lane < kDwRows ? lane : kDwRows);
-    const int first = runs.lower_bound(v < runs.vocab ? v : runs.vocab), next = __shfl_down(first, 1, 64);
-    if (lane < kDwRows) bound = make_int2(first, next);
-  }
+  if (!runs.bounds)
+    bound = few_positions(few, (int)runs.n, v0, runs.vocab, few_lds);
+  else if (lane < kDwRows && v0 + lane < runs.vocab)
+    bound = runs.bounds[v0 + lane];
+  auto position = [&](int64_t i) { return runs.bounds ? runs.positions[i] : few_lds.positions[i]; };
   RowSum<T, NC> sum(col, d);
   auto write = [&](int v) {
 #pragma unroll
@@ -520,7 +562,7 @@ __global__ __launch_bounds__(256) void k_embed_rows(Runs runs, const T* dy, int6
     int at = begin[0];
 #pragma unroll
     for (int k = 1; k < kWaveRows; ++k) at = i >= end[k] ? begin[k] - end[k] : at;
-    const int pos = i < total ? runs.positions[at + i] : 0;
+    const int pos = i < total ? position(at + i) : 0;
     const int n = total - i0 < 64 ? total - i0 : 64;
     for (int j = 0; j < n; j += U) {
       typename Vec<T>::raw v[U][NC];
@@ -563,7 +605,7 @@ __global__ __launch_bounds__(256) void k_embed_rows(Runs runs, const T* dy, int6
       const int end = (w + 1) * each < count ? (w + 1) * each : count;
       for (int at = w * each; at < end; at += 64) {
         const int mine = end - at < 64 ? end - at : 64;
-        const int pos = lane < mine ? runs.positions[from + at + lane] : 0;
+        const int pos = lane < mine ? position(from + at + lane) : 0;
         sum.template add<T, U>(dy, mine, [&](int i) { return (int64_t)__builtin_amdgcn_readlane(pos, i) * lddy; });
       }
     };

@@ -210,7 +210,8 @@ struct EmbedWorkspace {
   int64_t even, odd, keys, positions, bounds, counts, pieces, blocks, total;
 };
 EmbedWorkspace embed_workspace(int64_t n, int64_t vocab, int64_t d) {
-  EmbedWorkspace w;
+  EmbedWorkspace w{};
+  if (n <= kFew) return w;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t p = at;
@@ -243,8 +244,7 @@ Runs sort_tokens(const void* tokens, int token_bytes, int64_t n, int64_t vocab, 
   const SortOut last{nullptr, (int*)(ws + w.keys), (int*)(ws + w.positions)};
   int2* bounds = (int2*)(ws + w.bounds);
   if (n <= kSortOne) {
-    if (n <= kDirect) bounds = nullptr;
-    const int64_t clears = bounds ? ceil_div(vocab, 4 * kSortOneThreads) : 0;
+    const int64_t clears = ceil_div(vocab, 4 * kSortOneThreads);
     const unsigned groups = 1 + (unsigned)(clears < 256 ? clears : 256);
     k_sort_one<<<groups, kSortOneThreads, 0, st>>>(tok, s, passes, bits, even, odd, last, bounds);
   } else {
@@ -491,7 +491,9 @@ int mec_embedding_backward(const void* tokens, int token_bytes, int64_t n, const
   hipStream_t st = (hipStream_t)stream;
   char* ws = (char*)workspace;
   float *pieces = (float*)(ws + w.pieces), *blocks = (float*)(ws + w.blocks);
-  const Runs runs = sort_tokens(tokens, token_bytes, n, vocab, padding_idx, w, ws, st);
+  const FewTokens few{{tokens, token_bytes == 8}, padding_idx};
+  const Runs runs = n <= kFew ? Runs{nullptr, nullptr, n, (int)vocab, nullptr}
+                              : sort_tokens(tokens, token_bytes, n, vocab, padding_idx, w, ws, st);
   with_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int N = Vec<T>::N;
@@ -504,7 +506,7 @@ int mec_embedding_backward(const void* tokens, int token_bytes, int64_t n, const
       constexpr int NC = decltype(nc)::value;
       with_past(vocab * d * sizeof(T), [&](auto past) {
         k_embed_rows<T, NC, decltype(past)::value><<<dim3(groups, (unsigned)ceil_div(d, NC * 64 * N)), 256, 0, st>>>(
-            runs, (const T*)grad_out, ldg, (int)d, scale, pieces, blocks, (T*)grad_weight);
+            runs, few, (const T*)grad_out, ldg, (int)d, scale, pieces, blocks, (T*)grad_weight);
       });
     };
     // (1024 columns by a wave: more of them in 16 bits take too many registers)
