@@ -5,8 +5,6 @@ from __future__ import annotations
 
 import torch
 
-from torch.autograd.function import once_differentiable
-
 from . import _function as _f
 from . import _lib
 
@@ -73,17 +71,34 @@ def rows_of(logits: torch.Tensor) -> tuple[torch.Tensor, int, tuple[int, int, in
     return logits, logits.data_ptr(), (n0 * n1, n1, s0, s1)
 
 
+class _Once(torch.autograd.Function):
+    """Passes a gradient on; a derivative through it is refused."""
+
+    @staticmethod
+    def forward(ctx, grad):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("memoryefficientclip_amd: the operators over a vocabulary cannot be differentiated twice")
+
+
 def backward_of(grad):
     """``Function.backward`` from `grad(ctx, *grad_outputs)`, which is differentiable once.
 
-    The wrapper that says so costs as much as the rest of a small backward (autograd
-    runs it on a thread of its own, where Python code is several times slower than
-    on the caller's), so it is taken only where a second derivative could be asked
-    for: under ``create_graph``."""
-    guarded = once_differentiable(grad)
+    Under ``create_graph`` the gradients depend on the inputs, whether or not what
+    arrived from above does (the gradient of a plain sum is a constant), so each is
+    marked: a term in it would otherwise be taken for a constant without a word.
+    Otherwise nothing is added, since autograd runs this on a thread of its own,
+    where Python code is several times slower than on the caller's."""
 
     def backward(ctx, *grad_outputs):
-        return guarded(ctx, *grad_outputs) if torch.is_grad_enabled() else grad(ctx, *grad_outputs)
+        if not torch.is_grad_enabled():
+            return grad(ctx, *grad_outputs)
+        with torch.no_grad():
+            found = grad(ctx, *grad_outputs)
+        return tuple(g if g is None else _Once.apply(g.requires_grad_())
+                     for g in (found if isinstance(found, tuple) else (found,)))
 
     return staticmethod(backward)
 
