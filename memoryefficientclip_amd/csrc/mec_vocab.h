@@ -888,17 +888,19 @@ struct DistillState {
 
 // Loss and gradient (for grad_output 1) of a row by one workgroup.  With ONE the
 // row is one segment and stays in registers from its only read to the gradient's
-// write.  Of a longer row the last segment stays in registers and the one before
-// it in LDS (128 KB: up to 131072 16-bit logits are read once); what is left is
-// read a second time.  Bound by memory: two workgroups of 1024 threads share a CU
-// with ONE, so that one reads while the other writes (8192 x 49408 bf16, a quarter
-// without a teacher: 288 us, 4.9 TB/s); a longer row has the CU to itself (4096 x
-// 200000 bf16: 750 us, 4.4 TB/s of what has to move, a third of the reads twice).
+// write.  Of a longer row the last segment stays in registers, the one before it in
+// LDS and the one before that in registers again (192 KB of a row with 512 threads,
+// 384 KB with 1024); what is left is read a second time.  Bound by memory: with
+// ONE or 512 threads two or more workgroups share a CU, so that one reads while the
+// other writes (8192 x 49408 bf16, a quarter without a teacher: 288 us, 4.9 TB/s;
+// 8192 x 70001: 512 us, 4.5 TB/s; 4096 x 200000, half of the row read twice, from
+// the cache past L2: 705 us, 4.6 TB/s of the first reads and the writes); 1024
+// threads with more than a segment have the CU to themselves (1024 x 400000 bf16:
+// 412 us, 4.0 TB/s).  Which of the two: row_shape.
 template <class T, int THREADS, bool ONE, bool PAST>
-__global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap map, int n, Teacher teacher,
-                                                         float inv_t, float scale, TeacherRows have, int mean,
-                                                         float* row_loss, DistillState state, T* dx, int segments,
-                                                         int len) {
+__global__ __launch_bounds__(THREADS, ONE ? 1 : 4) void k_distill_row(
+    const T* logits, RowMap map, int n, Teacher teacher, float inv_t, float scale, TeacherRows have, int mean,
+    float* row_loss, DistillState state, T* dx, int segments, int len) {
   constexpr int N = Vec<T>::N, kWaves = THREADS / 64;
   extern __shared__ float teacher_lds[];
   __shared__ float2 wave_sums[kWaves];
@@ -909,6 +911,7 @@ __global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap
   const T* x = logits + map(r);
   T* y = dx + r * n;
   Segment<T, THREADS> v;
+  [[maybe_unused]] typename Vec<T>::raw kept[ONE ? 1 : kSegChunks];
   // (the first segment is the short one, up to a boundary: the others fill the registers)
   const int shift = misaligned(x);
   const int first_size = ONE ? n : (n - (segments - 1) * len + shift + N - 1) / N * N - shift;
@@ -956,6 +959,9 @@ __global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap
 #pragma unroll
         for (int c = 0; c < kSegChunks; ++c)
           if (c * Segment<T, THREADS>::kChunk < v.span) held[c][tid] = v.v[c];
+      } else if (i == segments - 3) {
+#pragma unroll
+        for (int c = 0; c < kSegChunks; ++c) kept[c] = v.v[c];
       }
     }
   });
@@ -996,6 +1002,10 @@ __global__ __launch_bounds__(THREADS) void k_distill_row(const T* logits, RowMap
 #pragma unroll
         for (int c = 0; c < kSegChunks; ++c)
           if (c * Segment<T, THREADS>::kChunk < v.span) v.v[c] = held[c][tid];
+      } else if (i == segments - 3) {
+        v.shape(x + base, size);
+#pragma unroll
+        for (int c = 0; c < kSegChunks; ++c) v.v[c] = kept[c];
       } else {
         v.template load<true>(x + base, size);
       }

@@ -172,7 +172,7 @@ int64_t scores_workspace(int64_t rows, int64_t vocab, int top_k, int dtype) {
 }
 
 // The workgroup that makes a row's loss and gradient: the fewest threads that hold
-// it in registers, else 1024 and several segments.
+// it in registers, else several segments.
 struct RowShape {
   int threads, segments, len;
 };
@@ -180,9 +180,15 @@ RowShape row_shape(int64_t vocab, int dtype, bool aligned) {
   const int64_t vec = dtype == MEC_DTYPE_F32 ? 4 : 8;
   for (int threads = 256; threads <= 1024; threads *= 2)
     if (vocab + (aligned ? 0 : 1) <= vec * kSegChunks * threads) return RowShape{threads, 1, (int)vocab};
+  // Two workgroups of 512 threads on a CU read and write at the same time, one of
+  // 1024 holds twice as much of a row.  512 / 1024 threads, bf16: 8192 x 70001 512 /
+  // 697 us, 4096 x 128256 442 / 508, 4096 x 200000 705 / 729, 4096 x 212000 794 / 760,
+  // 2048 x 250002 530 / 483; fp32 (half the arithmetic a byte): 4096 x 36000 239 /
+  // 297, 4096 x 49408 342 / 368, 2048 x 70000 262 / 258, 2048 x 100003 403 / 378.
+  const int threads = vocab <= (dtype == MEC_DTYPE_F32 ? 65536 : 204800) ? 512 : 1024;
   // (the first segment may begin off a boundary, and end up to a vector later for it)
-  const int64_t len = vec * kSegChunks * 1024 - (aligned ? 0 : vec);
-  return RowShape{1024, (int)ceil_div(vocab, len), (int)len};
+  const int64_t len = vec * kSegChunks * threads - (aligned ? 0 : vec);
+  return RowShape{threads, (int)ceil_div(vocab, len), (int)len};
 }
 
 // Workspace of mec_distill_forward, in bytes from its start.
@@ -387,14 +393,17 @@ int mec_distill_forward(const void* logits, int64_t rows, int64_t inner, int64_t
               shape.len);
         });
       };
-      if (shape.segments > 1)
-        run(std::integral_constant<int, 1024>{}, std::false_type{});
-      else if (shape.threads == 256)
+      const bool one = shape.segments == 1;
+      if (shape.threads == 256)
         run(std::integral_constant<int, 256>{}, std::true_type{});
-      else if (shape.threads == 512)
+      else if (shape.threads == 512 && one)
         run(std::integral_constant<int, 512>{}, std::true_type{});
-      else
+      else if (shape.threads == 512)
+        run(std::integral_constant<int, 512>{}, std::false_type{});
+      else if (one)
         run(std::integral_constant<int, 1024>{}, std::true_type{});
+      else
+        run(std::integral_constant<int, 1024>{}, std::false_type{});
       return;
     }
     const Cut cut = cut_rows(rows, vocab, dtype, x.aligned());
