@@ -494,8 +494,8 @@ int mec_distill_backward(const void* logits, int64_t rows, int64_t inner, int64_
 int mec_embedding(const void* tokens, int token_bytes, int64_t n, const void* weight, int64_t ldw, int64_t vocab,
                   int64_t d, int dtype, float scale, void* out, void* stream);
 
-/* Bytes of mec_embedding_backward's workspace (16-byte aligned); < 0 on bad
- * arguments. */
+/* Bytes of mec_embedding_backward's workspace (16-byte aligned); 0: none (up to
+ * 512 tokens); < 0 on bad arguments. */
 int64_t mec_embedding_workspace_bytes(int64_t n, int64_t vocab, int64_t d, int dtype);
 
 /* grad_weight[v] = scale * the sum of grad_out's rows (row stride ldg >= d) whose
