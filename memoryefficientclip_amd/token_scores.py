@@ -49,18 +49,18 @@ def _scores(logits, tokens, top_k, temperature, ignore_index, keep):
         top_log_probs.data_ptr() if top_k else None, state.data_ptr() if keep else None, ws, nbytes, stream))
     if rc:
         raise _lib.error("mec_token_scores", rc)
-    kept = (held, tokens, entropy, state, (rows, vocab, code, token_bytes, ignore_index, temperature, logits.shape))
+    kept = (held, rows, tokens, entropy, state), (vocab, code, token_bytes, ignore_index, temperature)
     return (log_probs, entropy, top_tokens, top_log_probs), kept
 
 
 def _logits_grad(ctx, g_log_probs, g_entropy, _g_tokens, _g_top):
     if g_log_probs is None and g_entropy is None:
         return None, None, None, None, None
-    held, tokens, entropy, state = ctx.saved_tensors
-    rows, vocab, code, token_bytes, ignore_index, temperature, shape = ctx.mec
+    held, rows, tokens, entropy, state = _v.saved_logits(ctx)
+    vocab, code, token_bytes, ignore_index, temperature = ctx.mec
     gl = None if g_log_probs is None else g_log_probs.contiguous()
     gh = None if g_entropy is None else g_entropy.contiguous()
-    dx = held.new_empty(shape)
+    dx = held.new_empty(held.shape)
     lib = _lib.load()
     rc = _v.launch(held.device.index, 0, lambda ws, stream: lib.mec_token_scores_backward(
         held.data_ptr(), *rows, vocab, code, tokens.data_ptr(), token_bytes, ignore_index, temperature,
@@ -78,8 +78,8 @@ class _TokenScoresFn(torch.autograd.Function):
         if top_k:
             ctx.mark_non_differentiable(out[2], out[3])
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(*kept[:4])
-        ctx.mec = kept[4]
+        _v.save_logits(ctx, *kept[0])
+        ctx.mec = kept[1]
         return out
 
     backward = _v.backward_of(_logits_grad)

@@ -1,0 +1,43 @@
+"""Saved-tensor hooks may bring the values that a backward needs back in other memory
+and other strides: what the kernels are told has to be of the tensor that came back."""
+import pytest
+import torch
+
+import library_stub as stub
+import memoryefficientclip_amd as mec
+
+CUTS = [lambda x: x[:, :-1], lambda x: x[:, 1:], lambda x: x[..., 3:40], lambda x: x.transpose(0, 1),
+        lambda x: x[:, :1].expand(4, 5, 50), lambda x: x[..., ::2], lambda x: x]
+
+
+@pytest.fixture
+def lib(monkeypatch):
+    return stub.install(monkeypatch)
+
+
+def logits(cut):
+    g = torch.Generator().manual_seed(1)
+    leaf = torch.randn(4, 6, 50, generator=g).requires_grad_(True)
+    return cut(leaf)
+
+
+@pytest.mark.parametrize("cut", CUTS)
+def test_token_scores_backward(lib, cut):
+    x = logits(cut)
+    tokens = torch.arange(x[..., 0].numel()).reshape(x.shape[:-1]) % x.shape[-1]
+    with stub.copying_hooks() as back:
+        r = mec.token_log_probs(x, tokens)
+        (r.log_probs.sum() + r.entropy.sum()).backward()
+    (args,), v = lib.calls["mec_token_scores_backward"], x.shape[-1]
+    assert args[5] == v
+    assert torch.equal(stub.rows_at(back, *args[:5], v), x.detach().reshape(-1, v))
+    assert torch.equal(stub.rows_at(back, args[7], 1, 1, 0, 0, tokens.numel())[0], tokens.reshape(-1))
+
+
+@pytest.mark.parametrize("unpack", [lambda t: t.half(), lambda t: t[..., :-1], lambda t: t.to("meta")])
+def test_other_values_than_were_saved_are_refused(lib, unpack):
+    x = logits(lambda x: x)
+    with pytest.raises(RuntimeError, match="saved-tensor hook returned"):
+        with stub.copying_hooks(unpack):
+            mec.token_log_probs(x, torch.zeros(4, 6, dtype=torch.int64)).log_probs.sum().backward()
+    assert "mec_token_scores_backward" not in lib.calls
