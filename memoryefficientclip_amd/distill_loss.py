@@ -43,20 +43,20 @@ def _loss(logits, teacher_tokens, teacher_logits, temperature, weight, reduction
         nbytes, stream))
     if rc:
         raise _lib.error("mec_distill_forward", rc)
-    kept = (held, teacher_tokens, teacher_logits, state,
-            (rows, vocab, code, token_bytes, teacher_code, k, temperature, weight, reduction, logits.shape), dx)
+    kept = ((held, rows, teacher_tokens, teacher_logits, state),
+            (vocab, code, token_bytes, teacher_code, k, temperature, weight, reduction), dx)
     return loss, kept
 
 
 def _logits_grad(ctx, grad_output):
-    held, teacher_tokens, teacher_logits, state = ctx.saved_tensors
-    rows, vocab, code, token_bytes, teacher_code, k, temperature, weight, reduction, shape = ctx.mec
+    held, rows, teacher_tokens, teacher_logits, state = _v.saved_logits(ctx)
+    vocab, code, token_bytes, teacher_code, k, temperature, weight, reduction = ctx.mec
     go = grad_output.contiguous()
     # (handed out once: its new owner may change it)
     dx, ctx.made = ctx.made, None
     made = dx is not None
     if not made:
-        dx = held.new_empty(shape)
+        dx = held.new_empty(held.shape)
     lib = _lib.load()
     rc = _v.launch(held.device.index, 0, lambda ws, stream: lib.mec_distill_backward(
         held.data_ptr(), *rows, vocab, code, teacher_tokens.data_ptr(), token_bytes, teacher_logits.data_ptr(),
@@ -71,8 +71,8 @@ class _DistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher_tokens, teacher_logits, temperature, weight, reduction):
         loss, kept = _loss(logits, teacher_tokens, teacher_logits, temperature, weight, reduction, True)
-        ctx.save_for_backward(*kept[:4])
-        ctx.mec, ctx.made = kept[4:]
+        _v.save_logits(ctx, *kept[0])
+        ctx.mec, ctx.made = kept[1:]
         return loss
 
     backward = _v.backward_of(_logits_grad)

@@ -34,3 +34,27 @@ def test_token_scores(cut, dtype, pin):
     with save_on_cpu(pin_memory=pin):
         got = grad()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("pin", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("cut", CUTS)
+def test_distillation(cut, dtype, pin):
+    """Where the backward makes the gradient: no common grad_output, one other than 1, a second backward."""
+    x = logits(dtype)
+    shape = (*cut(x).shape[:-1], 5)
+    g = torch.Generator().manual_seed(2)
+    tokens = torch.randint(0, cut(x).shape[-1], shape, generator=g).to(DEV)
+    z = torch.randn(shape, generator=g).to(DEV)
+
+    def grads():
+        rows = mec.TopKDistillationLoss(1.5, "none")(cut(x), tokens, z)
+        yield torch.autograd.grad(rows.sum(), x)[0]
+        loss = mec.TopKDistillationLoss(1.5)(cut(x), tokens, z)
+        yield torch.autograd.grad(3.0 * loss, x, retain_graph=True)[0]
+        yield torch.autograd.grad(loss, x)[0]
+
+    want = list(grads())
+    with save_on_cpu(pin_memory=pin):
+        got = list(grads())
+    assert all(torch.equal(a, b) for a, b in zip(got, want, strict=True))

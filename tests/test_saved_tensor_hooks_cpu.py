@@ -41,3 +41,28 @@ def test_other_values_than_were_saved_are_refused(lib, unpack):
         with stub.copying_hooks(unpack):
             mec.token_log_probs(x, torch.zeros(4, 6, dtype=torch.int64)).log_probs.sum().backward()
     assert "mec_token_scores_backward" not in lib.calls
+
+
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+@pytest.mark.parametrize("cut", CUTS)
+def test_distillation_backward(lib, cut, reduction):
+    x = logits(cut)
+    v, shape = x.shape[-1], (*x.shape[:-1], 3)
+    g = torch.Generator().manual_seed(2)
+    tokens, z = torch.randint(0, v, shape, generator=g), torch.randn(shape, generator=g)
+    with stub.copying_hooks() as back:
+        loss = mec.TopKDistillationLoss(reduction=reduction)(x, tokens, z)
+        loss.sum().backward(torch.tensor(3.0))
+    (args,) = lib.calls["mec_distill_backward"]
+    assert args[5] == v
+    assert torch.equal(stub.rows_at(back, *args[:5], v), x.detach().reshape(-1, v))
+    for at, want in ((7, tokens), (9, z)):
+        assert torch.equal(stub.rows_at(back, args[at], 1, 1, 0, 0, want.numel())[0], want.reshape(-1))
+
+
+def test_distillation_refuses_other_values(lib):
+    x = logits(lambda x: x)
+    with pytest.raises(RuntimeError, match="saved-tensor hook returned"):
+        with stub.copying_hooks(lambda t: t.half()):
+            mec.TopKDistillationLoss()(x, torch.zeros(4, 6, 2, dtype=torch.int64), torch.zeros(4, 6, 2)).backward()
+    assert "mec_distill_backward" not in lib.calls
