@@ -64,6 +64,20 @@ def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     return t, t.stride(0)
 
 
+def layout(t: torch.Tensor) -> tuple:
+    return t.shape, t.stride(), t.dtype, t.device
+
+
+def check_unpacked(t: torch.Tensor, saved: tuple) -> None:
+    """`t` came back for a saved tensor of the `saved` layout: a saved-tensor hook
+    (offloading, checkpointing) may bring the values back in other memory with
+    other strides, and nothing else may differ."""
+    shape, _, dtype, device = saved
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        raise RuntimeError(f"memoryefficientclip_amd: saved a tensor {tuple(shape)} of {dtype} on {device}, and a "
+                           f"saved-tensor hook returned {tuple(t.shape)} of {t.dtype} on {t.device}")
+
+
 # the current stream's handle without building a torch.cuda.Stream object
 # (about 2 us of host time per call at N = 1024, where the step is host-bound)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -156,6 +170,7 @@ def forward(ctx, x: torch.Tensor, y: torch.Tensor, temperature: float, mode: int
     if rc:
         raise _lib.error("mec_forward", rc)
     ctx.save_for_backward(x, y, ws)
+    ctx.mec_saved = layout(x), layout(y)
     ctx.mec = (ldx, ldy, n, d, dt, mode, int(normalize), temperature,
                math.sqrt(n / temperature) if stable else 1.0 / temperature)
     return loss
@@ -166,6 +181,13 @@ def backward(ctx, grad_output: torch.Tensor, need_x: bool, need_y: bool):
     refuse_graph_capture()
     x, y, ws = ctx.saved_tensors
     ldx, ldy, n, d, dt, mode, normalize, temperature, grad_scale = ctx.mec
+    saved_x, saved_y = ctx.mec_saved
+    if layout(x) != saved_x:
+        check_unpacked(x, saved_x)
+        x, ldx = _rows(x)
+    if layout(y) != saved_y:
+        check_unpacked(y, saved_y)
+        y, ldy = _rows(y)
     if mode & 0xFF == _lib.MODE_LIT:
         need_y = False
     if not (need_x or need_y):

@@ -71,32 +71,19 @@ def rows_of(logits: torch.Tensor) -> tuple[torch.Tensor, int, tuple[int, int, in
     return logits, logits.data_ptr(), (n0 * n1, n1, s0, s1)
 
 
-def layout(t: torch.Tensor) -> tuple:
-    return t.shape, t.stride(), t.dtype, t.device
-
-
-def check_unpacked(t: torch.Tensor, saved: tuple) -> None:
-    """`t` came back for a tensor of the `saved` layout: only its strides may be others."""
-    shape, _, dtype, device = saved
-    if t.shape != shape or t.dtype != dtype or t.device != device:
-        raise RuntimeError(f"memoryefficientclip_amd: saved a tensor {tuple(shape)} of {dtype} on {device}, and a "
-                           f"saved-tensor hook returned {tuple(t.shape)} of {t.dtype} on {t.device}")
-
-
 def save_logits(ctx, held: torch.Tensor, rows: tuple[int, int, int, int], *others: torch.Tensor) -> None:
     """Saves what ``rows_of`` returned for the logits, and other tensors (contiguous)."""
     ctx.save_for_backward(held, *others)
-    ctx.mec_logits = rows, layout(held)
+    ctx.mec_logits = rows, _f.layout(held)
 
 
 def saved_logits(ctx) -> tuple:
-    """(held, rows, *others) as save_logits had them.  A saved-tensor hook (offloading,
-    checkpointing) may bring the values back in other memory with other strides: the
-    rows are those of the tensor that came back."""
+    """(held, rows, *others) as save_logits had them; the rows are those of the tensor
+    that came back."""
     held, *others = ctx.saved_tensors
     rows, saved = ctx.mec_logits
-    if layout(held) != saved:
-        check_unpacked(held, saved)
+    if _f.layout(held) != saved:
+        _f.check_unpacked(held, saved)
         held, _, rows = rows_of(held)
     return held, rows, *(t.contiguous() for t in others)
 

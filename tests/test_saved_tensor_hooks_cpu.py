@@ -66,3 +66,24 @@ def test_distillation_refuses_other_values(lib):
         with stub.copying_hooks(lambda t: t.half()):
             mec.TopKDistillationLoss()(x, torch.zeros(4, 6, 2, dtype=torch.int64), torch.zeros(4, 6, 2)).backward()
     assert "mec_distill_backward" not in lib.calls
+
+
+@pytest.mark.parametrize("cut", [lambda x: x[:, 2:8], lambda x: x[:, 1:], lambda x: x[::2], lambda x: x.t()[:6],
+                                 lambda x: x[:, ::2], lambda x: x[1:2], lambda x: x])
+def test_contrastive_backward(lib, cut):
+    g = torch.Generator().manual_seed(3)
+    x, y = (torch.randn(10, 10, generator=g).requires_grad_(True) for _ in range(2))
+    with stub.copying_hooks() as back:
+        mec.MemoryEfficientCLIPLoss()(cut(x), cut(y)).backward()
+    (args,), (n, d) = lib.calls["mec_backward"], cut(x).shape
+    assert args[4:6] == (n, d)
+    for at, want in ((0, cut(x)), (2, cut(y))):
+        assert torch.equal(stub.rows_at(back, args[at], n, 1, args[at + 1], 0, d), want.detach())
+
+
+def test_contrastive_refuses_other_values(lib):
+    x = torch.randn(10, 10).requires_grad_(True)
+    with pytest.raises(RuntimeError, match="saved-tensor hook returned"):
+        with stub.copying_hooks(lambda t: t.half()):
+            mec.MemoryEfficientCLIPLoss()(x, x).backward()
+    assert "mec_backward" not in lib.calls
