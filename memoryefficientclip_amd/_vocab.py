@@ -4,6 +4,7 @@ layout of logits, scratch and the calls into the HIP library
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _function as _f
 from . import _lib
@@ -69,6 +70,13 @@ def rows_of(logits: torch.Tensor) -> tuple[torch.Tensor, int, tuple[int, int, in
         return logits, logits.data_ptr(), (merged[0][0], 1, merged[0][1], 0)
     (n0, s0), (n1, s1) = merged
     return logits, logits.data_ptr(), (n0 * n1, n1, s0, s1)
+
+
+def wants_autograd(t: torch.Tensor) -> bool:
+    """Whether a call on `t` has to go through its autograd function: where a gradient
+    is asked for, and where `t` has a tangent, which the function refuses.  Without
+    either the call is made directly, for less host time."""
+    return (t.requires_grad and torch.is_grad_enabled()) or forward_ad.unpack_dual(t).tangent is not None
 
 
 def save_logits(ctx, held: torch.Tensor, rows: tuple[int, int, int, int], *others: torch.Tensor) -> None:

@@ -130,7 +130,7 @@ class TopKDistillationLoss(nn.Module):
             return student_logits.sum(-1, dtype=torch.float32) if reduction == _lib.REDUCE_NONE else \
                 student_logits.sum(dtype=torch.float32)
         args = (student_logits, teacher_tokens, teacher_logits.detach(), self.temperature, self.weight, reduction)
-        if student_logits.requires_grad and torch.is_grad_enabled():
+        if _v.wants_autograd(student_logits):
             return _DistillFn.apply(*args)
         return _loss(*args, False)[0]
 

@@ -91,7 +91,7 @@ def scaled_embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 
     if tokens.numel() == 0:
         return weight[:0].sum() * scale + torch.empty((*tokens.shape, d), dtype=weight.dtype, device=weight.device)
     tokens = tokens.contiguous()
-    if weight.requires_grad and torch.is_grad_enabled():
+    if _v.wants_autograd(weight):
         return _EmbeddingFn.apply(tokens, weight, scale, int(padding_idx))
     return _lookup(tokens, weight, scale)
 

@@ -120,7 +120,7 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, 
         zero = logits.sum(-1, dtype=torch.float32)  # (no element: the graph's link to the logits)
         none = torch.empty((*tokens.shape, top_k), dtype=torch.int64, device=logits.device)
         return TokenScores(zero, zero.clone(), none if top_k else None, none.float() if top_k else None)
-    if logits.requires_grad and torch.is_grad_enabled():
+    if _v.wants_autograd(logits):
         return TokenScores(*_TokenScoresFn.apply(logits, tokens, top_k, temperature, int(ignore_index)))
     return TokenScores(*_scores(logits, tokens, top_k, temperature, int(ignore_index), False)[0])
 
