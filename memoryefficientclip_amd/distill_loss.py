@@ -21,6 +21,27 @@ from . import _vocab as _v
 _REDUCTIONS = {"none": _lib.REDUCE_NONE, "sum": _lib.REDUCE_SUM, "mean": _lib.REDUCE_MEAN}
 
 
+def _check(student_logits, teacher_tokens, teacher_logits):
+    _v.check_gpu("student_logits", student_logits)
+    _v.check_gpu("teacher_tokens", teacher_tokens, student_logits.device)
+    _v.check_gpu("teacher_logits", teacher_logits, student_logits.device)
+    _v.refuse_graph_capture()
+    _v.check_float("student_logits", student_logits)
+    _v.check_float("teacher_logits", teacher_logits)
+    _v.check_tokens("teacher_tokens", teacher_tokens)
+    if teacher_tokens.shape != teacher_logits.shape:
+        raise ValueError(f"teacher_tokens {tuple(teacher_tokens.shape)} and teacher_logits "
+                         f"{tuple(teacher_logits.shape)} differ in shape")
+    if min(student_logits.dim(), teacher_tokens.dim()) < 1 or student_logits.shape[:-1] != teacher_tokens.shape[:-1]:
+        raise ValueError(f"student_logits {tuple(student_logits.shape)} and teacher_tokens "
+                         f"{tuple(teacher_tokens.shape)} need the same positions")
+    vocab, k = student_logits.shape[-1], teacher_tokens.shape[-1]
+    if not 1 <= vocab <= _lib.MAX_VOCAB:
+        raise ValueError(f"the vocabulary must have 1 to {_lib.MAX_VOCAB} tokens, got {vocab}")
+    if not 1 <= k <= _lib.MAX_TEACHER_K:
+        raise ValueError(f"a position needs 1 to {_lib.MAX_TEACHER_K} teacher entries, got {k}")
+
+
 def _loss(logits, teacher_tokens, teacher_logits, temperature, weight, reduction, need):
     """The loss, and with `need` what the backward needs."""
     code, teacher_code, token_bytes = _v.code_of(logits), _v.code_of(teacher_logits), teacher_tokens.element_size()
@@ -64,12 +85,14 @@ def _logits_grad(ctx, grad_output):
         stream))
     if rc:
         raise _lib.error("mec_distill_backward", rc)
-    return dx, None, None, None, None, None
+    return dx, None, None, None, None, None, None
 
 
 class _DistillFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, teacher_tokens, teacher_logits, temperature, weight, reduction):
+    def forward(ctx, logits, teacher_tokens, teacher_logits, temperature, weight, reduction, traced):
+        if traced:
+            _check(logits, teacher_tokens, teacher_logits)
         loss, kept = _loss(logits, teacher_tokens, teacher_logits, temperature, weight, reduction, True)
         _v.save_logits(ctx, *kept[0])
         ctx.mec, ctx.made = kept[1:]
@@ -106,24 +129,7 @@ class TopKDistillationLoss(nn.Module):
             raise ValueError(f"weight must be finite, got {weight}")
 
     def forward(self, student_logits, teacher_tokens, teacher_logits):
-        _v.check_gpu("student_logits", student_logits)
-        _v.check_gpu("teacher_tokens", teacher_tokens, student_logits.device)
-        _v.check_gpu("teacher_logits", teacher_logits, student_logits.device)
-        _v.refuse_graph_capture()
-        _v.check_float("student_logits", student_logits)
-        _v.check_float("teacher_logits", teacher_logits)
-        _v.check_tokens("teacher_tokens", teacher_tokens)
-        if teacher_tokens.shape != teacher_logits.shape:
-            raise ValueError(f"teacher_tokens {tuple(teacher_tokens.shape)} and teacher_logits "
-                             f"{tuple(teacher_logits.shape)} differ in shape")
-        if min(student_logits.dim(), teacher_tokens.dim()) < 1 or student_logits.shape[:-1] != teacher_tokens.shape[:-1]:
-            raise ValueError(f"student_logits {tuple(student_logits.shape)} and teacher_tokens "
-                             f"{tuple(teacher_tokens.shape)} need the same positions")
-        vocab, k = student_logits.shape[-1], teacher_tokens.shape[-1]
-        if not 1 <= vocab <= _lib.MAX_VOCAB:
-            raise ValueError(f"the vocabulary must have 1 to {_lib.MAX_VOCAB} tokens, got {vocab}")
-        if not 1 <= k <= _lib.MAX_TEACHER_K:
-            raise ValueError(f"a position needs 1 to {_lib.MAX_TEACHER_K} teacher entries, got {k}")
+        _check(student_logits, teacher_tokens, teacher_logits)
         reduction = _REDUCTIONS[self.reduction]
         if student_logits.numel() == 0:
             # no position: the graph's link to the logits
@@ -131,7 +137,7 @@ class TopKDistillationLoss(nn.Module):
                 student_logits.sum(dtype=torch.float32)
         args = (student_logits, teacher_tokens, teacher_logits.detach(), self.temperature, self.weight, reduction)
         if _v.wants_autograd(student_logits):
-            return _DistillFn.apply(*args)
+            return _DistillFn.apply(*args, torch.jit.is_tracing())
         return _loss(*args, False)[0]
 
 

@@ -18,6 +18,20 @@ from . import _vocab as _v
 _MAX_TOKENS, _MAX_VOCAB, _MAX_DIM = 1 << 23, 1 << 22, 1 << 16
 
 
+def _check(tokens, weight):
+    _v.check_gpu("weight", weight)
+    _v.check_gpu("tokens", tokens, weight.device)
+    _v.refuse_graph_capture()
+    _v.check_float("weight", weight)
+    _v.check_tokens("tokens", tokens)
+    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"weight must be [V, D] with V, D >= 1, got {tuple(weight.shape)}")
+    vocab, d = weight.shape
+    if vocab > _MAX_VOCAB or d > _MAX_DIM or tokens.numel() > _MAX_TOKENS:
+        raise ValueError(f"{tokens.numel()} tokens of {vocab} x {d} exceed the maxima {_MAX_TOKENS}, {_MAX_VOCAB} x "
+                         f"{_MAX_DIM}")
+
+
 def _lookup(tokens, weight, scale):
     w, ldw = _f._rows(weight)
     vocab, d = w.shape
@@ -42,12 +56,15 @@ def _weight_grad(ctx, grad_output):
         dw.data_ptr(), ws, nbytes, stream))
     if rc:
         raise _lib.error("mec_embedding_backward", rc)
-    return None, dw, None, None
+    return None, dw, None, None, None
 
 
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, tokens, weight, scale, padding_idx):
+    def forward(ctx, tokens, weight, scale, padding_idx, traced):
+        if traced:
+            _check(tokens, weight)
+            tokens = tokens.contiguous()
         out = _lookup(tokens, weight, scale)
         ctx.save_for_backward(tokens)
         (vocab, d), n, code = weight.shape, tokens.numel(), _v.code_of(weight)
@@ -68,17 +85,8 @@ def scaled_embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 
     looked up like any other).  A token outside [0, V) gives a row of NaN and
     has no part in the gradient.  Up to 2^23 tokens, V up to 2^22, D up to 2^16.
     """
-    _v.check_gpu("weight", weight)
-    _v.check_gpu("tokens", tokens, weight.device)
-    _v.refuse_graph_capture()
-    _v.check_float("weight", weight)
-    _v.check_tokens("tokens", tokens)
-    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
-        raise ValueError(f"weight must be [V, D] with V, D >= 1, got {tuple(weight.shape)}")
+    _check(tokens, weight)
     vocab, d = weight.shape
-    if vocab > _MAX_VOCAB or d > _MAX_DIM or tokens.numel() > _MAX_TOKENS:
-        raise ValueError(f"{tokens.numel()} tokens of {vocab} x {d} exceed the maxima {_MAX_TOKENS}, {_MAX_VOCAB} x "
-                         f"{_MAX_DIM}")
     scale = float(scale)
     if not math.isfinite(scale):
         raise ValueError(f"scale must be finite, got {scale}")
@@ -92,7 +100,7 @@ def scaled_embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 
         return weight[:0].sum() * scale + torch.empty((*tokens.shape, d), dtype=weight.dtype, device=weight.device)
     tokens = tokens.contiguous()
     if _v.wants_autograd(weight):
-        return _EmbeddingFn.apply(tokens, weight, scale, int(padding_idx))
+        return _EmbeddingFn.apply(tokens, weight, scale, int(padding_idx), torch.jit.is_tracing())
     return _lookup(tokens, weight, scale)
 
 

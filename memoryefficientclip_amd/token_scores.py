@@ -27,6 +27,21 @@ class TokenScores(NamedTuple):
     top_log_probs: torch.Tensor | None
 
 
+def _check(logits, tokens, top_k):
+    _v.check_gpu("logits", logits)
+    _v.check_gpu("tokens", tokens, logits.device)
+    _v.refuse_graph_capture()
+    if logits.dim() < 1 or logits.shape[:-1] != tokens.shape:
+        raise ValueError(f"logits {tuple(logits.shape)} need one row for each of the tokens {tuple(tokens.shape)}")
+    _v.check_float("logits", logits)
+    _v.check_tokens("tokens", tokens)
+    vocab, top_k = logits.shape[-1], int(top_k)
+    if not 1 <= vocab <= _lib.MAX_VOCAB:
+        raise ValueError(f"the vocabulary must have 1 to {_lib.MAX_VOCAB} tokens, got {vocab}")
+    if not 0 <= top_k <= min(vocab, _lib.MAX_TOP_K):
+        raise ValueError(f"top_k must be in [0, {min(vocab, _lib.MAX_TOP_K)}], got {top_k}")
+
+
 def _scores(logits, tokens, top_k, temperature, ignore_index, keep):
     """Results, and with `keep` what the backward needs of them."""
     code, token_bytes = _v.code_of(logits), tokens.element_size()
@@ -55,7 +70,7 @@ def _scores(logits, tokens, top_k, temperature, ignore_index, keep):
 
 def _logits_grad(ctx, g_log_probs, g_entropy, _g_tokens, _g_top):
     if g_log_probs is None and g_entropy is None:
-        return None, None, None, None, None
+        return None, None, None, None, None, None
     held, rows, tokens, entropy, state = _v.saved_logits(ctx)
     vocab, code, token_bytes, ignore_index, temperature = ctx.mec
     gl = None if g_log_probs is None else g_log_probs.contiguous()
@@ -68,12 +83,14 @@ def _logits_grad(ctx, g_log_probs, g_entropy, _g_tokens, _g_top):
         None if gh is None else gh.data_ptr(), dx.data_ptr(), stream))
     if rc:
         raise _lib.error("mec_token_scores_backward", rc)
-    return dx, None, None, None, None
+    return dx, None, None, None, None, None
 
 
 class _TokenScoresFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, tokens, top_k, temperature, ignore_index):
+    def forward(ctx, logits, tokens, top_k, temperature, ignore_index, traced):
+        if traced:
+            _check(logits, tokens, top_k)
         out, kept = _scores(logits, tokens, top_k, temperature, ignore_index, True)
         if top_k:
             ctx.mark_non_differentiable(out[2], out[3])
@@ -103,25 +120,16 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, 
     fp32, bf16 and fp16 logits, read in place (any row strides), V up to 2^19 and
     ``top_k`` up to 128; int64 or int32 tokens.
     """
-    _v.check_gpu("logits", logits)
-    _v.check_gpu("tokens", tokens, logits.device)
-    _v.refuse_graph_capture()
-    if logits.dim() < 1 or logits.shape[:-1] != tokens.shape:
-        raise ValueError(f"logits {tuple(logits.shape)} need one row for each of the tokens {tuple(tokens.shape)}")
-    _v.check_float("logits", logits)
-    _v.check_tokens("tokens", tokens)
-    vocab, top_k = logits.shape[-1], int(top_k)
-    if not 1 <= vocab <= _lib.MAX_VOCAB:
-        raise ValueError(f"the vocabulary must have 1 to {_lib.MAX_VOCAB} tokens, got {vocab}")
-    if not 0 <= top_k <= min(vocab, _lib.MAX_TOP_K):
-        raise ValueError(f"top_k must be in [0, {min(vocab, _lib.MAX_TOP_K)}], got {top_k}")
+    _check(logits, tokens, top_k)
+    top_k = int(top_k)
     temperature = _v.check_temperature(temperature)
     if tokens.numel() == 0:
         zero = logits.sum(-1, dtype=torch.float32)  # (no element: the graph's link to the logits)
         none = torch.empty((*tokens.shape, top_k), dtype=torch.int64, device=logits.device)
         return TokenScores(zero, zero.clone(), none if top_k else None, none.float() if top_k else None)
     if _v.wants_autograd(logits):
-        return TokenScores(*_TokenScoresFn.apply(logits, tokens, top_k, temperature, int(ignore_index)))
+        return TokenScores(*_TokenScoresFn.apply(logits, tokens, top_k, temperature, int(ignore_index),
+                                                 torch.jit.is_tracing()))
     return TokenScores(*_scores(logits, tokens, top_k, temperature, int(ignore_index), False)[0])
 
 
