@@ -74,9 +74,11 @@ def rows_of(logits: torch.Tensor) -> tuple[torch.Tensor, int, tuple[int, int, in
 
 def wants_autograd(t: torch.Tensor) -> bool:
     """Whether a call on `t` has to go through its autograd function: where a gradient
-    is asked for, and where `t` has a tangent, which the function refuses.  Without
-    either the call is made directly, for less host time."""
-    return (t.requires_grad and torch.is_grad_enabled()) or forward_ad.unpack_dual(t).tangent is not None
+    is asked for, where `t` has a tangent, which the function refuses, and in a trace,
+    which records the function (of a direct call it records the empty results).
+    Otherwise the call is made directly, for less host time."""
+    return ((t.requires_grad and torch.is_grad_enabled()) or forward_ad.unpack_dual(t).tangent is not None
+            or torch.jit.is_tracing())
 
 
 def save_logits(ctx, held: torch.Tensor, rows: tuple[int, int, int, int], *others: torch.Tensor) -> None:

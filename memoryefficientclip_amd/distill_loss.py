@@ -93,7 +93,8 @@ class _DistillFn(torch.autograd.Function):
     def forward(ctx, logits, teacher_tokens, teacher_logits, temperature, weight, reduction, traced):
         if traced:
             _check(logits, teacher_tokens, teacher_logits)
-        loss, kept = _loss(logits, teacher_tokens, teacher_logits, temperature, weight, reduction, True)
+        loss, kept = _loss(logits, teacher_tokens, teacher_logits, temperature, weight, reduction,
+                           ctx.needs_input_grad[0])
         _v.save_logits(ctx, *kept[0])
         ctx.mec, ctx.made = kept[1:]
         return loss

@@ -56,3 +56,30 @@ def check_trace(lib, op, example, wrong, message):
 def test_a_traced_function_checks_its_inputs(lib, op, wrong, message):
     """Traced with a gradient; other inputs than were traced, which no kernel may be started on."""
     check_trace(lib, op, torch.randn(3, 5).requires_grad_(True), wrong, message)
+
+
+@pytest.mark.parametrize("op,wrong,message", WRONG)
+def test_a_function_traced_without_a_gradient_checks_its_inputs(lib, op, wrong, message):
+    check_trace(lib, op, torch.randn(3, 5), wrong, message)
+
+
+@pytest.mark.parametrize("wanted", [False, True])
+@pytest.mark.parametrize("op,call", zip(OPERATORS, CALLS))
+def test_a_traced_function_calls_the_library(lib, op, call, wanted):
+    x = torch.randn(3, 5).requires_grad_(wanted)
+    traced = torch.jit.trace(op, x, check_trace=False)
+    lib.calls.clear()
+    y = torch.randn(3, 5)
+    assert traced(y).shape == op(y).shape
+    got, want = lib.calls[call]
+    # the operator's numbers, and the tensor that the trace was called with
+    numbers = [[a for a in args if isinstance(a, (int, float)) and abs(a) < 1 << 30] for args in (got, want)]
+    assert numbers[0] == numbers[1] and y.data_ptr() in got
+
+
+@pytest.mark.parametrize("op", OPERATORS)
+def test_a_gradient_through_a_traced_function(lib, op):
+    traced = torch.jit.trace(op, torch.randn(3, 5), check_trace=False)
+    x = torch.randn(3, 5).requires_grad_(True)
+    traced(x).sum().backward()
+    assert x.grad.shape == x.shape and any(name.endswith("_backward") for name in lib.calls)
