@@ -22,7 +22,7 @@ def scores(x, tok, tt, tz):
 
 
 OPERATORS = [scores, lambda x, tok, tt, tz: (mec.TopKDistillationLoss(2.0)(x, tt, tz),),
-             lambda x, tok, tt, tz: (mec.scaled_embedding(tok, x, 1.5),)]
+             lambda x, tok, tt, tz: (mec.scaled_embedding(tok % x.shape[0], x, 1.5),)]
 
 
 @pytest.mark.parametrize("wanted", [False, True])
@@ -30,7 +30,7 @@ OPERATORS = [scores, lambda x, tok, tt, tz: (mec.TopKDistillationLoss(2.0)(x, tt
 def test_traced(op, wanted):
     x, *others = inputs(6, 900, 0)
     traced = torch.jit.trace(op, (x.requires_grad_(wanted), *others))
-    for seed, rows, vocab in ((1, 6, 900), (2, 11, 70001)):
+    for seed, rows, vocab in ((1, 6, 900), (2, 11, 50001)):
         x, *others = inputs(rows, vocab, seed)
         with torch.no_grad():
             assert all(torch.equal(a, b) for a, b in zip(traced(x, *others), op(x, *others), strict=True))
