@@ -113,6 +113,17 @@ def refuse_graph_capture() -> None:
                            "call it outside the captured region")
 
 
+_dispatch_mode = getattr(torch._C, "_get_dispatch_mode", None)
+
+
+def refuse_make_fx() -> None:
+    """Raise under ``make_fx``, which records the tensor operations of a call: here
+    the allocation of the results, and nothing that writes them."""
+    if _dispatch_mode is not None and _dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise RuntimeError("memoryefficientclip_amd: make_fx cannot record these operators; their kernels are started "
+                           "past PyTorch's dispatcher")
+
+
 def compute_dtype(dtype: torch.dtype) -> int:
     """C-ABI dtype code for inputs of `dtype` under the current
     ``torch.get_float32_matmul_precision()`` (fp32 only: "high" selects the
@@ -132,6 +143,7 @@ def forward(ctx, x: torch.Tensor, y: torch.Tensor, temperature: float, mode: int
             stable: bool) -> torch.Tensor:
     check_inputs(x, y)
     refuse_graph_capture()
+    refuse_make_fx()
     temperature = float(temperature)
     if not (temperature > 0.0 and math.isfinite(temperature)):
         raise ValueError(f"temperature must be finite and > 0, got {temperature}")

@@ -16,6 +16,9 @@ def refuse_graph_capture() -> None:
                            "capture; call them outside the captured region")
 
 
+refuse_make_fx = _f.refuse_make_fx
+
+
 def check_gpu(name: str, t: torch.Tensor, device: torch.device | None = None) -> None:
     """`t` is a tensor on the GPU (AssertionError else, as the losses raise it), on `device` if given."""
     if not isinstance(t, torch.Tensor):

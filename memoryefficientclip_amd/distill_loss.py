@@ -26,6 +26,7 @@ def _check(student_logits, teacher_tokens, teacher_logits):
     _v.check_gpu("teacher_tokens", teacher_tokens, student_logits.device)
     _v.check_gpu("teacher_logits", teacher_logits, student_logits.device)
     _v.refuse_graph_capture()
+    _v.refuse_make_fx()
     _v.check_float("student_logits", student_logits)
     _v.check_float("teacher_logits", teacher_logits)
     _v.check_tokens("teacher_tokens", teacher_tokens)

@@ -22,6 +22,7 @@ def _check(tokens, weight):
     _v.check_gpu("weight", weight)
     _v.check_gpu("tokens", tokens, weight.device)
     _v.refuse_graph_capture()
+    _v.refuse_make_fx()
     _v.check_float("weight", weight)
     _v.check_tokens("tokens", tokens)
     if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:

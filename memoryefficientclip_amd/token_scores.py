@@ -31,6 +31,7 @@ def _check(logits, tokens, top_k):
     _v.check_gpu("logits", logits)
     _v.check_gpu("tokens", tokens, logits.device)
     _v.refuse_graph_capture()
+    _v.refuse_make_fx()
     if logits.dim() < 1 or logits.shape[:-1] != tokens.shape:
         raise ValueError(f"logits {tuple(logits.shape)} need one row for each of the tokens {tuple(tokens.shape)}")
     _v.check_float("logits", logits)

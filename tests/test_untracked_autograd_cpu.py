@@ -83,3 +83,18 @@ def test_a_gradient_through_a_traced_function(lib, op):
     x = torch.randn(3, 5).requires_grad_(True)
     traced(x).sum().backward()
     assert x.grad.shape == x.shape and any(name.endswith("_backward") for name in lib.calls)
+
+
+@pytest.mark.parametrize("wanted", [False, True])
+@pytest.mark.parametrize("op", [*OPERATORS, lambda x: mec.MemoryEfficientCLIPLoss()(x, x)])
+def test_make_fx_is_refused(lib, op, wanted):
+    """It records tensor operations alone: of these calls, the empty results."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = torch.randn(3, 5).requires_grad_(wanted)
+    op(x)
+    lib.calls.clear()
+    with pytest.raises(RuntimeError, match="make_fx"):
+        make_fx(op)(x)
+    assert not lib.calls
+    op(x)
