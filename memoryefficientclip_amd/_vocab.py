@@ -102,10 +102,10 @@ def saved_logits(ctx) -> tuple:
 
 
 class _Once(torch.autograd.Function):
-    """Passes a gradient on; a derivative through it is refused."""
+    """Passes a gradient on that depends on other tensors; a derivative through it is refused."""
 
     @staticmethod
-    def forward(ctx, grad):
+    def forward(ctx, grad, *others):
         return grad.view_as(grad)
 
     @staticmethod
@@ -116,18 +116,18 @@ class _Once(torch.autograd.Function):
 def backward_of(grad):
     """``Function.backward`` from `grad(ctx, *grad_outputs)`, which is differentiable once.
 
-    Under ``create_graph`` the gradients depend on the inputs, whether or not what
-    arrived from above does (the gradient of a plain sum is a constant), so each is
-    marked: a term in it would otherwise be taken for a constant without a word.
-    Otherwise nothing is added, since autograd runs this on a thread of its own,
-    where Python code is several times slower than on the caller's."""
+    Under ``create_graph`` the gradients depend on the saved inputs and on what
+    arrived from above, and are tied to them: a derivative through them would
+    otherwise be taken for zero without a word.  Otherwise nothing is added, since
+    autograd runs this on a thread of its own, where Python code is several times
+    slower than on the caller's."""
 
     def backward(ctx, *grad_outputs):
         if not torch.is_grad_enabled():
             return grad(ctx, *grad_outputs)
         with torch.no_grad():
             found = grad(ctx, *grad_outputs)
-        return tuple(g if g is None else _Once.apply(g.requires_grad_())
+        return tuple(g if g is None else _Once.apply(g.requires_grad_(), *grad_outputs, *ctx.saved_tensors)
                      for g in (found if isinstance(found, tuple) else (found,)))
 
     return staticmethod(backward)

@@ -43,10 +43,9 @@ def _check(student_logits, teacher_tokens, teacher_logits):
         raise ValueError(f"a position needs 1 to {_lib.MAX_TEACHER_K} teacher entries, got {k}")
 
 
-def _loss(logits, teacher_tokens, teacher_logits, temperature, weight, reduction, need):
-    """The loss, and with `need` what the backward needs."""
+def _loss(logits, rows, teacher_tokens, teacher_logits, temperature, weight, reduction, need):
+    """The loss, and with `need` what the backward needs; logits and their rows as ``rows_of`` has them."""
     code, teacher_code, token_bytes = _v.code_of(logits), _v.code_of(teacher_logits), teacher_tokens.element_size()
-    held, px, rows = _v.rows_of(logits)
     teacher_tokens, teacher_logits = teacher_tokens.contiguous(), teacher_logits.contiguous()
     vocab, k, dev = logits.shape[-1], teacher_tokens.shape[-1], logits.device
     loss = torch.empty(logits.shape[:-1] if reduction == _lib.REDUCE_NONE else (), dtype=torch.float32, device=dev)
@@ -60,12 +59,12 @@ def _loss(logits, teacher_tokens, teacher_logits, temperature, weight, reduction
     lib = _lib.load()
     nbytes = lib.mec_distill_workspace_bytes(rows[0], vocab, k, code, int(dx is not None))
     rc = _v.launch(dev.index, nbytes, lambda ws, stream: lib.mec_distill_forward(
-        px, *rows, vocab, code, teacher_tokens.data_ptr(), token_bytes, teacher_logits.data_ptr(), teacher_code, k,
-        temperature, weight, reduction, loss.data_ptr(), state.data_ptr(), None if dx is None else dx.data_ptr(), ws,
-        nbytes, stream))
+        logits.data_ptr(), *rows, vocab, code, teacher_tokens.data_ptr(), token_bytes, teacher_logits.data_ptr(),
+        teacher_code, k, temperature, weight, reduction, loss.data_ptr(), state.data_ptr(),
+        None if dx is None else dx.data_ptr(), ws, nbytes, stream))
     if rc:
         raise _lib.error("mec_distill_forward", rc)
-    kept = ((held, rows, teacher_tokens, teacher_logits, state),
+    kept = ((logits, rows, teacher_tokens, teacher_logits, state),
             (vocab, code, token_bytes, teacher_code, k, temperature, weight, reduction), dx)
     return loss, kept
 
@@ -91,10 +90,11 @@ def _logits_grad(ctx, grad_output):
 
 class _DistillFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, teacher_tokens, teacher_logits, temperature, weight, reduction, traced):
-        if traced:
+    def forward(ctx, logits, rows, teacher_tokens, teacher_logits, temperature, weight, reduction):
+        if rows is None:
             _check(logits, teacher_tokens, teacher_logits)
-        loss, kept = _loss(logits, teacher_tokens, teacher_logits, temperature, weight, reduction,
+            logits, _, rows = _v.rows_of(logits)
+        loss, kept = _loss(logits, rows, teacher_tokens, teacher_logits, temperature, weight, reduction,
                            ctx.needs_input_grad[0])
         _v.save_logits(ctx, *kept[0])
         ctx.mec, ctx.made = kept[1:]
@@ -137,10 +137,12 @@ class TopKDistillationLoss(nn.Module):
             # no position: the graph's link to the logits
             return student_logits.sum(-1, dtype=torch.float32) if reduction == _lib.REDUCE_NONE else \
                 student_logits.sum(dtype=torch.float32)
-        args = (student_logits, teacher_tokens, teacher_logits.detach(), self.temperature, self.weight, reduction)
+        student_logits, _, rows = _v.rows_of(student_logits)
+        args = (teacher_tokens, teacher_logits.detach(), self.temperature, self.weight, reduction)
         if _v.wants_autograd(student_logits):
-            return _DistillFn.apply(*args, torch.jit.is_tracing())
-        return _loss(*args, False)[0]
+            # (a trace calls this again, with other inputs)
+            return _DistillFn.apply(student_logits, None if torch.jit.is_tracing() else rows, *args)
+        return _loss(student_logits, rows, *args, False)[0]
 
 
 __all__ = ["TopKDistillationLoss"]

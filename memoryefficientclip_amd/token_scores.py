@@ -43,10 +43,9 @@ def _check(logits, tokens, top_k):
         raise ValueError(f"top_k must be in [0, {min(vocab, _lib.MAX_TOP_K)}], got {top_k}")
 
 
-def _scores(logits, tokens, top_k, temperature, ignore_index, keep):
-    """Results, and with `keep` what the backward needs of them."""
+def _scores(logits, rows, tokens, top_k, temperature, ignore_index, keep):
+    """Results, and with `keep` what the backward needs of them; logits and their rows as ``rows_of`` has them."""
     code, token_bytes = _v.code_of(logits), tokens.element_size()
-    held, px, rows = _v.rows_of(logits)
     tokens = tokens.contiguous()
     vocab, dev, shape = logits.shape[-1], logits.device, tokens.shape
     log_probs = torch.empty(shape, dtype=torch.float32, device=dev)
@@ -60,12 +59,12 @@ def _scores(logits, tokens, top_k, temperature, ignore_index, keep):
     lib = _lib.load()
     nbytes = lib.mec_token_scores_workspace_bytes(rows[0], vocab, top_k, code)
     rc = _v.launch(dev.index, nbytes, lambda ws, stream: lib.mec_token_scores(
-        px, *rows, vocab, code, tokens.data_ptr(), token_bytes, ignore_index, temperature, top_k,
+        logits.data_ptr(), *rows, vocab, code, tokens.data_ptr(), token_bytes, ignore_index, temperature, top_k,
         log_probs.data_ptr(), entropy.data_ptr(), top_tokens.data_ptr() if top_k else None,
         top_log_probs.data_ptr() if top_k else None, state.data_ptr() if keep else None, ws, nbytes, stream))
     if rc:
         raise _lib.error("mec_token_scores", rc)
-    kept = (held, rows, tokens, entropy, state), (vocab, code, token_bytes, ignore_index, temperature)
+    kept = (logits, rows, tokens, entropy, state), (vocab, code, token_bytes, ignore_index, temperature)
     return (log_probs, entropy, top_tokens, top_log_probs), kept
 
 
@@ -89,10 +88,11 @@ def _logits_grad(ctx, g_log_probs, g_entropy, _g_tokens, _g_top):
 
 class _TokenScoresFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, tokens, top_k, temperature, ignore_index, traced):
-        if traced:
+    def forward(ctx, logits, rows, tokens, top_k, temperature, ignore_index):
+        if rows is None:
             _check(logits, tokens, top_k)
-        out, kept = _scores(logits, tokens, top_k, temperature, ignore_index, True)
+            logits, _, rows = _v.rows_of(logits)
+        out, kept = _scores(logits, rows, tokens, top_k, temperature, ignore_index, True)
         if top_k:
             ctx.mark_non_differentiable(out[2], out[3])
         ctx.set_materialize_grads(False)
@@ -128,10 +128,12 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, 
         zero = logits.sum(-1, dtype=torch.float32)  # (no element: the graph's link to the logits)
         none = torch.empty((*tokens.shape, top_k), dtype=torch.int64, device=logits.device)
         return TokenScores(zero, zero.clone(), none if top_k else None, none.float() if top_k else None)
+    logits, _, rows = _v.rows_of(logits)
     if _v.wants_autograd(logits):
-        return TokenScores(*_TokenScoresFn.apply(logits, tokens, top_k, temperature, int(ignore_index),
-                                                 torch.jit.is_tracing()))
-    return TokenScores(*_scores(logits, tokens, top_k, temperature, int(ignore_index), False)[0])
+        # (a trace calls this again, with other inputs)
+        rows = None if torch.jit.is_tracing() else rows
+        return TokenScores(*_TokenScoresFn.apply(logits, rows, tokens, top_k, temperature, int(ignore_index)))
+    return TokenScores(*_scores(logits, rows, tokens, top_k, temperature, int(ignore_index), False)[0])
 
 
 __all__ = ["TokenScores", "token_log_probs"]
