@@ -64,20 +64,20 @@ def _loss(logits, rows, teacher_tokens, teacher_logits, temperature, weight, red
         None if dx is None else dx.data_ptr(), ws, nbytes, stream))
     if rc:
         raise _lib.error("mec_distill_forward", rc)
-    kept = ((logits, rows, teacher_tokens, teacher_logits, state),
-            (vocab, code, token_bytes, teacher_code, k, temperature, weight, reduction), dx)
+    kept = ((logits, rows, teacher_tokens, teacher_logits, state) + (() if dx is None else (dx,)),
+            (vocab, code, token_bytes, teacher_code, k, temperature, weight, reduction))
     return loss, kept
 
 
 def _logits_grad(ctx, grad_output):
-    held, rows, teacher_tokens, teacher_logits, state = _v.saved_logits(ctx)
+    held, rows, teacher_tokens, teacher_logits, state, *dx = _v.saved_logits(ctx)
     vocab, code, token_bytes, teacher_code, k, temperature, weight, reduction = ctx.mec
     go = grad_output.contiguous()
-    # (handed out once: its new owner may change it)
-    dx, ctx.made = ctx.made, None
-    made = dx is not None
-    if not made:
-        dx = held.new_empty(held.shape)
+    # The forward's gradient is handed out once, since its new owner may change it: as a
+    # tensor of its own on the same memory (autograd copies one that others hold, and
+    # takes a change of it for one of what is saved).
+    made, ctx.made = ctx.made, False
+    dx = dx[0].data if made else held.new_empty(held.shape)
     lib = _lib.load()
     rc = _v.launch(held.device.index, 0, lambda ws, stream: lib.mec_distill_backward(
         held.data_ptr(), *rows, vocab, code, teacher_tokens.data_ptr(), token_bytes, teacher_logits.data_ptr(),
@@ -97,7 +97,7 @@ class _DistillFn(torch.autograd.Function):
         loss, kept = _loss(logits, rows, teacher_tokens, teacher_logits, temperature, weight, reduction,
                            ctx.needs_input_grad[0])
         _v.save_logits(ctx, *kept[0])
-        ctx.mec, ctx.made = kept[1:]
+        ctx.mec, ctx.made = kept[1], len(kept[0]) > 5
         return loss
 
     backward = _v.backward_of(_logits_grad)

@@ -3,6 +3,7 @@ the kernels read what came back, wherever and in whatever strides it lies."""
 import pytest
 import torch
 from torch.autograd.graph import save_on_cpu
+from torch.utils.checkpoint import checkpoint
 
 import memoryefficientclip_amd as mec
 
@@ -82,3 +83,41 @@ def test_contrastive_losses(cut, loss, dtype, n):
     bound = 2.0 ** -24 * (2 * n + 128) + (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -23)
     for a, b in zip(got, want):
         assert (a is None and b is None) or ((a - b).abs().max() <= bound * b.abs().max()).item()
+
+
+def distillation(dtype):
+    x = logits(dtype)
+    g = torch.Generator().manual_seed(4)
+    tokens = torch.randint(0, 1003, (4, 6, 5), generator=g).to(DEV)
+    z = torch.randn(4, 6, 5, generator=g).to(DEV)
+    return x, lambda x: mec.TopKDistillationLoss(1.5)(x * 1.0, tokens, z)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_the_forwards_gradient(dtype):
+    x, loss = distillation(dtype)
+    want, = torch.autograd.grad(loss(x), x)
+    with save_on_cpu():
+        got, = torch.autograd.grad(loss(x), x)
+    assert torch.equal(got, want)
+    got, = torch.autograd.grad(checkpoint(loss, x, use_reentrant=False), x)
+    assert torch.equal(got, want)
+    # summed with another gradient of the same logits, twice over a graph that is kept
+    y = x * 1.0
+    total = loss(y) + y.float().square().sum()
+    a, = torch.autograd.grad(total, x, retain_graph=True)
+    kept = a.clone()
+    a.zero_()
+    b, = torch.autograd.grad(total, x)
+    torch.testing.assert_close(b, kept, rtol=2.0 ** -6 if dtype == torch.bfloat16 else 4e-6, atol=1e-6)
+
+
+def test_a_checkpointed_region_keeps_no_gradient():
+    rows, vocab = 64, 50001
+    x = torch.randn(rows, vocab, device=DEV, requires_grad=True)
+    tokens, z = torch.zeros(rows, 2, dtype=torch.int64, device=DEV), torch.zeros(rows, 2, device=DEV)
+    before = torch.cuda.memory_allocated()
+    loss = checkpoint(lambda x: mec.TopKDistillationLoss()(x, tokens, z), x, use_reentrant=False)
+    assert torch.cuda.memory_allocated() - before < rows * vocab
+    loss.backward()
+    assert x.grad.shape == x.shape

@@ -1,7 +1,10 @@
 """Saved-tensor hooks may bring the values that a backward needs back in other memory
 and other strides: what the kernels are told has to be of the tensor that came back."""
+import gc
+
 import pytest
 import torch
+from torch.utils.checkpoint import checkpoint
 
 import library_stub as stub
 import memoryefficientclip_amd as mec
@@ -87,3 +90,49 @@ def test_contrastive_refuses_other_values(lib):
         with stub.copying_hooks(lambda t: t.half()):
             mec.MemoryEfficientCLIPLoss()(x, x).backward()
     assert "mec_backward" not in lib.calls
+
+
+def test_the_forwards_gradient_is_a_saved_tensor(lib):
+    """It is the largest thing from forward to backward: offloading and checkpointing have to see it."""
+    x = logits(lambda x: x)
+    tokens, z = torch.zeros(4, 6, 2, dtype=torch.int64), torch.zeros(4, 6, 2)
+    with stub.copying_hooks() as back:
+        loss = mec.TopKDistillationLoss()(x, tokens, z)
+        loss.backward()
+    (forward,), (backward,) = lib.calls["mec_distill_forward"], lib.calls["mec_distill_backward"]
+    pointers = [t.data_ptr() for t in back]
+    assert forward[17] is not None and forward[17] not in pointers
+    # what came back is what is handed out
+    assert backward[17] == 1 and backward[18] in pointers
+
+
+def test_a_checkpointed_region_keeps_no_gradient(lib):
+    x = logits(lambda x: x)
+    tokens, z = torch.zeros(4, 6, 2, dtype=torch.int64), torch.zeros(4, 6, 2)
+    loss = checkpoint(lambda x: mec.TopKDistillationLoss()(x * 1.0, tokens, z), x, use_reentrant=False)
+    gc.collect()
+    assert [t for t in gc.get_objects() if type(t) is torch.Tensor and t.shape == x.shape and t is not x] == []
+    loss.backward()
+    first, again = lib.calls["mec_distill_forward"]
+    (backward,) = lib.calls["mec_distill_backward"]
+    assert backward[17] == 1 and backward[18] == again[17]
+
+
+def test_the_forwards_gradient_is_handed_out_once(lib):
+    x = logits(lambda x: x)
+    loss = mec.TopKDistillationLoss()(x, torch.zeros(4, 6, 2, dtype=torch.int64), torch.zeros(4, 6, 2))
+    first, = torch.autograd.grad(loss, x, retain_graph=True)
+    (forward,) = lib.calls["mec_distill_forward"]
+    assert first.data_ptr() == forward[17]  # (no copy)
+    first.zero_()
+    second, = torch.autograd.grad(loss, x)
+    assert second.data_ptr() != first.data_ptr()
+    assert [(args[17], args[18]) for args in lib.calls["mec_distill_backward"]] == [(1, first.data_ptr()),
+                                                                                   (0, second.data_ptr())]
+
+
+def test_the_forwards_gradient_becomes_the_leafs(lib):
+    """AccumulateGrad takes it over without a copy."""
+    x = logits(lambda x: x)
+    mec.TopKDistillationLoss()(x, torch.zeros(4, 6, 2, dtype=torch.int64), torch.zeros(4, 6, 2)).backward()
+    assert x.grad.data_ptr() == lib.calls["mec_distill_forward"][0][17]
