@@ -48,6 +48,9 @@ def _lookup(tokens, weight, scale):
 
 def _weight_grad(ctx, grad_output):
     tokens, = ctx.saved_tensors
+    if _f.layout(tokens) != ctx.mec_tokens:
+        _f.check_unpacked(tokens, ctx.mec_tokens)
+        tokens = tokens.contiguous()
     vocab, d, n, code, index, scale, padding_idx, nbytes = ctx.mec
     dy, ldg = (grad_output, d) if grad_output.is_contiguous() else _f._rows(grad_output.reshape(-1, d))
     dw = dy.new_empty((vocab, d))
@@ -68,6 +71,7 @@ class _EmbeddingFn(torch.autograd.Function):
             tokens = tokens.contiguous()
         out = _lookup(tokens, weight, scale)
         ctx.save_for_backward(tokens)
+        ctx.mec_tokens = _f.layout(tokens)
         (vocab, d), n, code = weight.shape, tokens.numel(), _v.code_of(weight)
         ctx.mec = (vocab, d, n, code, weight.device.index, scale, padding_idx,
                    _lib.load().mec_embedding_workspace_bytes(n, vocab, d, code))

@@ -1,5 +1,6 @@
 """Saved-tensor hooks may bring the values that a backward needs back in other memory
 and other strides: what the kernels are told has to be of the tensor that came back."""
+import ctypes
 import gc
 
 import pytest
@@ -136,3 +137,23 @@ def test_the_forwards_gradient_becomes_the_leafs(lib):
     x = logits(lambda x: x)
     mec.TopKDistillationLoss()(x, torch.zeros(4, 6, 2, dtype=torch.int64), torch.zeros(4, 6, 2)).backward()
     assert x.grad.data_ptr() == lib.calls["mec_distill_forward"][0][17]
+
+
+def test_embedding_backward(lib):
+    tokens = torch.arange(12).reshape(3, 4)
+    w = torch.randn(12, 5).requires_grad_(True)
+    read = []
+
+    def backward(*args):
+        read.append(torch.frombuffer(bytearray(ctypes.string_at(args[0], 12 * args[1])), dtype=torch.int64))
+        return 0
+
+    lib.mec_embedding_backward = backward
+    with stub.copying_hooks(lambda t: t.t().contiguous().t()):
+        mec.scaled_embedding(tokens, w).sum().backward()
+    assert torch.equal(read[0], tokens.reshape(-1))
+    for unpack in (lambda t: t.int(), lambda t: t[:2]):
+        with pytest.raises(RuntimeError, match="saved-tensor hook returned"):
+            with stub.copying_hooks(unpack):
+                mec.scaled_embedding(tokens, w).sum().backward()
+    assert len(read) == 1
