@@ -61,7 +61,8 @@ def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     """Tensor with unit column stride and its row stride (elements)."""
     if t.stride(1) != 1 or t.stride(0) < t.shape[1]:
         t = t.contiguous()
-    return t, t.stride(0)
+    # (one row is contiguous whatever its stride)
+    return t, max(t.stride(0), t.shape[1])
 
 
 def layout(t: torch.Tensor) -> tuple:
