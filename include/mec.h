@@ -447,7 +447,8 @@ int mec_token_scores(const void* logits, int64_t rows, int64_t inner, int64_t ou
                      float* top_log_probs, float* state, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Gradient of the logits for the gradients of log_probs and entropy (either may
- * be NULL: zero), from what mec_token_scores left in state and entropy. */
+ * be NULL: zero), from what mec_token_scores left in state and entropy.  A token
+ * outside [0, vocab) makes its row NaN where its gradient of log_probs is not 0. */
 int mec_token_scores_backward(const void* logits, int64_t rows, int64_t inner, int64_t outer_stride,
                               int64_t inner_stride, int64_t vocab, int dtype, const void* tokens, int token_bytes,
                               int64_t ignore_index, float temperature, const float* state, const float* entropy,

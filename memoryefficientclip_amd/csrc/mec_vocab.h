@@ -729,7 +729,9 @@ __global__ __launch_bounds__(kRowThreads) void k_scores_grad(const T* logits, Ro
   else
     v.template load<false>(x0 + base, range.size);
   const Reference ref(stats[r], inv_t * (1.f / kLn2));
-  const float ls = logf(s), gl = bad ? NAN : g_log_probs ? g_log_probs[r] : 0.f, gh = g_entropy ? g_entropy[r] : 0.f;
+  const float ls = logf(s), gh = g_entropy ? g_entropy[r] : 0.f;
+  float gl = g_log_probs ? g_log_probs[r] : 0.f;
+  if (bad && gl != 0.f) gl = NAN;  // (the entropy does not depend on the token)
   // e (a + b t) = -(1/T) p (g_l + g_h (log p + entropy))
   const float f = none ? 0.f : -inv_t / s, a = f * (gl + gh * (entropy[r] - ls)), b = f * gh * kLn2;
   const int at = (int)(bad ? 0 : tok) - base;

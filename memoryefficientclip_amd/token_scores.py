@@ -114,8 +114,9 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, 
       before everything; ``None`` for ``top_k=0``.
 
     Positions whose token is ``ignore_index`` score 0, with top tokens -1, and
-    have no gradient; other tokens outside [0, V) score NaN.  Logits of -inf are
-    tokens that cannot occur; where none can, every log probability is -inf, the
+    have no gradient; other tokens outside [0, V) score NaN (the entropy of their
+    position and its gradient do not depend on them).  Logits of -inf are tokens
+    that cannot occur; where none can, every log probability is -inf, the
     entropy 0 and the gradient 0.
 
     fp32, bf16 and fp16 logits, read in place (any row strides), V up to 2^19 and
