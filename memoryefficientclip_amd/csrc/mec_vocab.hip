@@ -103,12 +103,17 @@ int check_workspace(const void* workspace, int64_t bytes, int64_t need) {
   return MEC_OK;
 }
 
-int check_teacher(const void* tokens, int token_bytes, const void* logits, int dtype, int64_t k) {
-  if (int rc = check_tokens(tokens, token_bytes)) return rc;
-  if (logits == nullptr) return fail(MEC_ERR_INVALID, "teacher_logits must be non-null");
+int check_teacher_k(int64_t k) {
   if (k < 1) return fail(MEC_ERR_INVALID, "k=%lld must be >= 1", (long long)k);
   if (k > MEC_MAX_TEACHER_K)
     return fail(MEC_ERR_UNSUPPORTED, "k=%lld exceeds the maximum %d", (long long)k, MEC_MAX_TEACHER_K);
+  return MEC_OK;
+}
+
+int check_teacher(const void* tokens, int token_bytes, const void* logits, int dtype, int64_t k) {
+  if (int rc = check_tokens(tokens, token_bytes)) return rc;
+  if (logits == nullptr) return fail(MEC_ERR_INVALID, "teacher_logits must be non-null");
+  if (int rc = check_teacher_k(k)) return rc;
   return check_dtype(dtype);
 }
 
@@ -346,8 +351,7 @@ int mec_token_scores_backward(const void* logits, int64_t rows, int64_t inner, i
 int64_t mec_distill_workspace_bytes(int64_t rows, int64_t vocab, int64_t k, int dtype, int with_grad) {
   g_err.clear();
   int rc = check_sizes(rows, vocab, dtype);
-  if (!rc && (k < 1 || k > MEC_MAX_TEACHER_K))
-    rc = fail(MEC_ERR_INVALID, "k=%lld out of range [1, %d]", (long long)k, MEC_MAX_TEACHER_K);
+  if (!rc) rc = check_teacher_k(k);
   return rc ? rc : distill_workspace(rows, vocab, dtype, with_grad != 0).total;
 }
 
