@@ -59,21 +59,24 @@ def check_inputs(x: torch.Tensor, y: torch.Tensor) -> None:
 
 def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     """Tensor with unit column stride and its row stride (elements)."""
-    if t.stride(1) != 1 or t.stride(0) < t.shape[1]:
+    ld, d = t.stride(0), t.shape[1]
+    if t.stride(1) != 1 or ld < d:
         t = t.contiguous()
-    # (one row is contiguous whatever its stride)
-    return t, max(t.stride(0), t.shape[1])
+        ld = max(t.stride(0), d)  # (one row is contiguous whatever its stride)
+    return t, ld
 
 
 def layout(t: torch.Tensor) -> tuple:
-    return t.shape, t.stride(), t.dtype, t.device
+    """What tells in the backward whether a saved tensor came back as it was: a
+    saved-tensor hook (offloading, checkpointing) may bring the values back in other
+    memory with other strides.  (With the strides and the type the same, the bytes
+    stand for the shape: less host time.)"""
+    return t.stride(), t.dtype, t.nbytes, t.device
 
 
-def check_unpacked(t: torch.Tensor, saved: tuple) -> None:
-    """`t` came back for a saved tensor of the `saved` layout: a saved-tensor hook
-    (offloading, checkpointing) may bring the values back in other memory with
-    other strides, and nothing else may differ."""
-    shape, _, dtype, device = saved
+def check_unpacked(t: torch.Tensor, saved: tuple, shape: tuple) -> None:
+    """`t` came back in another layout: only its strides may be others."""
+    _, dtype, _, device = saved
     if t.shape != shape or t.dtype != dtype or t.device != device:
         raise RuntimeError(f"memoryefficientclip_amd: saved a tensor {tuple(shape)} of {dtype} on {device}, and a "
                            f"saved-tensor hook returned {tuple(t.shape)} of {t.dtype} on {t.device}")
@@ -114,13 +117,14 @@ def refuse_graph_capture() -> None:
                            "call it outside the captured region")
 
 
-_dispatch_mode = getattr(torch._C, "_get_dispatch_mode", None)
+_dispatch_mode = getattr(torch._C, "_get_dispatch_mode", lambda key: None)
+_PROXY = getattr(getattr(torch._C, "_TorchDispatchModeKey", None), "PROXY", None)
 
 
 def refuse_make_fx() -> None:
     """Raise under ``make_fx``, which records the tensor operations of a call: here
     the allocation of the results, and nothing that writes them."""
-    if _dispatch_mode is not None and _dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+    if _dispatch_mode(_PROXY) is not None:
         raise RuntimeError("memoryefficientclip_amd: make_fx cannot record these operators; their kernels are started "
                            "past PyTorch's dispatcher")
 
@@ -196,10 +200,10 @@ def backward(ctx, grad_output: torch.Tensor, need_x: bool, need_y: bool):
     ldx, ldy, n, d, dt, mode, normalize, temperature, grad_scale = ctx.mec
     saved_x, saved_y = ctx.mec_saved
     if layout(x) != saved_x:
-        check_unpacked(x, saved_x)
+        check_unpacked(x, saved_x, (n, d))
         x, ldx = _rows(x)
     if layout(y) != saved_y:
-        check_unpacked(y, saved_y)
+        check_unpacked(y, saved_y, (n, d))
         y, ldy = _rows(y)
     if mode & 0xFF == _lib.MODE_LIT:
         need_y = False

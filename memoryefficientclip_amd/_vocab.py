@@ -75,30 +75,34 @@ def rows_of(logits: torch.Tensor) -> tuple[torch.Tensor, int, tuple[int, int, in
     return logits, logits.data_ptr(), (n0 * n1, n1, s0, s1)
 
 
+# (torch.jit.is_tracing, in half of its time)
+is_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
+
+
 def wants_autograd(t: torch.Tensor) -> bool:
     """Whether a call on `t` has to go through its autograd function: where a gradient
     is asked for, where `t` has a tangent, which the function refuses, and in a trace,
     which records the function (of a direct call it records the empty results).
     Otherwise the call is made directly, for less host time."""
-    return ((t.requires_grad and torch.is_grad_enabled()) or forward_ad.unpack_dual(t).tangent is not None
-            or torch.jit.is_tracing())
+    return ((t.requires_grad and torch.is_grad_enabled()) or is_tracing()
+            or (getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None))
 
 
 def save_logits(ctx, held: torch.Tensor, rows: tuple[int, int, int, int], *others: torch.Tensor) -> None:
     """Saves what ``rows_of`` returned for the logits, and other tensors (contiguous)."""
     ctx.save_for_backward(held, *others)
-    ctx.mec_logits = rows, _f.layout(held)
+    ctx.mec_logits = rows, _f.layout(held), held.shape
 
 
-def saved_logits(ctx) -> tuple:
-    """(held, rows, *others) as save_logits had them; the rows are those of the tensor
+def saved_logits(ctx) -> list:
+    """[held, rows, *others] as save_logits had them; the rows are those of the tensor
     that came back."""
     held, *others = ctx.saved_tensors
-    rows, saved = ctx.mec_logits
+    rows, saved, shape = ctx.mec_logits
     if _f.layout(held) != saved:
-        _f.check_unpacked(held, saved)
+        _f.check_unpacked(held, saved, shape)
         held, _, rows = rows_of(held)
-    return held, rows, *(t.contiguous() for t in others)
+    return [held, rows, *[t.contiguous() for t in others]]
 
 
 class _Once(torch.autograd.Function):

@@ -91,11 +91,12 @@ def _logits_grad(ctx, grad_output):
 class _DistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, rows, teacher_tokens, teacher_logits, temperature, weight, reduction):
+        need = True
         if rows is None:
             _check(logits, teacher_tokens, teacher_logits)
+            need = ctx.needs_input_grad[0]
             logits, _, rows = _v.rows_of(logits)
-        loss, kept = _loss(logits, rows, teacher_tokens, teacher_logits, temperature, weight, reduction,
-                           ctx.needs_input_grad[0])
+        loss, kept = _loss(logits, rows, teacher_tokens, teacher_logits, temperature, weight, reduction, need)
         _v.save_logits(ctx, *kept[0])
         ctx.mec, ctx.made = kept[1], len(kept[0]) > 5
         return loss
@@ -141,7 +142,7 @@ class TopKDistillationLoss(nn.Module):
         args = (teacher_tokens, teacher_logits.detach(), self.temperature, self.weight, reduction)
         if _v.wants_autograd(student_logits):
             # (a trace calls this again, with other inputs)
-            return _DistillFn.apply(student_logits, None if torch.jit.is_tracing() else rows, *args)
+            return _DistillFn.apply(student_logits, None if _v.is_tracing() else rows, *args)
         return _loss(student_logits, rows, *args, False)[0]
 
 

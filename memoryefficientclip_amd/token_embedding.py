@@ -25,12 +25,13 @@ def _check(tokens, weight):
     _v.refuse_make_fx()
     _v.check_float("weight", weight)
     _v.check_tokens("tokens", tokens)
-    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
-        raise ValueError(f"weight must be [V, D] with V, D >= 1, got {tuple(weight.shape)}")
-    vocab, d = weight.shape
-    if vocab > _MAX_VOCAB or d > _MAX_DIM or tokens.numel() > _MAX_TOKENS:
-        raise ValueError(f"{tokens.numel()} tokens of {vocab} x {d} exceed the maxima {_MAX_TOKENS}, {_MAX_VOCAB} x "
-                         f"{_MAX_DIM}")
+    shape, n = weight.shape, tokens.numel()
+    if len(shape) != 2 or shape[0] < 1 or shape[1] < 1:
+        raise ValueError(f"weight must be [V, D] with V, D >= 1, got {tuple(shape)}")
+    vocab, d = shape
+    if vocab > _MAX_VOCAB or d > _MAX_DIM or n > _MAX_TOKENS:
+        raise ValueError(f"{n} tokens of {vocab} x {d} exceed the maxima {_MAX_TOKENS}, {_MAX_VOCAB} x {_MAX_DIM}")
+    return vocab, d, n
 
 
 def _lookup(tokens, weight, scale):
@@ -48,8 +49,9 @@ def _lookup(tokens, weight, scale):
 
 def _weight_grad(ctx, grad_output):
     tokens, = ctx.saved_tensors
-    if _f.layout(tokens) != ctx.mec_tokens:
-        _f.check_unpacked(tokens, ctx.mec_tokens)
+    saved, shape = ctx.mec_tokens
+    if _f.layout(tokens) != saved:
+        _f.check_unpacked(tokens, saved, shape)
         tokens = tokens.contiguous()
     vocab, d, n, code, index, scale, padding_idx, nbytes = ctx.mec
     dy, ldg = (grad_output, d) if grad_output.is_contiguous() else _f._rows(grad_output.reshape(-1, d))
@@ -71,7 +73,7 @@ class _EmbeddingFn(torch.autograd.Function):
             tokens = tokens.contiguous()
         out = _lookup(tokens, weight, scale)
         ctx.save_for_backward(tokens)
-        ctx.mec_tokens = _f.layout(tokens)
+        ctx.mec_tokens = _f.layout(tokens), tokens.shape
         (vocab, d), n, code = weight.shape, tokens.numel(), _v.code_of(weight)
         ctx.mec = (vocab, d, n, code, weight.device.index, scale, padding_idx,
                    _lib.load().mec_embedding_workspace_bytes(n, vocab, d, code))
@@ -90,8 +92,7 @@ def scaled_embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 
     looked up like any other).  A token outside [0, V) gives a row of NaN and
     has no part in the gradient.  Up to 2^23 tokens, V up to 2^22, D up to 2^16.
     """
-    _check(tokens, weight)
-    vocab, d = weight.shape
+    vocab, d, n = _check(tokens, weight)
     scale = float(scale)
     if not math.isfinite(scale):
         raise ValueError(f"scale must be finite, got {scale}")
@@ -101,11 +102,11 @@ def scaled_embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 
         raise ValueError(f"padding_idx must be in [{-vocab}, {vocab}), got {padding_idx}")
     elif padding_idx < 0:
         padding_idx += vocab
-    if tokens.numel() == 0:
+    if n == 0:
         return weight[:0].sum() * scale + torch.empty((*tokens.shape, d), dtype=weight.dtype, device=weight.device)
     tokens = tokens.contiguous()
     if _v.wants_autograd(weight):
-        return _EmbeddingFn.apply(tokens, weight, scale, int(padding_idx), torch.jit.is_tracing())
+        return _EmbeddingFn.apply(tokens, weight, scale, int(padding_idx), _v.is_tracing())
     return _lookup(tokens, weight, scale)
 
 

@@ -132,7 +132,7 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, 
     logits, _, rows = _v.rows_of(logits)
     if _v.wants_autograd(logits):
         # (a trace calls this again, with other inputs)
-        rows = None if torch.jit.is_tracing() else rows
+        rows = None if _v.is_tracing() else rows
         return TokenScores(*_TokenScoresFn.apply(logits, rows, tokens, top_k, temperature, int(ignore_index)))
     return TokenScores(*_scores(logits, rows, tokens, top_k, temperature, int(ignore_index), False)[0])
 
