@@ -480,12 +480,13 @@ __device__ __forceinline__ void write_ignored(const ScoresOut& out, int64_t r, i
 // One workgroup per segment of a row.  With one segment the row's results, else
 // parts[row][seg] = (m, S, U) and the segment's top k keys.
 //
-// Bound by the read and by the vector unit about alike: a value costs an unpack
-// twice (maximum, sums), half a maximum, three fma-like operations and an
-// exponential, which takes four times their cycles.  256 threads and 8 vectors each:
-// 51 to 67 registers, so that seven or eight workgroups share a CU and one's sums
-// hide the others' loads.  8192 x 49408 bf16 in 138 us (5.9 TB/s); with the 32 top
-// tokens, 4096 x 131072 bf16, a tenth of them ignored, 190 us (5.1 TB/s).
+// Bound by the vector unit, busy 93% of the time (98% with top tokens), with the read
+// close behind: 10 instructions a value (14 with 32 top tokens), the exponential for
+// two: an unpack twice (maximum, sums), half a maximum, three fma-like operations and
+// what goes round them.  256 threads and 8 vectors each: 51 to 67 registers, so that
+// seven or eight workgroups share a CU and one's sums hide the others' loads.  8192 x
+// 49408 bf16 in 138 us (5.9 TB/s); with the 32 top tokens, 4096 x 131072 bf16, a tenth
+// of them ignored, 190 us (5.1 TB/s).
 template <class T, bool TOP>
 __global__ __launch_bounds__(kRowThreads) void k_scores(const T* logits, RowMap map, int n, Tokens tokens,
                                                         int64_t ignore, float inv_t, int k, ScoresOut out,
@@ -892,13 +893,13 @@ struct DistillState {
 // row is one segment and stays in registers from its only read to the gradient's
 // write.  Of a longer row the last segment stays in registers, the one before it in
 // LDS and the one before that in registers again (192 KB of a row with 512 threads,
-// 384 KB with 1024); what is left is read a second time.  Bound by memory: with
-// ONE or 512 threads two or more workgroups share a CU, so that one reads while the
-// other writes (8192 x 49408 bf16, a quarter without a teacher: 288 us, 4.9 TB/s;
-// 8192 x 70001: 512 us, 4.5 TB/s; 4096 x 200000, half of the row read twice, from
-// the cache past L2: 705 us, 4.6 TB/s of the first reads and the writes); 1024
-// threads with more than a segment have the CU to themselves (1024 x 400000 bf16:
-// 412 us, 4.0 TB/s).  Which of the two: row_shape.
+// 384 KB with 1024); what is left is read a second time.  Bound by memory (the vector
+// unit is busy 75 to 82% of the time): with ONE or 512 threads two or more workgroups
+// share a CU, so that one reads while the other writes (8192 x 49408 bf16, a quarter
+// without a teacher: 288 us, 4.9 TB/s; 8192 x 70001: 512 us, 4.5 TB/s; 4096 x 200000,
+// half of the row read twice: 2.5 GB past L2 and 1.7 written in 705 us, 4.6 TB/s
+// without the second reads); 1024 threads with more than a segment have the CU to
+// themselves (1024 x 400000 bf16: 412 us, 4.0 TB/s).  Which of the two: row_shape.
 template <class T, int THREADS, bool ONE, bool PAST>
 __global__ __launch_bounds__(THREADS, ONE ? 1 : 4) void k_distill_row(
     const T* logits, RowMap map, int n, Teacher teacher, float inv_t, float scale, TeacherRows have, int mean,

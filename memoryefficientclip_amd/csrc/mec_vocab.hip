@@ -186,10 +186,11 @@ RowShape row_shape(int64_t vocab, int dtype, bool aligned) {
   for (int threads = 256; threads <= 1024; threads *= 2)
     if (vocab + (aligned ? 0 : 1) <= vec * kSegChunks * threads) return RowShape{threads, 1, (int)vocab};
   // Two workgroups of 512 threads on a CU read and write at the same time, one of
-  // 1024 holds twice as much of a row.  512 / 1024 threads, bf16: 8192 x 70001 512 /
-  // 697 us, 4096 x 128256 442 / 508, 4096 x 200000 705 / 729, 4096 x 212000 794 / 760,
-  // 2048 x 250002 530 / 483; fp32 (half the arithmetic a byte): 4096 x 36000 239 /
-  // 297, 4096 x 49408 342 / 368, 2048 x 70000 262 / 258, 2048 x 100003 403 / 378.
+  // 1024 holds twice as much of a row.  512 / 1024 threads, with rows for every CU
+  // (fewer were not compared), bf16: 8192 x 70001 512 / 697 us, 4096 x 128256 442 /
+  // 508, 4096 x 200000 705 / 729, 4096 x 212000 794 / 760, 2048 x 250002 530 / 483;
+  // fp32 (half the arithmetic a byte): 4096 x 36000 239 / 297, 4096 x 49408 342 / 368,
+  // 2048 x 70000 262 / 258, 2048 x 100003 403 / 378.
   const int threads = vocab <= (dtype == MEC_DTYPE_F32 ? 65536 : 204800) ? 512 : 1024;
   // (the first segment may begin off a boundary, and end up to a vector later for it)
   const int64_t len = vec * kSegChunks * threads - (aligned ? 0 : vec);
