@@ -82,6 +82,13 @@ def check_unpacked(t: torch.Tensor, saved: tuple, shape: tuple) -> None:
                            f"saved-tensor hook returned {tuple(t.shape)} of {t.dtype} on {t.device}")
 
 
+def check_unpacked_bytes(t: torch.Tensor, nbytes: int) -> None:
+    """For a tensor that the kernels read as one piece in the form that it was saved in."""
+    if t.nbytes != nbytes:
+        raise RuntimeError(f"memoryefficientclip_amd: saved a tensor of {nbytes} bytes, and a saved-tensor hook "
+                           f"returned {tuple(t.shape)} of {t.dtype}, {t.nbytes} bytes")
+
+
 # the current stream's handle without building a torch.cuda.Stream object
 # (about 2 us of host time per call at N = 1024, where the step is host-bound)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -187,7 +194,7 @@ def forward(ctx, x: torch.Tensor, y: torch.Tensor, temperature: float, mode: int
     if rc:
         raise _lib.error("mec_forward", rc)
     ctx.save_for_backward(x, y, ws)
-    ctx.mec_saved = layout(x), layout(y)
+    ctx.mec_saved = layout(x), layout(y), ws.nbytes
     ctx.mec = (ldx, ldy, n, d, dt, mode, int(normalize), temperature,
                math.sqrt(n / temperature) if stable else 1.0 / temperature)
     return loss
@@ -198,7 +205,9 @@ def backward(ctx, grad_output: torch.Tensor, need_x: bool, need_y: bool):
     refuse_graph_capture()
     x, y, ws = ctx.saved_tensors
     ldx, ldy, n, d, dt, mode, normalize, temperature, grad_scale = ctx.mec
-    saved_x, saved_y = ctx.mec_saved
+    saved_x, saved_y, ws_bytes = ctx.mec_saved
+    check_unpacked_bytes(ws, ws_bytes)
+    ws = ws.contiguous()
     if layout(x) != saved_x:
         check_unpacked(x, saved_x, (n, d))
         x, ldx = _rows(x)

@@ -91,17 +91,20 @@ def wants_autograd(t: torch.Tensor) -> bool:
 def save_logits(ctx, held: torch.Tensor, rows: tuple[int, int, int, int], *others: torch.Tensor) -> None:
     """Saves what ``rows_of`` returned for the logits, and other tensors (contiguous)."""
     ctx.save_for_backward(held, *others)
-    ctx.mec_logits = rows, _f.layout(held), held.shape
+    ctx.mec_logits = rows, _f.layout(held), held.shape, [t.nbytes for t in others]
 
 
 def saved_logits(ctx) -> list:
     """[held, rows, *others] as save_logits had them; the rows are those of the tensor
     that came back."""
     held, *others = ctx.saved_tensors
-    rows, saved, shape = ctx.mec_logits
+    rows, saved, shape, nbytes = ctx.mec_logits
     if _f.layout(held) != saved:
         _f.check_unpacked(held, saved, shape)
         held, _, rows = rows_of(held)
+    if [t.nbytes for t in others] != nbytes:
+        for t, n in zip(others, nbytes):
+            _f.check_unpacked_bytes(t, n)
     return [held, rows, *[t.contiguous() for t in others]]
 
 

@@ -9,7 +9,7 @@ from memoryefficientclip_amd import _function, _lib, _vocab
 
 class Library:
     """Records calls: ``calls[name]`` is the list of their arguments.  No call wants scratch, and the
-    contrastive losses' plan is a workspace of one number in the inputs' own type."""
+    contrastive losses' plan is a workspace of one number."""
 
     def __init__(self):
         self.calls = {}

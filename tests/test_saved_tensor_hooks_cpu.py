@@ -157,3 +157,25 @@ def test_embedding_backward(lib):
             with stub.copying_hooks(unpack):
                 mec.scaled_embedding(tokens, w).sum().backward()
     assert len(read) == 1
+
+
+def narrow(t):
+    """What is held in 32 bits or more comes back in half of them."""
+    return t.to({torch.float32: torch.float16, torch.int64: torch.int32}.get(t.dtype, t.dtype))
+
+
+@pytest.mark.parametrize("kinds", [{torch.float32}, {torch.int64}])
+def test_other_tensors_than_the_logits_are_refused_too(lib, kinds):
+    """bf16 logits come back as they were, and what is saved beside them in fewer bytes than the kernels read."""
+    x = torch.randn(4, 6, 50).bfloat16().requires_grad_(True)
+    tokens, z = torch.zeros(4, 6, 2, dtype=torch.int64), torch.zeros(4, 6, 2)
+    calls = [lambda: mec.token_log_probs(x, tokens[..., 0]).entropy, lambda: mec.TopKDistillationLoss()(x, tokens, z),
+             lambda: mec.TopKDistillationLoss(reduction="none")(x, tokens, z)]
+    if torch.float32 in kinds:
+        y = torch.randn(10, 8).bfloat16().requires_grad_(True)
+        calls.append(lambda: mec.MemoryEfficientCLIPLoss()(y, y))
+    for call in calls:
+        with pytest.raises(RuntimeError, match="saved-tensor hook returned"):
+            with stub.copying_hooks(lambda t: narrow(t) if t.dtype in kinds else t):
+                call().sum().backward()
+    assert not any(name.endswith("_backward") for name in lib.calls)
