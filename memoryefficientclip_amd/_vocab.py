@@ -55,8 +55,12 @@ def rows_of(logits: torch.Tensor) -> tuple[torch.Tensor, int, tuple[int, int, in
     """(tensor to hold, data pointer, (rows, inner, outer stride, inner stride)) of
     logits [..., V]: read in place where the rows lie on a grid of two strides (any
     2-d tensor with unit column stride, slices of a 3-d one), else copied."""
+    if logits.is_contiguous():
+        vocab = logits.shape[-1]
+        rows = logits.numel() // vocab
+        return logits, logits.data_ptr(), (rows, 1, vocab if rows > 1 else 0, 0)
     if logits.stride(-1) != 1 and logits.shape[-1] > 1:
-        logits = logits.contiguous()
+        return rows_of(logits.contiguous())
     dims = [(n, s) for n, s in zip(logits.shape[:-1], logits.stride()[:-1]) if n != 1]
     # neighbouring dimensions that are one
     merged: list[tuple[int, int]] = []

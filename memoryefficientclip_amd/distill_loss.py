@@ -30,13 +30,14 @@ def _check(student_logits, teacher_tokens, teacher_logits):
     _v.check_float("student_logits", student_logits)
     _v.check_float("teacher_logits", teacher_logits)
     _v.check_tokens("teacher_tokens", teacher_tokens)
-    if teacher_tokens.shape != teacher_logits.shape:
-        raise ValueError(f"teacher_tokens {tuple(teacher_tokens.shape)} and teacher_logits "
-                         f"{tuple(teacher_logits.shape)} differ in shape")
-    if min(student_logits.dim(), teacher_tokens.dim()) < 1 or student_logits.shape[:-1] != teacher_tokens.shape[:-1]:
-        raise ValueError(f"student_logits {tuple(student_logits.shape)} and teacher_tokens "
-                         f"{tuple(teacher_tokens.shape)} need the same positions")
-    vocab, k = student_logits.shape[-1], teacher_tokens.shape[-1]
+    shape, teacher_shape = student_logits.shape, teacher_tokens.shape
+    if teacher_shape != teacher_logits.shape:
+        raise ValueError(f"teacher_tokens {tuple(teacher_shape)} and teacher_logits {tuple(teacher_logits.shape)} differ "
+                         f"in shape")
+    if min(len(shape), len(teacher_shape)) < 1 or shape[:-1] != teacher_shape[:-1]:
+        raise ValueError(f"student_logits {tuple(shape)} and teacher_tokens {tuple(teacher_shape)} need the same "
+                         f"positions")
+    vocab, k = shape[-1], teacher_shape[-1]
     if not 1 <= vocab <= _lib.MAX_VOCAB:
         raise ValueError(f"the vocabulary must have 1 to {_lib.MAX_VOCAB} tokens, got {vocab}")
     if not 1 <= k <= _lib.MAX_TEACHER_K:
@@ -47,15 +48,16 @@ def _loss(logits, rows, teacher_tokens, teacher_logits, temperature, weight, red
     """The loss, and with `need` what the backward needs; logits and their rows as ``rows_of`` has them."""
     code, teacher_code, token_bytes = _v.code_of(logits), _v.code_of(teacher_logits), teacher_tokens.element_size()
     teacher_tokens, teacher_logits = teacher_tokens.contiguous(), teacher_logits.contiguous()
-    vocab, k, dev = logits.shape[-1], teacher_tokens.shape[-1], logits.device
-    loss = torch.empty(logits.shape[:-1] if reduction == _lib.REDUCE_NONE else (), dtype=torch.float32, device=dev)
+    shape, k, dev = logits.shape, teacher_tokens.shape[-1], logits.device
+    vocab = shape[-1]
+    loss = torch.empty(shape[:-1] if reduction == _lib.REDUCE_NONE else (), dtype=torch.float32, device=dev)
     state = torch.empty(2 * rows[0] + 1, dtype=torch.float32, device=dev)
     # The gradient for grad_output 1 is made while the row is at hand: the
     # logits are read once for loss and gradient.  fp16 programs scale their
     # losses, so there grad_output is not 1 and the backward makes it.
     dx = None
     if need and reduction != _lib.REDUCE_NONE and logits.dtype != torch.float16:
-        dx = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        dx = torch.empty(shape, dtype=logits.dtype, device=dev)
     lib = _lib.load()
     nbytes = lib.mec_distill_workspace_bytes(rows[0], vocab, k, code, int(dx is not None))
     rc = _v.launch(dev.index, nbytes, lambda ws, stream: lib.mec_distill_forward(

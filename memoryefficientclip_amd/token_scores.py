@@ -32,11 +32,12 @@ def _check(logits, tokens, top_k):
     _v.check_gpu("tokens", tokens, logits.device)
     _v.refuse_graph_capture()
     _v.refuse_make_fx()
-    if logits.dim() < 1 or logits.shape[:-1] != tokens.shape:
-        raise ValueError(f"logits {tuple(logits.shape)} need one row for each of the tokens {tuple(tokens.shape)}")
+    shape = logits.shape
+    if len(shape) < 1 or shape[:-1] != tokens.shape:
+        raise ValueError(f"logits {tuple(shape)} need one row for each of the tokens {tuple(tokens.shape)}")
     _v.check_float("logits", logits)
     _v.check_tokens("tokens", tokens)
-    vocab, top_k = logits.shape[-1], int(top_k)
+    vocab, top_k = shape[-1], int(top_k)
     if not 1 <= vocab <= _lib.MAX_VOCAB:
         raise ValueError(f"the vocabulary must have 1 to {_lib.MAX_VOCAB} tokens, got {vocab}")
     if not 0 <= top_k <= min(vocab, _lib.MAX_TOP_K):
