@@ -1,6 +1,7 @@
 /*
  * mec.h — C ABI of the MI355X (gfx950) memory-efficient CLIP / LiT loss, and of
- * operators over a vocabulary for the text tower (the last part).
+ * operators over a vocabulary for the text tower and of the towers' attention
+ * (the last two parts).
  *
  * This library replaces the four Triton kernels and the PyTorch glue of the
  * reference's autograd Functions (b0nce/MemoryEfficientCLIP):
@@ -505,6 +506,109 @@ int64_t mec_embedding_workspace_bytes(int64_t n, int64_t vocab, int64_t d, int d
 int mec_embedding_backward(const void* tokens, int token_bytes, int64_t n, const void* grad_out, int64_t ldg,
                            int64_t vocab, int64_t d, int dtype, float scale, int64_t padding_idx, void* grad_weight,
                            void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- The attention of a tower ----
+ *
+ * The rotation of queries and keys by positions on several axes, with the norm
+ * of each head in the same pass, and attention, each with its gradient.  No
+ * counterpart in the reference.  The conventions above hold (error codes,
+ * streams, no allocation, no synchronisation, no graph capture), and:
+ *   - heads: [batch, tokens, heads, head_dim] with unit stride of the features
+ *     and any other strides >= 0 (in elements), at any alignment (mec_heads_t).
+ *     Results are written without gaps in this order.
+ *   - dtype: MEC_DTYPE_F32, MEC_DTYPE_BF16 or MEC_DTYPE_F16; sums, norms and the
+ *     softmax's statistics are held in fp32, angles in 64 bits.
+ *   - all results are deterministic. */
+typedef struct {
+  const void* data;
+  int64_t batch_stride, token_stride, head_stride;
+} mec_heads_t;
+
+#define MEC_MAX_AXES 8
+#define MEC_POSITION_INT32 0
+#define MEC_POSITION_INT64 1
+#define MEC_POSITION_F32 2
+
+/* With norm, a head is first divided by sqrt(mean x^2 + eps) and multiplied by
+ * its side's weight (head_dim values, NULL: ones).  Its head_dim / 2 pairs are
+ * (x[p], x[p + head_dim / 2]), or (x[2p], x[2p + 1]) if interleaved; the first
+ * sections[0] pairs belong to axis 0, the next sections[1] to axis 1, and so on.
+ * Pair p is turned by position * frequency: (a cos - b sin, b cos + a sin);
+ * frequencies: head_dim / 2 doubles on the device (radians per position; 0 leaves
+ * a pair as it is), or NULL: theta^(-j / n) for the j-th of an axis's n pairs.
+ * positions: [tokens, axes], or [batch, tokens, axes] if positions_per_batch.
+ * A side with no heads is left out.  Up to 2^31 - 1 tokens, head_dim even and
+ * <= 256, 2^16 heads. */
+typedef struct {
+  int64_t batch, tokens, query_heads, key_heads, head_dim;
+  int32_t dtype, weight_dtype, norm, interleaved;
+  float eps;
+  int32_t axes, sections[MEC_MAX_AXES];
+  int32_t position_type, positions_per_batch;
+  double theta;
+  const void *query_weight, *key_weight, *positions;
+  const double* frequencies;
+} mec_rotary_t;
+
+/* out_query [batch, tokens, query_heads, head_dim] and out_key. */
+int mec_norm_rotary(const mec_rotary_t* rotary, const mec_heads_t* query, const mec_heads_t* key, void* out_query,
+                    void* out_key, void* stream);
+
+/* Bytes of mec_norm_rotary_backward's workspace (16-byte aligned) where a weight's
+ * gradient is asked for, on the current device; < 0 on bad arguments. */
+int64_t mec_norm_rotary_workspace_bytes(const mec_rotary_t* rotary);
+
+/* Gradients of query, key (without gaps) and of the weights (weight_dtype, head_dim
+ * values) for those of out_query and out_key.  With norm each may be NULL: not
+ * asked for; without, query and key are not read and may be NULL, and there are no
+ * weights. */
+int mec_norm_rotary_backward(const mec_rotary_t* rotary, const mec_heads_t* query, const mec_heads_t* key,
+                             const mec_heads_t* grad_out_query, const mec_heads_t* grad_out_key, void* grad_query,
+                             void* grad_key, void* grad_query_weight, void* grad_key_weight, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+
+/* softmax(scale query key^T) value over the keys that a query sees.
+ * query [batch, queries, heads, head_dim], key and value [batch, keys, key_heads,
+ * head_dim]; head h looks at key head h / (heads / key_heads), key_heads divides
+ * heads.  query_lengths, key_lengths: batch values each (length_bytes 4 or 8 a
+ * value), NULL: all full; values are taken into [0, queries], [0, keys].  Queries
+ * and keys at or beyond their length are not read: such a query's result and
+ * gradient, and such a key's gradient, are 0.  causal: query i of nq sees the keys
+ * j <= i + nk - nq of nk (lengths: the last query sees the last key).  A query that
+ * sees no key, or only scores of -inf, has result 0 and gradient 0, and no key or
+ * value that it does not see has a part in its result, whatever it holds.
+ * head_dim 1 to 128; batch * key_heads, queries * heads / key_heads and keys at most
+ * 2^30; scale finite and > 0. */
+#define MEC_MAX_HEAD_DIM 128
+typedef struct {
+  int64_t batch, queries, keys, heads, key_heads, head_dim;
+  int32_t dtype, causal;
+  float scale;
+  int32_t length_bytes;
+  const void *query_lengths, *key_lengths;
+} mec_attention_t;
+
+/* Bytes of mec_attention's workspace (16-byte aligned), on the current device; 0:
+ * none; < 0 on bad arguments. */
+int64_t mec_attention_workspace_bytes(const mec_attention_t* attention);
+
+/* out [batch, queries, heads, head_dim]; lse: NULL, or batch * heads * queries floats
+ * for mec_attention_backward. */
+int mec_attention(const mec_attention_t* attention, const mec_heads_t* query, const mec_heads_t* key,
+                  const mec_heads_t* value, void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                  void* stream);
+
+/* Bytes of mec_attention_backward's workspace (16-byte aligned), on the current
+ * device; < 0 on bad arguments. */
+int64_t mec_attention_backward_workspace_bytes(const mec_attention_t* attention);
+
+/* Gradients of query, key and value (without gaps) for that of out, from what
+ * mec_attention left in out and lse.  grad_query, or grad_key and grad_value, may be
+ * NULL: not asked for. */
+int mec_attention_backward(const mec_attention_t* attention, const mec_heads_t* query, const mec_heads_t* key,
+                           const mec_heads_t* value, const void* out, const float* lse, const mec_heads_t* grad_out,
+                           void* grad_query, void* grad_key, void* grad_value, void* workspace,
+                           int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

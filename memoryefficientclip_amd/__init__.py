@@ -5,7 +5,7 @@ Drop-in replacement for b0nce/MemoryEfficientCLIP's ``clip_loss`` and
 backed by hand-written HIP kernels in ``lib/libmec.so`` (C ABI:
 ``include/mec.h``).  Beside it, the vocabulary side of the text tower: scaled
 token embedding, token log probabilities and distillation from a teacher's top
-logits.
+logits; and the towers' attention, with the rotation of its queries and keys.
 """
 from .clip_loss import (
     MemoryEfficientCLIPLoss,
@@ -22,6 +22,8 @@ from .lit_loss import (
 )
 from .token_embedding import ScaledTokenEmbedding, scaled_embedding
 from .token_scores import TokenScores, token_log_probs
+from .tower_attention import attention
+from .tower_rotary import norm_rotary
 
 __version__ = "0.1.0"
 
@@ -37,6 +39,8 @@ __all__ = [
     "ScaledTokenEmbedding",
     "TokenScores",
     "TopKDistillationLoss",
+    "attention",
+    "norm_rotary",
     "scaled_embedding",
     "token_log_probs",
 ]

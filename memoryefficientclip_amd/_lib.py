@@ -80,6 +80,13 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "mec_embedding_workspace_bytes": (_i64, [_i64, _i64, _i64, _int]),
     "mec_embedding_backward": (_int, [_vp, _int, _i64, _vp, _i64, _i64, _i64, _int, _f32, _i64, _vp, _vp, _i64,
                                       _vp]),
+    "mec_norm_rotary": (_int, [_vp, _vp, _vp, _vp, _vp, _vp]),
+    "mec_norm_rotary_workspace_bytes": (_i64, [_vp]),
+    "mec_norm_rotary_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "mec_attention_workspace_bytes": (_i64, [_vp]),
+    "mec_attention": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "mec_attention_backward_workspace_bytes": (_i64, [_vp]),
+    "mec_attention_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
 }
 MAX_VOCAB = 1 << 19  # MEC_MAX_VOCAB
 MAX_TOP_K = 128  # MEC_MAX_TOP_K
@@ -94,6 +101,33 @@ class BackwardPlan(ctypes.Structure):
                 ("noalloc_block_rows", ctypes.c_int64), ("noalloc_scratch_bytes", ctypes.c_int64),
                 ("contract_tile_rows", ctypes.c_int32), ("contract_tile_features", ctypes.c_int32),
                 ("narrow_tiles", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+MAX_AXES = 8  # MEC_MAX_AXES
+MAX_HEAD_DIM = 128  # MEC_MAX_HEAD_DIM
+
+
+class Heads(ctypes.Structure):
+    """mec_heads_t (include/mec.h)."""
+    _fields_ = [("data", _vp), ("batch_stride", _i64), ("token_stride", _i64), ("head_stride", _i64)]
+
+
+class Rotary(ctypes.Structure):
+    """mec_rotary_t (include/mec.h)."""
+    _fields_ = [("batch", _i64), ("tokens", _i64), ("query_heads", _i64), ("key_heads", _i64), ("head_dim", _i64),
+                ("dtype", ctypes.c_int32), ("weight_dtype", ctypes.c_int32), ("norm", ctypes.c_int32),
+                ("interleaved", ctypes.c_int32), ("eps", _f32), ("axes", ctypes.c_int32),
+                ("sections", ctypes.c_int32 * MAX_AXES), ("position_type", ctypes.c_int32),
+                ("positions_per_batch", ctypes.c_int32), ("theta", ctypes.c_double), ("query_weight", _vp),
+                ("key_weight", _vp), ("positions", _vp), ("frequencies", _vp)]
+
+
+class Attention(ctypes.Structure):
+    """mec_attention_t (include/mec.h)."""
+    _fields_ = [("batch", _i64), ("queries", _i64), ("keys", _i64), ("heads", _i64), ("key_heads", _i64),
+                ("head_dim", _i64), ("dtype", ctypes.c_int32), ("causal", ctypes.c_int32), ("scale", _f32),
+                ("length_bytes", ctypes.c_int32), ("query_lengths", _vp), ("key_lengths", _vp)]
+
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

@@ -1,6 +1,6 @@
-"""Host side shared by the operators over a vocabulary: argument checks, the
-layout of logits, scratch and the calls into the HIP library
-(``include/mec.h``)."""
+"""Host side shared by the operators over a vocabulary, and in part by those of a
+tower's attention: argument checks, the layout of logits, scratch and the calls
+into the HIP library (``include/mec.h``)."""
 from __future__ import annotations
 
 import torch
@@ -121,7 +121,7 @@ class _Once(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad):
-        raise RuntimeError("memoryefficientclip_amd: the operators over a vocabulary cannot be differentiated twice")
+        raise RuntimeError("memoryefficientclip_amd: these operators cannot be differentiated twice")
 
 
 def backward_of(grad):
@@ -162,5 +162,19 @@ def launch(index: int, nbytes: int, call) -> int:
     finally:
         if ws is not None:
             torch.cuda.caching_allocator_delete(ws)
+        if cur != index:
+            torch.cuda.set_device(cur)
+
+
+def launch_sized(index: int, size, call) -> int:
+    """``launch`` with the scratch that ``size()`` asks for on device `index`:
+    ``call(workspace, nbytes, stream)``."""
+    cur = torch.cuda.current_device()
+    if cur != index:
+        torch.cuda.set_device(index)
+    try:
+        nbytes = size()
+        return launch(index, nbytes, lambda ws, stream: call(ws, nbytes, stream))
+    finally:
         if cur != index:
             torch.cuda.set_device(cur)

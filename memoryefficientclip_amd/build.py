@@ -45,7 +45,7 @@ def hipcc() -> str:
 
 
 def sources() -> list[Path]:
-    return [CSRC / "mec_abi.hip", CSRC / "mec_vocab.hip"]
+    return [CSRC / f"{name}.hip" for name in ("mec_abi", "mec_vocab", "mec_rotary", "mec_attention")]
 
 
 def _run(cmd: list[str], verbose: bool) -> None:

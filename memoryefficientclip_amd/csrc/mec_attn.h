@@ -1,0 +1,296 @@
+// Attention on the MFMA cores: what its forward and backward kernels share.
+//
+//   s_ij = scale q_i . k_j,  p_ij = exp(s_ij) / sum over the keys that i sees,
+//   o_i = sum_j p_ij v_j
+// and for a gradient do of o, with delta_i = do_i . o_i,
+//   dv_j = sum_i p_ij do_i,  ds_ij = p_ij (do_i . v_j - delta_i),
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i.
+// No matrix of scores is kept: the forward leaves one number a row,
+// lse_i = log2 sum_j exp(s_ij), from which the backward makes p_ij anew.
+//
+// Tiles.  A wave works on 32 rows of its own ("columns" of the MFMA's result,
+// one a lane: lanes l and l + 32 share one) against blocks of 32 rows of a tile
+// in LDS.  v_mfma_f32_32x32x16 leaves a lane 16 of the 32 block rows,
+// 8 (i / 4) + 4 (l / 32) + i % 4 in register i.  As the next product sums over
+// just these rows, in any order that both operands share, registers 8 s .. 8 s + 7
+// rounded to 16 bits are its right operand as they stand, and its left operand,
+// the other tile transposed, is read from LDS in that order by
+// ds_read_b64_tr_b16: probabilities never leave their lane.  fp32 runs the same
+// kernels on v_mfma_f32_32x32x2, eight to a step of 16.
+//
+// LDS holds a tile as rows of VPR 16-byte vectors, vector v of row r in place
+// v ^ swz(r): 16 rows at one vector (row reads) lie in 16 different groups of 4
+// banks, and so do 4 rows by 4 vectors (transposed reads).
+#pragma once
+#include "mec_vec.h"
+
+namespace mec {
+namespace attn {
+
+constexpr uint32_t OOB = 0x80000000u;  // buffer offset that reads as zero
+constexpr float kInf = __builtin_inff();
+constexpr float kLog2e = 1.44269504088896340736f;
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char Lds;
+
+// Heads as the callers give them: element (b, t, h, i) at p[b * batch + t * token + h * head + i].
+struct View {
+  const void* p;
+  int64_t batch, token, head;
+};
+
+struct Problem {
+  View q, k, v, g;  // g: the gradient of the result
+  int queries, keys, heads, key_heads, group, d;
+  int64_t pairs;    // batch * key_heads
+  int causal;
+  float scale, c;   // c = scale log2(e)
+  const void *query_lengths, *key_lengths;
+  int length64;
+  // number of queries and keys of batch entry b, each within what there is
+  __device__ __forceinline__ int length(const void* p, int64_t b, int all) const {
+    if (p == nullptr) return all;
+    const int64_t n = length64 ? ((const int64_t*)p)[b] : (int64_t)((const int32_t*)p)[b];
+    return n < 0 ? 0 : n > all ? all : (int)n;
+  }
+  __device__ __forceinline__ int nq(int64_t b) const { return length(query_lengths, b, queries); }
+  __device__ __forceinline__ int nk(int64_t b) const { return length(key_lengths, b, keys); }
+};
+
+// Workgroup id in a launch of `n` (a multiple of 8, over x and y), such that
+// neighbouring ids run on one XCD and share what they read in its L2; n or more
+// for the workgroups beyond.
+__device__ __forceinline__ int64_t group_id(int64_t n) {
+  const int64_t bid = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  return bid < n ? (bid & 7) * (n >> 3) + (bid >> 3) : n;
+}
+
+// 8 consecutive k of a row or column, and the products of 32 x 16 by 16 x 32.
+template <class T>
+struct Ops {
+  static constexpr bool F32 = std::is_same<T, float>::value, F16 = std::is_same<T, _Float16>::value;
+  struct Frag32 {
+    float v[8];
+  };
+  using Frag = typename std::conditional<F32, Frag32, i16x8>::type;
+  static constexpr int EPV = 16 / sizeof(T);
+  // fp16 probabilities are kept 2^6 times as large: beside a row's largest (1 to 2^8,
+  // as the running maximum may lag by 8) those down to 2^-30 are not flushed
+  static constexpr float BIAS = F16 ? 6.f : 0.f;
+  // in the backward, where they are at most 1, 2^14 times
+  static constexpr float GRAD_BIAS = F16 ? 14.f : 0.f, GRAD_UNIT = F16 ? 0x1p-14f : 1.f;
+
+  static __device__ __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) {
+    if constexpr (F32) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) c = mfma_f32_32x32x2(a.v[e], b.v[e], c);
+      return c;
+    } else {
+      return mfma16_32x32x16<F16>(a, b, c);
+    }
+  }
+  // registers 8 s .. 8 s + 7 as a right operand, rounded to T
+  static __device__ __forceinline__ Frag pack(const f32x16& x, int s) {
+    Frag f;
+    if constexpr (F32) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f.v[e] = x[8 * s + e];
+    } else {
+      u32x4 r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        r[e] = F16 ? pack2_f16(x[8 * s + 2 * e], x[8 * s + 2 * e + 1]) : pack2_bf16(x[8 * s + 2 * e], x[8 * s + 2 * e + 1]);
+      f = __builtin_bit_cast(i16x8, r);
+    }
+    return f;
+  }
+  // k 16 s + 8 half .. + 7 of a row of d elements in memory
+  static __device__ __forceinline__ Frag load_row(const T* row, bool valid, int s, int half, int d) {
+    const int at = 16 * s + 8 * half, n = valid ? d - at : 0;
+    Frag f;
+    if constexpr (F32) {
+      const auto lo = load_raw(row + at, n), hi = load_raw(row + at + 4, n - 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f.v[e] = __uint_as_float(lo[e]);
+        f.v[4 + e] = __uint_as_float(hi[e]);
+      }
+    } else {
+      f = __builtin_bit_cast(i16x8, (u32x4)load_raw(row + at, n));
+    }
+    return f;
+  }
+  static __device__ __forceinline__ float dot(const Frag& a, const Frag& b) {
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (F32)
+        sum += a.v[e] * b.v[e];
+      else if constexpr (F16)
+        sum += (float)__builtin_bit_cast(f16x8, a)[e] * (float)__builtin_bit_cast(f16x8, b)[e];
+      else
+        sum += bf16_to_f32((uint16_t)a[e]) * bf16_to_f32((uint16_t)b[e]);
+    }
+    return sum;
+  }
+};
+
+// A tile of rows of 32 DB elements in LDS.
+template <class T, int DB>
+struct Tile {
+  using O = Ops<T>;
+  using Frag = typename O::Frag;
+  static constexpr int EPV = O::EPV, VPR = 32 * DB / EPV, RB = 16 * VPR;
+  static __device__ __forceinline__ int swz(int r) {
+    if constexpr (VPR % 16 == 0)
+      return ((r & 3) << 2) | ((r >> 2) & 3);
+    else if constexpr (VPR % 16 == 8)
+      return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+    else
+      return (r >> 2) & 3;
+  }
+  // k 16 s + 8 (lane / 32) .. + 7 of row row0 + lane % 32 (row0 a multiple of 32)
+  static __device__ __forceinline__ Frag row(Lds* tile, int row0, int s, int lane) {
+    const int r = lane & 31, half = lane >> 5, x = swz(r);
+    Lds* at = tile + (row0 + r) * RB;
+    if constexpr (O::F32) {
+      Frag f;
+      const f32x4 lo = *(__attribute__((address_space(3))) f32x4*)(at + (((4 * s + 2 * half) ^ x) << 4));
+      const f32x4 hi = *(__attribute__((address_space(3))) f32x4*)(at + (((4 * s + 2 * half + 1) ^ x) << 4));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f.v[e] = lo[e];
+        f.v[4 + e] = hi[e];
+      }
+      return f;
+    } else {
+      return *(__attribute__((address_space(3))) i16x8*)(at + (((2 * s + half) ^ x) << 4));
+    }
+  }
+  // column 32 db + lane % 32, rows row0 + 4 (lane / 32) + {0 .. 3, 8 .. 11} (row0 a multiple of 16)
+  static __device__ __forceinline__ Frag col(Lds* tile, int row0, int db, int lane) {
+    const int half = lane >> 5;
+    if constexpr (O::F32) {
+      Frag f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int r = row0 + 4 * half + 8 * (e >> 2) + (e & 3);
+        const int v = (8 * db + ((lane & 31) >> 2)) ^ swz(r);
+        f.v[e] = *(__attribute__((address_space(3))) float*)(tile + r * RB + (v << 4) + 4 * (lane & 3));
+      }
+      return f;
+    } else {
+      // (lane j of 16 points at 4 columns of row j / 4 and receives column j of 4 rows)
+      const int j = lane & 15, v = 4 * db + 2 * ((lane >> 4) & 1) + ((j & 3) >> 1);
+      const int r0 = row0 + 4 * half + (j >> 2), r1 = r0 + 8;
+      typedef __attribute__((address_space(3))) i16x4 Quad;
+      const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Quad*)(tile + r0 * RB + ((v ^ swz(r0)) << 4) + 8 * (j & 1)));
+      const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Quad*)(tile + r1 * RB + ((v ^ swz(r1)) << 4) + 8 * (j & 1)));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+};
+
+// ROWS rows of a matrix on their way from memory through the registers of NT
+// threads into a tile.
+template <class T, int DB, int ROWS, int NT>
+struct Loader {
+  using Tl = Tile<T, DB>;
+  static constexpr int NV = ROWS * Tl::VPR / NT;
+  static_assert(NV * NT == ROWS * Tl::VPR, "the vectors divide evenly");
+  const char* base;
+  int64_t pitch;  // bytes between rows
+  int d, t;
+  bool whole;     // rows of whole 16-byte vectors on 4-byte boundaries, offsets within a tile in 31 bits
+  u32x4 r[NV];
+
+  // (uniform but for t)
+  __device__ __forceinline__ void init(const View& v, int64_t b, int h, int d_, int t_) {
+    base = (const char*)((const T*)v.p + b * v.batch + (int64_t)h * v.head);
+    pitch = v.token * (int64_t)sizeof(T);
+    d = d_;
+    t = t_;
+    whole = d % Tl::EPV == 0 && ((uintptr_t)base & 3) == 0 && (pitch & 3) == 0 && pitch < (int64_t)1 << 24;
+  }
+  // rows row0 .. row0 + ROWS - 1, those from `valid` rows on as zeros
+  __device__ __forceinline__ void load(int row0, int valid) {
+    const char* p = base + row0 * pitch;
+    if (whole) {
+      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int at = t + i * NT, row = at / Tl::VPR, v = at % Tl::VPR;
+        const uint32_t off = row < valid && v * Tl::EPV < d ? (uint32_t)(row * (int)pitch + v * 16) : OOB;
+        r[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int at = t + i * NT, row = at / Tl::VPR, v = at % Tl::VPR;
+        r[i] = load_raw((const T*)(p + row * pitch) + v * Tl::EPV, row < valid ? d - v * Tl::EPV : 0);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(Lds* tile) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int at = t + i * NT, row = at / Tl::VPR, v = at % Tl::VPR;
+      *(__attribute__((address_space(3))) u32x4*)(tile + row * Tl::RB + ((v ^ Tl::swz(row)) << 4)) = r[i];
+    }
+  }
+};
+
+// The other half of the wave's value.
+__device__ __forceinline__ float other_half(float v) {
+  const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float((threadIdx.x & 32) ? sw[0] : sw[1]);
+}
+
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// 4 consecutive elements at p, the first n of them.
+template <class T>
+__device__ __forceinline__ void store4(T* p, int n, float a, float b, float c, float d) {
+  if (n >= 4) {
+    if constexpr (sizeof(T) == 4) {
+      typedef float raw __attribute__((ext_vector_type(4), aligned(4)));
+      *(raw*)p = raw{a, b, c, d};
+    } else {
+      typedef uint32_t raw __attribute__((ext_vector_type(2), aligned(2)));
+      if constexpr (std::is_same<T, _Float16>::value)
+        *(raw*)p = raw{pack2_f16(a, b), pack2_f16(c, d)};
+      else
+        *(raw*)p = raw{pack2_bf16(a, b), pack2_bf16(c, d)};
+    }
+  } else {
+    if (n > 0) put(p, a);
+    if (n > 1) put(p + 1, b);
+    if (n > 2) put(p + 2, c);
+  }
+}
+// A lane's column of the accumulators, times f: 32 DB elements, d of them valid, at p.
+template <class T, int DB>
+__device__ __forceinline__ void store_column(T* p, int d, const f32x16 (&acc)[DB], float f, int lane) {
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = 32 * db + 8 * i + 4 * (lane >> 5);
+      store4(p + at, d - at, acc[db][4 * i] * f, acc[db][4 * i + 1] * f, acc[db][4 * i + 2] * f, acc[db][4 * i + 3] * f);
+    }
+}
+
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+
+}  // namespace attn
+}  // namespace mec
