@@ -45,7 +45,8 @@ def hipcc() -> str:
 
 
 def sources() -> list[Path]:
-    return [CSRC / f"{name}.hip" for name in ("mec_abi", "mec_vocab", "mec_rotary", "mec_attention")]
+    return [CSRC / f"{name}.hip" for name in ("mec_abi", "mec_vocab", "mec_rotary", "mec_attention",
+                                           "mec_attention_backward")]
 
 
 def _run(cmd: list[str], verbose: bool) -> None:

@@ -169,6 +169,11 @@ struct Tile {
       return *(__attribute__((address_space(3))) i16x8*)(at + (((2 * s + half) ^ x) << 4));
     }
   }
+  // (16-bit types) the same, written
+  static __device__ __forceinline__ void put_row(Lds* tile, int row0, int s, int lane, const Frag& f) {
+    const int r = lane & 31;
+    *(__attribute__((address_space(3))) i16x8*)(tile + (row0 + r) * RB + (((2 * s + (lane >> 5)) ^ swz(r)) << 4)) = f;
+  }
   // column 32 db + lane % 32, rows row0 + 4 (lane / 32) + {0 .. 3, 8 .. 11} (row0 a multiple of 16)
   static __device__ __forceinline__ Frag col(Lds* tile, int row0, int db, int lane) {
     const int half = lane >> 5;

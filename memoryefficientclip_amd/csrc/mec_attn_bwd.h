@@ -10,6 +10,8 @@
 // in fp16, to steps of 2^-24 and up to 65504, as the gradients that go out are.
 // k_attn_dq also leaves delta = do . o for k_attn_dkv.
 #pragma once
+#include <climits>
+
 #include "mec_attn.h"
 
 namespace mec {
@@ -21,11 +23,21 @@ struct Backward {
   static constexpr int DB = (KS + 1) / 2, WAVES = 4, NT = 64 * WAVES, ROWS = 32 * WAVES;
   using Tl = Tile<T, DB>;
   // rows of the tiles that are walked over
-  static constexpr int KEYS = O::F32 ? 32 : 64, QUERIES = O::F32 || DB > 3 ? 32 : 64;
+  static constexpr int KEYS = O::F32 || DB > 3 ? 32 : 64, QUERIES = O::F32 || DB > 3 ? 32 : 64;
+  // the values of a wave's keys stay in LDS where keys, values and both gradients take
+  // more registers than two waves on a SIMD have
+  static constexpr bool V_LDS = !O::F32 && DB > 3;
+  // The forward's result has the errors of 16 bits, and so has do . o; where few keys share a row's weight
+  // this is the largest error of dq and dk (heads of 64, 77 tokens, causal, bf16: 0.0031 of their size, 0.0023
+  // with a delta of fp32).  delta is also sum_j p_ij do_i . v_j: with d for do . o, eps = sum_j p_ij (do_i . v_j - d)
+  // is what it lacks.  Up to KEYS_EXACT keys it is summed along with dq, and dq corrected by -eps sum_j p_ij k_j
+  // (its product costs no reads of LDS), or, where registers are short, summed in a first walk over the keys.
+  static constexpr int KEYS_EXACT = O::F32 ? 0 : 512;
+  static constexpr bool TWICE = DB > 2;
 };
 
 template <class T, int KS>
-__global__ __launch_bounds__(256) void k_attn_dq(Problem a, int64_t items, int64_t ids, int row_tiles, const T* out,
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void k_attn_dq(Problem a, int64_t items, int64_t ids, int row_tiles, const T* out,
                                                  const float* lse, float* delta, T* dq) {
   using B = Backward<T, KS>;
   using O = Ops<T>;
@@ -51,9 +63,12 @@ __global__ __launch_bounds__(256) void k_attn_dq(Problem a, int64_t items, int64
   const int last = min((row0 + B::ROWS - 1) / a.group, nq - 1);
   int end = row0 / a.group >= nq ? 0 : a.causal ? min(nk, last + shift + 1) : nk;
   if (end < 0) end = 0;
-  if (dq == nullptr) end = 0;
+  const bool exact = end <= B::KEYS_EXACT;
+  if (dq == nullptr && !exact) end = 0;
   const int all = a.causal ? min(nk, wave_row0 / a.group + shift + 1) : nk;
-  const int wave_end = a.causal ? min(nk, min((wave_row0 + 31) / a.group, nq - 1) + shift + 1) : nk;
+  const int wave_end = wave_row0 / a.group >= nq ? 0
+                       : a.causal               ? min(nk, min((wave_row0 + 31) / a.group, nq - 1) + shift + 1)
+                                                : nk;
   const int see = a.causal ? min(nk, qi + shift + 1) : nk;
 
   const int64_t at = (b * a.heads + qh) * (int64_t)a.queries + qi;  // of lse and delta
@@ -71,11 +86,14 @@ __global__ __launch_bounds__(256) void k_attn_dq(Problem a, int64_t items, int64
     }
     dot += other_half(dot);
     if (live) l2 = lse[at];
-    if (half == 0 && row < rows) delta[at] = dot;
   }
-  f32x16 acc[DB];
+  f32x16 acc[DB], mean[B::TWICE ? 1 : DB];  // dq / scale, sum_j p_ij k_j
 #pragma unroll
-  for (int db = 0; db < DB; ++db) acc[db] = zero16();
+  for (int db = 0; db < DB; ++db) {
+    acc[db] = zero16();
+    mean[B::TWICE ? 0 : db] = zero16();
+  }
+  float eps = 0.f;
   const int tiles = (end + KEYS - 1) / KEYS;
   if (tiles > 0) {
     Loader<T, DB, KEYS, B::NT> lk, lv;
@@ -83,17 +101,23 @@ __global__ __launch_bounds__(256) void k_attn_dq(Problem a, int64_t items, int64
     lv.init(a.v, b, kh, a.d, threadIdx.x);
     lk.load(0, nk);
     lv.load(0, nk);
-    for (int i = 0; i < tiles; ++i) {
+    // (the first walk: below 0)
+    for (int i = B::TWICE && exact ? -tiles : 0; i < tiles; ++i) {
       Lds* const tk = lds + (i & 1 ? 2 * TILE : 0);
       Lds* const tv = tk + TILE;
       lk.store(tk);
       lv.store(tv);
       __syncthreads();
       if (i + 1 < tiles) {
-        lk.load((i + 1) * KEYS, nk - (i + 1) * KEYS);
-        lv.load((i + 1) * KEYS, nk - (i + 1) * KEYS);
+        const int next = (i + 1 < 0 ? i + 1 + tiles : i + 1) * KEYS;
+        lk.load(next, nk - next);
+        lv.load(next, nk - next);
       }
-      const int key0 = i * KEYS;
+      if (B::TWICE && i == 0 && exact) {
+        dot += eps + other_half(eps);
+        eps = 0.f;
+      }
+      const int key0 = (i < 0 ? i + tiles : i) * KEYS;
       if (key0 >= wave_end) continue;
       const bool masked = key0 + KEYS > all;
 #pragma unroll
@@ -105,21 +129,51 @@ __global__ __launch_bounds__(256) void k_attn_dq(Problem a, int64_t items, int64
           p = O::mma(Tl::row(tv, 32 * kb, ks, lane), g[ks], p);
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = fast_exp2(fmaf(s[e], a.c, -l2)) * (p[e] - dot);
+        for (int e = 0; e < 16; ++e) {
+          s[e] = fast_exp2(fmaf(s[e], a.c, -l2));
+          p[e] = s[e] * (p[e] - dot);
+        }
         if (masked) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            s[e] = key0 + 32 * kb + 8 * (e >> 2) + 4 * half + (e & 3) < see ? s[e] : 0.f;
+          for (int e = 0; e < 16; ++e) {
+            const bool in = key0 + 32 * kb + 8 * (e >> 2) + 4 * half + (e & 3) < see;
+            s[e] = in ? s[e] : 0.f;
+            p[e] = in ? p[e] : 0.f;
+          }
+        }
+        if (!O::F32 && exact) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) eps += p[e];
+          if (B::TWICE && i < 0) continue;
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const Frag ds = O::pack(s, h);
+          const Frag ds = O::pack(p, h);
+          if (!O::F32 && !B::TWICE && exact) {
+            const Frag ps = O::pack(s, h);
 #pragma unroll
-          for (int db = 0; db < DB; ++db) acc[db] = O::mma(Tl::col(tk, 32 * kb + 16 * h, db, lane), ds, acc[db]);
+            for (int db = 0; db < DB; ++db) {
+              const Frag kt = Tl::col(tk, 32 * kb + 16 * h, db, lane);
+              acc[db] = O::mma(kt, ds, acc[db]);
+              mean[db] = O::mma(kt, ps, mean[db]);
+            }
+          } else {
+#pragma unroll
+            for (int db = 0; db < DB; ++db) acc[db] = O::mma(Tl::col(tk, 32 * kb + 16 * h, db, lane), ds, acc[db]);
+          }
         }
       }
     }
   }
+  if (!O::F32 && !B::TWICE && exact) {
+    eps += other_half(eps);
+    dot += eps;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[db][e] -= eps * mean[db][e];
+  }
+  if (half == 0 && row < rows) delta[at] = dot;
   if (row >= rows || dq == nullptr) return;
   if (!live || l2 == kInf)
 #pragma unroll
@@ -128,14 +182,14 @@ __global__ __launch_bounds__(256) void k_attn_dq(Problem a, int64_t items, int64
 }
 
 template <class T, int KS>
-__global__ __launch_bounds__(256) void k_attn_dkv(Problem a, int64_t items, int64_t ids, int key_tiles,
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void k_attn_dkv(Problem a, int64_t items, int64_t ids, int key_tiles,
                                                   const float* lse, const float* delta, T* dk, T* dv) {
   using B = Backward<T, KS>;
   using O = Ops<T>;
   using Frag = typename O::Frag;
   using Tl = typename B::Tl;
   constexpr int DB = B::DB, QUERIES = B::QUERIES, NB = QUERIES / 32, TILE = QUERIES * Tl::RB;
-  __shared__ alignas(16) char s_lds[4 * TILE];
+  __shared__ alignas(16) char s_lds[4 * TILE + (B::V_LDS ? B::ROWS * Tl::RB : 0)];
   __shared__ alignas(16) float s_row[2][2][QUERIES];  // lse, delta of the tile's queries
   Lds* const lds = (Lds*)s_lds;
   const int64_t id = group_id(ids);
@@ -153,7 +207,7 @@ __global__ __launch_bounds__(256) void k_attn_dkv(Problem a, int64_t items, int6
   // queries that see any key of the workgroup, of the wave; those from which on all see all of the wave's; and
   // those from which on this key is seen
   const int begin = key0 >= nk ? nq : a.causal ? max(0, key0 - shift) : 0;
-  const int wave_begin = wave_key0 >= nk ? nq : a.causal ? wave_key0 - shift : 0;
+  const int wave_begin = wave_key0 >= nk ? INT_MAX : a.causal ? wave_key0 - shift : 0;
   const int all = a.causal ? wave_key0 + 31 - shift : 0;
   const int seen = a.causal ? key - shift : 0;
 
@@ -162,14 +216,19 @@ __global__ __launch_bounds__(256) void k_attn_dkv(Problem a, int64_t items, int6
   for (int db = 0; db < DB; ++db) ak[db] = av[db] = zero16();
   const int first = begin / QUERIES, each = (nq + QUERIES - 1) / QUERIES - first;
   if (each > 0) {
-    Frag k[KS], v[KS];
+    Frag k[KS], v[B::V_LDS ? 1 : KS];
+    Lds* const values = lds + 4 * TILE;
     {
       const T* pk = (const T*)a.k.p + b * a.k.batch + (int64_t)key * a.k.token + (int64_t)kh * a.k.head;
       const T* pv = (const T*)a.v.p + b * a.v.batch + (int64_t)key * a.v.token + (int64_t)kh * a.v.head;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         k[s] = O::load_row(pk, live, s, half, a.d);
-        v[s] = O::load_row(pv, live, s, half, a.d);
+        const Frag x = O::load_row(pv, live, s, half, a.d);
+        if constexpr (B::V_LDS)
+          Tl::put_row(values, 32 * wave, s, lane, x);  // (read by this wave alone)
+        else
+          v[s] = x;
       }
     }
     Loader<T, DB, QUERIES, B::NT> lq, lg;
@@ -209,7 +268,10 @@ __global__ __launch_bounds__(256) void k_attn_dkv(Problem a, int64_t items, int6
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           s = O::mma(Tl::row(tq, 32 * qb, ks, lane), k[ks], s);
-          p = O::mma(Tl::row(tg, 32 * qb, ks, lane), v[ks], p);
+          if constexpr (B::V_LDS)
+            p = O::mma(Tl::row(tg, 32 * qb, ks, lane), Tl::row(values, 32 * wave, ks, lane), p);
+          else
+            p = O::mma(Tl::row(tg, 32 * qb, ks, lane), v[ks], p);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {

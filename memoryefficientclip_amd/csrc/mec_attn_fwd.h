@@ -41,7 +41,7 @@ struct Forward {
 };
 
 template <class T, int KS, int WM, int WK>
-__global__ __launch_bounds__(64 * WM * WK) void k_attn_forward(Problem a, int64_t items, int64_t ids, int row_tiles,
+__global__ __launch_bounds__(64 * WM * WK, sizeof(T) == 4 || (WM == 1 && KS == 8) ? 1 : 2) void k_attn_forward(Problem a, int64_t items, int64_t ids, int row_tiles,
                                                                int splits, T* out, float* lse, Parts parts) {
   using F = Forward<T, KS, WM, WK>;
   using O = Ops<T>;
@@ -72,7 +72,9 @@ __global__ __launch_bounds__(64 * WM * WK) void k_attn_forward(Problem a, int64_
   int end = row0 / a.group >= nq ? 0 : a.causal ? min(nk, last + shift + 1) : nk;
   if (end < 0) end = 0;
   const int all = a.causal ? min(nk, wave_row0 / a.group + shift + 1) : nk;
-  const int wave_end = a.causal ? min(nk, min((wave_row0 + 31) / a.group, nq - 1) + shift + 1) : nk;
+  const int wave_end = wave_row0 / a.group >= nq ? 0
+                       : a.causal               ? min(nk, min((wave_row0 + 31) / a.group, nq - 1) + shift + 1)
+                                                : nk;
   const int see = a.causal ? min(nk, qi + shift + 1) : nk;  // this row sees the keys below
 
   f32x16 o[DB];
