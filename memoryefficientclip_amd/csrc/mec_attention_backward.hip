@@ -2,10 +2,31 @@
 // plain host code, then stream-ordered kernel launches.  Nothing here allocates
 // device memory or synchronises the host.
 #include "mec_attn_bwd.h"
+#include "mec_attn_whole.h"
 #include "mec_attn_host.h"
 
 using namespace mec;
 using namespace mec::attn;
+
+namespace {
+
+// Waves and LDS of k_attn_whole_grad, 0 waves where it does not fit or does not pay.
+struct Whole {
+  int waves;
+  size_t lds;
+};
+Whole plan_whole(const Problem& a, int dtype) {
+  const int size = dtype == MEC_DTYPE_F32 ? 4 : 2, steps = a.d <= 32 ? 2 : a.d <= 64 ? 4 : a.d <= 96 ? 6 : 8;
+  const int row = 16 * steps * size, most = whole_waves(steps, size);
+  const int64_t nq = (a.queries + 31) & ~31, nk = (a.keys + 31) & ~31;
+  const int64_t lds = 2 * (nq + nk) * row + 8 * nq;
+  const int blocks = (int)((nq > nk ? nq : nk) / 32);
+  // (wider heads do not fit into the registers; queries leave through the place of keys and values)
+  if (steps > whole_steps(size) || a.group != 1 || lds > kWholeLds || blocks > most || nq > 2 * nk) return {0, 0};
+  return {blocks, (size_t)lds};
+}
+
+}  // namespace
 
 extern "C" {
 
@@ -22,7 +43,7 @@ int mec_attention_backward(const mec_attention_t* attention, const mec_heads_t* 
                            int64_t workspace_bytes, void* stream) {
   g_err.clear();
   Problem a{};
-  Grid gq{}, gk{};
+  Grid gq{}, gk{}, gw{};
   int rc = check_attention(attention, &a);
   if (!rc) rc = check_heads(query, "query");
   if (!rc) rc = check_heads(key, "key");
@@ -36,6 +57,7 @@ int mec_attention_backward(const mec_attention_t* attention, const mec_heads_t* 
   const int row_tiles = (int)ceil_div(rows, 128), key_tiles = (int)ceil_div(a.keys, 128);
   if (!rc) rc = make_grid(a.pairs * row_tiles, &gq);
   if (!rc) rc = make_grid(a.pairs * key_tiles, &gk);
+  if (!rc) rc = make_grid(a.pairs, &gw);
   if (rc || (!grad_query && !grad_key)) return rc;
   a.q = view(query);
   a.k = view(key);
@@ -43,9 +65,17 @@ int mec_attention_backward(const mec_attention_t* attention, const mec_heads_t* 
   a.g = view(grad_out);
   hipStream_t st = (hipStream_t)stream;
   float* delta = (float*)workspace;
+  const Whole whole = plan_whole(a, attention->dtype);
   with_kernel(attention->dtype, a.d, [&](auto* t, auto ks) {
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int KS = decltype(ks)::value;
+    if constexpr (KS <= whole_steps(sizeof(T))) {
+      if (whole.waves) {
+        k_attn_whole_grad<T, KS><<<gw.dims, 64 * whole.waves, whole.lds, st>>>(
+            a, gw.items, gw.ids, (const T*)out, lse, (T*)grad_query, (T*)grad_key, (T*)grad_value);
+        return;
+      }
+    }
     k_attn_dq<T, KS><<<gq.dims, 256, 0, st>>>(a, gq.items, gq.ids, row_tiles, (const T*)out, lse, delta, (T*)grad_query);
     if (grad_key)
       k_attn_dkv<T, KS><<<gk.dims, 256, 0, st>>>(a, gk.items, gk.ids, key_tiles, lse, delta, (T*)grad_key,

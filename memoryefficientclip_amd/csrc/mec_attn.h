@@ -258,36 +258,79 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 
-// 4 consecutive elements at p, the first n of them.
-template <class T>
-__device__ __forceinline__ void store4(T* p, int n, float a, float b, float c, float d) {
-  if (n >= 4) {
-    if constexpr (sizeof(T) == 4) {
-      typedef float raw __attribute__((ext_vector_type(4), aligned(4)));
-      *(raw*)p = raw{a, b, c, d};
-    } else {
-      typedef uint32_t raw __attribute__((ext_vector_type(2), aligned(2)));
-      if constexpr (std::is_same<T, _Float16>::value)
-        *(raw*)p = raw{pack2_f16(a, b), pack2_f16(c, d)};
-      else
-        *(raw*)p = raw{pack2_bf16(a, b), pack2_bf16(c, d)};
-    }
-  } else {
-    if (n > 0) put(p, a);
-    if (n > 1) put(p + 1, b);
-    if (n > 2) put(p + 2, c);
-  }
-}
-// A lane's column of the accumulators, times f: 32 DB elements, d of them valid, at p.
+// A wave's 32 columns of the accumulators, rounded to T, on their way to rows of d
+// elements.  They pass through LDS (32 rows of a tile, of which the wave alone has the
+// use), so that 16 bytes a lane and whole lines leave the CU: 8 bytes a lane, 32 rows at
+// a time, are four times the requests, which short sequences wait for.
 template <class T, int DB>
-__device__ __forceinline__ void store_column(T* p, int d, const f32x16 (&acc)[DB], float f, int lane) {
+struct Rows {
+  using Tl = Tile<T, DB>;
+  typedef typename std::conditional<sizeof(T) == 4, float, uint32_t>::type E;
+  typedef E Four __attribute__((ext_vector_type(sizeof(T))));  // 4 elements
+  Four v[DB][4];
+
+  __device__ __forceinline__ void pack(const f32x16 (&acc)[DB], float f) {
 #pragma unroll
-  for (int db = 0; db < DB; ++db)
+    for (int db = 0; db < DB; ++db)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = 32 * db + 8 * i + 4 * (lane >> 5);
-      store4(p + at, d - at, acc[db][4 * i] * f, acc[db][4 * i + 1] * f, acc[db][4 * i + 2] * f, acc[db][4 * i + 3] * f);
+      for (int i = 0; i < 4; ++i) {
+        const float a = acc[db][4 * i] * f, b = acc[db][4 * i + 1] * f, c = acc[db][4 * i + 2] * f,
+                    d = acc[db][4 * i + 3] * f;
+        if constexpr (sizeof(T) == 4)
+          v[db][i] = Four{a, b, c, d};
+        else if constexpr (std::is_same<T, _Float16>::value)
+          v[db][i] = Four{pack2_f16(a, b), pack2_f16(c, d)};
+        else
+          v[db][i] = Four{pack2_bf16(a, b), pack2_bf16(c, d)};
+      }
+  }
+  __device__ __forceinline__ void put(Lds* mine, int lane) const {
+    const int r = lane & 31, half = lane >> 5, x = Tl::swz(r);
+    Lds* const to = mine + r * Tl::RB;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4)
+          *(__attribute__((address_space(3))) Four*)(to + (((8 * db + 2 * i + half) ^ x) << 4)) = v[db][i];
+        else
+          *(__attribute__((address_space(3))) Four*)(to + (((4 * db + i) ^ x) << 4) + 8 * half) = v[db][i];
+      }
+  }
+  // row(r): where row r goes, nullptr: nowhere
+  template <class Row>
+  static __device__ __forceinline__ void flush(Lds* mine, int d, int lane, Row row) {
+    constexpr int EPV = Tl::EPV, VPR = Tl::VPR;
+    wave_sync();
+#pragma unroll
+    for (int i = 0; i < VPR / 2; ++i) {
+      const int at = i * 64 + lane, r = at / VPR, vec = at % VPR, n = d - vec * EPV;
+      T* p = row(r);
+      if (p != nullptr && n > 0) {
+        const u32x4 x4 = *(__attribute__((address_space(3))) u32x4*)(mine + r * Tl::RB + ((vec ^ Tl::swz(r)) << 4));
+        p += vec * EPV;
+        if (n >= EPV) {
+          *(typename Vec<T>::raw*)p = x4;
+        } else {
+#pragma unroll
+          for (int e = 0; e < EPV - 1; ++e)
+            if (e < n) {
+              if constexpr (sizeof(T) == 4)
+                p[e] = __uint_as_float(x4[e]);
+              else
+                p[e] = __builtin_bit_cast(T, (uint16_t)(x4[e / 2] >> (16 * (e & 1))));
+            }
+        }
+      }
     }
+  }
+};
+template <class T, int DB, class Row>
+__device__ __forceinline__ void store_rows(Lds* mine, const f32x16 (&acc)[DB], float f, int d, int lane, Row row) {
+  Rows<T, DB> rows;
+  rows.pack(acc, f);
+  rows.put(mine, lane);
+  Rows<T, DB>::flush(mine, d, lane, row);
 }
 
 __device__ __forceinline__ f32x16 zero16() {

@@ -174,11 +174,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void k_attn_dq(Problem
       for (int e = 0; e < 16; ++e) acc[db][e] -= eps * mean[db][e];
   }
   if (half == 0 && row < rows) delta[at] = dot;
-  if (row >= rows || dq == nullptr) return;
+  if (dq == nullptr) return;
   if (!live || l2 == kInf)
 #pragma unroll
     for (int db = 0; db < DB; ++db) acc[db] = zero16();
-  store_column<T, DB>(dq + ((b * a.queries + qi) * a.heads + qh) * (int64_t)a.d, a.d, acc, a.scale, lane);
+  __syncthreads();  // (the tiles are no longer read)
+  store_rows<T, DB>(lds + 32 * wave * Tl::RB, acc, a.scale, a.d, lane, [&](int r) -> T* {
+    const int to = wave_row0 + r;
+    return to < rows ? dq + ((b * a.queries + to / a.group) * a.heads + kh * a.group + to % a.group) * (int64_t)a.d
+                     : nullptr;
+  });
 }
 
 template <class T, int KS>
@@ -303,13 +308,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void k_attn_dkv(Proble
       }
     }
   }
-  if (key >= a.keys) return;
   if (!live)
 #pragma unroll
     for (int db = 0; db < DB; ++db) ak[db] = av[db] = zero16();
-  const int64_t at = ((b * a.keys + key) * a.key_heads + kh) * (int64_t)a.d;
-  store_column<T, DB>(dk + at, a.d, ak, a.scale, lane);
-  store_column<T, DB>(dv + at, a.d, av, O::GRAD_UNIT, lane);
+  __syncthreads();  // (the tiles are no longer read)
+  const auto to = [&](T* p) {
+    return [&, p](int r) -> T* {
+      return wave_key0 + r < a.keys ? p + ((b * a.keys + wave_key0 + r) * a.key_heads + kh) * (int64_t)a.d : nullptr;
+    };
+  };
+  store_rows<T, DB>(lds + 32 * wave * Tl::RB, ak, a.scale, a.d, lane, to(dk));
+  wave_sync();
+  store_rows<T, DB>(lds + 32 * wave * Tl::RB, av, O::GRAD_UNIT, a.d, lane, to(dv));
 }
 
 }  // namespace attn

@@ -218,10 +218,15 @@ __global__ __launch_bounds__(64 * WM * WK, sizeof(T) == 4 || (WM == 1 && KS == 8
       }
     }
   } else {
-    if (row >= rows) return;
     const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-    store_column<T, DB>(out + ((b * a.queries + qi) * a.heads + qh) * (int64_t)a.d, a.d, o, inv, lane);
-    if (lse && half == 0) lse[(b * a.heads + qh) * (int64_t)a.queries + qi] = l == 0.f ? kInf : m - O::BIAS + log2f(l);
+    if (lse && half == 0 && row < rows)
+      lse[(b * a.heads + qh) * (int64_t)a.queries + qi] = l == 0.f ? kInf : m - O::BIAS + log2f(l);
+    __syncthreads();  // (the tiles are no longer read)
+    store_rows<T, DB>(lds + 32 * wave * Tl::RB, o, inv, a.d, lane, [&](int r) -> T* {
+      const int at = wave_row0 + r;
+      return at < rows ? out + ((b * a.queries + at / a.group) * a.heads + kh * a.group + at % a.group) * (int64_t)a.d
+                       : nullptr;
+    });
   }
 }
 

@@ -1,0 +1,271 @@
+// Attention of short sequences, whose tiles fit into LDS as a whole: the texts and
+// patches of a contrastive batch.  A workgroup takes all tokens of one key head.
+//
+// Beside the kernels that walk over tiles this saves their barriers, their second
+// reading of the inputs in the backward, and the time until a tile has arrived,
+// which here is spent once: everything is on its way to LDS before the first
+// product, by loads that pass no registers.
+#pragma once
+#include "mec_attn.h"
+
+namespace mec {
+namespace attn {
+
+// most waves of a workgroup: registers for 3 or 2 on a SIMD
+constexpr int whole_waves(int steps, int size) { return steps <= 4 && size == 2 ? 12 : 8; }
+constexpr int whole_steps(int size) { return size == 2 ? 6 : 4; }  // of 16 features: the widest heads
+constexpr int kWholeLds = 160 * 1024;  // of a CU
+
+extern __shared__ __align__(16) char s_whole[];
+
+// Rows [0, valid) of a head into a tile of `rows` rows (a multiple of 32), the rest as zeros.
+template <class T, int DB>
+__device__ __forceinline__ void fetch(Lds* tile, const View& v, int64_t b, int h, int valid, int rows, int d, int wave,
+                                      int waves) {
+  using Tl = Tile<T, DB>;
+  constexpr int VPR = Tl::VPR;
+  const char* base = (const char*)((const T*)v.p + b * v.batch + (int64_t)h * v.head);
+  const int64_t pitch = v.token * (int64_t)sizeof(T);
+  const int lane = threadIdx.x & 63, blocks = rows * VPR / 64;
+  if (d % Tl::EPV == 0 && ((uintptr_t)base & 15) == 0 && (pitch & 15) == 0 && pitch < (1 << 20)) {
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, 0x00020000);
+    for (int i = wave; i < blocks; i += waves) {
+      // lane l fills place l of the i-th 64
+      const int at = i * 64 + lane, row = at / VPR, vec = (at % VPR) ^ Tl::swz(row);
+      const uint32_t off = row < valid && vec * Tl::EPV < d ? (uint32_t)(row * (int)pitch + vec * 16) : OOB;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(tile + i * 1024), 16, off,
+                                               0, 0, 0);
+    }
+  } else {
+    for (int i = wave; i < blocks; i += waves) {
+      const int at = i * 64 + lane, row = at / VPR, vec = (at % VPR) ^ Tl::swz(row);
+      const u32x4 r = load_raw((const T*)(base + row * pitch) + vec * Tl::EPV, row < valid ? d - vec * Tl::EPV : 0);
+      *(__attribute__((address_space(3))) u32x4*)(tile + at * 16) = r;
+    }
+  }
+}
+
+// Loads into LDS and the waves' writes to it are there for all waves.
+__device__ __forceinline__ void loads_and_writes_done() {
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): loads that pass no registers too
+  __syncthreads();
+}
+
+// The gradients of one head (heads == key_heads).  Each wave has a block of 32 queries
+// and one of 32 keys: first S^T, dP^T and dQ^T of the queries as in k_attn_dq, with
+// delta made whole (see there), then S, dP, dV^T and dK^T of the keys as in k_attn_dkv.
+// LDS: K, V, Q, dO, and lse and delta of the queries.
+template <class T, int KS>
+__global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_grad(Problem a, int64_t items, int64_t ids,
+                                                                                     const T* out, const float* lse,
+                                                                                     T* dq, T* dk, T* dv) {
+  using O = Ops<T>;
+  using Frag = typename O::Frag;
+  constexpr int DB = (KS + 1) / 2;
+  using Tl = Tile<T, DB>;
+  // a wave's keys and values, in registers; of fp32 and of wide heads they are read from LDS
+  constexpr bool HELD = !O::F32 && DB <= 2;
+  // see Backward: d + eps is delta
+  constexpr bool MEAN = !O::F32 && DB <= 2, TWICE = !O::F32 && DB > 2;
+  const int64_t id = group_id(ids);
+  if (id >= items) return;
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int64_t b = id / a.key_heads;
+  const int h = (int)(id - b * a.key_heads);
+  const int nq = a.nq(b), nk = a.nk(b), shift = nk - nq;
+  const int q_rows = (a.queries + 31) & ~31, k_rows = (a.keys + 31) & ~31;
+  Lds* const tk = (Lds*)s_whole;
+  Lds* const tv = tk + k_rows * Tl::RB;
+  Lds* const tq = tv + k_rows * Tl::RB;
+  Lds* const tg = tq + q_rows * Tl::RB;
+  typedef __attribute__((address_space(3))) float LdsFloat;
+  typedef __attribute__((address_space(3))) f32x4 LdsFour;
+  LdsFloat* const s_lse = (LdsFloat*)(tg + q_rows * Tl::RB);
+  LdsFloat* const s_delta = s_lse + q_rows;
+  const int64_t head0 = (b * a.heads + h) * (int64_t)a.queries;  // of lse
+  const int first = 32 * wave;                                  // of the wave's queries, and of its keys
+  const int qi = first + (lane & 31), key = qi;
+  const bool live = qi < nq;
+  const int end = first >= nq || nk == 0 ? 0 : a.causal ? min(nk, min(first + 31, nq - 1) + shift + 1) : nk;
+  Frag o[O::F32 || TWICE ? 1 : KS];  // (the result: on its way from memory along with the tiles)
+  float l2 = kInf;
+  if (nq > 0 && nk > 0) {
+    // (blocks that the lengths leave empty are not touched)
+    const int nq32 = (nq + 31) & ~31, nk32 = (nk + 31) & ~31;
+    fetch<T, DB>(tk, a.k, b, h, nk, nk32, a.d, wave, waves);
+    fetch<T, DB>(tq, a.q, b, h, nq, nq32, a.d, wave, waves);
+    fetch<T, DB>(tv, a.v, b, h, nk, nk32, a.d, wave, waves);
+    fetch<T, DB>(tg, a.g, b, h, nq, nq32, a.d, wave, waves);
+    if (live) l2 = lse[head0 + qi];
+    if constexpr (MEAN) {
+      const T* po = out + ((b * a.queries + qi) * a.heads + h) * (int64_t)a.d;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) o[s] = O::load_row(po, live, s, half, a.d);
+    }
+    if (half == 0 && first < nq) s_lse[qi] = l2 - O::GRAD_BIAS;
+  }
+  loads_and_writes_done();
+  Rows<T, DB> packed;  // dq
+  {
+    f32x16 acc[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db) acc[db] = zero16();
+    float dot = 0.f;
+    if (end > 0) {
+      const int see = a.causal ? min(nk, qi + shift + 1) : nk, all = a.causal ? min(nk, first + shift + 1) : nk;
+      Frag q[KS], g[KS];
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        q[s] = Tl::row(tq, first, s, lane);
+        g[s] = Tl::row(tg, first, s, lane);
+        if constexpr (MEAN) dot += O::dot(g[s], o[s]);
+        if constexpr (O::F32)
+          dot += O::dot(g[s], O::load_row(out + ((b * a.queries + qi) * a.heads + h) * (int64_t)a.d, live, s, half, a.d));
+      }
+      dot += other_half(dot);
+      f32x16 mean[MEAN ? DB : 1];
+#pragma unroll
+      for (int db = 0; db < (MEAN ? DB : 1); ++db) mean[db] = zero16();
+      float eps = 0.f;
+      for (int walk = TWICE ? 0 : 1; walk < 2; ++walk) {
+        for (int key0 = 0; key0 < end; key0 += 32) {
+          f32x16 s = zero16(), p = zero16();
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            s = O::mma(Tl::row(tk, key0, ks, lane), q[ks], s);
+            p = O::mma(Tl::row(tv, key0, ks, lane), g[ks], p);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            s[e] = fast_exp2(fmaf(s[e], a.c, -l2));
+            p[e] = s[e] * (p[e] - dot);
+          }
+          if (key0 + 32 > all) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const bool in = key0 + 8 * (e >> 2) + 4 * half + (e & 3) < see;
+              s[e] = in ? s[e] : 0.f;
+              p[e] = in ? p[e] : 0.f;
+            }
+          }
+          if (!O::F32) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) eps += p[e];
+          }
+          if (TWICE && walk == 0) continue;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const Frag ds = O::pack(p, x), ps = O::pack(s, x);
+#pragma unroll
+            for (int db = 0; db < DB; ++db) {
+              const Frag kt = Tl::col(tk, key0 + 16 * x, db, lane);
+              acc[db] = O::mma(kt, ds, acc[db]);
+              if constexpr (MEAN) mean[db] = O::mma(kt, ps, mean[db]);
+            }
+          }
+        }
+        if (TWICE && walk == 0) {
+          dot += eps + other_half(eps);
+          eps = 0.f;
+        }
+      }
+      if constexpr (MEAN) {
+        eps += other_half(eps);
+        dot += eps;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[db][e] -= eps * mean[db][e];
+      }
+      if (!live || l2 == kInf)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[db] = zero16();
+    }
+    if (half == 0 && first < nq) s_delta[qi] = dot * O::GRAD_UNIT;
+    packed.pack(acc, a.scale);
+  }
+  const auto to = [&](T* p, int n, int heads) {
+    return [=](int r) -> T* { return first + r < n ? p + ((b * n + first + r) * heads + h) * (int64_t)a.d : nullptr; };
+  };
+  __syncthreads();  // delta is there, and other waves' keys and values are no longer read
+  Frag k[HELD ? KS : 1], v[HELD ? KS : 1];
+  if constexpr (HELD) {
+    if (first < nk) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        k[s] = Tl::row(tk, first, s, lane);
+        v[s] = Tl::row(tv, first, s, lane);
+      }
+    }
+    if (dq) {
+      __syncthreads();  // nor is any key or value
+      if (first < a.queries) {
+        packed.put(tk + first * Tl::RB, lane);
+        Rows<T, DB>::flush(tk + first * Tl::RB, a.d, lane, to(dq, a.queries, a.heads));
+      }
+      __syncthreads();
+    }
+  }
+  if (dk) {
+    f32x16 ak[DB], av[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db) ak[db] = av[db] = zero16();
+    const int begin = first >= nk ? nq : a.causal ? max(0, first - shift) & ~31 : 0;
+    const int all = a.causal ? first + 31 - shift : 0, seen = a.causal ? key - shift : 0;
+    for (int q0 = begin; q0 < nq; q0 += 32) {
+      f32x16 s = zero16(), p = zero16();
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        s = O::mma(Tl::row(tq, q0, ks, lane), HELD ? k[HELD ? ks : 0] : Tl::row(tk, first, ks, lane), s);
+        p = O::mma(Tl::row(tg, q0, ks, lane), HELD ? v[HELD ? ks : 0] : Tl::row(tv, first, ks, lane), p);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const f32x4 ls = *(LdsFour*)(s_lse + q0 + 8 * e + 4 * half), dl = *(LdsFour*)(s_delta + q0 + 8 * e + 4 * half);
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          s[4 * e + f] = fast_exp2(fmaf(s[4 * e + f], a.c, -ls[f]));
+          p[4 * e + f] = s[4 * e + f] * fmaf(p[4 * e + f], O::GRAD_UNIT, -dl[f]);
+        }
+      }
+      if (q0 < all) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const bool in = q0 + 8 * (e >> 2) + 4 * half + (e & 3) >= seen;
+          s[e] = in ? s[e] : 0.f;
+          p[e] = in ? p[e] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const Frag fp = O::pack(s, x), fs = O::pack(p, x);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          av[db] = O::mma(Tl::col(tg, q0 + 16 * x, db, lane), fp, av[db]);
+          ak[db] = O::mma(Tl::col(tq, q0 + 16 * x, db, lane), fs, ak[db]);
+        }
+      }
+    }
+    if (first < a.keys) {
+      if (key >= nk)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) ak[db] = av[db] = zero16();
+      // (this wave's keys and values are no longer read)
+      store_rows<T, DB>(tk + first * Tl::RB, ak, a.scale, a.d, lane, to(dk, a.keys, a.key_heads));
+      store_rows<T, DB>(tv + first * Tl::RB, av, O::GRAD_UNIT, a.d, lane, to(dv, a.keys, a.key_heads));
+    }
+  }
+  if constexpr (!HELD) {
+    if (dq) {
+      __syncthreads();  // queries are no longer read
+      if (first < a.queries) {
+        packed.put(tq + first * Tl::RB, lane);
+        Rows<T, DB>::flush(tq + first * Tl::RB, a.d, lane, to(dq, a.queries, a.heads));
+      }
+    }
+  }
+}
+
+}  // namespace attn
+}  // namespace mec
