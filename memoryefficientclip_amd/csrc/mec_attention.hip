@@ -2,6 +2,7 @@
 // plain host code, then stream-ordered kernel launches.  Nothing here allocates
 // device memory or synchronises the host.
 #include "mec_attn_fwd.h"
+#include "mec_attn_whole.h"
 #include "mec_attn_host.h"
 
 using namespace mec;
@@ -12,18 +13,36 @@ namespace {
 // How the forward's work is cut.
 struct Plan {
   bool few;        // few rows a key head: the waves of a workgroup share them
+  int whole;       // waves of the form for short sequences, 0: not that one
+  size_t lds;      // ... and its LDS
   int row_tiles, splits;
   int64_t parts_o, parts_ml;  // bytes
 };
 constexpr int kWave = 4;
 
-int plan_forward(const Problem& a, Plan* out) {
+// Waves of k_attn_whole_forward and its LDS, 0 where another form is taken: up to 64 KB, of which two workgroups
+// and more share a CU, and not for few rows of many keys, whose loads want more waves.  256 x 12 heads of 64, us, this
+// form and the one that walks over tiles: 77 tokens 29 and 36, 197 tokens (56 KB) 82 and 106, 257 (72 KB) 184 and 149;
+// 160 tokens of 16-bit heads of 72 (60 KB) 93 and 110, 197 (84 KB) 161 and 137.
+int whole_forward(const Problem& a, int dtype, int64_t rows, size_t* lds) {
+  const int size = dtype == MEC_DTYPE_F32 ? 4 : 2, steps = a.d <= 32 ? 2 : a.d <= 64 ? 4 : a.d <= 96 ? 6 : 8;
+  const int64_t blocks = ceil_div(rows, 32), key_blocks = ceil_div(a.keys, 32);
+  *lds = (size_t)(key_blocks * 2 * 32 * 16 * steps * size);
+  // (rows leave through the place of keys and values)
+  const bool fits = blocks <= whole_waves(steps, size) && *lds <= 64 * 1024 && blocks <= 2 * key_blocks;
+  return fits && key_blocks <= 4 * blocks ? (int)blocks : 0;
+}
+
+int plan_forward(const Problem& a, int dtype, Plan* out) {
   const int64_t rows = (int64_t)a.queries * a.group;
   Plan p{};
   p.few = rows <= 32;
   p.row_tiles = (int)ceil_div(rows, p.few ? 32 : 128);
   p.splits = 1;
-  if (p.few) {
+  p.whole = whole_forward(a, dtype, rows, &p.lds);
+  if (p.whole) {
+    p.row_tiles = 1;
+  } else if (p.few) {
     int cus = 0;
     if (int rc = compute_units(&cus)) return rc;
     // two workgroups a CU, and two tiles of 32 keys a wave
@@ -48,7 +67,7 @@ int64_t mec_attention_workspace_bytes(const mec_attention_t* attention) {
   Problem a{};
   Plan p{};
   int rc = check_attention(attention, &a);
-  if (!rc) rc = plan_forward(a, &p);
+  if (!rc) rc = plan_forward(a, attention->dtype, &p);
   return rc ? rc : p.parts_o + p.parts_ml;
 }
 
@@ -65,7 +84,7 @@ int mec_attention(const mec_attention_t* attention, const mec_heads_t* query, co
   if (!rc) rc = check_heads(value, "value");
   if (!rc && !out) rc = fail(MEC_ERR_INVALID, "out must be non-null");
   if (!rc) rc = check_not_capturing(stream);
-  if (!rc) rc = plan_forward(a, &p);
+  if (!rc) rc = plan_forward(a, attention->dtype, &p);
   if (!rc) rc = check_scratch(workspace, workspace_bytes, p.parts_o + p.parts_ml);
   if (!rc) rc = make_grid(a.pairs * p.row_tiles * p.splits, &g);
   if (rc) return rc;
@@ -77,7 +96,9 @@ int mec_attention(const mec_attention_t* attention, const mec_heads_t* query, co
   with_kernel(attention->dtype, a.d, [&](auto* t, auto ks) {
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int KS = decltype(ks)::value;
-    if (p.few) {
+    if (p.whole) {
+      k_attn_whole_forward<T, KS><<<g.dims, 64 * p.whole, p.lds, st>>>(a, g.items, g.ids, (T*)out, lse);
+    } else if (p.few) {
       k_attn_forward<T, KS, 1, kWave>
           <<<g.dims, 64 * kWave, 0, st>>>(a, g.items, g.ids, p.row_tiles, p.splits, (T*)out, lse, parts);
       if (p.splits > 1) {

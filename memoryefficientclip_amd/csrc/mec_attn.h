@@ -258,6 +258,32 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 
+// The running maximum m (in units of log2) after scores s, times c: sum l and accumulators o are
+// rescaled where it grew by more than 8 in any row.
+template <class O, int NB, int DB>
+__device__ __forceinline__ void grow(const f32x16 (&s)[NB], float c, float& m, float& l, f32x16 (&o)[DB]) {
+  float top = s[0][0];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) top = fmaxf(top, s[b][e]);
+  top = fmaxf(top, other_half(top)) * c;
+  if (__any(top > m + 8.f)) {
+    const float now = fmaxf(m, top), f = now == -kInf ? 1.f : fast_exp2(m - now);
+    m = now;
+    l *= f;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[db][e] *= f;
+  }
+}
+template <class O, int DB>
+__device__ __forceinline__ void grow(const f32x16& s, float c, float& m, float& l, f32x16 (&o)[DB]) {
+  const f32x16 one[1] = {s};
+  grow<O>(one, c, m, l, o);
+}
+
 // A wave's 32 columns of the accumulators, rounded to T, on their way to rows of d
 // elements.  They pass through LDS (32 rows of a tile, of which the wave alone has the
 // use), so that 16 bytes a lane and whole lines leave the CU: 8 bytes a lane, 32 rows at

@@ -133,21 +133,7 @@ __global__ __launch_bounds__(64 * WM * WK, sizeof(T) == 4 || (WM == 1 && KS == 8
           for (int e = 0; e < 16; ++e)
             s[kb][e] = key0 + 32 * kb + 8 * (e >> 2) + 4 * half + (e & 3) < see ? s[kb][e] : -kInf;
       }
-      float top = s[0][0];
-#pragma unroll
-      for (int kb = 0; kb < NB; ++kb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, s[kb][e]);
-      top = fmaxf(top, other_half(top)) * a.c;
-      if (__any(top > m + 8.f)) {
-        const float now = fmaxf(m, top), f = now == -kInf ? 1.f : fast_exp2(m - now);
-        m = now;
-        l *= f;
-#pragma unroll
-        for (int db = 0; db < DB; ++db)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[db][e] *= f;
-      }
+      grow<O>(s, a.c, m, l, o);
       const float ref = (m == -kInf ? 0.f : m) - O::BIAS;
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb)

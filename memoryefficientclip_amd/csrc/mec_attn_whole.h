@@ -18,7 +18,9 @@ constexpr int kWholeLds = 160 * 1024;  // of a CU
 
 extern __shared__ __align__(16) char s_whole[];
 
-// Rows [0, valid) of a head into a tile of `rows` rows (a multiple of 32), the rest as zeros.
+// Rows [0, valid) of a head into `rows` rows (a multiple of 32), the rest as zeros: in
+// blocks of 32, with as much room after each for the block of another matrix, which is
+// then at a distance that the reading instructions hold.
 template <class T, int DB>
 __device__ __forceinline__ void fetch(Lds* tile, const View& v, int64_t b, int h, int valid, int rows, int d, int wave,
                                       int waves) {
@@ -30,17 +32,17 @@ __device__ __forceinline__ void fetch(Lds* tile, const View& v, int64_t b, int h
   if (d % Tl::EPV == 0 && ((uintptr_t)base & 15) == 0 && (pitch & 15) == 0 && pitch < (1 << 20)) {
     const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, 0x00020000);
     for (int i = wave; i < blocks; i += waves) {
-      // lane l fills place l of the i-th 64
+      // lane l fills place l of the i-th 64, VPR / 2 of which are a block
       const int at = i * 64 + lane, row = at / VPR, vec = (at % VPR) ^ Tl::swz(row);
       const uint32_t off = row < valid && vec * Tl::EPV < d ? (uint32_t)(row * (int)pitch + vec * 16) : OOB;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(tile + i * 1024), 16, off,
-                                               0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(tile + (i + i / (VPR / 2) * (VPR / 2)) * 1024),
+                                               16, off, 0, 0, 0);
     }
   } else {
     for (int i = wave; i < blocks; i += waves) {
       const int at = i * 64 + lane, row = at / VPR, vec = (at % VPR) ^ Tl::swz(row);
       const u32x4 r = load_raw((const T*)(base + row * pitch) + vec * Tl::EPV, row < valid ? d - vec * Tl::EPV : 0);
-      *(__attribute__((address_space(3))) u32x4*)(tile + at * 16) = r;
+      *(__attribute__((address_space(3))) u32x4*)(tile + (at + i / (VPR / 2) * 32 * VPR) * 16) = r;
     }
   }
 }
@@ -49,6 +51,84 @@ __device__ __forceinline__ void fetch(Lds* tile, const View& v, int64_t b, int h
 __device__ __forceinline__ void loads_and_writes_done() {
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): loads that pass no registers too
   __syncthreads();
+}
+
+// The forward: each wave has a block of 32 rows (r = query * group + head), as in
+// k_attn_forward; LDS holds K and V.
+template <class T, int KS>
+__global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T)), sizeof(T) == 4 || KS > 6 ? 2 : KS > 4 ? 3 : 5) void
+k_attn_whole_forward(Problem a, int64_t items, int64_t ids, T* out, float* lse) {
+  using O = Ops<T>;
+  using Frag = typename O::Frag;
+  constexpr int DB = (KS + 1) / 2;
+  using Tl = Tile<T, DB>;
+  constexpr int BLOCK = 32 * Tl::RB;
+  const int64_t id = group_id(ids);
+  if (id >= items) return;
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int64_t b = id / a.key_heads;
+  const int kh = (int)(id - b * a.key_heads);
+  const int nq = a.nq(b), nk = a.nk(b), shift = nk - nq;
+  Lds* const tk = (Lds*)s_whole;
+  const int first = 32 * wave, row = first + (lane & 31), rows = a.queries * a.group;
+  const int qi = row / a.group, qh = kh * a.group + row % a.group;
+  const bool live = qi < nq;
+  const int see = a.causal ? min(nk, qi + shift + 1) : nk;
+  const int all = a.causal ? min(nk, first / a.group + shift + 1) : nk;
+  const int end = first / a.group >= nq ? 0 : a.causal ? min(nk, min((first + 31) / a.group, nq - 1) + shift + 1) : nk;
+  Frag q[KS];
+  if (nq > 0 && nk > 0) {
+    const int nk32 = (nk + 31) & ~31;
+    fetch<T, DB>(tk, a.k, b, kh, nk, nk32, a.d, wave, waves);
+    fetch<T, DB>(tk + BLOCK, a.v, b, kh, nk, nk32, a.d, wave, waves);
+    const T* p = (const T*)a.q.p + b * a.q.batch + (int64_t)qi * a.q.token + (int64_t)qh * a.q.head;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) q[s] = O::load_row(p, live, s, half, a.d);
+  }
+  loads_and_writes_done();
+  f32x16 o[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) o[db] = zero16();
+  float m = -kInf, l = 0.f;
+  Lds* at = tk;
+  for (int key0 = 0; key0 < end; key0 += 32, at += 2 * BLOCK) {
+    f32x16 s = zero16();
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) s = O::mma(Tl::row(at, 0, ks, lane), q[ks], s);
+    if (key0 + 32 > all) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = key0 + 8 * (e >> 2) + 4 * half + (e & 3) < see ? s[e] : -kInf;
+    }
+    grow<O>(s, a.c, m, l, o);
+    const float ref = (m == -kInf ? 0.f : m) - O::BIAS;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      s[e] = fast_exp2(fmaf(s[e], a.c, -ref));
+      l += s[e];
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const Frag p = O::pack(s, x);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db] = O::mma(Tl::col(at + BLOCK, 16 * x, db, lane), p, o[db]);
+    }
+  }
+  l += other_half(l);
+  if (!live || l == 0.f) {
+    l = 0.f;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) o[db] = zero16();
+  }
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+  if (lse && half == 0 && row < rows)
+    lse[(b * a.heads + qh) * (int64_t)a.queries + qi] = l == 0.f ? kInf : m - O::BIAS + log2f(l);
+  __syncthreads();  // (keys and values are no longer read)
+  store_rows<T, DB>(tk + wave * BLOCK, o, inv, a.d, lane, [&](int r) -> T* {
+    const int to = first + r;
+    return to < rows ? out + ((b * a.queries + to / a.group) * a.heads + kh * a.group + to % a.group) * (int64_t)a.d
+                     : nullptr;
+  });
 }
 
 // The gradients of one head (heads == key_heads).  Each wave has a block of 32 queries
@@ -75,14 +155,16 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
   const int h = (int)(id - b * a.key_heads);
   const int nq = a.nq(b), nk = a.nk(b), shift = nk - nq;
   const int q_rows = (a.queries + 31) & ~31, k_rows = (a.keys + 31) & ~31;
+  // (blocks of K and V, and of Q and dO, in turn)
+  constexpr int BLOCK = 32 * Tl::RB;
   Lds* const tk = (Lds*)s_whole;
-  Lds* const tv = tk + k_rows * Tl::RB;
-  Lds* const tq = tv + k_rows * Tl::RB;
-  Lds* const tg = tq + q_rows * Tl::RB;
+  Lds* const tq = tk + 2 * k_rows * Tl::RB;
   typedef __attribute__((address_space(3))) float LdsFloat;
   typedef __attribute__((address_space(3))) f32x4 LdsFour;
-  LdsFloat* const s_lse = (LdsFloat*)(tg + q_rows * Tl::RB);
+  LdsFloat* const s_lse = (LdsFloat*)(tq + 2 * q_rows * Tl::RB);
   LdsFloat* const s_delta = s_lse + q_rows;
+  Lds* const my_k = tk + 2 * wave * BLOCK;
+  Lds* const my_q = tq + 2 * wave * BLOCK;
   const int64_t head0 = (b * a.heads + h) * (int64_t)a.queries;  // of lse
   const int first = 32 * wave;                                  // of the wave's queries, and of its keys
   const int qi = first + (lane & 31), key = qi;
@@ -95,8 +177,8 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
     const int nq32 = (nq + 31) & ~31, nk32 = (nk + 31) & ~31;
     fetch<T, DB>(tk, a.k, b, h, nk, nk32, a.d, wave, waves);
     fetch<T, DB>(tq, a.q, b, h, nq, nq32, a.d, wave, waves);
-    fetch<T, DB>(tv, a.v, b, h, nk, nk32, a.d, wave, waves);
-    fetch<T, DB>(tg, a.g, b, h, nq, nq32, a.d, wave, waves);
+    fetch<T, DB>(tk + BLOCK, a.v, b, h, nk, nk32, a.d, wave, waves);
+    fetch<T, DB>(tq + BLOCK, a.g, b, h, nq, nq32, a.d, wave, waves);
     if (live) l2 = lse[head0 + qi];
     if constexpr (MEAN) {
       const T* po = out + ((b * a.queries + qi) * a.heads + h) * (int64_t)a.d;
@@ -117,8 +199,8 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
       Frag q[KS], g[KS];
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        q[s] = Tl::row(tq, first, s, lane);
-        g[s] = Tl::row(tg, first, s, lane);
+        q[s] = Tl::row(my_q, 0, s, lane);
+        g[s] = Tl::row(my_q + BLOCK, 0, s, lane);
         if constexpr (MEAN) dot += O::dot(g[s], o[s]);
         if constexpr (O::F32)
           dot += O::dot(g[s], O::load_row(out + ((b * a.queries + qi) * a.heads + h) * (int64_t)a.d, live, s, half, a.d));
@@ -129,12 +211,13 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
       for (int db = 0; db < (MEAN ? DB : 1); ++db) mean[db] = zero16();
       float eps = 0.f;
       for (int walk = TWICE ? 0 : 1; walk < 2; ++walk) {
-        for (int key0 = 0; key0 < end; key0 += 32) {
+        Lds* at = tk;
+        for (int key0 = 0; key0 < end; key0 += 32, at += 2 * BLOCK) {
           f32x16 s = zero16(), p = zero16();
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) {
-            s = O::mma(Tl::row(tk, key0, ks, lane), q[ks], s);
-            p = O::mma(Tl::row(tv, key0, ks, lane), g[ks], p);
+            s = O::mma(Tl::row(at, 0, ks, lane), q[ks], s);
+            p = O::mma(Tl::row(at + BLOCK, 0, ks, lane), g[ks], p);
           }
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
@@ -159,7 +242,7 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
             const Frag ds = O::pack(p, x), ps = O::pack(s, x);
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
-              const Frag kt = Tl::col(tk, key0 + 16 * x, db, lane);
+              const Frag kt = Tl::col(at, 16 * x, db, lane);
               acc[db] = O::mma(kt, ds, acc[db]);
               if constexpr (MEAN) mean[db] = O::mma(kt, ps, mean[db]);
             }
@@ -182,7 +265,7 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
 #pragma unroll
         for (int db = 0; db < DB; ++db) acc[db] = zero16();
     }
-    if (half == 0 && first < nq) s_delta[qi] = dot * O::GRAD_UNIT;
+    if (half == 0 && first < nq) s_delta[qi] = dot;
     packed.pack(acc, a.scale);
   }
   const auto to = [&](T* p, int n, int heads) {
@@ -194,15 +277,15 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
     if (first < nk) {
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        k[s] = Tl::row(tk, first, s, lane);
-        v[s] = Tl::row(tv, first, s, lane);
+        k[s] = Tl::row(my_k, 0, s, lane);
+        v[s] = Tl::row(my_k + BLOCK, 0, s, lane);
       }
     }
     if (dq) {
       __syncthreads();  // nor is any key or value
       if (first < a.queries) {
-        packed.put(tk + first * Tl::RB, lane);
-        Rows<T, DB>::flush(tk + first * Tl::RB, a.d, lane, to(dq, a.queries, a.heads));
+        packed.put(tk + wave * BLOCK, lane);
+        Rows<T, DB>::flush(tk + wave * BLOCK, a.d, lane, to(dq, a.queries, a.heads));
       }
       __syncthreads();
     }
@@ -213,20 +296,27 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
     for (int db = 0; db < DB; ++db) ak[db] = av[db] = zero16();
     const int begin = first >= nk ? nq : a.causal ? max(0, first - shift) & ~31 : 0;
     const int all = a.causal ? first + 31 - shift : 0, seen = a.causal ? key - shift : 0;
-    for (int q0 = begin; q0 < nq; q0 += 32) {
-      f32x16 s = zero16(), p = zero16();
+    Lds* at = tq + begin * 2 * Tl::RB;
+    for (int q0 = begin; q0 < nq; q0 += 32, at += 2 * BLOCK) {
+      f32x16 s = zero16(), p;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const f32x4 dl = *(LdsFour*)(s_delta + q0 + 8 * e + 4 * half);
+#pragma unroll
+        for (int f = 0; f < 4; ++f) p[4 * e + f] = -dl[f];
+      }
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        s = O::mma(Tl::row(tq, q0, ks, lane), HELD ? k[HELD ? ks : 0] : Tl::row(tk, first, ks, lane), s);
-        p = O::mma(Tl::row(tg, q0, ks, lane), HELD ? v[HELD ? ks : 0] : Tl::row(tv, first, ks, lane), p);
+        s = O::mma(Tl::row(at, 0, ks, lane), HELD ? k[HELD ? ks : 0] : Tl::row(my_k, 0, ks, lane), s);
+        p = O::mma(Tl::row(at + BLOCK, 0, ks, lane), HELD ? v[HELD ? ks : 0] : Tl::row(my_k + BLOCK, 0, ks, lane), p);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const f32x4 ls = *(LdsFour*)(s_lse + q0 + 8 * e + 4 * half), dl = *(LdsFour*)(s_delta + q0 + 8 * e + 4 * half);
+        const f32x4 ls = *(LdsFour*)(s_lse + q0 + 8 * e + 4 * half);
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
           s[4 * e + f] = fast_exp2(fmaf(s[4 * e + f], a.c, -ls[f]));
-          p[4 * e + f] = s[4 * e + f] * fmaf(p[4 * e + f], O::GRAD_UNIT, -dl[f]);
+          p[4 * e + f] = s[4 * e + f] * (O::GRAD_UNIT * p[4 * e + f]);
         }
       }
       if (q0 < all) {
@@ -242,8 +332,8 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
         const Frag fp = O::pack(s, x), fs = O::pack(p, x);
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
-          av[db] = O::mma(Tl::col(tg, q0 + 16 * x, db, lane), fp, av[db]);
-          ak[db] = O::mma(Tl::col(tq, q0 + 16 * x, db, lane), fs, ak[db]);
+          av[db] = O::mma(Tl::col(at + BLOCK, 16 * x, db, lane), fp, av[db]);
+          ak[db] = O::mma(Tl::col(at, 16 * x, db, lane), fs, ak[db]);
         }
       }
     }
@@ -252,16 +342,16 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
 #pragma unroll
         for (int db = 0; db < DB; ++db) ak[db] = av[db] = zero16();
       // (this wave's keys and values are no longer read)
-      store_rows<T, DB>(tk + first * Tl::RB, ak, a.scale, a.d, lane, to(dk, a.keys, a.key_heads));
-      store_rows<T, DB>(tv + first * Tl::RB, av, O::GRAD_UNIT, a.d, lane, to(dv, a.keys, a.key_heads));
+      store_rows<T, DB>(my_k, ak, a.scale, a.d, lane, to(dk, a.keys, a.key_heads));
+      store_rows<T, DB>(my_k + BLOCK, av, O::GRAD_UNIT, a.d, lane, to(dv, a.keys, a.key_heads));
     }
   }
   if constexpr (!HELD) {
     if (dq) {
       __syncthreads();  // queries are no longer read
       if (first < a.queries) {
-        packed.put(tq + first * Tl::RB, lane);
-        Rows<T, DB>::flush(tq + first * Tl::RB, a.d, lane, to(dq, a.queries, a.heads));
+        packed.put(my_q, lane);
+        Rows<T, DB>::flush(my_q, a.d, lane, to(dq, a.queries, a.heads));
       }
     }
   }
