@@ -45,8 +45,9 @@ def hipcc() -> str:
 
 
 def sources() -> list[Path]:
-    return [CSRC / f"{name}.hip" for name in ("mec_abi", "mec_vocab", "mec_rotary", "mec_attention",
-                                           "mec_attention_backward")]
+    names = ["mec_abi", "mec_vocab", "mec_rotary", "mec_attention", "mec_attention_backward", "mec_attn_bwd_f32",
+             "mec_attn_bwd_bf16", "mec_attn_bwd_f16"]
+    return [CSRC / f"{name}.hip" for name in names]
 
 
 def _run(cmd: list[str], verbose: bool) -> None:

@@ -97,10 +97,10 @@ int mec_attention(const mec_attention_t* attention, const mec_heads_t* query, co
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int KS = decltype(ks)::value;
     if (p.whole) {
-      k_attn_whole_forward<T, KS><<<g.dims, 64 * p.whole, p.lds, st>>>(a, g.items, g.ids, (T*)out, lse);
+      k_attn_whole_forward<T, KS><<<g.dims, 64 * p.whole, p.lds, st>>>(a, g.items, (T*)out, lse);
     } else if (p.few) {
       k_attn_forward<T, KS, 1, kWave>
-          <<<g.dims, 64 * kWave, 0, st>>>(a, g.items, g.ids, p.row_tiles, p.splits, (T*)out, lse, parts);
+          <<<g.dims, 64 * kWave, 0, st>>>(a, g.items, p.row_tiles, p.splits, (T*)out, lse, parts);
       if (p.splits > 1) {
         const int64_t rows = a.pairs * a.queries * a.group, groups = ceil_div(rows, 4);
         const int64_t x = groups < (1 << 20) ? groups : (1 << 20);
@@ -108,7 +108,7 @@ int mec_attention(const mec_attention_t* attention, const mec_heads_t* query, co
                                                                                         (T*)out, lse);
       }
     } else {
-      k_attn_forward<T, KS, kWave, 1><<<g.dims, 64 * kWave, 0, st>>>(a, g.items, g.ids, p.row_tiles, 1, (T*)out, lse, parts);
+      k_attn_forward<T, KS, kWave, 1><<<g.dims, 64 * kWave, 0, st>>>(a, g.items, p.row_tiles, 1, (T*)out, lse, parts);
     }
   });
   return check_launch("mec_attention");

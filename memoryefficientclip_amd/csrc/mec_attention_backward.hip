@@ -1,22 +1,14 @@
 // C-ABI entry points of attention's backward (include/mec.h): argument validation in
 // plain host code, then stream-ordered kernel launches.  Nothing here allocates
 // device memory or synchronises the host.
-#include "mec_attn_bwd.h"
+#include "mec_attn_cut.h"
 #include "mec_attn_whole.h"
-#include "mec_attn_host.h"
 
 using namespace mec;
 using namespace mec::attn;
 
 namespace {
 
-// Waves and LDS of k_attn_whole_grad, 0 waves where it does not fit.  Where it does it was the faster form at all
-// sizes, 2 to 256 x 12 heads (256 x 12 heads of 64, us, this form and two kernels that walk over tiles: 77 tokens 68
-// and 131, 197 tokens 297 and 354, 257 tokens 414 and 571; fp32, 77 tokens, 395 and 459).
-struct Whole {
-  int waves;
-  size_t lds;
-};
 Whole plan_whole(const Problem& a, int dtype) {
   const int size = dtype == MEC_DTYPE_F32 ? 4 : 2, steps = a.d <= 32 ? 2 : a.d <= 64 ? 4 : a.d <= 96 ? 6 : 8;
   const int row = 16 * steps * size, most = whole_waves(steps, size);
@@ -28,6 +20,28 @@ Whole plan_whole(const Problem& a, int dtype) {
   return {blocks, (size_t)lds};
 }
 
+int plan_cut(const Problem& a, const Whole& whole, Cut* out) {
+  Cut c{};
+  int cus = 0;
+  if (int rc = compute_units(&cus)) return rc;
+  const int64_t rows = (int64_t)a.queries * a.group;
+  c.splits = 1;
+  if (!whole.waves) {
+    c.few_rows = a.pairs * ceil_div(rows, 128) < cus;
+    c.few_keys = a.pairs * ceil_div(a.keys, 128) < cus;
+    c.row_tiles = (int)ceil_div(rows, c.few_rows ? 32 : 128);
+    c.key_tiles = (int)ceil_div(a.keys, c.few_keys ? 32 : 128);
+    c.delta = round256(a.pairs * rows * 4);
+    // about 8 workgroups a CU, 8 tiles of queries or more each
+    const int64_t want = 8 * cus / (a.pairs * c.key_tiles), most = a.group * ceil_div(a.queries, 64) / 8;
+    const int64_t s = want < most ? want : most;
+    c.splits = (int)(s < 1 ? 1 : s);
+    if (c.splits > 1) c.parts = c.splits * a.pairs * a.keys * 2 * a.d * 4;
+  }
+  *out = c;
+  return MEC_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -35,8 +49,10 @@ extern "C" {
 int64_t mec_attention_backward_workspace_bytes(const mec_attention_t* attention) {
   g_err.clear();
   Problem a{};
+  Cut c{};
   int rc = check_attention(attention, &a);
-  return rc ? rc : a.pairs * a.queries * a.group * (int64_t)sizeof(float);
+  if (!rc) rc = plan_cut(a, plan_whole(a, attention->dtype), &c);
+  return rc ? rc : c.delta + c.parts;
 }
 
 int mec_attention_backward(const mec_attention_t* attention, const mec_heads_t* query, const mec_heads_t* key,
@@ -45,7 +61,9 @@ int mec_attention_backward(const mec_attention_t* attention, const mec_heads_t* 
                            int64_t workspace_bytes, void* stream) {
   g_err.clear();
   Problem a{};
-  Grid gq{}, gk{}, gw{};
+  Whole whole{};
+  Cut c{};
+  Grid gq{}, gk{}, gj{};
   int rc = check_attention(attention, &a);
   if (!rc) rc = check_heads(query, "query");
   if (!rc) rc = check_heads(key, "key");
@@ -53,13 +71,15 @@ int mec_attention_backward(const mec_attention_t* attention, const mec_heads_t* 
   if (!rc) rc = check_heads(grad_out, "grad_out");
   if (!rc && (!out || !lse)) rc = fail(MEC_ERR_INVALID, "out and lse must be non-null");
   if (!rc && (!grad_key != !grad_value)) rc = fail(MEC_ERR_INVALID, "grad_key and grad_value go together");
-  if (!rc) rc = check_scratch(workspace, workspace_bytes, a.pairs * a.queries * a.group * (int64_t)sizeof(float));
   if (!rc) rc = check_not_capturing(stream);
-  const int64_t rows = (int64_t)a.queries * a.group;
-  const int row_tiles = (int)ceil_div(rows, 128), key_tiles = (int)ceil_div(a.keys, 128);
-  if (!rc) rc = make_grid(a.pairs * row_tiles, &gq);
-  if (!rc) rc = make_grid(a.pairs * key_tiles, &gk);
-  if (!rc) rc = make_grid(a.pairs, &gw);
+  if (!rc) {
+    whole = plan_whole(a, attention->dtype);
+    rc = plan_cut(a, whole, &c);
+  }
+  if (!rc) rc = check_scratch(workspace, workspace_bytes, c.delta + c.parts);
+  if (!rc) rc = make_grid(a.pairs * (whole.waves ? 1 : c.row_tiles), &gq);
+  if (!rc && !whole.waves) rc = make_grid(a.pairs * c.key_tiles * c.splits, &gk);
+  if (!rc && c.splits > 1) rc = make_grid(ceil_div(a.pairs * a.keys, 4), &gj);
   if (rc || (!grad_query && !grad_key)) return rc;
   a.q = view(query);
   a.k = view(key);
@@ -67,22 +87,9 @@ int mec_attention_backward(const mec_attention_t* attention, const mec_heads_t* 
   a.g = view(grad_out);
   hipStream_t st = (hipStream_t)stream;
   float* delta = (float*)workspace;
-  const Whole whole = plan_whole(a, attention->dtype);
-  with_kernel(attention->dtype, a.d, [&](auto* t, auto ks) {
-    using T = std::remove_pointer_t<decltype(t)>;
-    constexpr int KS = decltype(ks)::value;
-    if constexpr (KS <= whole_steps(sizeof(T))) {
-      if (whole.waves) {
-        k_attn_whole_grad<T, KS><<<gw.dims, 64 * whole.waves, whole.lds, st>>>(
-            a, gw.items, gw.ids, (const T*)out, lse, (T*)grad_query, (T*)grad_key, (T*)grad_value);
-        return;
-      }
-    }
-    k_attn_dq<T, KS><<<gq.dims, 256, 0, st>>>(a, gq.items, gq.ids, row_tiles, (const T*)out, lse, delta, (T*)grad_query);
-    if (grad_key)
-      k_attn_dkv<T, KS><<<gk.dims, 256, 0, st>>>(a, gk.items, gk.ids, key_tiles, lse, delta, (T*)grad_key,
-                                                 (T*)grad_value);
-  });
+  float* parts = c.splits > 1 ? (float*)((char*)workspace + c.delta) : nullptr;
+  const Launch l{a, whole, c, gq, gk, gj, lse, delta, parts, out, grad_query, grad_key, grad_value, st};
+  with_element_type(attention->dtype, [&](auto* t) { launch_backward<std::remove_pointer_t<decltype(t)>>(l); });
   return check_launch("mec_attention_backward");
 }
 

@@ -53,19 +53,35 @@ struct Problem {
   __device__ __forceinline__ int length(const void* p, int64_t b, int all) const {
     if (p == nullptr) return all;
     const int64_t n = length64 ? ((const int64_t*)p)[b] : (int64_t)((const int32_t*)p)[b];
-    return n < 0 ? 0 : n > all ? all : (int)n;
+    return __builtin_amdgcn_readfirstlane(n < 0 ? 0 : n > all ? all : (int)n);  // (the same in all lanes: scalar)
   }
   __device__ __forceinline__ int nq(int64_t b) const { return length(query_lengths, b, queries); }
   __device__ __forceinline__ int nk(int64_t b) const { return length(key_lengths, b, keys); }
 };
 
-// Workgroup id in a launch of `n` (a multiple of 8, over x and y), such that
-// neighbouring ids run on one XCD and share what they read in its L2; n or more
-// for the workgroups beyond.
-__device__ __forceinline__ int64_t group_id(int64_t n) {
-  const int64_t bid = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
-  return bid < n ? (bid & 7) * (n >> 3) + (bid >> 3) : n;
-}
+// What the workgroups of a launch take: `tiles` items of each pair of batch entry and
+// key head.  Workgroups run on the 8 XCDs in turn, each with an L2 of its own.  With many
+// pairs an XCD has all items of its pairs, one pair after another, which share what they
+// read.  With few pairs the first items of all pairs come first (where causal, the
+// longest), and an XCD has a pair's items in turn with others: in the order of many
+// pairs some XCDs would have all the long items, the others all the short ones.
+struct Items {
+  int64_t count, ids;  // of items; the same, as a multiple of 8
+  static constexpr int MANY = 64;
+  __device__ __forceinline__ bool take(int64_t pairs, int tiles, int64_t& pair, int& tile) const {
+    int64_t id = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    if (id >= ids) return false;
+    if (pairs >= MANY) {
+      id = (id & 7) * (ids >> 3) + (id >> 3);
+      pair = id / tiles;
+      tile = (int)(id - pair * tiles);
+    } else {
+      tile = (int)(id / pairs);
+      pair = id - tile * pairs;
+    }
+    return id < count;
+  }
+};
 
 // 8 consecutive k of a row or column, and the products of 32 x 16 by 16 x 32.
 template <class T>

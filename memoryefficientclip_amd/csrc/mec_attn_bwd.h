@@ -9,6 +9,13 @@
 // in a pass of its own.  Gradients of the scores are rounded to T like the results:
 // in fp16, to steps of 2^-24 and up to 65504, as the gradients that go out are.
 // k_attn_dq also leaves delta = do . o for k_attn_dkv.
+//
+// WM = 4: the four waves of a workgroup have 32 rows (keys) each and share tiles,
+// two in LDS, the next on its way in registers.  WM = 1, where that would leave the
+// device empty: they share 32 rows (keys) and take every fourth tile of 32, each in
+// LDS of its own, and add up what they have in the end.  k_attn_dkv's queries are
+// split over `splits` workgroups besides, whose fp32 sums k_attn_dkv_join adds, where
+// there are few keys, or the first ones are seen by many more queries than the last.
 #pragma once
 #include <climits>
 
@@ -17,46 +24,68 @@
 namespace mec {
 namespace attn {
 
-template <class T, int KS>
+template <class T, int KS, int WM>
 struct Backward {
   using O = Ops<T>;
-  static constexpr int DB = (KS + 1) / 2, WAVES = 4, NT = 64 * WAVES, ROWS = 32 * WAVES;
+  static constexpr int DB = (KS + 1) / 2, WAVES = 4, NT = 64 * WAVES, WK = WAVES / WM, ROWS = 32 * WM;
+  static_assert(WM == 1 || WM == 4, "");
   using Tl = Tile<T, DB>;
   // rows of the tiles that are walked over
-  static constexpr int KEYS = O::F32 || DB > 3 ? 32 : 64, QUERIES = O::F32 || DB > 3 ? 32 : 64;
+  static constexpr int STEP = WM == 1 || O::F32 || DB > 3 ? 32 : 64;
+  static constexpr int TILE = STEP * Tl::RB, BUFS = WM == 1 ? 1 : 2;
+  static constexpr int TILES = 2 * TILE * BUFS * WK;  // of all waves
+  // (what leaves passes through the same LDS)
+  static_assert(WM == 1 ? WK * 32 * 32 * DB * 4 <= TILES : 128 * Tl::RB <= TILES, "");
   // the values of a wave's keys stay in LDS where keys, values and both gradients take
   // more registers than two waves on a SIMD have
   static constexpr bool V_LDS = !O::F32 && DB > 3;
   // The forward's result has the errors of 16 bits, and so has do . o; where few keys share a row's weight
   // this is the largest error of dq and dk (heads of 64, 77 tokens, causal, bf16: 0.0031 of their size, 0.0023
   // with a delta of fp32).  delta is also sum_j p_ij do_i . v_j: with d for do . o, eps = sum_j p_ij (do_i . v_j - d)
-  // is what it lacks.  Up to KEYS_EXACT keys it is summed along with dq, and dq corrected by -eps sum_j p_ij k_j
-  // (its product costs no reads of LDS), or, where registers are short, summed in a first walk over the keys.
+  // is what it lacks.  Up to this many keys it is summed in a first walk over them.
   static constexpr int KEYS_EXACT = O::F32 ? 0 : 512;
-  static constexpr bool TWICE = DB > 2;
 };
 
-template <class T, int KS>
-__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void k_attn_dq(Problem a, int64_t items, int64_t ids, int row_tiles, const T* out,
-                                                 const float* lse, float* delta, T* dq) {
-  using B = Backward<T, KS>;
+// A row of the sums of a workgroup's waves, [WK][32][32 DB] in LDS.
+template <int WK, int DB>
+__device__ __forceinline__ float joined(const float* sums, int r, int e) {
+  float v = 0.f;
+#pragma unroll
+  for (int i = 0; i < WK; ++i) v += sums[(i * 32 + r) * 32 * DB + e];
+  return v;
+}
+template <int DB>
+__device__ __forceinline__ void put_sums(float* sums, const f32x16 (&acc)[DB], int wave, int lane) {
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *(f32x4*)(sums + ((wave * 32 + (lane & 31)) * DB + db) * 32 + 8 * i + 4 * (lane >> 5)) =
+          f32x4{acc[db][4 * i], acc[db][4 * i + 1], acc[db][4 * i + 2], acc[db][4 * i + 3]};
+}
+
+template <class T, int KS, int WM>
+__global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2) void k_attn_dq(
+    Problem a, Items items, int row_tiles, const T* out, const float* lse, float* delta, T* dq) {
+  using B = Backward<T, KS, WM>;
   using O = Ops<T>;
   using Frag = typename O::Frag;
   using Tl = typename B::Tl;
-  constexpr int DB = B::DB, KEYS = B::KEYS, NB = KEYS / 32, TILE = KEYS * Tl::RB;
-  __shared__ alignas(16) char s_lds[4 * TILE];
+  constexpr int DB = B::DB, STEP = B::STEP, NB = STEP / 32, WK = B::WK;
+  __shared__ alignas(16) char s_lds[B::TILES];
+  __shared__ float s_eps[WM == 1 ? WK : 1][32];
   Lds* const lds = (Lds*)s_lds;
-  const int64_t id = group_id(ids);
-  if (id >= items) return;
+  int64_t pair;
+  int tile;
+  if (!items.take(a.pairs, row_tiles, pair, tile)) return;
+  tile = row_tiles - 1 - tile;  // (where causal, the last rows see most keys)
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t pair = id / row_tiles;
-  const int tile = row_tiles - 1 - (int)(id - pair * row_tiles);
   const int64_t b = pair / a.key_heads;
   const int kh = (int)(pair - b * a.key_heads);
   const int nq = a.nq(b), nk = a.nk(b), shift = nk - nq;
   const int rows = a.queries * a.group;
-  const int row0 = tile * B::ROWS, wave_row0 = row0 + 32 * wave;
+  const int row0 = tile * B::ROWS, wave_row0 = row0 + (WM == 1 ? 0 : 32 * wave);
   const int row = wave_row0 + (lane & 31);
   const int qi = row / a.group, qh = kh * a.group + row % a.group;
   const bool live = qi < nq;
@@ -87,126 +116,130 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void k_attn_dq(Problem
     dot += other_half(dot);
     if (live) l2 = lse[at];
   }
-  f32x16 acc[DB], mean[B::TWICE ? 1 : DB];  // dq / scale, sum_j p_ij k_j
+  f32x16 acc[DB];  // dq / scale
 #pragma unroll
-  for (int db = 0; db < DB; ++db) {
-    acc[db] = zero16();
-    mean[B::TWICE ? 0 : db] = zero16();
-  }
-  float eps = 0.f;
-  const int tiles = (end + KEYS - 1) / KEYS;
+  for (int db = 0; db < DB; ++db) acc[db] = zero16();
+  const int tiles = (end + STEP - 1) / STEP;
   if (tiles > 0) {
-    Loader<T, DB, KEYS, B::NT> lk, lv;
-    lk.init(a.k, b, kh, a.d, threadIdx.x);
-    lv.init(a.v, b, kh, a.d, threadIdx.x);
-    lk.load(0, nk);
-    lv.load(0, nk);
-    // (the first walk: below 0)
-    for (int i = B::TWICE && exact ? -tiles : 0; i < tiles; ++i) {
-      Lds* const tk = lds + (i & 1 ? 2 * TILE : 0);
-      Lds* const tv = tk + TILE;
-      lk.store(tk);
-      lv.store(tv);
-      __syncthreads();
-      if (i + 1 < tiles) {
-        const int next = (i + 1 < 0 ? i + 1 + tiles : i + 1) * KEYS;
-        lk.load(next, nk - next);
-        lv.load(next, nk - next);
+    Loader<T, DB, STEP, 64 * WM> lk, lv;
+    const int t = WM == 1 ? lane : threadIdx.x;
+    lk.init(a.k, b, kh, a.d, t);
+    lv.init(a.v, b, kh, a.d, t);
+    Lds* const mine = lds + (WM == 1 ? wave * 2 * B::TILE : 0);
+    const int first = WM == 1 ? wave : 0;
+    int turn = 0;  // (a tile's place in LDS)
+#pragma unroll 1
+    for (int walk = exact ? 0 : 1; walk < 2; ++walk) {
+      float eps = 0.f;
+      if (first < tiles) {
+        lk.load(first * STEP, nk - first * STEP);
+        lv.load(first * STEP, nk - first * STEP);
       }
-      if (B::TWICE && i == 0 && exact) {
-        dot += eps + other_half(eps);
-        eps = 0.f;
-      }
-      const int key0 = (i < 0 ? i + tiles : i) * KEYS;
-      if (key0 >= wave_end) continue;
-      const bool masked = key0 + KEYS > all;
-#pragma unroll
-      for (int kb = 0; kb < NB; ++kb) {
-        f32x16 s = zero16(), p = zero16();
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          s = O::mma(Tl::row(tk, 32 * kb, ks, lane), q[ks], s);
-          p = O::mma(Tl::row(tv, 32 * kb, ks, lane), g[ks], p);
+      for (int i = first; i < tiles; i += WK, ++turn) {
+        Lds* const tk = mine + (B::BUFS == 2 && (turn & 1) ? 2 * B::TILE : 0);
+        Lds* const tv = tk + B::TILE;
+        lk.store(tk);
+        lv.store(tv);
+        if constexpr (WM == 1)
+          wave_sync();
+        else
+          __syncthreads();
+        if (i + WK < tiles) {
+          lk.load((i + WK) * STEP, nk - (i + WK) * STEP);
+          lv.load((i + WK) * STEP, nk - (i + WK) * STEP);
         }
+        const int key0 = i * STEP;
+        if (key0 >= wave_end) continue;
+        const bool masked = key0 + STEP > all;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          s[e] = fast_exp2(fmaf(s[e], a.c, -l2));
-          p[e] = s[e] * (p[e] - dot);
-        }
-        if (masked) {
+        for (int kb = 0; kb < NB; ++kb) {
+          f32x16 s = zero16(), p = zero16();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const bool in = key0 + 32 * kb + 8 * (e >> 2) + 4 * half + (e & 3) < see;
-            s[e] = in ? s[e] : 0.f;
-            p[e] = in ? p[e] : 0.f;
+          for (int ks = 0; ks < KS; ++ks) {
+            s = O::mma(Tl::row(tk, 32 * kb, ks, lane), q[ks], s);
+            p = O::mma(Tl::row(tv, 32 * kb, ks, lane), g[ks], p);
           }
-        }
-        if (!O::F32 && exact) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) eps += p[e];
-          if (B::TWICE && i < 0) continue;
-        }
+          for (int e = 0; e < 16; ++e) p[e] = fast_exp2(fmaf(s[e], a.c, -l2)) * (p[e] - dot);
+          if (masked) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const Frag ds = O::pack(p, h);
-          if (!O::F32 && !B::TWICE && exact) {
-            const Frag ps = O::pack(s, h);
+            for (int e = 0; e < 16; ++e)
+              p[e] = key0 + 32 * kb + 8 * (e >> 2) + 4 * half + (e & 3) < see ? p[e] : 0.f;
+          }
+          if constexpr (!O::F32) {
+            // (one loop for both walks: the compiler's two copies of it take 50 registers more)
+            int w = walk;
+            asm volatile("" : "+v"(w));
+            if (__builtin_amdgcn_readfirstlane(w) == 0) {
 #pragma unroll
-            for (int db = 0; db < DB; ++db) {
-              const Frag kt = Tl::col(tk, 32 * kb + 16 * h, db, lane);
-              acc[db] = O::mma(kt, ds, acc[db]);
-              mean[db] = O::mma(kt, ps, mean[db]);
+              for (int e = 0; e < 16; ++e) eps += p[e];
+              continue;
             }
-          } else {
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const Frag ds = O::pack(p, h);
 #pragma unroll
             for (int db = 0; db < DB; ++db) acc[db] = O::mma(Tl::col(tk, 32 * kb + 16 * h, db, lane), ds, acc[db]);
           }
         }
       }
+      if (walk == 0) {
+        eps += other_half(eps);
+        if constexpr (WM == 1) {
+          if (half == 0) s_eps[wave][lane] = eps;
+          __syncthreads();
+          eps = 0.f;
+#pragma unroll
+          for (int i = 0; i < WK; ++i) eps += s_eps[i][lane & 31];
+        }
+        dot += eps;
+      }
     }
   }
-  if (!O::F32 && !B::TWICE && exact) {
-    eps += other_half(eps);
-    dot += eps;
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[db][e] -= eps * mean[db][e];
-  }
-  if (half == 0 && row < rows) delta[at] = dot;
+  if (half == 0 && row < rows && (WM > 1 || wave == 0)) delta[at] = dot;
   if (dq == nullptr) return;
   if (!live || l2 == kInf)
 #pragma unroll
     for (int db = 0; db < DB; ++db) acc[db] = zero16();
+  const auto to = [&](int r) -> T* {
+    const int x = wave_row0 + r;
+    return x < rows ? dq + ((b * a.queries + x / a.group) * a.heads + kh * a.group + x % a.group) * (int64_t)a.d : nullptr;
+  };
   __syncthreads();  // (the tiles are no longer read)
-  store_rows<T, DB>(lds + 32 * wave * Tl::RB, acc, a.scale, a.d, lane, [&](int r) -> T* {
-    const int to = wave_row0 + r;
-    return to < rows ? dq + ((b * a.queries + to / a.group) * a.heads + kh * a.group + to % a.group) * (int64_t)a.d
-                     : nullptr;
-  });
+  if constexpr (WM == 1) {
+    put_sums<DB>((float*)s_lds, acc, wave, lane);
+    __syncthreads();
+    for (int r = wave; r < 32; r += WK)
+      if (T* p = to(r))
+        for (int e = lane; e < a.d; e += 64) put(p + e, a.scale * joined<WK, DB>((float*)s_lds, r, e));
+  } else {
+    store_rows<T, DB>(lds + 32 * wave * Tl::RB, acc, a.scale, a.d, lane, to);
+  }
 }
 
-template <class T, int KS>
-__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void k_attn_dkv(Problem a, int64_t items, int64_t ids, int key_tiles,
-                                                  const float* lse, const float* delta, T* dk, T* dv) {
-  using B = Backward<T, KS>;
+template <class T, int KS, int WM>
+__global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2) void k_attn_dkv(
+    Problem a, Items items, int key_tiles, int splits, const float* lse, const float* delta, T* dk, T* dv, float* parts) {
+  using B = Backward<T, KS, WM>;
   using O = Ops<T>;
   using Frag = typename O::Frag;
   using Tl = typename B::Tl;
-  constexpr int DB = B::DB, QUERIES = B::QUERIES, NB = QUERIES / 32, TILE = QUERIES * Tl::RB;
-  __shared__ alignas(16) char s_lds[4 * TILE + (B::V_LDS ? B::ROWS * Tl::RB : 0)];
-  __shared__ alignas(16) float s_row[2][2][QUERIES];  // lse, delta of the tile's queries
+  constexpr int DB = B::DB, STEP = B::STEP, NB = STEP / 32, WK = B::WK;
+  __shared__ alignas(16) char s_lds[B::TILES + (B::V_LDS ? B::ROWS * Tl::RB : 0)];
+  __shared__ alignas(16) float s_row[WK][B::BUFS][2][STEP];  // lse, delta of the tile's queries
   Lds* const lds = (Lds*)s_lds;
-  const int64_t id = group_id(ids);
-  if (id >= items) return;
+  int64_t pair;
+  int tile;  // (where causal, the first keys are seen by most queries)
+  if (!items.take(a.pairs, key_tiles * splits, pair, tile)) return;
+  const int split = tile % splits;
+  tile /= splits;
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t pair = id / key_tiles;
-  const int tile = (int)(id - pair * key_tiles);  // (where causal, the first keys are seen by most queries)
   const int64_t b = pair / a.key_heads;
   const int kh = (int)(pair - b * a.key_heads);
   const int nq = a.nq(b), nk = a.nk(b), shift = nk - nq;
-  const int key0 = tile * B::ROWS, wave_key0 = key0 + 32 * wave;
+  const int key0 = tile * B::ROWS, wave_key0 = key0 + (WM == 1 ? 0 : 32 * wave);
   const int key = wave_key0 + (lane & 31);
   const bool live = key < nk;
   // queries that see any key of the workgroup, of the wave; those from which on all see all of the wave's; and
@@ -219,10 +252,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void k_attn_dkv(Proble
   f32x16 ak[DB], av[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) ak[db] = av[db] = zero16();
-  const int first = begin / QUERIES, each = (nq + QUERIES - 1) / QUERIES - first;
-  if (each > 0) {
+  // the tiles of all heads, and this workgroup's share of them
+  const int first = begin / STEP, each = (nq + STEP - 1) / STEP - first;
+  const int tiles = each > 0 ? each * a.group : 0, share = (tiles + splits - 1) / splits;
+  const int stop = min(tiles, (split + 1) * share);
+  if (split * share < stop) {
     Frag k[KS], v[B::V_LDS ? 1 : KS];
-    Lds* const values = lds + 4 * TILE;
+    Lds* const values = lds + B::TILES + (WM == 1 ? 0 : 32 * wave * Tl::RB);
     {
       const T* pk = (const T*)a.k.p + b * a.k.batch + (int64_t)key * a.k.token + (int64_t)kh * a.k.head;
       const T* pv = (const T*)a.v.p + b * a.v.batch + (int64_t)key * a.v.token + (int64_t)kh * a.v.head;
@@ -230,42 +266,53 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void k_attn_dkv(Proble
       for (int s = 0; s < KS; ++s) {
         k[s] = O::load_row(pk, live, s, half, a.d);
         const Frag x = O::load_row(pv, live, s, half, a.d);
-        if constexpr (B::V_LDS)
-          Tl::put_row(values, 32 * wave, s, lane, x);  // (read by this wave alone)
-        else
+        if constexpr (B::V_LDS) {
+          // (WM = 4: read by this wave alone; WM = 1: by all, which write the same)
+          Tl::put_row(values, 0, s, lane, x);
+        } else {
           v[s] = x;
+        }
       }
     }
-    Loader<T, DB, QUERIES, B::NT> lq, lg;
-    float r_row = 0.f;  // threads below 2 QUERIES: a value of s_row on its way
-    const int t = threadIdx.x;
+    Loader<T, DB, STEP, 64 * WM> lq, lg;
+    float r_row[2] = {0.f, 0.f};  // a query's lse and delta on their way (WM = 4: one of them)
+    const int t = WM == 1 ? lane : threadIdx.x;
+    int loaded = -1;  // head
     auto load = [&](int at) {
-      const int h = kh * a.group + at / each, q0 = (first + at % each) * QUERIES;
-      if (at % each == 0 || at == 0) {
+      const int h = kh * a.group + at / each, q0 = (first + at % each) * STEP;
+      if (h != loaded) {
         lq.init(a.q, b, h, a.d, t);
         lg.init(a.g, b, h, a.d, t);
+        loaded = h;
       }
       lq.load(q0, nq - q0);
       lg.load(q0, nq - q0);
-      if (t < 2 * QUERIES) {
-        const int i = q0 + t % QUERIES;
-        const float* p = (t < QUERIES ? lse : delta) + (b * a.heads + h) * (int64_t)a.queries;
-        const float x = i < nq ? p[i] : t < QUERIES ? kInf : 0.f;
-        r_row = t < QUERIES ? x - O::GRAD_BIAS : x * O::GRAD_UNIT;
+      const int64_t head0 = (b * a.heads + h) * (int64_t)a.queries;
+      const int i = q0 + t % STEP;
+      if (t < 2 * STEP) {
+        const float x = i < nq ? (t < STEP ? lse : delta)[head0 + i] : t < STEP ? kInf : 0.f;
+        r_row[0] = t < STEP ? x - O::GRAD_BIAS : x * O::GRAD_UNIT;
       }
     };
-    load(0);
-    const int tiles = each * a.group;
-    for (int i = 0; i < tiles; ++i) {
-      Lds* const tq = lds + (i & 1 ? 2 * TILE : 0);
-      Lds* const tg = tq + TILE;
+    Lds* const mine = lds + (WM == 1 ? wave * 2 * B::TILE : 0);
+    const int begin_at = split * share + (WM == 1 ? wave : 0);
+    if (begin_at < stop) load(begin_at);
+    int turn = 0;
+    for (int i = begin_at; i < stop; i += WK, ++turn) {
+      const int buf = B::BUFS == 2 ? turn & 1 : 0;
+      Lds* const tq = mine + buf * 2 * B::TILE;
+      Lds* const tg = tq + B::TILE;
+      auto& row = s_row[WM == 1 ? wave : 0][buf];
       lq.store(tq);
       lg.store(tg);
-      if (t < 2 * QUERIES) s_row[i & 1][t / QUERIES][t % QUERIES] = r_row;
-      __syncthreads();
-      if (i + 1 < tiles) load(i + 1);
-      const int q0 = (first + i % each) * QUERIES;
-      if (q0 + QUERIES <= wave_begin) continue;
+      if (t < 2 * STEP) row[t / STEP][t % STEP] = r_row[0];
+      if constexpr (WM == 1)
+        wave_sync();
+      else
+        __syncthreads();
+      if (i + WK < stop) load(i + WK);
+      const int q0 = (first + i % each) * STEP;
+      if (q0 + STEP <= wave_begin) continue;
       const bool masked = q0 < all;
 #pragma unroll
       for (int qb = 0; qb < NB; ++qb) {
@@ -274,14 +321,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void k_attn_dkv(Proble
         for (int ks = 0; ks < KS; ++ks) {
           s = O::mma(Tl::row(tq, 32 * qb, ks, lane), k[ks], s);
           if constexpr (B::V_LDS)
-            p = O::mma(Tl::row(tg, 32 * qb, ks, lane), Tl::row(values, 32 * wave, ks, lane), p);
+            p = O::mma(Tl::row(tg, 32 * qb, ks, lane), Tl::row(values, 0, ks, lane), p);
           else
             p = O::mma(Tl::row(tg, 32 * qb, ks, lane), v[ks], p);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const f32x4 l2 = *(const f32x4*)&s_row[i & 1][0][32 * qb + 8 * e + 4 * half];
-          const f32x4 dl = *(const f32x4*)&s_row[i & 1][1][32 * qb + 8 * e + 4 * half];
+          const f32x4 l2 = *(const f32x4*)&row[0][32 * qb + 8 * e + 4 * half];
+          const f32x4 dl = *(const f32x4*)&row[1][32 * qb + 8 * e + 4 * half];
 #pragma unroll
           for (int f = 0; f < 4; ++f) {
             s[4 * e + f] = fast_exp2(fmaf(s[4 * e + f], a.c, -l2[f]));
@@ -311,15 +358,72 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void k_attn_dkv(Proble
   if (!live)
 #pragma unroll
     for (int db = 0; db < DB; ++db) ak[db] = av[db] = zero16();
-  __syncthreads();  // (the tiles are no longer read)
+  // where row r of dk or dv, or of a part's sums (dk's, then dv's d values), goes
   const auto to = [&](T* p) {
     return [&, p](int r) -> T* {
       return wave_key0 + r < a.keys ? p + ((b * a.keys + wave_key0 + r) * a.key_heads + kh) * (int64_t)a.d : nullptr;
     };
   };
-  store_rows<T, DB>(lds + 32 * wave * Tl::RB, ak, a.scale, a.d, lane, to(dk));
-  wave_sync();
-  store_rows<T, DB>(lds + 32 * wave * Tl::RB, av, O::GRAD_UNIT, a.d, lane, to(dv));
+  const auto part = [&](int r) -> float* {
+    return wave_key0 + r < a.keys ? parts + ((split * a.pairs + pair) * a.keys + wave_key0 + r) * 2 * a.d : nullptr;
+  };
+  __syncthreads();  // (the tiles are no longer read)
+  if constexpr (WM == 1) {
+    float* const sums = (float*)s_lds;
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      put_sums<DB>(sums, side ? av : ak, wave, lane);
+      __syncthreads();
+      for (int r = wave; r < 32; r += WK)
+        if (wave_key0 + r < a.keys)
+          for (int e = lane; e < a.d; e += 64) {
+            const float x = joined<WK, DB>(sums, r, e);
+            if (parts)
+              part(r)[side * a.d + e] = x;
+            else
+              put((side ? to(dv) : to(dk))(r) + e, x * (side ? O::GRAD_UNIT : a.scale));
+          }
+      __syncthreads();
+    }
+  } else if (parts) {
+    float* const p = part(lane & 31);
+    if (p) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int x = 32 * db + 8 * (e >> 2) + 4 * half + (e & 3);
+          if (x < a.d) {
+            p[x] = ak[db][e];
+            p[a.d + x] = av[db][e];
+          }
+        }
+    }
+  } else {
+    store_rows<T, DB>(lds + 32 * wave * Tl::RB, ak, a.scale, a.d, lane, to(dk));
+    wave_sync();
+    store_rows<T, DB>(lds + 32 * wave * Tl::RB, av, O::GRAD_UNIT, a.d, lane, to(dv));
+  }
+}
+
+// dk and dv from the parts' sums: a wave a key.
+template <class T>
+__global__ __launch_bounds__(256) void k_attn_dkv_join(Problem a, int64_t all_keys, int splits, const float* parts, T* dk,
+                                                       T* dv) {
+  const int64_t at = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (at >= all_keys) return;
+  const int lane = threadIdx.x & 63;
+  const int64_t pair = at / a.keys, b = pair / a.key_heads;
+  const int key = (int)(at - pair * a.keys), kh = (int)(pair - b * a.key_heads);
+  const int64_t to = ((b * a.keys + key) * a.key_heads + kh) * (int64_t)a.d;
+  for (int e = lane; e < 2 * a.d; e += 64) {
+    float v = 0.f;
+    for (int s = 0; s < splits; ++s) v += parts[(s * all_keys + at) * 2 * a.d + e];
+    if (e < a.d)
+      put(dk + to + e, v * a.scale);
+    else
+      put(dv + to + e - a.d, v * Ops<T>::GRAD_UNIT);
+  }
 }
 
 }  // namespace attn

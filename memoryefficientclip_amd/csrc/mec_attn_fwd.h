@@ -41,7 +41,7 @@ struct Forward {
 };
 
 template <class T, int KS, int WM, int WK>
-__global__ __launch_bounds__(64 * WM * WK, sizeof(T) == 4 || (WM == 1 && KS == 8) ? 1 : 2) void k_attn_forward(Problem a, int64_t items, int64_t ids, int row_tiles,
+__global__ __launch_bounds__(64 * WM * WK, sizeof(T) == 4 || (WM == 1 && KS == 8) ? 1 : 2) void k_attn_forward(Problem a, Items items, int row_tiles,
                                                                int splits, T* out, float* lse, Parts parts) {
   using F = Forward<T, KS, WM, WK>;
   using O = Ops<T>;
@@ -50,14 +50,13 @@ __global__ __launch_bounds__(64 * WM * WK, sizeof(T) == 4 || (WM == 1 && KS == 8
   constexpr int DB = F::DB, NB = F::NB, KEYS = F::KEYS;
   __shared__ alignas(16) char s_lds[F::LDS];
   Lds* const lds = (Lds*)s_lds;
-  const int64_t id = group_id(ids);
-  if (id >= items) return;
+  int64_t pair;
+  int in;
+  if (!items.take(a.pairs, row_tiles * splits, pair, in)) return;
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // pair-major, the last rows (the longest where causal) first
-  const int per = row_tiles * splits;
-  const int64_t pair = id / per;
-  const int in = (int)(id - pair * per), split = in % splits, tile = row_tiles - 1 - in / splits;
+  // (the last rows, where causal those that see most, first)
+  const int split = in % splits, tile = row_tiles - 1 - in / splits;
   const int64_t b = pair / a.key_heads;
   const int kh = (int)(pair - b * a.key_heads);
   const int nq = a.nq(b), nk = a.nk(b), shift = nk - nq;

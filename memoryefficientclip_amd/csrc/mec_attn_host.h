@@ -53,35 +53,37 @@ inline int check_attention(const mec_attention_t* p, Problem* out) {
 
 inline View view(const mec_heads_t* h) { return View{h->data, h->batch_stride, h->token_stride, h->head_stride}; }
 
-// A launch of `items` workgroups: a multiple of 8 ids over x and y.
+// A launch of `count` workgroups.
 struct Grid {
-  int64_t items, ids;
+  Items items;
   dim3 dims;
 };
-inline int make_grid(int64_t items, Grid* g) {
-  g->items = items;
-  g->ids = (items + 7) & ~int64_t(7);
-  const int64_t x = g->ids < (1 << 20) ? g->ids : (1 << 20), y = ceil_div(g->ids, x);
-  if (y > 65535) return fail(MEC_ERR_UNSUPPORTED, "%lld workgroups are too many", (long long)items);
+inline int make_grid(int64_t count, Grid* g) {
+  const int64_t ids = (count + 7) & ~int64_t(7), x = ids < (1 << 20) ? ids : (1 << 20), y = ceil_div(ids, x);
+  if (y > 65535) return fail(MEC_ERR_UNSUPPORTED, "%lld workgroups are too many", (long long)count);
+  g->items = {count, ids};
   g->dims = dim3((unsigned)x, (unsigned)y);
   return MEC_OK;
 }
 
-// f(T*, integral_constant<KS>): KS steps of 16 features
+// f(integral_constant<KS>): KS steps of 16 features
+template <class F>
+void with_steps(int d, F f) {
+  if (d <= 32)
+    f(std::integral_constant<int, 2>{});
+  else if (d <= 64)
+    f(std::integral_constant<int, 4>{});
+  else if (d <= 80)
+    f(std::integral_constant<int, 5>{});
+  else if (d <= 96)
+    f(std::integral_constant<int, 6>{});
+  else
+    f(std::integral_constant<int, 8>{});
+}
+// f(T*, integral_constant<KS>)
 template <class F>
 void with_kernel(int dtype, int d, F f) {
-  with_element_type(dtype, [&](auto* t) {
-    if (d <= 32)
-      f(t, std::integral_constant<int, 2>{});
-    else if (d <= 64)
-      f(t, std::integral_constant<int, 4>{});
-    else if (d <= 80)
-      f(t, std::integral_constant<int, 5>{});
-    else if (d <= 96)
-      f(t, std::integral_constant<int, 6>{});
-    else
-      f(t, std::integral_constant<int, 8>{});
-  });
+  with_element_type(dtype, [&](auto* t) { with_steps(d, [&](auto ks) { f(t, ks); }); });
 }
 
 }  // namespace attn

@@ -57,14 +57,15 @@ __device__ __forceinline__ void loads_and_writes_done() {
 // k_attn_forward; LDS holds K and V.
 template <class T, int KS>
 __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T)), sizeof(T) == 4 || KS > 6 ? 2 : KS > 4 ? 3 : 5) void
-k_attn_whole_forward(Problem a, int64_t items, int64_t ids, T* out, float* lse) {
+k_attn_whole_forward(Problem a, Items items, T* out, float* lse) {
   using O = Ops<T>;
   using Frag = typename O::Frag;
   constexpr int DB = (KS + 1) / 2;
   using Tl = Tile<T, DB>;
   constexpr int BLOCK = 32 * Tl::RB;
-  const int64_t id = group_id(ids);
-  if (id >= items) return;
+  int64_t id;
+  int tile;
+  if (!items.take(a.pairs, 1, id, tile)) return;
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int64_t b = id / a.key_heads;
@@ -136,8 +137,8 @@ k_attn_whole_forward(Problem a, int64_t items, int64_t ids, T* out, float* lse) 
 // delta made whole (see there), then S, dP, dV^T and dK^T of the keys as in k_attn_dkv.
 // LDS: K, V, Q, dO, and lse and delta of the queries.
 template <class T, int KS>
-__global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_grad(Problem a, int64_t items, int64_t ids,
-                                                                                     const T* out, const float* lse,
+__global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_grad(Problem a, Items items, const T* out,
+                                                                                     const float* lse,
                                                                                      T* dq, T* dk, T* dv) {
   using O = Ops<T>;
   using Frag = typename O::Frag;
@@ -147,8 +148,9 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
   constexpr bool HELD = !O::F32 && DB <= 2;
   // see Backward: d + eps is delta
   constexpr bool MEAN = !O::F32 && DB <= 2, TWICE = !O::F32 && DB > 2;
-  const int64_t id = group_id(ids);
-  if (id >= items) return;
+  int64_t id;
+  int tile;
+  if (!items.take(a.pairs, 1, id, tile)) return;
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int64_t b = id / a.key_heads;
