@@ -36,17 +36,18 @@ int whole_forward(const Problem& a, int dtype, int64_t rows, size_t* lds) {
 int plan_forward(const Problem& a, int dtype, Plan* out) {
   const int64_t rows = (int64_t)a.queries * a.group;
   Plan p{};
-  p.few = rows <= 32;
+  int cus = 0;
+  if (int rc = compute_units(&cus)) return rc;
+  // (128 rows a workgroup would leave the device empty: the waves share 32)
+  p.few = rows <= 32 || a.pairs * ceil_div(rows, 128) < cus;
   p.row_tiles = (int)ceil_div(rows, p.few ? 32 : 128);
   p.splits = 1;
   p.whole = whole_forward(a, dtype, rows, &p.lds);
   if (p.whole) {
     p.row_tiles = 1;
   } else if (p.few) {
-    int cus = 0;
-    if (int rc = compute_units(&cus)) return rc;
-    // two workgroups a CU, and two tiles of 32 keys a wave
-    const int64_t want = ceil_div(2 * cus, a.pairs * p.row_tiles), most = ceil_div(a.keys, 32 * kWave * 2);
+    // two workgroups a CU, and four tiles of 32 keys a wave
+    const int64_t want = ceil_div(2 * cus, a.pairs * p.row_tiles), most = ceil_div(a.keys, 32 * kWave * 4);
     const int64_t s = want < most ? want : most;
     p.splits = (int)(s < 1 ? 1 : s);
   }

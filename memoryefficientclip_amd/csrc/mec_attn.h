@@ -167,6 +167,45 @@ struct Tile {
     else
       return (r >> 2) & 3;
   }
+  // A lane's part of the addresses below.  Of 16-bit rows all of them are two numbers, xor and plus constants (a row's
+  // beginning is a multiple of the xored bits): held as such they take 2 registers, where the compiler keeps up to 16
+  // (see `again`).
+  static constexpr bool XOR = !O::F32;
+  static constexpr int STEPS = VPR % 16 == 0 ? 7 : VPR % 16 == 8 ? 3 : 1;  // the bits of a step that are xored
+  struct At {
+    int lane, row, col;
+    __device__ __forceinline__ explicit At(int l) : lane(l), row(0), col(0) {
+      if constexpr (XOR) {
+        const int r = l & 31, half = l >> 5, j = l & 15;
+        row = r * RB + ((half ^ swz(r)) << 4);
+        const int w = 2 * ((l >> 4) & 1) + ((j & 3) >> 1), high = swz(j >> 2) & ~3;
+        col = (4 * half + (j >> 2)) * RB + ((high | (w ^ half)) << 4) + 8 * (j & 1);
+      }
+    }
+    // from here on the addresses are made anew, not kept from before
+    __device__ __forceinline__ void again() {
+      if constexpr (XOR) asm volatile("" : "+v"(row), "+v"(col));
+    }
+  };
+  static __device__ __forceinline__ Frag row(Lds* tile, int row0, int s, const At& at) {
+    if constexpr (XOR)
+      return *(__attribute__((address_space(3))) i16x8*)(tile + row0 * RB + (at.row ^ ((s & STEPS) << 5)) +
+                                                         ((s & ~STEPS) << 5));
+    else
+      return row(tile, row0, s, at.lane);
+  }
+  static __device__ __forceinline__ Frag col(Lds* tile, int row0, int db, const At& at) {
+    if constexpr (XOR) {
+      typedef __attribute__((address_space(3))) i16x4 Quad;
+      // (whole rows of 8 or 16 vectors: the block of 4 vectors is xored, too)
+      const int x = STEPS > 1 ? at.col ^ (db << 6) : at.col, plus = STEPS > 1 ? 0 : db << 6;
+      const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Quad*)(tile + row0 * RB + x + plus));
+      const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Quad*)(tile + (row0 + 8) * RB + (x ^ 32) + plus));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+      return col(tile, row0, db, at.lane);
+    }
+  }
   // k 16 s + 8 (lane / 32) .. + 7 of row row0 + lane % 32 (row0 a multiple of 32)
   static __device__ __forceinline__ Frag row(Lds* tile, int row0, int s, int lane) {
     const int r = lane & 31, half = lane >> 5, x = swz(r);
@@ -262,6 +301,88 @@ struct Loader {
     }
   }
 };
+
+// ROWS rows of a matrix on their way from memory into a tile, past the registers where
+// rows are whole 16-byte vectors on 16-byte boundaries.  The loads of a tile are in flight
+// while the one before is read: each of the two is an LDS array of its own, which tells the
+// compiler that reads of the one need not wait for the other.
+template <class T, int DB, int ROWS, int WAVES>
+struct Fetcher {
+  using Tl = Tile<T, DB>;
+  static constexpr int VPR = Tl::VPR, BLOCKS = ROWS * VPR / 64, NB = (BLOCKS + WAVES - 1) / WAVES;
+  const char* base;
+  int64_t pitch;  // bytes between rows
+  int d, lane, wave;
+  bool whole;
+  uint32_t off[NB];
+
+  __device__ __forceinline__ void init(const View& v, int64_t b, int h, int d_, int wave_, int lane_) {
+    base = (const char*)((const T*)v.p + b * v.batch + (int64_t)h * v.head);
+    pitch = v.token * (int64_t)sizeof(T);
+    d = d_;
+    lane = lane_;
+    wave = wave_;
+    whole = d % Tl::EPV == 0 && ((uintptr_t)base & 15) == 0 && (pitch & 15) == 0 && pitch < (int64_t)1 << 24;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      // (lane l of the block fills its place l)
+      const int at = (i * WAVES + wave) * 64 + lane, row = at / VPR, vec = (at % VPR) ^ Tl::swz(row);
+      off[i] = vec * Tl::EPV < d ? (uint32_t)(row * (int)pitch + vec * 16) : OOB;
+    }
+  }
+  // another head of the same matrix
+  __device__ __forceinline__ void move(const View& v, int64_t b, int h) {
+    base = (const char*)((const T*)v.p + b * v.batch + (int64_t)h * v.head);
+  }
+  // rows row0 .. row0 + ROWS - 1, those from `valid` rows on as zeros
+  __device__ __forceinline__ void load(Lds* tile, int row0, int valid) const {
+    const char* p = base + row0 * pitch;
+    if (whole) {
+      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int block = i * WAVES + wave;
+        if (BLOCKS % WAVES == 0 || block < BLOCKS) {
+          const uint32_t o = valid >= ROWS || (block * 64 + lane) / VPR < valid ? off[i] : OOB;
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(tile + block * 1024), 16,
+                                                   o, 0, 0, 0);
+        }
+      }
+    } else {
+      for (int block = wave; block < BLOCKS; block += WAVES) {
+        const int at = block * 64 + lane, row = at / VPR, vec = (at % VPR) ^ Tl::swz(row);
+        *(__attribute__((address_space(3))) u32x4*)(tile + at * 16) =
+            load_raw((const T*)(p + row * pitch) + vec * Tl::EPV, row < valid ? d - vec * Tl::EPV : 0);
+      }
+    }
+  }
+};
+// Loads into LDS, and the waves' reads and writes of it, are done for all waves.
+__device__ __forceinline__ void loads_done() {
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): loads that pass no registers too
+  __syncthreads();
+}
+// load(i, 0 or 1) and use(i, 0 or 1) of the tiles first .. last - 1 in two places in turn, the next on its
+// way while one is used.  Ends with all uses done.
+template <class Load, class Use>
+__device__ __forceinline__ void walk_tiles(int first, int last, Load load, Use use) {
+  std::integral_constant<int, 0> a;
+  std::integral_constant<int, 1> b;
+  if (first >= last) return;
+  load(first, a);
+  loads_done();
+#pragma unroll 1
+  for (int i = first;;) {
+    if (i + 1 < last) load(i + 1, b);
+    use(i, a);
+    loads_done();
+    if (++i >= last) break;
+    if (i + 1 < last) load(i + 1, a);
+    use(i, b);
+    loads_done();
+    if (++i >= last) break;
+  }
+}
 
 // The other half of the wave's value.
 __device__ __forceinline__ float other_half(float v) {
@@ -373,6 +494,12 @@ __device__ __forceinline__ void store_rows(Lds* mine, const f32x16 (&acc)[DB], f
   rows.pack(acc, f);
   rows.put(mine, lane);
   Rows<T, DB>::flush(mine, d, lane, row);
+}
+
+// 32 rows of LDS for wave 0 .. 3 in the two places of tiles: each holds the rows of two waves, or of all.
+template <int STEP, int RB>
+__device__ __forceinline__ Lds* wave_rows(char* a, char* b, int wave) {
+  return STEP == 64 || wave < 2 ? (Lds*)a + 32 * wave * RB : (Lds*)b + 32 * (wave - 2) * RB;
 }
 
 __device__ __forceinline__ f32x16 zero16() {

@@ -32,12 +32,12 @@ struct Backward {
   using Tl = Tile<T, DB>;
   // rows of the tiles that are walked over
   static constexpr int STEP = WM == 1 || O::F32 || DB > 3 ? 32 : 64;
-  static constexpr int TILE = STEP * Tl::RB, BUFS = WM == 1 ? 1 : 2;
-  static constexpr int TILES = 2 * TILE * BUFS * WK;  // of all waves
+  static constexpr int TILE = STEP * Tl::RB;
+  static constexpr int PLACE = 2 * TILE * WK;  // of a tile of each wave that has its own; WM = 4: there are two
   // (what leaves passes through the same LDS)
-  static_assert(WM == 1 ? WK * 32 * 32 * DB * 4 <= TILES : 128 * Tl::RB <= TILES, "");
-  // the values of a wave's keys stay in LDS where keys, values and both gradients take
-  // more registers than two waves on a SIMD have
+  static_assert(WM == 4 || WK * 32 * 32 * DB * 4 <= PLACE, "");
+  // the values of a wave's keys, or the result's gradients of its rows, stay in LDS where
+  // all that a wave holds takes more registers than two waves on a SIMD have
   static constexpr bool V_LDS = !O::F32 && DB > 3;
   // The forward's result has the errors of 16 bits, and so has do . o; where few keys share a row's weight
   // this is the largest error of dq and dk (heads of 64, 77 tokens, causal, bf16: 0.0031 of their size, 0.0023
@@ -72,14 +72,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
   using Frag = typename O::Frag;
   using Tl = typename B::Tl;
   constexpr int DB = B::DB, STEP = B::STEP, NB = STEP / 32, WK = B::WK;
-  __shared__ alignas(16) char s_lds[B::TILES];
+  __shared__ alignas(16) char s_lds[B::PLACE], s_next[WM == 1 ? 16 : B::PLACE];
   __shared__ float s_eps[WM == 1 ? WK : 1][32];
-  Lds* const lds = (Lds*)s_lds;
+  constexpr bool G_LDS = B::V_LDS && WM > 1;
+  __shared__ alignas(16) char s_grads[G_LDS ? B::ROWS * Tl::RB : 16];
   int64_t pair;
   int tile;
   if (!items.take(a.pairs, row_tiles, pair, tile)) return;
   tile = row_tiles - 1 - tile;  // (where causal, the last rows see most keys)
   const int lane = threadIdx.x & 63, half = lane >> 5;
+  const typename Tl::At lane_at(lane);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t b = pair / a.key_heads;
   const int kh = (int)(pair - b * a.key_heads);
@@ -101,7 +103,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
   const int see = a.causal ? min(nk, qi + shift + 1) : nk;
 
   const int64_t at = (b * a.heads + qh) * (int64_t)a.queries + qi;  // of lse and delta
-  Frag q[KS], g[KS];
+  Frag q[KS], g[G_LDS ? 1 : KS];
+  Lds* const grads = (Lds*)s_grads + 32 * wave * Tl::RB;
   float dot = 0.f, l2 = kInf;
   {
     const T* pg = (const T*)a.g.p + b * a.g.batch + (int64_t)qi * a.g.token + (int64_t)qh * a.g.head;
@@ -109,8 +112,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
     const T* pq = (const T*)a.q.p + b * a.q.batch + (int64_t)qi * a.q.token + (int64_t)qh * a.q.head;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      g[s] = O::load_row(pg, live, s, half, a.d);
-      dot += O::dot(g[s], O::load_row(po, live, s, half, a.d));
+      const Frag x = O::load_row(pg, live, s, half, a.d);
+      dot += O::dot(x, O::load_row(po, live, s, half, a.d));
+      if constexpr (G_LDS)
+        Tl::put_row(grads, 0, s, lane, x);  // (read by this wave alone)
+      else
+        g[s] = x;
       q[s] = O::load_row(pq, live, s, half, a.d);
     }
     dot += other_half(dot);
@@ -121,68 +128,88 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
   for (int db = 0; db < DB; ++db) acc[db] = zero16();
   const int tiles = (end + STEP - 1) / STEP;
   if (tiles > 0) {
-    Loader<T, DB, STEP, 64 * WM> lk, lv;
-    const int t = WM == 1 ? lane : threadIdx.x;
-    lk.init(a.k, b, kh, a.d, t);
-    lv.init(a.v, b, kh, a.d, t);
-    Lds* const mine = lds + (WM == 1 ? wave * 2 * B::TILE : 0);
     const int first = WM == 1 ? wave : 0;
-    int turn = 0;  // (a tile's place in LDS)
-#pragma unroll 1
-    for (int walk = exact ? 0 : 1; walk < 2; ++walk) {
-      float eps = 0.f;
-      if (first < tiles) {
-        lk.load(first * STEP, nk - first * STEP);
-        lv.load(first * STEP, nk - first * STEP);
+    float eps = 0.f;
+    int walk = exact ? 0 : 1;
+    const auto use = [&](Lds* tk, int i) {
+      auto at = lane_at;
+      at.again();
+      Lds* const tv = tk + B::TILE;
+      const int key0 = i * STEP;
+      if (key0 >= wave_end) return;
+      const bool masked = key0 + STEP > all;
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb) {
+        f32x16 s = zero16(), p = zero16();
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          s = O::mma(Tl::row(tk, 32 * kb, ks, at), q[ks], s);
+          if constexpr (G_LDS)
+            p = O::mma(Tl::row(tv, 32 * kb, ks, at), Tl::row(grads, 0, ks, at), p);
+          else
+            p = O::mma(Tl::row(tv, 32 * kb, ks, at), g[ks], p);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) p[e] = fast_exp2(fmaf(s[e], a.c, -l2)) * (p[e] - dot);
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            p[e] = key0 + 32 * kb + 8 * (e >> 2) + 4 * half + (e & 3) < see ? p[e] : 0.f;
+        }
+        if constexpr (!O::F32) {
+          // (one loop for both walks: the compiler's two copies of it take 50 registers more)
+          int w = walk;
+          asm volatile("" : "+v"(w));
+          if (__builtin_amdgcn_readfirstlane(w) == 0) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) eps += p[e];
+            continue;
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const Frag ds = O::pack(p, h);
+#pragma unroll
+          for (int db = 0; db < DB; ++db) acc[db] = O::mma(Tl::col(tk, 32 * kb + 16 * h, db, at), ds, acc[db]);
+        }
       }
-      for (int i = first; i < tiles; i += WK, ++turn) {
-        Lds* const tk = mine + (B::BUFS == 2 && (turn & 1) ? 2 * B::TILE : 0);
-        Lds* const tv = tk + B::TILE;
-        lk.store(tk);
-        lv.store(tv);
-        if constexpr (WM == 1)
+    };
+    Loader<T, DB, STEP, 64> lk, lv;
+    Fetcher<T, DB, STEP, WM> fk, fv;
+    if constexpr (WM == 1) {
+      lk.init(a.k, b, kh, a.d, lane);
+      lv.init(a.v, b, kh, a.d, lane);
+    } else {
+      fk.init(a.k, b, kh, a.d, wave, lane);
+      fv.init(a.v, b, kh, a.d, wave, lane);
+    }
+#pragma unroll 1
+    for (; walk < 2; ++walk) {
+      if constexpr (WM == 1) {
+        Lds* const tk = (Lds*)s_lds + wave * 2 * B::TILE;
+        if (first < tiles) {
+          lk.load(first * STEP, nk - first * STEP);
+          lv.load(first * STEP, nk - first * STEP);
+        }
+        for (int i = first; i < tiles; i += WK) {
+          lk.store(tk);
+          lv.store(tk + B::TILE);
           wave_sync();
-        else
-          __syncthreads();
-        if (i + WK < tiles) {
-          lk.load((i + WK) * STEP, nk - (i + WK) * STEP);
-          lv.load((i + WK) * STEP, nk - (i + WK) * STEP);
+          if (i + WK < tiles) {
+            lk.load((i + WK) * STEP, nk - (i + WK) * STEP);
+            lv.load((i + WK) * STEP, nk - (i + WK) * STEP);
+          }
+          use(tk, i);
         }
-        const int key0 = i * STEP;
-        if (key0 >= wave_end) continue;
-        const bool masked = key0 + STEP > all;
-#pragma unroll
-        for (int kb = 0; kb < NB; ++kb) {
-          f32x16 s = zero16(), p = zero16();
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            s = O::mma(Tl::row(tk, 32 * kb, ks, lane), q[ks], s);
-            p = O::mma(Tl::row(tv, 32 * kb, ks, lane), g[ks], p);
-          }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) p[e] = fast_exp2(fmaf(s[e], a.c, -l2)) * (p[e] - dot);
-          if (masked) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              p[e] = key0 + 32 * kb + 8 * (e >> 2) + 4 * half + (e & 3) < see ? p[e] : 0.f;
-          }
-          if constexpr (!O::F32) {
-            // (one loop for both walks: the compiler's two copies of it take 50 registers more)
-            int w = walk;
-            asm volatile("" : "+v"(w));
-            if (__builtin_amdgcn_readfirstlane(w) == 0) {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) eps += p[e];
-              continue;
-            }
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const Frag ds = O::pack(p, h);
-#pragma unroll
-            for (int db = 0; db < DB; ++db) acc[db] = O::mma(Tl::col(tk, 32 * kb + 16 * h, db, lane), ds, acc[db]);
-          }
-        }
+      } else {
+        walk_tiles(
+            first, tiles,
+            [&](int i, auto place) {
+              Lds* const tk = (Lds*)(place ? s_next : s_lds);
+              fk.load(tk, i * STEP, nk - i * STEP);
+              fv.load(tk + B::TILE, i * STEP, nk - i * STEP);
+            },
+            [&](int i, auto place) { use((Lds*)(place ? s_next : s_lds), i); });
       }
       if (walk == 0) {
         eps += other_half(eps);
@@ -194,6 +221,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
           for (int i = 0; i < WK; ++i) eps += s_eps[i][lane & 31];
         }
         dot += eps;
+        eps = 0.f;
       }
     }
   }
@@ -206,15 +234,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
     const int x = wave_row0 + r;
     return x < rows ? dq + ((b * a.queries + x / a.group) * a.heads + kh * a.group + x % a.group) * (int64_t)a.d : nullptr;
   };
-  __syncthreads();  // (the tiles are no longer read)
   if constexpr (WM == 1) {
+    __syncthreads();  // (the tiles are no longer read)
     put_sums<DB>((float*)s_lds, acc, wave, lane);
     __syncthreads();
     for (int r = wave; r < 32; r += WK)
       if (T* p = to(r))
         for (int e = lane; e < a.d; e += 64) put(p + e, a.scale * joined<WK, DB>((float*)s_lds, r, e));
   } else {
-    store_rows<T, DB>(lds + 32 * wave * Tl::RB, acc, a.scale, a.d, lane, to);
+    store_rows<T, DB>(wave_rows<STEP, Tl::RB>(s_lds, s_next, wave), acc, a.scale, a.d, lane, to);
   }
 }
 
@@ -226,15 +254,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
   using Frag = typename O::Frag;
   using Tl = typename B::Tl;
   constexpr int DB = B::DB, STEP = B::STEP, NB = STEP / 32, WK = B::WK;
-  __shared__ alignas(16) char s_lds[B::TILES + (B::V_LDS ? B::ROWS * Tl::RB : 0)];
-  __shared__ alignas(16) float s_row[WK][B::BUFS][2][STEP];  // lse, delta of the tile's queries
-  Lds* const lds = (Lds*)s_lds;
+  __shared__ alignas(16) char s_lds[B::PLACE], s_next[WM == 1 ? 16 : B::PLACE];
+  __shared__ alignas(16) char s_values[B::V_LDS ? B::ROWS * Tl::RB : 16];
+  // lse and delta of the tile's queries
+  __shared__ alignas(16) float s_row[WK][2][64], s_next_row[2][64];
   int64_t pair;
   int tile;  // (where causal, the first keys are seen by most queries)
   if (!items.take(a.pairs, key_tiles * splits, pair, tile)) return;
   const int split = tile % splits;
   tile /= splits;
   const int lane = threadIdx.x & 63, half = lane >> 5;
+  const typename Tl::At lane_at(lane);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t b = pair / a.key_heads;
   const int kh = (int)(pair - b * a.key_heads);
@@ -258,7 +288,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
   const int stop = min(tiles, (split + 1) * share);
   if (split * share < stop) {
     Frag k[KS], v[B::V_LDS ? 1 : KS];
-    Lds* const values = lds + B::TILES + (WM == 1 ? 0 : 32 * wave * Tl::RB);
+    Lds* const values = (Lds*)s_values + (WM == 1 ? 0 : 32 * wave * Tl::RB);
     {
       const T* pk = (const T*)a.k.p + b * a.k.batch + (int64_t)key * a.k.token + (int64_t)kh * a.k.head;
       const T* pv = (const T*)a.v.p + b * a.v.batch + (int64_t)key * a.v.token + (int64_t)kh * a.v.head;
@@ -274,65 +304,32 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
         }
       }
     }
-    Loader<T, DB, STEP, 64 * WM> lq, lg;
-    float r_row[2] = {0.f, 0.f};  // a query's lse and delta on their way (WM = 4: one of them)
-    const int t = WM == 1 ? lane : threadIdx.x;
-    int loaded = -1;  // head
-    auto load = [&](int at) {
-      const int h = kh * a.group + at / each, q0 = (first + at % each) * STEP;
-      if (h != loaded) {
-        lq.init(a.q, b, h, a.d, t);
-        lg.init(a.g, b, h, a.d, t);
-        loaded = h;
-      }
-      lq.load(q0, nq - q0);
-      lg.load(q0, nq - q0);
-      const int64_t head0 = (b * a.heads + h) * (int64_t)a.queries;
-      const int i = q0 + t % STEP;
-      if (t < 2 * STEP) {
-        const float x = i < nq ? (t < STEP ? lse : delta)[head0 + i] : t < STEP ? kInf : 0.f;
-        r_row[0] = t < STEP ? x - O::GRAD_BIAS : x * O::GRAD_UNIT;
-      }
-    };
-    Lds* const mine = lds + (WM == 1 ? wave * 2 * B::TILE : 0);
-    const int begin_at = split * share + (WM == 1 ? wave : 0);
-    if (begin_at < stop) load(begin_at);
-    int turn = 0;
-    for (int i = begin_at; i < stop; i += WK, ++turn) {
-      const int buf = B::BUFS == 2 ? turn & 1 : 0;
-      Lds* const tq = mine + buf * 2 * B::TILE;
+    const auto use = [&](Lds* tq, const float* row, int i) {
+      auto at = lane_at;
+      at.again();
       Lds* const tg = tq + B::TILE;
-      auto& row = s_row[WM == 1 ? wave : 0][buf];
-      lq.store(tq);
-      lg.store(tg);
-      if (t < 2 * STEP) row[t / STEP][t % STEP] = r_row[0];
-      if constexpr (WM == 1)
-        wave_sync();
-      else
-        __syncthreads();
-      if (i + WK < stop) load(i + WK);
       const int q0 = (first + i % each) * STEP;
-      if (q0 + STEP <= wave_begin) continue;
+      if (q0 + STEP <= wave_begin) return;
       const bool masked = q0 < all;
 #pragma unroll
       for (int qb = 0; qb < NB; ++qb) {
         f32x16 s = zero16(), p = zero16();
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          s = O::mma(Tl::row(tq, 32 * qb, ks, lane), k[ks], s);
+          s = O::mma(Tl::row(tq, 32 * qb, ks, at), k[ks], s);
           if constexpr (B::V_LDS)
-            p = O::mma(Tl::row(tg, 32 * qb, ks, lane), Tl::row(values, 0, ks, lane), p);
+            p = O::mma(Tl::row(tg, 32 * qb, ks, at), Tl::row(values, 0, ks, at), p);
           else
-            p = O::mma(Tl::row(tg, 32 * qb, ks, lane), v[ks], p);
+            p = O::mma(Tl::row(tg, 32 * qb, ks, at), v[ks], p);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const f32x4 l2 = *(const f32x4*)&row[0][32 * qb + 8 * e + 4 * half];
-          const f32x4 dl = *(const f32x4*)&row[1][32 * qb + 8 * e + 4 * half];
+          const f32x4 l2 = *(const f32x4*)(row + 32 * qb + 8 * e + 4 * half);
+          const f32x4 dl = *(const f32x4*)(row + 64 + 32 * qb + 8 * e + 4 * half);
 #pragma unroll
           for (int f = 0; f < 4; ++f) {
-            s[4 * e + f] = fast_exp2(fmaf(s[4 * e + f], a.c, -l2[f]));
-            p[4 * e + f] = s[4 * e + f] * fmaf(p[4 * e + f], O::GRAD_UNIT, -dl[f]);
+            s[4 * e + f] = fast_exp2(fmaf(s[4 * e + f], a.c, O::GRAD_BIAS - l2[f]));
+            p[4 * e + f] = s[4 * e + f] * (O::GRAD_UNIT * (p[4 * e + f] - dl[f]));
           }
         }
         if (masked) {
@@ -348,11 +345,61 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
           const Frag fp = O::pack(s, h), fs = O::pack(p, h);
 #pragma unroll
           for (int db = 0; db < DB; ++db) {
-            av[db] = O::mma(Tl::col(tg, 32 * qb + 16 * h, db, lane), fp, av[db]);
-            ak[db] = O::mma(Tl::col(tq, 32 * qb + 16 * h, db, lane), fs, ak[db]);
+            av[db] = O::mma(Tl::col(tg, 32 * qb + 16 * h, db, at), fp, av[db]);
+            ak[db] = O::mma(Tl::col(tq, 32 * qb + 16 * h, db, at), fs, ak[db]);
           }
         }
       }
+    };
+    const int begin_at = split * share;
+    if constexpr (WM == 1) {
+      Loader<T, DB, STEP, 64> lq, lg;
+      float r_row = 0.f;  // a query's lse or delta on its way
+      const auto load = [&](int at) {
+        const int h = kh * a.group + at / each, q0 = (first + at % each) * STEP;
+        lq.init(a.q, b, h, a.d, lane);
+        lg.init(a.g, b, h, a.d, lane);
+        lq.load(q0, nq - q0);
+        lg.load(q0, nq - q0);
+        const int i = q0 + (lane & 31);
+        // (of rows that are none Q and dO are 0)
+        r_row = i < nq ? (half ? delta : lse)[(b * a.heads + h) * (int64_t)a.queries + i] : 0.f;
+      };
+      Lds* const tq = (Lds*)s_lds + wave * 2 * B::TILE;
+      if (begin_at + wave < stop) load(begin_at + wave);
+      for (int i = begin_at + wave; i < stop; i += WK) {
+        lq.store(tq);
+        lg.store(tq + B::TILE);
+        s_row[wave][half][lane & 31] = r_row;
+        wave_sync();
+        if (i + WK < stop) load(i + WK);
+        use(tq, s_row[wave][0], i);
+      }
+    } else {
+      Fetcher<T, DB, STEP, WM> fq, fg;
+      fq.init(a.q, b, kh * a.group, a.d, wave, lane);
+      fg.init(a.g, b, kh * a.group, a.d, wave, lane);
+      walk_tiles(
+          begin_at, stop,
+          [&](int at, auto place) {
+            const int h = kh * a.group + at / each, q0 = (first + at % each) * STEP;
+            fq.move(a.q, b, h);
+            fg.move(a.g, b, h);
+            Lds* const tq = (Lds*)(place ? s_next : s_lds);
+            fq.load(tq, q0, nq - q0);
+            fg.load(tq + B::TILE, q0, nq - q0);
+            if (wave < 2) {
+              // (lse by the first wave, delta by the second; of rows that are none 0, as their Q and dO)
+              const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
+                  (void*)((wave ? delta : lse) + (b * a.heads + h) * (int64_t)a.queries + q0), 0, 0x7fffffff, 0x00020000);
+              Lds* const to = (Lds*)(place ? &s_next_row[0][0] : &s_row[0][0][0]) + wave * 256;
+              __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)to, 4,
+                                                       lane < STEP && q0 + lane < nq ? 4 * lane : OOB, 0, 0, 0);
+            }
+          },
+          [&](int i, auto place) {
+            use((Lds*)(place ? s_next : s_lds), place ? &s_next_row[0][0] : &s_row[0][0][0], i);
+          });
     }
   }
   if (!live)
@@ -367,8 +414,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
   const auto part = [&](int r) -> float* {
     return wave_key0 + r < a.keys ? parts + ((split * a.pairs + pair) * a.keys + wave_key0 + r) * 2 * a.d : nullptr;
   };
-  __syncthreads();  // (the tiles are no longer read)
   if constexpr (WM == 1) {
+    __syncthreads();  // (the tiles are no longer read)
     float* const sums = (float*)s_lds;
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
@@ -400,9 +447,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
         }
     }
   } else {
-    store_rows<T, DB>(lds + 32 * wave * Tl::RB, ak, a.scale, a.d, lane, to(dk));
+    Lds* const mine = wave_rows<STEP, Tl::RB>(s_lds, s_next, wave);
+    store_rows<T, DB>(mine, ak, a.scale, a.d, lane, to(dk));
     wave_sync();
-    store_rows<T, DB>(lds + 32 * wave * Tl::RB, av, O::GRAD_UNIT, a.d, lane, to(dv));
+    store_rows<T, DB>(mine, av, O::GRAD_UNIT, a.d, lane, to(dv));
   }
 }
 

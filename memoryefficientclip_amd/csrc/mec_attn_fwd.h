@@ -34,9 +34,10 @@ struct Forward {
   using Tl = Tile<T, DB>;
   static constexpr int NT = 64 * WM * WK, ROWS = 32 * WM;
   static constexpr int KEYS = WM == 1 || O::F32 ? 32 : 64, NB = KEYS / 32;
-  static constexpr int TILE = KEYS * Tl::RB, BUFS = WM == 1 ? 1 : 2;
+  static constexpr int TILE = KEYS * Tl::RB;
   static constexpr int JOIN = WM == 1 ? WK * 32 * (32 * DB + 2) * 4 : 0;
-  static constexpr int LDS0 = 2 * TILE * BUFS * WK, LDS = LDS0 > JOIN ? LDS0 : JOIN;
+  // keys and values of a tile of each wave that has its own
+  static constexpr int LDS0 = 2 * TILE * WK, LDS = LDS0 > JOIN ? LDS0 : JOIN;
   static_assert(WM == 1 || WK == 1, "");
 };
 
@@ -48,12 +49,12 @@ __global__ __launch_bounds__(64 * WM * WK, sizeof(T) == 4 || (WM == 1 && KS == 8
   using Frag = typename O::Frag;
   using Tl = typename F::Tl;
   constexpr int DB = F::DB, NB = F::NB, KEYS = F::KEYS;
-  __shared__ alignas(16) char s_lds[F::LDS];
-  Lds* const lds = (Lds*)s_lds;
+  __shared__ alignas(16) char s_lds[F::LDS], s_next[WM == 1 ? 16 : F::LDS];
   int64_t pair;
   int in;
   if (!items.take(a.pairs, row_tiles * splits, pair, in)) return;
   const int lane = threadIdx.x & 63, half = lane >> 5;
+  const typename Tl::At lane_at(lane);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // (the last rows, where causal those that see most, first)
   const int split = in % splits, tile = row_tiles - 1 - in / splits;
@@ -96,34 +97,18 @@ __global__ __launch_bounds__(64 * WM * WK, sizeof(T) == 4 || (WM == 1 && KS == 8
 #pragma unroll
       for (int s = 0; s < KS; ++s) q[s] = O::load_row(p, live, s, half, a.d);
     }
-    Loader<T, DB, KEYS, 64 * WM> lk, lv;
-    const int t = WM == 1 ? lane : threadIdx.x;
-    lk.init(a.k, b, kh, a.d, t);
-    lv.init(a.v, b, kh, a.d, t);
-    lk.load(first * KEYS, nk - first * KEYS);
-    lv.load(first * KEYS, nk - first * KEYS);
-    Lds* const mine = lds + (WM == 1 ? wave * 2 * F::TILE : 0);
-    for (int i = first; i < tiles; i += WK) {
-      Lds* const tk = mine + (F::BUFS == 2 && (i & 1) ? 2 * F::TILE : 0);
+    const auto use = [&](Lds* tk, int i) {
+      auto at = lane_at;
+      at.again();
       Lds* const tv = tk + F::TILE;
-      lk.store(tk);
-      lv.store(tv);
-      if constexpr (WM == 1)
-        wave_sync();
-      else
-        __syncthreads();
-      if (i + WK < tiles) {
-        lk.load((i + WK) * KEYS, nk - (i + WK) * KEYS);
-        lv.load((i + WK) * KEYS, nk - (i + WK) * KEYS);
-      }
       const int key0 = i * KEYS;
-      if (key0 >= wave_end) continue;
+      if (key0 >= wave_end) return;
       f32x16 s[NB];
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb) {
         s[kb] = zero16();
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s[kb] = O::mma(Tl::row(tk, 32 * kb, ks, lane), q[ks], s[kb]);
+        for (int ks = 0; ks < KS; ++ks) s[kb] = O::mma(Tl::row(tk, 32 * kb, ks, at), q[ks], s[kb]);
       }
       if (key0 + KEYS > all) {
 #pragma unroll
@@ -147,8 +132,38 @@ __global__ __launch_bounds__(64 * WM * WK, sizeof(T) == 4 || (WM == 1 && KS == 8
         for (int h = 0; h < 2; ++h) {
           const Frag p = O::pack(s[kb], h);
 #pragma unroll
-          for (int db = 0; db < DB; ++db) o[db] = O::mma(Tl::col(tv, 32 * kb + 16 * h, db, lane), p, o[db]);
+          for (int db = 0; db < DB; ++db) o[db] = O::mma(Tl::col(tv, 32 * kb + 16 * h, db, at), p, o[db]);
         }
+    };
+    if constexpr (WM == 1) {
+      Loader<T, DB, KEYS, 64> lk, lv;
+      lk.init(a.k, b, kh, a.d, lane);
+      lv.init(a.v, b, kh, a.d, lane);
+      lk.load(first * KEYS, nk - first * KEYS);
+      lv.load(first * KEYS, nk - first * KEYS);
+      Lds* const tk = (Lds*)s_lds + wave * 2 * F::TILE;
+      for (int i = first; i < tiles; i += WK) {
+        lk.store(tk);
+        lv.store(tk + F::TILE);
+        wave_sync();
+        if (i + WK < tiles) {
+          lk.load((i + WK) * KEYS, nk - (i + WK) * KEYS);
+          lv.load((i + WK) * KEYS, nk - (i + WK) * KEYS);
+        }
+        use(tk, i);
+      }
+    } else {
+      Fetcher<T, DB, KEYS, WM> fk, fv;
+      fk.init(a.k, b, kh, a.d, wave, lane);
+      fv.init(a.v, b, kh, a.d, wave, lane);
+      walk_tiles(
+          first, tiles,
+          [&](int i, auto place) {
+            Lds* const tk = (Lds*)(place ? s_next : s_lds);
+            fk.load(tk, i * KEYS, nk - i * KEYS);
+            fv.load(tk + F::TILE, i * KEYS, nk - i * KEYS);
+          },
+          [&](int i, auto place) { use((Lds*)(place ? s_next : s_lds), i); });
     }
   }
   l += other_half(l);
@@ -206,8 +221,8 @@ __global__ __launch_bounds__(64 * WM * WK, sizeof(T) == 4 || (WM == 1 && KS == 8
     const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
     if (lse && half == 0 && row < rows)
       lse[(b * a.heads + qh) * (int64_t)a.queries + qi] = l == 0.f ? kInf : m - O::BIAS + log2f(l);
-    __syncthreads();  // (the tiles are no longer read)
-    store_rows<T, DB>(lds + 32 * wave * Tl::RB, o, inv, a.d, lane, [&](int r) -> T* {
+    Lds* const mine = wave_rows<KEYS, Tl::RB>(s_lds, s_next, wave);  // (the tiles are no longer read)
+    store_rows<T, DB>(mine, o, inv, a.d, lane, [&](int r) -> T* {
       const int at = wave_row0 + r;
       return at < rows ? out + ((b * a.queries + at / a.group) * a.heads + kh * a.group + at % a.group) * (int64_t)a.d
                        : nullptr;

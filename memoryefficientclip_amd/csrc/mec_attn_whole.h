@@ -47,12 +47,6 @@ __device__ __forceinline__ void fetch(Lds* tile, const View& v, int64_t b, int h
   }
 }
 
-// Loads into LDS and the waves' writes to it are there for all waves.
-__device__ __forceinline__ void loads_and_writes_done() {
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): loads that pass no registers too
-  __syncthreads();
-}
-
 // The forward: each wave has a block of 32 rows (r = query * group + head), as in
 // k_attn_forward; LDS holds K and V.
 template <class T, int KS>
@@ -67,6 +61,7 @@ k_attn_whole_forward(Problem a, Items items, T* out, float* lse) {
   int tile;
   if (!items.take(a.pairs, 1, id, tile)) return;
   const int lane = threadIdx.x & 63, half = lane >> 5;
+  typename Tl::At lane_at(lane);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int64_t b = id / a.key_heads;
   const int kh = (int)(id - b * a.key_heads);
@@ -87,16 +82,17 @@ k_attn_whole_forward(Problem a, Items items, T* out, float* lse) {
 #pragma unroll
     for (int s = 0; s < KS; ++s) q[s] = O::load_row(p, live, s, half, a.d);
   }
-  loads_and_writes_done();
+  loads_done();
   f32x16 o[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) o[db] = zero16();
   float m = -kInf, l = 0.f;
   Lds* at = tk;
   for (int key0 = 0; key0 < end; key0 += 32, at += 2 * BLOCK) {
+    lane_at.again();
     f32x16 s = zero16();
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) s = O::mma(Tl::row(at, 0, ks, lane), q[ks], s);
+    for (int ks = 0; ks < KS; ++ks) s = O::mma(Tl::row(at, 0, ks, lane_at), q[ks], s);
     if (key0 + 32 > all) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = key0 + 8 * (e >> 2) + 4 * half + (e & 3) < see ? s[e] : -kInf;
@@ -112,7 +108,7 @@ k_attn_whole_forward(Problem a, Items items, T* out, float* lse) {
     for (int x = 0; x < 2; ++x) {
       const Frag p = O::pack(s, x);
 #pragma unroll
-      for (int db = 0; db < DB; ++db) o[db] = O::mma(Tl::col(at + BLOCK, 16 * x, db, lane), p, o[db]);
+      for (int db = 0; db < DB; ++db) o[db] = O::mma(Tl::col(at + BLOCK, 16 * x, db, lane_at), p, o[db]);
     }
   }
   l += other_half(l);
@@ -152,6 +148,7 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
   int tile;
   if (!items.take(a.pairs, 1, id, tile)) return;
   const int lane = threadIdx.x & 63, half = lane >> 5;
+  typename Tl::At lane_at(lane);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int64_t b = id / a.key_heads;
   const int h = (int)(id - b * a.key_heads);
@@ -189,7 +186,7 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
     }
     if (half == 0 && first < nq) s_lse[qi] = l2 - O::GRAD_BIAS;
   }
-  loads_and_writes_done();
+  loads_done();
   Rows<T, DB> packed;  // dq
   {
     f32x16 acc[DB];
@@ -201,8 +198,8 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
       Frag q[KS], g[KS];
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        q[s] = Tl::row(my_q, 0, s, lane);
-        g[s] = Tl::row(my_q + BLOCK, 0, s, lane);
+        q[s] = Tl::row(my_q, 0, s, lane_at);
+        g[s] = Tl::row(my_q + BLOCK, 0, s, lane_at);
         if constexpr (MEAN) dot += O::dot(g[s], o[s]);
         if constexpr (O::F32)
           dot += O::dot(g[s], O::load_row(out + ((b * a.queries + qi) * a.heads + h) * (int64_t)a.d, live, s, half, a.d));
@@ -215,11 +212,12 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
       for (int walk = TWICE ? 0 : 1; walk < 2; ++walk) {
         Lds* at = tk;
         for (int key0 = 0; key0 < end; key0 += 32, at += 2 * BLOCK) {
+    lane_at.again();
           f32x16 s = zero16(), p = zero16();
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) {
-            s = O::mma(Tl::row(at, 0, ks, lane), q[ks], s);
-            p = O::mma(Tl::row(at + BLOCK, 0, ks, lane), g[ks], p);
+            s = O::mma(Tl::row(at, 0, ks, lane_at), q[ks], s);
+            p = O::mma(Tl::row(at + BLOCK, 0, ks, lane_at), g[ks], p);
           }
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
@@ -244,7 +242,7 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
             const Frag ds = O::pack(p, x), ps = O::pack(s, x);
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
-              const Frag kt = Tl::col(at, 16 * x, db, lane);
+              const Frag kt = Tl::col(at, 16 * x, db, lane_at);
               acc[db] = O::mma(kt, ds, acc[db]);
               if constexpr (MEAN) mean[db] = O::mma(kt, ps, mean[db]);
             }
@@ -279,8 +277,8 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
     if (first < nk) {
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        k[s] = Tl::row(my_k, 0, s, lane);
-        v[s] = Tl::row(my_k + BLOCK, 0, s, lane);
+        k[s] = Tl::row(my_k, 0, s, lane_at);
+        v[s] = Tl::row(my_k + BLOCK, 0, s, lane_at);
       }
     }
     if (dq) {
@@ -300,6 +298,7 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
     const int all = a.causal ? first + 31 - shift : 0, seen = a.causal ? key - shift : 0;
     Lds* at = tq + begin * 2 * Tl::RB;
     for (int q0 = begin; q0 < nq; q0 += 32, at += 2 * BLOCK) {
+      lane_at.again();
       f32x16 s = zero16(), p;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -309,8 +308,8 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
       }
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        s = O::mma(Tl::row(at, 0, ks, lane), HELD ? k[HELD ? ks : 0] : Tl::row(my_k, 0, ks, lane), s);
-        p = O::mma(Tl::row(at + BLOCK, 0, ks, lane), HELD ? v[HELD ? ks : 0] : Tl::row(my_k + BLOCK, 0, ks, lane), p);
+        s = O::mma(Tl::row(at, 0, ks, lane_at), HELD ? k[HELD ? ks : 0] : Tl::row(my_k, 0, ks, lane_at), s);
+        p = O::mma(Tl::row(at + BLOCK, 0, ks, lane_at), HELD ? v[HELD ? ks : 0] : Tl::row(my_k + BLOCK, 0, ks, lane_at), p);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -334,8 +333,8 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
         const Frag fp = O::pack(s, x), fs = O::pack(p, x);
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
-          av[db] = O::mma(Tl::col(at + BLOCK, 16 * x, db, lane), fp, av[db]);
-          ak[db] = O::mma(Tl::col(at, 16 * x, db, lane), fs, ak[db]);
+          av[db] = O::mma(Tl::col(at + BLOCK, 16 * x, db, lane_at), fp, av[db]);
+          ak[db] = O::mma(Tl::col(at, 16 * x, db, lane_at), fs, ak[db]);
         }
       }
     }
