@@ -19,7 +19,7 @@
 #pragma once
 #include <climits>
 
-#include "mec_attn.h"
+#include "mec_attn_strict.h"
 
 namespace mec {
 namespace attn {
@@ -225,6 +225,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
       }
     }
   }
+  if (a.causal && any_nan<O>(acc)) {
+    float again[16 * DB];
+    strict_dq<T, KS>((const T*)a.q.p + b * a.q.batch + (int64_t)qi * a.q.token + (int64_t)qh * a.q.head,
+                     (const T*)a.g.p + b * a.g.batch + (int64_t)qi * a.g.token + (int64_t)qh * a.g.head, live,
+                     (const T*)a.k.p + b * a.k.batch + (int64_t)kh * a.k.head, a.k.token,
+                     (const T*)a.v.p + b * a.v.batch + (int64_t)kh * a.v.head, a.v.token, a.d,
+                     Range{WM == 1 ? wave : 0, tiles, WK, STEP}, wave_end, see, a.c, l2, dot, again);
+    take<DB>(acc, again);
+  }
   if (half == 0 && row < rows && (WM > 1 || wave == 0)) delta[at] = dot;
   if (dq == nullptr) return;
   if (!live || l2 == kInf)
@@ -401,6 +410,19 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
             use((Lds*)(place ? s_next : s_lds), place ? &s_next_row[0][0] : &s_row[0][0][0], i);
           });
     }
+  }
+  if (a.causal && (any_nan<O>(ak) || any_nan<O>(av))) {
+    float again[32 * DB];
+    const int h = kh * a.group;
+    const int64_t head0 = (b * a.heads + h) * (int64_t)a.queries;
+    const Queries<T> s{(const T*)a.q.p + b * a.q.batch + (int64_t)h * a.q.head,
+                       (const T*)a.g.p + b * a.g.batch + (int64_t)h * a.g.head,
+                       a.q.token, a.q.head, a.g.token, a.g.head, lse + head0, delta + head0, a.queries, nq, each, first};
+    strict_dkv<T, KS>((const T*)a.k.p + b * a.k.batch + (int64_t)key * a.k.token + (int64_t)kh * a.k.head,
+                      (const T*)a.v.p + b * a.v.batch + (int64_t)key * a.v.token + (int64_t)kh * a.v.head, live, s, a.d,
+                      Range{split * share + (WM == 1 ? wave : 0), stop, WK, STEP}, seen, a.c, again);
+    take<DB>(ak, again);
+    take<DB>(av, again + 16 * DB);
   }
   if (!live)
 #pragma unroll

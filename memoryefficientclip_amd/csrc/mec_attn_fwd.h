@@ -15,7 +15,7 @@
 // without a barrier, and meet at the end; the keys are split over `splits`
 // workgroups, which k_attn_join joins.
 #pragma once
-#include "mec_attn.h"
+#include "mec_attn_strict.h"
 
 namespace mec {
 namespace attn {
@@ -165,6 +165,16 @@ __global__ __launch_bounds__(64 * WM * WK, sizeof(T) == 4 || (WM == 1 && KS == 8
           },
           [&](int i, auto place) { use((Lds*)(place ? s_next : s_lds), i); });
     }
+  }
+  if (a.causal && any_nan<O>(o)) {
+    float again[16 * DB + 2];
+    strict_forward<T, KS>((const T*)a.q.p + b * a.q.batch + (int64_t)qi * a.q.token + (int64_t)qh * a.q.head, live,
+                          (const T*)a.k.p + b * a.k.batch + (int64_t)kh * a.k.head, a.k.token,
+                          (const T*)a.v.p + b * a.v.batch + (int64_t)kh * a.v.head, a.v.token, a.d,
+                          Range{first, tiles, WK, KEYS}, wave_end, see, a.c, again);
+    take<DB>(o, again);
+    m = again[16 * DB];
+    l = again[16 * DB + 1];
   }
   l += other_half(l);
   if (!live || l == 0.f) {

@@ -6,7 +6,9 @@
 // which here is spent once: everything is on its way to LDS before the first
 // product, by loads that pass no registers.
 #pragma once
-#include "mec_attn.h"
+#include <climits>
+
+#include "mec_attn_strict.h"
 
 namespace mec {
 namespace attn {
@@ -110,6 +112,16 @@ k_attn_whole_forward(Problem a, Items items, T* out, float* lse) {
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] = O::mma(Tl::col(at + BLOCK, 16 * x, db, lane_at), p, o[db]);
     }
+  }
+  if (a.causal && any_nan<O>(o)) {
+    float again[16 * DB + 2];
+    strict_forward<T, KS>((const T*)a.q.p + b * a.q.batch + (int64_t)qi * a.q.token + (int64_t)qh * a.q.head, live,
+                          (const T*)a.k.p + b * a.k.batch + (int64_t)kh * a.k.head, a.k.token,
+                          (const T*)a.v.p + b * a.v.batch + (int64_t)kh * a.v.head, a.v.token, a.d,
+                          Range{0, (end + 31) / 32, 1, 32}, end, see, a.c, again);
+    take<DB>(o, again);
+    m = again[16 * DB];
+    l = again[16 * DB + 1];
   }
   l += other_half(l);
   if (!live || l == 0.f) {
@@ -261,6 +273,15 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
 #pragma unroll
           for (int e = 0; e < 16; ++e) acc[db][e] -= eps * mean[db][e];
       }
+      if (a.causal && any_nan<O>(acc)) {
+        float again[16 * DB];
+        strict_dq<T, KS>((const T*)a.q.p + b * a.q.batch + (int64_t)qi * a.q.token + (int64_t)h * a.q.head,
+                         (const T*)a.g.p + b * a.g.batch + (int64_t)qi * a.g.token + (int64_t)h * a.g.head, live,
+                         (const T*)a.k.p + b * a.k.batch + (int64_t)h * a.k.head, a.k.token,
+                         (const T*)a.v.p + b * a.v.batch + (int64_t)h * a.v.head, a.v.token, a.d,
+                         Range{0, (end + 31) / 32, 1, 32}, end, see, a.c, l2, dot, again);
+        take<DB>(acc, again);
+      }
       if (!live || l2 == kInf)
 #pragma unroll
         for (int db = 0; db < DB; ++db) acc[db] = zero16();
@@ -337,6 +358,18 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
           ak[db] = O::mma(Tl::col(at, 16 * x, db, lane_at), fs, ak[db]);
         }
       }
+    }
+    if (a.causal && (any_nan<O>(ak) || any_nan<O>(av))) {
+      // (delta of all queries is in LDS alone)
+      float again[32 * DB];
+      const Queries<T> s{(const T*)a.q.p + b * a.q.batch + (int64_t)h * a.q.head,
+                         (const T*)a.g.p + b * a.g.batch + (int64_t)h * a.g.head,
+                         a.q.token, 0, a.g.token, 0, lse + head0, (const float*)s_delta, a.queries, nq, INT_MAX, 0};
+      strict_dkv<T, KS>((const T*)a.k.p + b * a.k.batch + (int64_t)key * a.k.token + (int64_t)h * a.k.head,
+                        (const T*)a.v.p + b * a.v.batch + (int64_t)key * a.v.token + (int64_t)h * a.v.head, key < nk, s,
+                        a.d, Range{begin / 32, (nq + 31) / 32, 1, 32}, seen, a.c, again);
+      take<DB>(ak, again);
+      take<DB>(av, again + 16 * DB);
     }
     if (first < a.keys) {
       if (key >= nk)

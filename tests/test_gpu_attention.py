@@ -23,7 +23,8 @@ def lengths(*n, dtype=torch.int32):
     return torch.tensor(n, dtype=dtype)
 
 
-def check(q, k, v, do, train=True, device=DEV, **how):
+def check(q, k, v, do, train=True, device=DEV, finite=False, **how):
+    """`finite`: what is inf in one may be NaN in the other."""
     want = ref.attention(q, k, v, do if train else None, **how)
     leaves = [t.to(device).requires_grad_(train) for t in (q, k, v)]
     on = {n: t.to(device) if isinstance(t, torch.Tensor) else t for n, t in how.items()}
@@ -34,7 +35,10 @@ def check(q, k, v, do, train=True, device=DEV, **how):
         got.update(zip(("dq", "dk", "dv"), (t.grad for t in leaves)))
     for name, (value, tolerance) in want.items():
         assert got[name].dtype == q.dtype and got[name].is_contiguous()
-        ref.close(name, got[name], value, tolerance)
+        x = got[name]
+        if finite:
+            x, value = (torch.where(torch.isfinite(y), y, math.nan) for y in (x, value))
+        ref.close(name, x, value, tolerance)
     return got
 
 
@@ -83,6 +87,50 @@ def test_padding_is_not_read(bad, dtype):
             t[b, length[b]:] = bad
     got = check(q, k, v, do, query_lengths=n, key_lengths=m)
     assert all(torch.isfinite(t).all() for t in got.values())
+
+
+# Sizes at which each of the forms runs: all tokens of a head in LDS; 32 rows or keys a workgroup; 128 of them; keys or
+# queries split over workgroups.
+FORMS = [(2, 77, 77, 2, 2), (1, 300, 420, 2, 1), (11, 300, 420, 8, 8), (1, 1300, 1300, 2, 1)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("what,bad", [("q", math.nan), ("k", math.nan), ("v", math.nan), ("v", math.inf),
+                                      ("do", math.nan), ("do", -math.inf)])
+@pytest.mark.parametrize("b,n,m,h,hk", FORMS[:3])
+def test_what_is_not_seen_has_no_part(b, n, m, h, hk, what, bad, dtype):
+    """An inf or a NaN in the middle of a causal sequence: earlier tokens do not see it."""
+    q, k, v, do = inputs(b, n, m, h, hk, 24, dtype, seed=n)
+    at = {"q": q, "k": k, "v": v, "do": do}[what]
+    at[0, at.shape[1] // 2, 0, 5] = bad
+    at[-1, at.shape[1] // 3, -1, :] = bad
+    # Through an inf the gradients are sums of infs of both signs and products of 0 and inf, NaN or inf by the order
+    # that they are formed in (do . o and sum_j p_ij do . v_j are the same number only while both are finite): they
+    # must not be finite where the formula's are not, nor the other way round.
+    check(q, k, v, do, finite=math.isinf(bad), causal=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("b,n,m,h,hk,d", [(*form, d) for form in FORMS for d in (16, 40, 64, 72, 96, 121, 128)
+                                          if form[0] * form[1] * d <= 11 * 300 * 72])
+def test_forms(b, n, m, h, hk, d, causal, dtype):
+    check(*inputs(b, n, m, h, hk, d, dtype, seed=d), causal=causal)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("b,n,m,h,hk", FORMS)
+def test_forms_of_padded_batches(b, n, m, h, hk, dtype):
+    g = torch.Generator().manual_seed(m)
+    nq, nk = (torch.randint(0, x + 1, (b,), generator=g, dtype=torch.int32) for x in (n, m))
+    check(*inputs(b, n, m, h, hk, 32, dtype, seed=b), causal=True, query_lengths=nq, key_lengths=nk)
+    check(*inputs(b, n, m, h, hk, 32, dtype, seed=b), query_lengths=nq, key_lengths=nk)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,m", [(2500, 20), (20, 2500), (3, 700)])
+def test_many_queries_of_few_keys_and_few_of_many(n, m, dtype):
+    check(*inputs(1, n, m, 2, 1, 64, dtype, seed=n))
 
 
 @pytest.mark.parametrize("dtype", TYPES)

@@ -88,9 +88,10 @@ def attention(q, k, v, do=None, causal=False, scale=None, query_lengths=None, ke
     edp = (d + 1) * E * (g.abs() @ vd.abs().transpose(2, 3))
     # (delta is made from the rounded result)
     edelta = (g.abs() * (tout + d * E * out.abs())).sum(3, keepdim=True)
-    ds = p * (dp - delta)
+    ds = (p * (dp - delta)).masked_fill(~see, 0.0)
     # (the backward's probabilities come from lse: the same e, and are not rounded on the way to ds)
     eds = (p * (e + 4 * E) + lost) * (dp - delta).abs() + p * (edp + edelta) + up * ds.abs()
+    eds = eds.masked_fill(~see, 0.0)
     if dtype == torch.float16:
         eds = eds + 2.0 ** -25 * see  # half of fp16's smallest step
     if dtype == torch.bfloat16:
