@@ -14,12 +14,13 @@
 // bits the angle of position 10^6 is off by up to 0.03.
 //
 // Bound by memory: x is read and y written once (backwards dy and x read, dx
-// written), all else is registers.  A wave takes a token with all of its query
-// and key heads, so that the angles of a token are formed once, one pair a
-// lane, and handed to the lanes that need them through LDS.  In a head's row a
+// written), all else is registers.  A wave takes a token's query heads, or its key
+// heads: all of them, so that the angles are formed once, one pair a lane, and
+// handed to the lanes that need them through LDS; one side, so that a lane holds
+// the weights, and the sums of their gradients, of one.  In a head's row a
 // lane holds VP pairs, both halves of each, so that the turn crosses no lanes;
 // a group of 2^lg lanes is a row, and only the norm's sum of squares crosses
-// them.  ROWS rows of a group are in flight at once.
+// them.  The next rows are on their way while the ones before are turned.
 #pragma once
 #include "mec_vec.h"
 
@@ -39,6 +40,7 @@ struct RotaryShape {
   int64_t rows;       // batch * tokens
   int tokens;
   int heads[2];       // of queries and keys (0: that side is left out)
+  int waves[2];       // of a workgroup's, those that take queries, then those that take keys
   int half;           // pairs of a head
   int lg;             // lanes of a row, as a power of 2
   int axes;
@@ -66,45 +68,49 @@ struct Bytes8<4> {
   typedef uint32_t type __attribute__((ext_vector_type(2), aligned(4)));
 };
 
-// VP elements at any alignment, the first n of them (the rest 0).
+// VP elements as they are in memory, at any alignment: 8 or 16 bytes.
 template <class T, int VP>
-__device__ __forceinline__ void load_some(const T* p, int n, float (&v)[VP]) {
-  if constexpr (VP * sizeof(T) == 16) {
-    load_row(p, n, v);
-  } else {
-    using raw = typename Bytes8<sizeof(T)>::type;
-    static_assert(VP * sizeof(T) == 8, "8 or 16 bytes");
-    if (n >= VP) {
-      const raw r = *(const raw*)p;
+struct Raw {
+  static constexpr bool WIDE = VP * sizeof(T) == 16;
+  static_assert(WIDE || VP * sizeof(T) == 8, "8 or 16 bytes");
+  using raw = typename std::conditional<WIDE, typename Vec<T>::raw, typename Bytes8<sizeof(T)>::type>::type;
+  static constexpr int WORDS = WIDE ? 4 : 2;
+  // the first n, the rest 0
+  static __device__ __forceinline__ raw load(const T* p, int n) {
+    if (n >= VP) return *(const raw*)p;
+    raw r;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if constexpr (sizeof(T) == 4) {
-          v[i] = __uint_as_float(r[i]);
-        } else if constexpr (std::is_same<T, uint16_t>::value) {
-          v[2 * i] = __uint_as_float(r[i] << 16);
-          v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
-        } else {
-          const f16x2 h = __builtin_bit_cast(f16x2, (uint32_t)r[i]);
-          v[2 * i] = (float)h[0];
-          v[2 * i + 1] = (float)h[1];
-        }
+    for (int i = 0; i < WORDS; ++i) r[i] = 0;
+#pragma unroll
+    for (int i = 0; i < VP; ++i)
+      if (i < n) {
+        if constexpr (sizeof(T) == 4)
+          r[i] = __float_as_uint(p[i]);
+        else
+          r[i / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, p[i]) << (16 * (i & 1));
       }
-    } else {
+    return r;
+  }
+  static __device__ __forceinline__ void unpack(const raw& r, float (&v)[VP]) {
 #pragma unroll
-      for (int i = 0; i < VP; ++i) v[i] = i < n ? value(p[i]) : 0.f;
+    for (int i = 0; i < WORDS; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        v[i] = __uint_as_float(r[i]);
+      } else if constexpr (std::is_same<T, uint16_t>::value) {
+        v[2 * i] = __uint_as_float(r[i] << 16);
+        v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+      } else {
+        const f16x2 h = __builtin_bit_cast(f16x2, (uint32_t)r[i]);
+        v[2 * i] = (float)h[0];
+        v[2 * i + 1] = (float)h[1];
+      }
     }
   }
-}
-template <class T, int VP>
-__device__ __forceinline__ void store_some(T* p, int n, const float (&v)[VP]) {
-  if constexpr (VP * sizeof(T) == 16) {
-    store_row(p, n, v);
-  } else {
-    using raw = typename Bytes8<sizeof(T)>::type;
+  static __device__ __forceinline__ void store(T* p, int n, const float (&v)[VP]) {
     if (n >= VP) {
       raw r;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < WORDS; ++i) {
         if constexpr (sizeof(T) == 4)
           r[i] = __float_as_uint(v[i]);
         else if constexpr (std::is_same<T, uint16_t>::value)
@@ -119,45 +125,52 @@ __device__ __forceinline__ void store_some(T* p, int n, const float (&v)[VP]) {
         if (i < n) put(p + i, v[i]);
     }
   }
-}
+};
 
-// The n pairs of a lane that begin at pair p0 of the row x.
+// The n pairs of a lane that begin at pair p0 of a row, as they are in memory.
 template <class T, int VP, bool IL>
-__device__ __forceinline__ void load_pairs(const T* x, int p0, int n, int half, float (&a)[VP], float (&b)[VP]) {
-  if constexpr (IL) {
-    float u[VP], v[VP];
-    load_some<T, VP>(x + 2 * p0, 2 * n, u);
-    load_some<T, VP>(x + 2 * p0 + VP, 2 * n - VP, v);
-#pragma unroll
-    for (int i = 0; i < VP / 2; ++i) {
-      a[i] = u[2 * i];
-      b[i] = u[2 * i + 1];
-      a[VP / 2 + i] = v[2 * i];
-      b[VP / 2 + i] = v[2 * i + 1];
-    }
-  } else {
-    load_some<T, VP>(x + p0, n, a);
-    load_some<T, VP>(x + half + p0, n, b);
+struct Pairs {
+  using R = Raw<T, VP>;
+  typename R::raw lo, hi;
+  __device__ __forceinline__ void load(const T* x, int p0, int n, int half) {
+    lo = R::load(x + (IL ? 2 * p0 : p0), IL ? 2 * n : n);
+    hi = R::load(x + (IL ? 2 * p0 + VP : half + p0), IL ? 2 * n - VP : n);
   }
-}
-template <class T, int VP, bool IL>
-__device__ __forceinline__ void store_pairs(T* x, int p0, int n, int half, const float (&a)[VP], const float (&b)[VP]) {
-  if constexpr (IL) {
-    float u[VP], v[VP];
+  __device__ __forceinline__ void unpack(float (&a)[VP], float (&b)[VP]) const {
+    if constexpr (IL) {
+      float u[VP], v[VP];
+      R::unpack(lo, u);
+      R::unpack(hi, v);
 #pragma unroll
-    for (int i = 0; i < VP / 2; ++i) {
-      u[2 * i] = a[i];
-      u[2 * i + 1] = b[i];
-      v[2 * i] = a[VP / 2 + i];
-      v[2 * i + 1] = b[VP / 2 + i];
+      for (int i = 0; i < VP / 2; ++i) {
+        a[i] = u[2 * i];
+        b[i] = u[2 * i + 1];
+        a[VP / 2 + i] = v[2 * i];
+        b[VP / 2 + i] = v[2 * i + 1];
+      }
+    } else {
+      R::unpack(lo, a);
+      R::unpack(hi, b);
     }
-    store_some<T, VP>(x + 2 * p0, 2 * n, u);
-    store_some<T, VP>(x + 2 * p0 + VP, 2 * n - VP, v);
-  } else {
-    store_some<T, VP>(x + p0, n, a);
-    store_some<T, VP>(x + half + p0, n, b);
   }
-}
+  static __device__ __forceinline__ void store(T* x, int p0, int n, int half, const float (&a)[VP], const float (&b)[VP]) {
+    if constexpr (IL) {
+      float u[VP], v[VP];
+#pragma unroll
+      for (int i = 0; i < VP / 2; ++i) {
+        u[2 * i] = a[i];
+        u[2 * i + 1] = b[i];
+        v[2 * i] = a[VP / 2 + i];
+        v[2 * i + 1] = b[VP / 2 + i];
+      }
+      R::store(x + 2 * p0, 2 * n, u);
+      R::store(x + 2 * p0 + VP, 2 * n - VP, v);
+    } else {
+      R::store(x + p0, n, a);
+      R::store(x + half + p0, n, b);
+    }
+  }
+};
 
 // Sum over the 2^lg lanes of a row.
 __device__ __forceinline__ float row_sum(float v, int lg) {
@@ -230,81 +243,104 @@ __device__ __forceinline__ void load_weights(const RotaryShape& s, int side, int
   }
 }
 
-// A wave's way over the tokens: `first`, `first + step`, ...
-struct TokenWalk {
-  int64_t first, step;
-  __device__ __forceinline__ TokenWalk() {
-    first = (int64_t)blockIdx.x * kRotaryWaves + (threadIdx.x >> 6);
-    step = (int64_t)gridDim.x * kRotaryWaves;
+// A wave's way over its side: the passes over a token's heads, 64 / 2^lg rows each, of the tokens
+// first, first + step, ...
+struct Walk {
+  int side, heads, groups, group, passes;
+  int64_t step, rows;
+  int64_t row;     // token, and where it lies
+  int64_t b, t;
+  int pass;
+  int tokens;
+  __device__ __forceinline__ Walk(const RotaryShape& s, int wave, int lane) {
+    side = wave >= s.waves[0];
+    heads = s.heads[side];
+    group = lane >> s.lg;
+    groups = 64 >> s.lg;
+    passes = (heads + groups - 1) / groups;
+    rows = s.rows;
+    tokens = s.tokens;
+    step = (int64_t)gridDim.x * s.waves[side];
+    pass = 0;
+    place((int64_t)blockIdx.x * s.waves[side] + (side ? wave - s.waves[0] : wave));
   }
+  __device__ __forceinline__ void place(int64_t r) {
+    row = r;
+    b = r / tokens;
+    t = r - b * tokens;
+  }
+  __device__ __forceinline__ bool done() const { return row >= rows; }
+  __device__ __forceinline__ void next() {
+    if (++pass == passes) {
+      pass = 0;
+      place(row + step);
+    }
+  }
+  __device__ __forceinline__ int head() const { return pass * groups + group; }
+  // this lane's row, and its pairs there (0: no row)
+  template <class T>
+  __device__ __forceinline__ const T* at(const HeadsView& v) const {
+    return (const T*)v.p + b * v.batch + t * v.token + (int64_t)head() * v.head;
+  }
+  __device__ __forceinline__ int pairs(int n) const { return !done() && head() < heads ? n : 0; }
 };
+// cos and sin of this lane's pairs of the walk's token
+template <int VP>
+__device__ __forceinline__ void angles(const Turns& turns, const RotaryShape& s, const Walk& w, int lane, float* cs,
+                                       float* sn, int p0, int n, float (&c)[VP], float (&z)[VP]) {
+  turns.turn(s, w.b * s.pos_batch + w.t * s.axes, lane, cs, sn);
+  wave_sync();
+#pragma unroll
+  for (int i = 0; i < VP; ++i) {
+    const bool in = i < n;
+    c[i] = in ? cs[p0 + i] : 0.f;
+    z[i] = in ? sn[p0 + i] : 0.f;
+  }
+  wave_sync();
+}
 
 template <class T, int VP, bool IL, bool NORM>
 __global__ __launch_bounds__(64 * kRotaryWaves) void k_rotary(RotaryShape s, HeadsView q, HeadsView k, T* yq, T* yk) {
-  constexpr int ROWS = 2;
+  using P = Pairs<T, VP, IL>;
   __shared__ alignas(16) float s_cos[kRotaryWaves][kMaxHalf + VP], s_sin[kRotaryWaves][kMaxHalf + VP];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   float *cs = s_cos[wave], *sn = s_sin[wave];
-  const int p0 = (lane & ((1 << s.lg) - 1)) * VP, n = s.half - p0;  // this lane's pairs
-  const int group = lane >> s.lg, groups = 64 >> s.lg;
-  const int heads = s.heads[0] + s.heads[1], d = 2 * s.half;
+  const int p0 = (lane & ((1 << s.lg) - 1)) * VP, n = s.half - p0, d = 2 * s.half;  // this lane's pairs
+  Walk w(s, wave, lane);
+  const HeadsView v = w.side ? k : q;
+  T* const y = w.side ? yk : yq;
+  if (w.done() || w.heads == 0) return;
+  P x;
+  x.load(w.at<T>(v), p0, w.pairs(n), s.half);
   Turns turns;
   turns.init(s, lane);
-  float wa[2][VP], wb[2][VP];
-  if constexpr (NORM) {
-    load_weights<VP, IL>(s, 0, p0, wa[0], wb[0]);
-    load_weights<VP, IL>(s, 1, p0, wa[1], wb[1]);
-  }
-  const TokenWalk walk;
-  for (int64_t row = walk.first; row < s.rows; row += walk.step) {
-    const int64_t b = row / s.tokens, t = row - b * s.tokens;
-    turns.turn(s, b * s.pos_batch + t * s.axes, lane, cs, sn);
-    wave_sync();
-    float c[VP], z[VP];
+  float wa[VP], wb[VP], c[VP], z[VP];
+  if constexpr (NORM) load_weights<VP, IL>(s, w.side, p0, wa, wb);
+  while (!w.done()) {
+    if (w.pass == 0) angles<VP>(turns, s, w, lane, cs, sn, p0, n, c, z);
+    float a[VP], b[VP], ya[VP], yb[VP];
+    x.unpack(a, b);
+    const int h = w.head();
+    T* const to = h < w.heads ? y + (w.row * w.heads + h) * d : nullptr;
+    w.next();
+    x.load(w.at<T>(v), p0, w.pairs(n), s.half);
+    if constexpr (NORM) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < VP; ++i) sum += a[i] * a[i] + b[i] * b[i];
+      const float r = rsqrtf(row_sum(sum, s.lg) / (float)d + s.eps);
+#pragma unroll
+      for (int i = 0; i < VP; ++i) {
+        a[i] *= r * wa[i];
+        b[i] *= r * wb[i];
+      }
+    }
 #pragma unroll
     for (int i = 0; i < VP; ++i) {
-      const bool in = i < n;
-      c[i] = in ? cs[p0 + i] : 0.f;
-      z[i] = in ? sn[p0 + i] : 0.f;
+      ya[i] = a[i] * c[i] - b[i] * z[i];
+      yb[i] = b[i] * c[i] + a[i] * z[i];
     }
-    wave_sync();
-    for (int h0 = group; h0 < heads; h0 += ROWS * groups) {
-      float xa[ROWS][VP], xb[ROWS][VP];
-#pragma unroll
-      for (int u = 0; u < ROWS; ++u) {
-        const int h = h0 + u * groups;
-        const bool key = h >= s.heads[0];
-        const HeadsView& v = key ? k : q;
-        const T* x = (const T*)v.p + b * v.batch + t * v.token + (int64_t)(key ? h - s.heads[0] : h) * v.head;
-        load_pairs<T, VP, IL>(x, p0, h < heads ? n : 0, s.half, xa[u], xb[u]);
-      }
-#pragma unroll
-      for (int u = 0; u < ROWS; ++u) {
-        const int h = h0 + u * groups;
-        const bool key = h >= s.heads[0];
-        if constexpr (NORM) {
-          float sum = 0.f;
-#pragma unroll
-          for (int i = 0; i < VP; ++i) sum += xa[u][i] * xa[u][i] + xb[u][i] * xb[u][i];
-          const float r = rsqrtf(row_sum(sum, s.lg) / (float)d + s.eps);
-#pragma unroll
-          for (int i = 0; i < VP; ++i) {
-            xa[u][i] *= r * (key ? wa[1][i] : wa[0][i]);
-            xb[u][i] *= r * (key ? wb[1][i] : wb[0][i]);
-          }
-        }
-        float ya[VP], yb[VP];
-#pragma unroll
-        for (int i = 0; i < VP; ++i) {
-          ya[i] = xa[u][i] * c[i] - xb[u][i] * z[i];
-          yb[i] = xb[u][i] * c[i] + xa[u][i] * z[i];
-        }
-        if (h < heads) {
-          T* y = key ? yk + (row * s.heads[1] + (h - s.heads[0])) * d : yq + (row * s.heads[0] + h) * d;
-          store_pairs<T, VP, IL>(y, p0, n, s.half, ya, yb);
-        }
-      }
-    }
+    if (to) P::store(to, p0, n, s.half, ya, yb);
   }
 }
 
@@ -314,100 +350,86 @@ template <class T, int VP, bool IL>
 __global__ __launch_bounds__(64 * kRotaryWaves) void k_rotary_norm_grad(RotaryShape s, HeadsView q, HeadsView k,
                                                                         HeadsView gq, HeadsView gk, T* dxq, T* dxk,
                                                                         float* parts) {
+  using P = Pairs<T, VP, IL>;
   __shared__ alignas(16) float s_cos[kRotaryWaves][kMaxHalf + VP], s_sin[kRotaryWaves][kMaxHalf + VP];
   __shared__ float s_dw[kRotaryWaves][2 * kMaxHalf];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   float *cs = s_cos[wave], *sn = s_sin[wave];
-  const int p0 = (lane & ((1 << s.lg) - 1)) * VP, n = s.half - p0;
-  const int group = lane >> s.lg, groups = 64 >> s.lg;
-  const int heads = s.heads[0] + s.heads[1], d = 2 * s.half;
-  Turns turns;
-  turns.init(s, lane);
-  float wa[2][VP], wb[2][VP], da[2][VP], db[2][VP];
+  const int p0 = (lane & ((1 << s.lg) - 1)) * VP, n = s.half - p0, d = 2 * s.half;
+  Walk w(s, wave, lane);
+  const HeadsView v = w.side ? k : q, g = w.side ? gk : gq;
+  T* const dx = w.side ? dxk : dxq;
+  float da[VP], db[VP];
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    load_weights<VP, IL>(s, e, p0, wa[e], wb[e]);
-#pragma unroll
-    for (int i = 0; i < VP; ++i) da[e][i] = db[e][i] = 0.f;
-  }
-  const TokenWalk walk;
-  for (int64_t row = walk.first; row < s.rows; row += walk.step) {
-    const int64_t b = row / s.tokens, t = row - b * s.tokens;
-    turns.turn(s, b * s.pos_batch + t * s.axes, lane, cs, sn);
-    wave_sync();
-    float c[VP], z[VP];
-#pragma unroll
-    for (int i = 0; i < VP; ++i) {
-      const bool in = i < n;
-      c[i] = in ? cs[p0 + i] : 0.f;
-      z[i] = in ? sn[p0 + i] : 0.f;
-    }
-    wave_sync();
-    for (int h = group; h < heads; h += groups) {
-      const bool key = h >= s.heads[0];
-      const int hh = key ? h - s.heads[0] : h;
-      const HeadsView &v = key ? k : q, &g = key ? gk : gq;
+  for (int i = 0; i < VP; ++i) da[i] = db[i] = 0.f;
+  if (!w.done() && w.heads > 0) {
+    P x, y;
+    x.load(w.at<T>(v), p0, w.pairs(n), s.half);
+    y.load(w.at<T>(g), p0, w.pairs(n), s.half);
+    Turns turns;
+    turns.init(s, lane);
+    float wa[VP], wb[VP], c[VP], z[VP];
+    load_weights<VP, IL>(s, w.side, p0, wa, wb);
+    while (!w.done()) {
+      if (w.pass == 0) angles<VP>(turns, s, w, lane, cs, sn, p0, n, c, z);
       float xa[VP], xb[VP], ga[VP], gb[VP];
-      load_pairs<T, VP, IL>((const T*)v.p + b * v.batch + t * v.token + (int64_t)hh * v.head, p0, n, s.half, xa, xb);
-      load_pairs<T, VP, IL>((const T*)g.p + b * g.batch + t * g.token + (int64_t)hh * g.head, p0, n, s.half, ga, gb);
+      x.unpack(xa, xb);
+      y.unpack(ga, gb);
+      const int h = w.head();
+      T* const to = dx != nullptr && h < w.heads ? dx + (w.row * w.heads + h) * d : nullptr;
+      w.next();
+      x.load(w.at<T>(v), p0, w.pairs(n), s.half);
+      y.load(w.at<T>(g), p0, w.pairs(n), s.half);
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < VP; ++i) sum += xa[i] * xa[i] + xb[i] * xb[i];
-      const float r = rsqrtf(row_sum(sum, s.lg) / (float)d + s.eps);
+      // (rows that are none are 0, and have no part in dw)
+      const float r = h < w.heads ? rsqrtf(row_sum(sum, s.lg) / (float)d + s.eps) : 0.f;
+      // dx = r g w - x r^3 mean(g w x)
       float dot = 0.f;
 #pragma unroll
       for (int i = 0; i < VP; ++i) {
         const float ta = ga[i] * c[i] + gb[i] * z[i], tb = gb[i] * c[i] - ga[i] * z[i];
-        xa[i] *= r;
-        xb[i] *= r;
-        const float wqa = ta * xa[i], wqb = tb * xb[i];
-        da[0][i] += key ? 0.f : wqa;
-        db[0][i] += key ? 0.f : wqb;
-        da[1][i] += key ? wqa : 0.f;
-        db[1][i] += key ? wqb : 0.f;
-        ga[i] = ta * (key ? wa[1][i] : wa[0][i]);
-        gb[i] = tb * (key ? wb[1][i] : wb[0][i]);
-        dot += ga[i] * xa[i] + gb[i] * xb[i];
+        const float ua = ta * xa[i], ub = tb * xb[i];
+        da[i] = fmaf(ua, r, da[i]);
+        db[i] = fmaf(ub, r, db[i]);
+        dot = fmaf(ua, wa[i], dot);
+        dot = fmaf(ub, wb[i], dot);
+        ga[i] = ta * (wa[i] * r);
+        gb[i] = tb * (wb[i] * r);
       }
-      const float mean = row_sum(dot, s.lg) / (float)d;
+      const float less = -(row_sum(dot, s.lg) / (float)d) * r * r * r;
 #pragma unroll
       for (int i = 0; i < VP; ++i) {
-        ga[i] = r * (ga[i] - xa[i] * mean);
-        gb[i] = r * (gb[i] - xb[i] * mean);
+        ga[i] = fmaf(xa[i], less, ga[i]);
+        gb[i] = fmaf(xb[i], less, gb[i]);
       }
-      T* dx = key ? dxk : dxq;
-      if (dx) store_pairs<T, VP, IL>(dx + (row * s.heads[key] + hh) * d, p0, n, s.half, ga, gb);
+      if (to) P::store(to, p0, n, s.half, ga, gb);
     }
   }
   if (parts == nullptr) return;
-  // over the groups of the wave, then over the waves, in this order
+  // over the groups of the wave, then over the side's waves, in this order
   for (int m = 1 << s.lg; m < 64; m <<= 1)
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+    for (int i = 0; i < VP; ++i) {
+      da[i] += __shfl_xor(da[i], m, 64);
+      db[i] += __shfl_xor(db[i], m, 64);
+    }
+  if (w.group == 0) {
 #pragma unroll
-      for (int i = 0; i < VP; ++i) {
-        da[e][i] += __shfl_xor(da[e][i], m, 64);
-        db[e][i] += __shfl_xor(db[e][i], m, 64);
+    for (int i = 0; i < VP; ++i)
+      if (i < n) {
+        const int p = p0 + i;
+        s_dw[wave][IL ? 2 * p : p] = da[i];
+        s_dw[wave][IL ? 2 * p + 1 : p + s.half] = db[i];
       }
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    if (group == 0) {
-#pragma unroll
-      for (int i = 0; i < VP; ++i)
-        if (i < n) {
-          const int p = p0 + i;
-          s_dw[wave][IL ? 2 * p : p] = da[e][i];
-          s_dw[wave][IL ? 2 * p + 1 : p + s.half] = db[e][i];
-        }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < d; i += 64 * kRotaryWaves) {
-      float v = 0.f;
-#pragma unroll
-      for (int w = 0; w < kRotaryWaves; ++w) v += s_dw[w][i];
-      parts[((int64_t)blockIdx.x * 2 + e) * d + i] = v;
-    }
-    __syncthreads();
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * d; i += 64 * kRotaryWaves) {
+    const int side = i >= d, from = side ? s.waves[0] : 0;
+    float sum = 0.f;
+    for (int u = 0; u < s.waves[side]; ++u) sum += s_dw[from + u][i - side * d];
+    parts[(int64_t)blockIdx.x * 2 * d + i] = sum;
   }
 }
 
@@ -420,6 +442,7 @@ __global__ __launch_bounds__(64 * kDwWaves) void k_rotary_dw(const float* parts,
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
   float v = 0.f;
   if (col < 2 * d)
+#pragma unroll 8
     for (int i = wave; i < n; i += kDwWaves) v += parts[(int64_t)i * 2 * d + col];
   s_sum[wave][lane] = v;
   __syncthreads();
