@@ -298,7 +298,22 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
   if (split * share < stop) {
     Frag k[KS], v[B::V_LDS ? 1 : KS];
     Lds* const values = (Lds*)s_values + (WM == 1 ? 0 : 32 * wave * Tl::RB);
-    {
+    if constexpr (WM == 4 && STEP == 64) {
+      // (through the tiles' places, in whole rows, not as fragments, 16 bytes of each of 32 rows at a time: one query of
+      // 729 keys, 256 x 16 heads of 72, 527 to 511 us)
+      Fetcher<T, DB, 128, WM> fk, fv;
+      fk.init(a.k, b, kh, a.d, wave, lane);
+      fv.init(a.v, b, kh, a.d, wave, lane);
+      fk.load((Lds*)s_lds, key0, nk - key0);
+      fv.load((Lds*)s_next, key0, nk - key0);
+      loads_done();
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        k[s] = Tl::row((Lds*)s_lds, 32 * wave, s, lane_at);
+        v[s] = Tl::row((Lds*)s_next, 32 * wave, s, lane_at);
+      }
+      __syncthreads();
+    } else {
       const T* pk = (const T*)a.k.p + b * a.k.batch + (int64_t)key * a.k.token + (int64_t)kh * a.k.head;
       const T* pv = (const T*)a.v.p + b * a.v.batch + (int64_t)key * a.v.token + (int64_t)kh * a.v.head;
 #pragma unroll

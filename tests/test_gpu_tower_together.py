@@ -73,3 +73,32 @@ def test_a_tower(causal):
     assert abs(loss.item() - loss64.item()) <= 2.0 ** -10 * abs(loss64.item())
     for name, got, want in zip(("embedding", "projection", "query norm", "key norm"), leaves, wide):
         ref.close(name, got.grad, want.grad, 2.0 ** -10 * want.grad.abs().max())
+
+
+def test_offloaded_and_recomputed():
+    """Saved tensors that go through the host, or are made again, give the same gradients."""
+    from torch.utils.checkpoint import checkpoint
+
+    g = torch.Generator().manual_seed(1)
+    qkv = torch.randn(3, 40, 8, 32, generator=g).to(DEV, torch.bfloat16)
+    w = torch.ones(32, device=DEV, dtype=torch.bfloat16)
+    pos, n = torch.arange(40, device=DEV)[:, None], torch.tensor([40, 0, 17], device=DEV)
+
+    def f(x, w):
+        q, k, v = x.split([4, 2, 2], 2)
+        q, k = mec.norm_rotary(q, k, pos, (16,), w, w, eps=1e-6)
+        return mec.attention(q, k, v, causal=True, query_lengths=n, key_lengths=n)
+
+    grads = []
+    for way in ("plain", "host", "again"):
+        leaves = [qkv.clone().requires_grad_(True), w.clone().requires_grad_(True)]
+        if way == "host":
+            with torch.autograd.graph.save_on_cpu():
+                out = f(*leaves)
+        elif way == "again":
+            out = checkpoint(f, *leaves, use_reentrant=False)
+        else:
+            out = f(*leaves)
+        out.float().square().sum().backward()
+        grads.append([t.grad for t in leaves])
+    assert all(torch.equal(a, b) for way in grads[1:] for a, b in zip(grads[0], way))
