@@ -122,6 +122,22 @@ struct Ops {
     }
     return f;
   }
+  // sum + the 8 values of a fragment
+  static __device__ __forceinline__ float add(const Frag& f, float sum) {
+    if constexpr (!F32) {
+      const uint32_t ones = F16 ? 0x3c003c00u : 0x3f803f80u;
+      const u32x4 r = __builtin_bit_cast(u32x4, f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (F16)
+          sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, (uint32_t)r[e]), __builtin_bit_cast(f16x2, ones), sum, false);
+        else
+          sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, (uint32_t)r[e]), __builtin_bit_cast(bf16x2, ones),
+                                                sum, false);
+      }
+    }
+    return sum;
+  }
   // k 16 s + 8 half .. + 7 of a row of d elements in memory
   static __device__ __forceinline__ Frag load_row(const T* row, bool valid, int s, int half, int d) {
     const int at = 16 * s + 8 * half, n = valid ? d - at : 0;

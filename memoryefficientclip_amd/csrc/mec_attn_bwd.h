@@ -43,7 +43,13 @@ struct Backward {
   // this is the largest error of dq and dk (heads of 64, 77 tokens, causal, bf16: 0.0031 of their size, 0.0023
   // with a delta of fp32).  delta is also sum_j p_ij do_i . v_j: with d for do . o, eps = sum_j p_ij (do_i . v_j - d)
   // is what it lacks.  Up to this many keys it is summed in a first walk over them.
-  static constexpr int KEYS_EXACT = O::F32 ? 0 : 512;
+  //
+  // dq = scale sum_j ds_ij k_j, and as the ds_ij add up to 0, the k_j might be less their mean, m_i = sum_j p_ij k_j:
+  // rounded ds_ij do not add up to 0, and their sum times m_i is an error that grows with scale.  Heads of up to 48
+  // have the registers for m_i: there dq is corrected by it, which takes what delta lacks along, at all lengths
+  // (bf16, heads of 32, 6396 keys: dq off by 0.0026 of its size, 0.0023 with it; heads of 16: 0.0027 and 0.0023).
+  static constexpr bool MEAN = !O::F32 && KS <= 3;
+  static constexpr int KEYS_EXACT = O::F32 || MEAN ? -1 : 512;
 };
 
 // A row of the sums of a workgroup's waves, [WK][32][32 DB] in LDS.
@@ -73,7 +79,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
   using Tl = typename B::Tl;
   constexpr int DB = B::DB, STEP = B::STEP, NB = STEP / 32, WK = B::WK;
   __shared__ alignas(16) char s_lds[B::PLACE], s_next[WM == 1 ? 16 : B::PLACE];
-  __shared__ float s_eps[WM == 1 ? WK : 1][32];
+  __shared__ float s_eps[WM == 1 ? 2 * WK : 1][32];
   constexpr bool G_LDS = B::V_LDS && WM > 1;
   __shared__ alignas(16) char s_grads[G_LDS ? B::ROWS * Tl::RB : 16];
   int64_t pair;
@@ -95,7 +101,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
   int end = row0 / a.group >= nq ? 0 : a.causal ? min(nk, last + shift + 1) : nk;
   if (end < 0) end = 0;
   const bool exact = end <= B::KEYS_EXACT;
-  if (dq == nullptr && !exact) end = 0;
+  if (dq == nullptr && !exact && !B::MEAN) end = 0;
   const int all = a.causal ? min(nk, wave_row0 / a.group + shift + 1) : nk;
   const int wave_end = wave_row0 / a.group >= nq ? 0
                        : a.causal               ? min(nk, min((wave_row0 + 31) / a.group, nq - 1) + shift + 1)
@@ -123,13 +129,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
     dot += other_half(dot);
     if (live) l2 = lse[at];
   }
-  f32x16 acc[DB];  // dq / scale
+  f32x16 acc[DB], mean[B::MEAN ? DB : 1];  // dq / scale; sum_j p_ij k_j
 #pragma unroll
-  for (int db = 0; db < DB; ++db) acc[db] = zero16();
+  for (int db = 0; db < DB; ++db) {
+    acc[db] = zero16();
+    mean[B::MEAN ? db : 0] = zero16();
+  }
+  float eps = 0.f, eps16 = 0.f;  // sums of the ds_ij, and of the rounded ones
   const int tiles = (end + STEP - 1) / STEP;
   if (tiles > 0) {
     const int first = WM == 1 ? wave : 0;
-    float eps = 0.f;
     int walk = exact ? 0 : 1;
     const auto use = [&](Lds* tk, int i) {
       auto at = lane_at;
@@ -150,11 +159,33 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
             p = O::mma(Tl::row(tv, 32 * kb, ks, at), g[ks], p);
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) p[e] = fast_exp2(fmaf(s[e], a.c, -l2)) * (p[e] - dot);
+        for (int e = 0; e < 16; ++e) {
+          s[e] = fast_exp2(fmaf(s[e], a.c, -l2));
+          p[e] = s[e] * (p[e] - dot);
+        }
         if (masked) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            p[e] = key0 + 32 * kb + 8 * (e >> 2) + 4 * half + (e & 3) < see ? p[e] : 0.f;
+          for (int e = 0; e < 16; ++e) {
+            const bool in = key0 + 32 * kb + 8 * (e >> 2) + 4 * half + (e & 3) < see;
+            s[e] = in ? s[e] : 0.f;
+            p[e] = in ? p[e] : 0.f;
+          }
+        }
+        if constexpr (B::MEAN) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) eps += p[e];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const Frag ds = O::pack(p, h), ps = O::pack(s, h);
+            eps16 = O::add(ds, eps16);
+#pragma unroll
+            for (int db = 0; db < DB; ++db) {
+              const Frag kt = Tl::col(tk, 32 * kb + 16 * h, db, at);
+              acc[db] = O::mma(kt, ds, acc[db]);
+              mean[db] = O::mma(kt, ps, mean[db]);
+            }
+          }
+          continue;
         }
         if constexpr (!O::F32) {
           // (one loop for both walks: the compiler's two copies of it take 50 registers more)
@@ -224,6 +255,29 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
         eps = 0.f;
       }
     }
+  }
+  if constexpr (B::MEAN) {
+    eps += other_half(eps);
+    eps16 += other_half(eps16);
+    if constexpr (WM == 1) {
+      // (each wave takes its share of the correction off: the sum of all times its part of the mean)
+      if (half == 0) {
+        s_eps[wave][lane] = eps;
+        s_eps[WK + wave][lane] = eps16;
+      }
+      __syncthreads();
+      eps = eps16 = 0.f;
+#pragma unroll
+      for (int i = 0; i < WK; ++i) {
+        eps += s_eps[i][lane & 31];
+        eps16 += s_eps[WK + i][lane & 31];
+      }
+    }
+    dot += eps;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[db][e] -= eps16 * mean[B::MEAN ? db : 0][e];
   }
   if (a.causal && any_nan<O>(acc)) {
     float again[16 * DB];

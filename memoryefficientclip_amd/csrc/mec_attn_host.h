@@ -71,6 +71,8 @@ template <class F>
 void with_steps(int d, F f) {
   if (d <= 32)
     f(std::integral_constant<int, 2>{});
+  else if (d <= 48)
+    f(std::integral_constant<int, 3>{});
   else if (d <= 64)
     f(std::integral_constant<int, 4>{});
   else if (d <= 80)

@@ -154,7 +154,7 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
   using Tl = Tile<T, DB>;
   // a wave's keys and values, in registers; of fp32 and of wide heads they are read from LDS
   constexpr bool HELD = !O::F32 && DB <= 2;
-  // see Backward: d + eps is delta
+  // see Backward: d + eps is delta, and dq is corrected by the sum of the rounded ds times the mean key
   constexpr bool MEAN = !O::F32 && DB <= 2, TWICE = !O::F32 && DB > 2;
   int64_t id;
   int tile;
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
       f32x16 mean[MEAN ? DB : 1];
 #pragma unroll
       for (int db = 0; db < (MEAN ? DB : 1); ++db) mean[db] = zero16();
-      float eps = 0.f;
+      float eps = 0.f, eps16 = 0.f;
       for (int walk = TWICE ? 0 : 1; walk < 2; ++walk) {
         Lds* at = tk;
         for (int key0 = 0; key0 < end; key0 += 32, at += 2 * BLOCK) {
@@ -252,6 +252,7 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const Frag ds = O::pack(p, x), ps = O::pack(s, x);
+            if constexpr (MEAN) eps16 = O::add(ds, eps16);
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
               const Frag kt = Tl::col(at, 16 * x, db, lane_at);
@@ -267,11 +268,12 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
       }
       if constexpr (MEAN) {
         eps += other_half(eps);
+        eps16 += other_half(eps16);
         dot += eps;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) acc[db][e] -= eps * mean[db][e];
+          for (int e = 0; e < 16; ++e) acc[db][e] -= eps16 * mean[db][e];
       }
       if (a.causal && any_nan<O>(acc)) {
         float again[16 * DB];
