@@ -578,7 +578,7 @@ int mec_norm_rotary_backward(const mec_rotary_t* rotary, const mec_heads_t* quer
  * sees no key, or only scores of -inf, has result 0 and gradient 0, and no key or
  * value that it does not see has a part in its result, whatever it holds.
  * head_dim 1 to 128; batch * key_heads, queries * heads / key_heads and keys at most
- * 2^30; scale finite and > 0. */
+ * 2^30; scale in [1e-30, 1e30]. */
 #define MEC_MAX_HEAD_DIM 128
 typedef struct {
   int64_t batch, queries, keys, heads, key_heads, head_dim;

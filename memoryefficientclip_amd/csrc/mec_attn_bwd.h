@@ -11,7 +11,7 @@
 // k_attn_dq also leaves delta = do . o for k_attn_dkv.
 //
 // WM = 4: the four waves of a workgroup have 32 rows (keys) each and share tiles,
-// two in LDS, the next on its way in registers.  WM = 1, where that would leave the
+// two in LDS, one of them on its way (Fetcher).  WM = 1, where that would leave the
 // device empty: they share 32 rows (keys) and take every fourth tile of 32, each in
 // LDS of its own, and add up what they have in the end.  k_attn_dkv's queries are
 // split over `splits` workgroups besides, whose fp32 sums k_attn_dkv_join adds, where

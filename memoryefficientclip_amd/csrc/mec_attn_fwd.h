@@ -9,8 +9,8 @@
 // The maximum lags: the accumulators are rescaled only where it grew by more than
 // 2^8, which after the first tiles hardly happens.
 //
-// WM > 1: WM waves of 32 rows each share tiles of KEYS keys, two in LDS, the next
-// on its way in registers.  WM = 1 is the form for few rows (single tokens): the
+// WM > 1: WM waves of 32 rows each share tiles of KEYS keys, two in LDS, one of them
+// on its way (Fetcher).  WM = 1 is the form for few rows (single tokens): the
 // WK waves of a workgroup take every WK-th tile of 32 keys, each in LDS of its own
 // without a barrier, and meet at the end; the keys are split over `splits`
 // workgroups, which k_attn_join joins.
@@ -20,10 +20,11 @@
 namespace mec {
 namespace attn {
 
-// log2 units: with m the maximum that the sums l and o are relative to, and a part's lse
+// What a workgroup has of its rows where the keys are split: the sum of the values, and m (the maximum that it is
+// relative to, in units of log2) and the sum of the probabilities.
 struct Parts {
-  float* o;     // [splits][pairs][rows][d]
-  float2* ml;   // [splits][pairs][rows]
+  float* o;    // [splits][pairs][rows][d]
+  float2* ml;  // [splits][pairs][rows]
 };
 
 template <class T, int KS, int WM, int WK>
@@ -35,15 +36,15 @@ struct Forward {
   static constexpr int NT = 64 * WM * WK, ROWS = 32 * WM;
   static constexpr int KEYS = WM == 1 || O::F32 ? 32 : 64, NB = KEYS / 32;
   static constexpr int TILE = KEYS * Tl::RB;
-  static constexpr int JOIN = WM == 1 ? WK * 32 * (32 * DB + 2) * 4 : 0;
-  // keys and values of a tile of each wave that has its own
-  static constexpr int LDS0 = 2 * TILE * WK, LDS = LDS0 > JOIN ? LDS0 : JOIN;
+  // keys and values of a tile of each wave that has its own, and in the end (WM = 1) what the waves have
+  static constexpr int TILES = 2 * TILE * WK, JOIN = WM == 1 ? WK * 32 * (32 * DB + 2) * 4 : 0;
+  static constexpr int LDS = TILES > JOIN ? TILES : JOIN;
   static_assert(WM == 1 || WK == 1, "");
 };
 
 template <class T, int KS, int WM, int WK>
-__global__ __launch_bounds__(64 * WM * WK, sizeof(T) == 4 || (WM == 1 && KS == 8) ? 1 : 2) void k_attn_forward(Problem a, Items items, int row_tiles,
-                                                               int splits, T* out, float* lse, Parts parts) {
+__global__ __launch_bounds__(64 * WM * WK, sizeof(T) == 4 || (WM == 1 && KS == 8) ? 1 : 2) void k_attn_forward(
+    Problem a, Items items, int row_tiles, int splits, T* out, float* lse, Parts parts) {
   using F = Forward<T, KS, WM, WK>;
   using O = Ops<T>;
   using Frag = typename O::Frag;

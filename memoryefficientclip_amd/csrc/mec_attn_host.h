@@ -30,7 +30,8 @@ inline int check_attention(const mec_attention_t* p, Problem* out) {
     return fail(MEC_ERR_UNSUPPORTED, "%lld x %lld key heads, %lld queries for %lld heads each, %lld keys exceed 2^30",
                 (long long)p->batch, (long long)p->key_heads, (long long)p->queries, (long long)group,
                 (long long)p->keys);
-  if (!(p->scale > 0.f && std::isfinite(p->scale))) return fail(MEC_ERR_INVALID, "scale must be finite and > 0");
+  // (times log2(e) it has to be finite, and times -inf to be -inf)
+  if (!(p->scale >= 1e-30f && p->scale <= 1e30f)) return fail(MEC_ERR_INVALID, "scale must be in [1e-30, 1e30]");
   if ((p->query_lengths || p->key_lengths) && p->length_bytes != 4 && p->length_bytes != 8)
     return fail(MEC_ERR_INVALID, "length_bytes=%d must be 4 or 8", p->length_bytes);
   Problem a{};

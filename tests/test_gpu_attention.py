@@ -263,3 +263,28 @@ def test_another_stream():
     stream.synchronize()
     for name, t in zip(("out", "dq", "dk", "dv"), (out, *(t.grad for t in leaves))):
         ref.close(name, t, *want[name])
+
+
+def test_a_cache_beyond_32_bits():
+    """A long cache of two texts, the second beyond 2^31 bytes, its end beyond 2^31 elements: one new token of each."""
+    n, hk, d = 1_100_000, 8, 128
+    g = torch.Generator(device=DEV).manual_seed(0)
+    k, v = (torch.empty(2, n, hk, d, device=DEV, dtype=torch.bfloat16) for _ in "kv")
+    for t, mean in ((k, 0.0), (v, 1.0)):
+        for b in range(2):
+            t[b].normal_(mean, 1.0, generator=g)
+    assert k.stride(0) * k.element_size() > 1 << 31 and k.numel() > 1 << 31
+    q = torch.randn(2, 1, 2 * hk, d, device=DEV, generator=g).bfloat16()
+    lengths = torch.tensor([n, n - 77], device=DEV)
+    out = mec.attention(q, k, v, causal=True, key_lengths=lengths)
+    for b in range(2):
+        for h in range(2 * hk):
+            m = lengths[b].item()
+            kd, vd = k[b, :m, h // 2].double(), v[b, :m, h // 2].double()
+            p = torch.softmax(kd @ q[b, 0, h].double() / d ** 0.5, 0)
+            want = p @ vd
+            # A score is off by (d + 2) E times the sizes of its terms, here 20 at most.  A lane adds up less than 10000
+            # probabilities, and its products; 32 parts are joined.  Probabilities and result are rounded to bf16.
+            u = ref.half_step(torch.bfloat16)
+            tolerance = (u + 2 * (d + 2) * ref.E * 20 + 10100 * ref.E) * (p @ vd.abs()) + u * want.abs()
+            ref.close(f"{b} {h}", out[b, 0, h], want.cpu(), tolerance.cpu())

@@ -63,7 +63,7 @@ def test_attention_refuses(no_capture):
         mec.attention(q.double(), k.double(), k.double())
     with pytest.raises(TypeError, match="mismatch"):
         mec.attention(q, k, k.half())
-    for s in (0.0, -1.0, math.inf, math.nan):
+    for s in (0.0, -1.0, math.inf, math.nan, 1e-31, 1e31):
         with pytest.raises(ValueError, match="scale"):
             mec.attention(q, k, k, scale=s)
     with pytest.raises(ValueError, match="query_lengths"):
@@ -140,7 +140,7 @@ def call_attention_backward(a, out=P, lse=P, dq=P, dk=P, dv=P, workspace=None, n
 BAD_ATTENTION = [(dict(dtype=4), -1), (dict(batch=0), -1), (dict(queries=0), -1), (dict(keys=0), -1), (dict(heads=0), -1),
                  (dict(key_heads=0), -1), (dict(key_heads=3), -1), (dict(head_dim=0), -1), (dict(head_dim=129), -2),
                  (dict(keys=(1 << 30) + 1), -2), (dict(queries=1 << 30), -2), (dict(batch=1 << 30), -2),
-                 (dict(heads=1 << 40, key_heads=1), -2), (dict(scale=0.0), -1), (dict(scale=math.nan), -1),
+                 (dict(heads=1 << 40, key_heads=1), -2), (dict(scale=0.0), -1), (dict(scale=1e-31), -1), (dict(scale=1e31), -1), (dict(scale=math.nan), -1),
                  (dict(scale=math.inf), -1), (dict(query_lengths=P, length_bytes=3), -1)]
 
 
