@@ -332,13 +332,15 @@ struct Fetcher {
   bool whole;
   uint32_t off[NB];
 
-  __device__ __forceinline__ void init(const View& v, int64_t b, int h, int d_, int wave_, int lane_) {
+  // (moves: `move` will be called)
+  __device__ __forceinline__ void init(const View& v, int64_t b, int h, int d_, int wave_, int lane_, bool moves = false) {
     base = (const char*)((const T*)v.p + b * v.batch + (int64_t)h * v.head);
     pitch = v.token * (int64_t)sizeof(T);
     d = d_;
     lane = lane_;
     wave = wave_;
-    whole = d % Tl::EPV == 0 && ((uintptr_t)base & 15) == 0 && (pitch & 15) == 0 && pitch < (int64_t)1 << 24;
+    const int64_t apart = moves ? v.head * (int64_t)sizeof(T) : 0;  // a head from the next
+    whole = d % Tl::EPV == 0 && (((uintptr_t)base | pitch | apart) & 15) == 0 && pitch < (int64_t)1 << 24;
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
       // (lane l of the block fills its place l)
@@ -346,7 +348,7 @@ struct Fetcher {
       off[i] = vec * Tl::EPV < d ? (uint32_t)(row * (int)pitch + vec * 16) : OOB;
     }
   }
-  // another head of the same matrix
+  // another head of the same matrix (`whole` holds for all of them: see init)
   __device__ __forceinline__ void move(const View& v, int64_t b, int h) {
     base = (const char*)((const T*)v.p + b * v.batch + (int64_t)h * v.head);
   }

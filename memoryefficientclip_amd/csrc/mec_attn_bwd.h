@@ -455,8 +455,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
       }
     } else {
       Fetcher<T, DB, STEP, WM> fq, fg;
-      fq.init(a.q, b, kh * a.group, a.d, wave, lane);
-      fg.init(a.g, b, kh * a.group, a.d, wave, lane);
+      fq.init(a.q, b, kh * a.group, a.d, wave, lane, a.group > 1);
+      fg.init(a.g, b, kh * a.group, a.d, wave, lane, a.group > 1);
       walk_tiles(
           begin_at, stop,
           [&](int at, auto place) {
