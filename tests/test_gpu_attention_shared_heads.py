@@ -50,3 +50,51 @@ def test_heads_on_other_boundaries_than_the_first(row, dtype):
     q, k, v, do = inputs(2, 40, 256, 8, 2, 64, dtype, seed=row)
     assert layout(q).stride()[1:3] == (8 * row, row)
     check(64, q, k, v, do, layout=layout)
+
+
+# batch, queries, keys, heads, key heads; of 256 compute units: 512 and 896 workgroups of 128 rows, 256 of 128 keys; in the
+# second, queries are split in two for each 128 keys
+FORMS = [(64, 70, 200, 12, 2), (64, 200, 129, 8, 2)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("d", [16, 40, 64, 72, 100, 128])
+@pytest.mark.parametrize("b,n,m,h,hk", FORMS)
+def test_forms_of_whole_batches(b, n, m, h, hk, d, causal, dtype):
+    check(b, *inputs(2, n, m, h, hk, d, dtype, seed=d), causal=causal)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("d", [40, 64, 128])
+@pytest.mark.parametrize("b,n,m,h,hk", FORMS)
+def test_padded_batches(b, n, m, h, hk, d, causal, dtype):
+    """Lengths of none, one, some and all; rows that see nothing."""
+    nq = torch.tensor([n, 0, 1, n - 31, n // 2, 3, n, 33], dtype=torch.int32)
+    nk = torch.tensor([m, 50, m, 65, 0, 1, 7, m - 1], dtype=torch.int32)
+    check(b, *inputs(8, n, m, h, hk, d, dtype, seed=d), causal=causal, query_lengths=nq, key_lengths=nk)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("what", ["q", "k", "v", "do"])
+@pytest.mark.parametrize("d", [40, 72, 128])
+@pytest.mark.parametrize("b,n,m,h,hk", FORMS)
+def test_what_is_not_seen_has_no_part(b, n, m, h, hk, d, what, dtype):
+    """A NaN in the middle of a causal sequence: earlier tokens do not see it."""
+    q, k, v, do = inputs(1, n, m, h, hk, d, dtype, seed=d)
+    at = {"q": q, "k": k, "v": v, "do": do}[what]
+    at[0, at.shape[1] // 2, -1, 5] = float("nan")
+    at[0, at.shape[1] // 3 * 2, 0, :] = float("nan")
+    check(b, q, k, v, do, causal=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 72, 128])
+@pytest.mark.parametrize("n,m,h,hk", [(300, 420, 4, 2), (1300, 1300, 2, 1), (40, 700, 2, 1)])
+def test_what_is_not_seen_has_no_part_in_long_sequences(n, m, h, hk, d, dtype):
+    """The same where a workgroup has 32 rows or keys, or keys and queries are split over workgroups."""
+    q, k, v, do = inputs(1, n, m, h, hk, d, dtype, seed=d)
+    k[0, m // 2, 0, 5] = v[0, m // 3 * 2, -1, 5] = float("nan")
+    q[0, n // 3, 0, 1] = do[0, n // 5, 0, 2] = float("nan")
+    check(1, q, k, v, do, causal=True)
