@@ -388,7 +388,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
       Lds* const tg = tq + B::TILE;
       const int q0 = (first + i % each) * STEP;
       if (q0 + STEP <= wave_begin) return;
-      const bool masked = q0 < all;
+      // (of rows beyond the queries Q and dO are 0, but 0 times a key that holds an inf is NaN)
+      const bool masked = q0 < all || q0 + STEP > nq;
 #pragma unroll
       for (int qb = 0; qb < NB; ++qb) {
         f32x16 s = zero16(), p = zero16();
@@ -413,7 +414,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
         if (masked) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const bool in = q0 + 32 * qb + 8 * (e >> 2) + 4 * half + (e & 3) >= seen;
+            const int i = q0 + 32 * qb + 8 * (e >> 2) + 4 * half + (e & 3);
+            const bool in = i >= seen && i < nq;
             s[e] = in ? s[e] : 0.f;
             p[e] = in ? p[e] : 0.f;
           }

@@ -224,7 +224,7 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
       for (int walk = TWICE ? 0 : 1; walk < 2; ++walk) {
         Lds* at = tk;
         for (int key0 = 0; key0 < end; key0 += 32, at += 2 * BLOCK) {
-    lane_at.again();
+          lane_at.again();
           f32x16 s = zero16(), p = zero16();
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) {
@@ -288,7 +288,8 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
 #pragma unroll
         for (int db = 0; db < DB; ++db) acc[db] = zero16();
     }
-    if (half == 0 && first < nq) s_delta[qi] = dot;
+    // (rows beyond the queries have none: 0 times a key or value that holds an inf is NaN)
+    if (half == 0 && first < nq) s_delta[qi] = live ? dot : 0.f;
     packed.pack(acc, a.scale);
   }
   const auto to = [&](T* p, int n, int heads) {
@@ -343,10 +344,11 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
           p[4 * e + f] = s[4 * e + f] * (O::GRAD_UNIT * p[4 * e + f]);
         }
       }
-      if (q0 < all) {
+      if (q0 < all || q0 + 32 > nq) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const bool in = q0 + 8 * (e >> 2) + 4 * half + (e & 3) >= seen;
+          const int i = q0 + 8 * (e >> 2) + 4 * half + (e & 3);
+          const bool in = i >= seen && i < nq;
           s[e] = in ? s[e] : 0.f;
           p[e] = in ? p[e] : 0.f;
         }
