@@ -6,9 +6,10 @@
 // share a key head for 32 keys a wave (four: S, dP, dV, dK).  S and dP are made
 // twice, seven products for the five that one kernel would need, which would have
 // to add its dQ over the key tiles in memory: with atomics in no fixed order, or
-// in a pass of its own.  Gradients of the scores are rounded to T like the results:
-// in fp16, to steps of 2^-24 and up to 65504, as the gradients that go out are.
-// k_attn_dq also leaves delta = do . o for k_attn_dkv.
+// in a pass of its own.  Gradients of the scores are rounded to T (the MFMA's operand);
+// in fp16 in units of their own (GradUnit).
+// k_attn_dq also leaves delta = do . o for k_attn_dkv, and what that lacks where it
+// has it (Backward): a product more in a first walk, or the mean key's.
 //
 // WM = 4: the four waves of a workgroup have 32 rows (keys) each and share tiles,
 // two in LDS, one of them on its way (Fetcher).  WM = 1, where that would leave the
@@ -136,6 +137,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
     mean[B::MEAN ? db : 0] = zero16();
   }
   float eps = 0.f, eps16 = 0.f;  // sums of the ds_ij, and of the rounded ones
+  GradUnit<O> unit;              // of them and of acc
   const int tiles = (end + STEP - 1) / STEP;
   if (tiles > 0) {
     const int first = WM == 1 ? wave : 0;
@@ -161,7 +163,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           s[e] = fast_exp2(fmaf(s[e], a.c, -l2));
-          p[e] = s[e] * (p[e] - dot);
+          p[e] = s[e] * unit.times(p[e], dot);
         }
         if (masked) {
 #pragma unroll
@@ -171,6 +173,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
             p[e] = in ? p[e] : 0.f;
           }
         }
+        unit.fit(p, [&](float f) {
+          scale_all(acc, f);
+          eps *= f;
+          eps16 *= f;
+        });
         if constexpr (B::MEAN) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) eps += p[e];
@@ -243,6 +250,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
             [&](int i, auto place) { use((Lds*)(place ? s_next : s_lds), i); });
       }
       if (walk == 0) {
+        if constexpr (O::F16) eps *= unit.back();
         eps += other_half(eps);
         if constexpr (WM == 1) {
           if (half == 0) s_eps[wave][lane] = eps;
@@ -255,6 +263,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
         eps = 0.f;
       }
     }
+  }
+  if constexpr (O::F16) {
+    scale_all(acc, unit.back());
+    eps *= unit.back();
+    eps16 *= unit.back();
   }
   if constexpr (B::MEAN) {
     eps += other_half(eps);
@@ -345,6 +358,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
   f32x16 ak[DB], av[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) ak[db] = av[db] = zero16();
+  GradUnit<O> unit(O::GRAD_UNIT);  // of ak, beside that of the probabilities
   // the tiles of all heads, and this workgroup's share of them
   const int first = begin / STEP, each = (nq + STEP - 1) / STEP - first;
   const int tiles = each > 0 ? each * a.group : 0, share = (tiles + splits - 1) / splits;
@@ -408,7 +422,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
 #pragma unroll
           for (int f = 0; f < 4; ++f) {
             s[4 * e + f] = fast_exp2(fmaf(s[4 * e + f], a.c, O::GRAD_BIAS - l2[f]));
-            p[4 * e + f] = s[4 * e + f] * (O::GRAD_UNIT * (p[4 * e + f] - dl[f]));
+            p[4 * e + f] = s[4 * e + f] * unit.times(p[4 * e + f], dl[f]);
           }
         }
         if (masked) {
@@ -420,6 +434,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
             p[e] = in ? p[e] : 0.f;
           }
         }
+        unit.fit(p, [&](float f) { scale_all(ak, f); });
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const Frag fp = O::pack(s, h), fs = O::pack(p, h);
@@ -482,6 +497,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (WM == 1 && KS > 4) ? 1 : 2)
           });
     }
   }
+  if constexpr (O::F16) scale_all(ak, O::GRAD_UNIT * unit.back());
   if (a.causal && (any_nan<O>(ak) || any_nan<O>(av))) {
     float again[32 * DB];
     const int h = kh * a.group;

@@ -221,6 +221,7 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
 #pragma unroll
       for (int db = 0; db < (MEAN ? DB : 1); ++db) mean[db] = zero16();
       float eps = 0.f, eps16 = 0.f;
+      GradUnit<O> unit;  // of them and of acc
       for (int walk = TWICE ? 0 : 1; walk < 2; ++walk) {
         Lds* at = tk;
         for (int key0 = 0; key0 < end; key0 += 32, at += 2 * BLOCK) {
@@ -234,7 +235,7 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             s[e] = fast_exp2(fmaf(s[e], a.c, -l2));
-            p[e] = s[e] * (p[e] - dot);
+            p[e] = s[e] * unit.times(p[e], dot);
           }
           if (key0 + 32 > all) {
 #pragma unroll
@@ -244,6 +245,11 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
               p[e] = in ? p[e] : 0.f;
             }
           }
+          unit.fit(p, [&](float f) {
+            scale_all(acc, f);
+            eps *= f;
+            eps16 *= f;
+          });
           if (!O::F32) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) eps += p[e];
@@ -262,9 +268,15 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
           }
         }
         if (TWICE && walk == 0) {
+          if constexpr (O::F16) eps *= unit.back();
           dot += eps + other_half(eps);
           eps = 0.f;
         }
+      }
+      if constexpr (O::F16) {
+        scale_all(acc, unit.back());
+        eps *= unit.back();
+        eps16 *= unit.back();
       }
       if constexpr (MEAN) {
         eps += other_half(eps);
@@ -318,6 +330,7 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
     f32x16 ak[DB], av[DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db) ak[db] = av[db] = zero16();
+    GradUnit<O> unit(O::GRAD_UNIT);  // of ak, beside that of the probabilities
     const int begin = first >= nk ? nq : a.causal ? max(0, first - shift) & ~31 : 0;
     const int all = a.causal ? first + 31 - shift : 0, seen = a.causal ? key - shift : 0;
     Lds* at = tq + begin * 2 * Tl::RB;
@@ -341,7 +354,7 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
           s[4 * e + f] = fast_exp2(fmaf(s[4 * e + f], a.c, -ls[f]));
-          p[4 * e + f] = s[4 * e + f] * (O::GRAD_UNIT * p[4 * e + f]);
+          p[4 * e + f] = s[4 * e + f] * unit.times(p[4 * e + f]);
         }
       }
       if (q0 < all || q0 + 32 > nq) {
@@ -353,6 +366,7 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
           p[e] = in ? p[e] : 0.f;
         }
       }
+      unit.fit(p, [&](float f) { scale_all(ak, f); });
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const Frag fp = O::pack(s, x), fs = O::pack(p, x);
@@ -363,6 +377,7 @@ __global__ __launch_bounds__(64 * whole_waves(KS, sizeof(T))) void k_attn_whole_
         }
       }
     }
+    if constexpr (O::F16) scale_all(ak, O::GRAD_UNIT * unit.back());
     if (a.causal && (any_nan<O>(ak) || any_nan<O>(av))) {
       // (delta of all queries is in LDS alone)
       float again[32 * DB];
