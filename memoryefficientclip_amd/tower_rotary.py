@@ -135,6 +135,10 @@ class _NormRotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, positions, query_weight, key_weight, frequencies, sections, eps, theta, traced):
         theta, interleaved = theta
+        if ctx.needs_input_grad[2] or ctx.needs_input_grad[5]:
+            # (it would be taken for zero without a word)
+            raise RuntimeError("memoryefficientclip_amd: norm_rotary has no gradient for positions and frequencies; detach "
+                               "them")
         if traced:
             _check(query, key, positions, sections, query_weight, key_weight, eps, frequencies)
             positions, query_weight, key_weight, frequencies = _plain(positions, query_weight, key_weight, frequencies)
@@ -152,7 +156,7 @@ class _NormRotaryFn(torch.autograd.Function):
 
 def _plain(positions, query_weight, key_weight, frequencies):
     return (positions.contiguous(), *(w if w is None else w.contiguous() for w in (query_weight, key_weight)),
-            frequencies if frequencies is None else frequencies.detach().double().contiguous())
+            frequencies if frequencies is None else frequencies.double().contiguous())
 
 
 def norm_rotary(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor, sections,
@@ -174,7 +178,8 @@ def norm_rotary(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor,
       [head_dim / 2] (float64 or float32; 0 leaves a pair as it is).
 
     Gradients flow to query, key and the weights; those of the weights are summed in fp32,
-    in a fixed order.  head_dim even, up to 256; up to 8 axes.
+    in a fixed order.  Positions or frequencies that ask for one are refused.  head_dim
+    even, up to 256; up to 8 axes.
     """
     sections = tuple(int(n) for n in sections)
     _check(query, key, positions, sections, query_weight, key_weight, eps, frequencies)
@@ -191,7 +196,7 @@ def norm_rotary(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor,
         return tuple(x * 1 + sum(links).to(x.dtype) if links else x * 1 for x in (query, key))
     positions, query_weight, key_weight, frequencies = _plain(positions, query_weight, key_weight, frequencies)
     args = (query, key, positions, query_weight, key_weight, frequencies, sections, eps)
-    if _h.wants_autograd(query, key, query_weight, key_weight):
+    if _h.wants_autograd(query, key, query_weight, key_weight, positions, frequencies):
         return _NormRotaryFn.apply(*args, (theta, bool(interleaved)), _v.is_tracing())
     return _turn(*args, theta, bool(interleaved))[:2]
 
