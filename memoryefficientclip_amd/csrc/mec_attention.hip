@@ -20,16 +20,21 @@ struct Plan {
 };
 constexpr int kWave = 4;
 
-// Waves of k_attn_whole_forward and its LDS, 0 where another form is taken: up to 64 KB, of which two workgroups
-// and more share a CU, and not for few rows of many keys, whose loads want more waves.  256 x 12 heads of 64, us, this
-// form and the one that walks over tiles: 77 tokens 29 and 36, 197 tokens (56 KB) 82 and 106, 257 (72 KB) 184 and 149;
-// 160 tokens of 16-bit heads of 72 (60 KB) 93 and 110, 197 (84 KB) 161 and 137.
+// Waves of k_attn_whole_forward and its LDS, 0 waves where another form is taken: of 16-bit types 48 KB of keys and values
+// (three workgroups share a CU), 40 KB beyond 128 keys and up to 256 keys, of fp32 64 KB; and not for few rows of many
+// keys, whose loads want more waves.  256 x 12 heads, us, this form and the one that walks over tiles.  bf16, heads of 64: 77
+// tokens 27 and 30, 160 (40 KB) 65 and 69, 176 (48 KB) 78 and 72, 225 (64 KB) 109 and 94; of 72: 96 tokens (36 KB) 38 and
+// 43, 128 (48 KB) 53 and 54, 160 (60 KB) 122 and 90; of 128: 96 tokens (48 KB) 71 and 72, 128 (64 KB) 95 and 88; of 32: 160
+// tokens 33 and 47, 225 (32 KB) 63 and 64, 257 (36 KB) 107 and 94.  fp32, heads of 64: 128 tokens (64 KB) 159 and 191; of
+// 32: 160 tokens (40 KB) 159 and 162, 224 (56 KB) 233 and 219, 256 (64 KB) 238 and 246.
 int whole_forward(const Problem& a, int dtype, int64_t rows, size_t* lds) {
-  const int size = dtype == MEC_DTYPE_F32 ? 4 : 2, steps = a.d <= 32 ? 2 : a.d <= 64 ? 4 : a.d <= 96 ? 6 : 8;
+  const bool f32 = dtype == MEC_DTYPE_F32;
+  const int size = f32 ? 4 : 2, steps = a.d <= 32 ? 2 : a.d <= 64 ? 4 : a.d <= 96 ? 6 : 8;
   const int64_t blocks = ceil_div(rows, 32), key_blocks = ceil_div(a.keys, 32);
+  const size_t most = f32 ? 64 * 1024 : key_blocks <= 4 ? 48 * 1024 : key_blocks <= 8 ? 40 * 1024 : 0;
   *lds = (size_t)(key_blocks * 2 * 32 * 16 * steps * size);
   // (rows leave through the place of keys and values)
-  const bool fits = blocks <= whole_waves(steps, size) && *lds <= 64 * 1024 && blocks <= 2 * key_blocks;
+  const bool fits = blocks <= whole_waves(steps, size) && *lds <= most && blocks <= 2 * key_blocks;
   return fits && key_blocks <= 4 * blocks ? (int)blocks : 0;
 }
 

@@ -5,9 +5,10 @@
 namespace mec {
 namespace attn {
 
-// Waves and LDS of k_attn_whole_grad, 0 waves where it does not fit.  Where it does it was the faster form at all
-// sizes, 2 to 256 x 12 heads (256 x 12 heads of 64, us, this form and two kernels that walk over tiles: 77 tokens 68
-// and 131, 197 tokens 297 and 354, 257 tokens 414 and 571; fp32, 77 tokens, 395 and 459).
+// Waves and LDS of k_attn_whole_grad, 0 waves where it does not fit.  Where it does it is the faster form at all sizes
+// (a step's time less the forward's, 256 x 12 heads, us, this form and two kernels that walk over tiles; bf16, heads of 64:
+// 77 tokens 135 and 138, 129 205 and 307, 197 306 and 398, 257 442 and 630; 1024 x 77 causal 230 and 580; heads of 32:
+// 77 tokens 140 and 146, 257 270 and 320; of 72: 77 tokens 128 and 173, 160 277 and 393; fp32, 77 tokens of 64, 391 and 467).
 struct Whole {
   int waves;
   size_t lds;
