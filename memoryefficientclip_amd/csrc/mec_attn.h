@@ -35,11 +35,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char Lds;
 
-// Heads as the callers give them: element (b, t, h, i) at p[b * batch + t * token + h * head + i].
-struct View {
-  const void* p;
-  int64_t batch, token, head;
-};
+using View = HeadsView;
 
 struct Problem {
   View q, k, v, g;  // g: the gradient of the result
@@ -406,11 +402,6 @@ __device__ __forceinline__ void walk_tiles(int first, int last, Load load, Use u
 __device__ __forceinline__ float other_half(float v) {
   const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float((threadIdx.x & 32) ? sw[0] : sw[1]);
-}
-
-__device__ __forceinline__ void wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
 }
 
 // The running maximum m (in units of log2) after scores s, times c: sum l and accumulators o are

@@ -30,12 +30,6 @@ constexpr int kRotaryWaves = 4;
 constexpr int kMaxAxes = 8;
 constexpr int kMaxHalf = 128;  // pairs of a head
 
-// Heads as the callers give them: element (b, t, h, i) at p[b * batch + t * token + h * head + i].
-struct HeadsView {
-  const void* p;
-  int64_t batch, token, head;
-};
-
 struct RotaryShape {
   int64_t rows;       // batch * tokens
   int tokens;
@@ -176,12 +170,6 @@ struct Pairs {
 __device__ __forceinline__ float row_sum(float v, int lg) {
   for (int m = 0; m < lg; ++m) v += __shfl_xor(v, 1 << m, 64);
   return v;
-}
-
-// What the lanes of a wave wrote to LDS is there for its other lanes.
-__device__ __forceinline__ void wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
 }
 
 // Turns per position and the axis of a lane's pairs (lane and lane + 64).

@@ -1,5 +1,5 @@
 // Rows of fp32, bf16 or fp16 elements in 16-byte vectors, at any alignment and
-// with any number of elements, as fp32 values.
+// with any number of elements, as fp32 values; heads in memory.
 #pragma once
 #include "mec_common.h"
 
@@ -78,6 +78,18 @@ __device__ __forceinline__ typename Vec<T>::raw load_raw(const T* p, int n) {
 template <class T>
 __device__ __forceinline__ void load_row(const T* p, int n, float (&v)[Vec<T>::N]) {
   Vec<T>::unpack(load_raw(p, n), v);
+}
+
+// Heads as the callers give them: element (b, t, h, i) at p[b * batch + t * token + h * head + i].
+struct HeadsView {
+  const void* p;
+  int64_t batch, token, head;
+};
+
+// What the lanes of a wave wrote to LDS is there for its other lanes.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
 
 // Outputs that pass half of the last-level cache (256 MB) are stored past it: there

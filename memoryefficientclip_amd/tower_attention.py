@@ -13,7 +13,6 @@ import math
 
 import torch
 
-from . import _function as _f
 from . import _heads as _h
 from . import _lib
 from . import _vocab as _v
