@@ -9,7 +9,7 @@
 // in a pass of its own.  Gradients of the scores are rounded to T (the MFMA's operand);
 // in fp16 in units of their own (GradUnit).
 // k_attn_dq also leaves delta = do . o for k_attn_dkv, and what that lacks where it
-// has it (Backward): a product more in a first walk, or the mean key's.
+// has it (Backward), from a first walk of two products, or along with the mean key.
 //
 // WM = 4: the four waves of a workgroup have 32 rows (keys) each and share tiles,
 // two in LDS, one of them on its way (Fetcher).  WM = 1, where that would leave the
